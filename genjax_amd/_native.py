@@ -42,8 +42,11 @@ def build(force: bool = False) -> str:
     # (the default of that cap) -- above it the copy stays, i.e. every lane writes ~2.5 KB of world tables to scratch
     # at kernel entry and indexes them there.  The 16- and 32-ray move kernels were over the cap (scratch 2.0-4.1 KB
     # per lane against 0.2-0.5 KB with the cap lifted).
+    # -packed-fp32-ops: no v_pk_{add,mul,fma}_f32 (some of their forms have given wrong results on this hardware);
+    # every element rounds as before, so results keep their bits.  (The host pass warns that it does not know the feature.)
     flags = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-ffp-contract=on",
-             "-mllvm", "-instcombine-max-copied-from-constant-users=1000000"] + \
+             "-mllvm", "-instcombine-max-copied-from-constant-users=1000000",
+             "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"] + \
         os.environ.get("GJX_EXTRA_HIPCC_FLAGS", "").split()
     stamp = os.path.join(objdir, "flags.txt")
     if not os.path.exists(stamp) or open(stamp).read() != " ".join(flags):
