@@ -33,6 +33,7 @@ from .distributions import (  # noqa: F401
     beta,
     categorical,
     flip,
+    linear_categorical,
     multivariate_normal,
     normal,
     uniform,

@@ -431,6 +431,110 @@ def categorical_logpdf(x, logits):
     return out.reshape(()) if scalar else out
 
 
+# --------------------------------------------------------------------------- #
+# categorical with linear logits, x W^T + b
+# --------------------------------------------------------------------------- #
+ELEMENT_TYPES = {torch.float32: 0, torch.bfloat16: 1}       # GJX_F32, GJX_BF16
+
+
+def _on_current_device(who, **tensors):
+    """Refuse tensors that are not on the current device (launches go to its current stream)."""
+    cur = torch.cuda.current_device() if torch.cuda.is_available() else None
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            raise GjxError(f"{who}: `{name}` must be a device tensor")
+        if t.device.index != cur:
+            raise GjxError(f"{who}: `{name}` lives on cuda:{t.device.index} but the current device is cuda:{cur}: launches "
+                           "go to the current device's stream (use torch.cuda.set_device / torch.cuda.device)")
+
+
+def _unit_stride(t):
+    """`t` itself when its last axis is contiguous and its rows do not overlap, else a contiguous copy."""
+    ok = t.stride(-1) == 1 or t.shape[-1] == 1
+    if t.dim() > 1:
+        ok = ok and t.stride(0) >= t.shape[-1]
+    return t if ok else t.contiguous()
+
+
+def _linear_args(who, x, weight, bias):
+    for name, t in (("x", x), ("weight", weight), ("bias", bias)):
+        if t is not None and not isinstance(t, torch.Tensor):
+            raise GjxError(f"{who}: `{name}` must be a tensor")
+    if x.dim() != 2 or weight.dim() != 2 or x.shape[1] != weight.shape[1] or weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise GjxError(f"{who}: x {tuple(x.shape)} and weight {tuple(weight.shape)} must be (n, width) and (vocab, width)")
+    if bias is not None and tuple(bias.shape) != (weight.shape[0],):
+        raise GjxError(f"{who}: bias {tuple(bias.shape)} must be ({weight.shape[0]},)")
+    if x.dtype not in ELEMENT_TYPES or any(t is not None and t.dtype != x.dtype for t in (weight, bias)):
+        raise GjxError(f"{who}: x, weight and bias must all be float32 or all bfloat16 (got {x.dtype}, {weight.dtype}"
+                       f"{'' if bias is None else f', {bias.dtype}'})")
+    _on_current_device(who, x=x, weight=weight, bias=bias)
+    return _unit_stride(x), _unit_stride(weight), None if bias is None else bias.contiguous()
+
+
+def _linear_head(x, weight):
+    return (C.c_void_p(x.data_ptr()), max(x.stride(0), x.shape[1]), C.c_void_p(weight.data_ptr()),
+            max(weight.stride(0), weight.shape[1]))
+
+
+def _linear_workspace(x, weight, grad):
+    n, (vocab, width) = x.shape[0], weight.shape
+    size = C.c_int64()
+    N.check(N.lib().gjx_linear_categorical_workspace(ELEMENT_TYPES[x.dtype], *_linear_head(x, weight), n, vocab, width, grad,
+                                                     C.byref(size)), "gjx_linear_categorical_workspace")
+    return torch.empty(max(size.value, 256), dtype=torch.uint8, device=x.device)
+
+
+def linear_categorical_logpdf(y, x, weight, bias=None):
+    """y: (n,) int32; x: (n, width), weight: (vocab, width), bias: (vocab,) or None -> (log p(y) (n,), logsumexp (n,))."""
+    who = "linear_categorical"
+    x, weight, bias = _linear_args(who, x, weight, bias)
+    n, (vocab, width) = x.shape[0], weight.shape
+    if y.dtype != torch.int32 or tuple(y.shape) != (n,):
+        raise GjxError(f"{who}: y must be int32 of shape ({n},), got {y.dtype} {tuple(y.shape)}")
+    _on_current_device(who, y=y)
+    lp = torch.empty(n, dtype=torch.float32, device=x.device)
+    lse = torch.empty(n, dtype=torch.float32, device=x.device)
+    if n > 0:
+        y = y.contiguous()
+        work = _linear_workspace(x, weight, 0)
+        N.check(N.lib().gjx_linear_categorical_logpdf(ELEMENT_TYPES[x.dtype], _ptr(y), *_linear_head(x, weight), _ptr(bias), n,
+                                                      vocab, width, _ptr(lp), _ptr(lse), _ptr(work), work.numel(), _stream()),
+                "gjx_linear_categorical_logpdf")
+    return lp, lse
+
+
+def linear_categorical_grad(y, x, weight, bias, lse, upstream, want=(True, True, True)):
+    """upstream x d log p / d(x, weight, bias), summed over the rows for weight and bias (entries not wanted: None)."""
+    x, weight, bias = _linear_args("linear_categorical", x, weight, bias)
+    n, (vocab, width) = x.shape[0], weight.shape
+    like = (x, weight, bias)
+    outs = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if w and t is not None else None for w, t in zip(want, like)]
+    if n == 0:
+        return [None if o is None else o.zero_() for o in outs]
+    if any(o is not None for o in outs):
+        y, upstream = y.contiguous(), _f32(upstream).contiguous()
+        work = _linear_workspace(x, weight, 1 if outs[0] is not None else 2)
+        N.check(N.lib().gjx_linear_categorical_grad(ELEMENT_TYPES[x.dtype], _ptr(y), *_linear_head(x, weight), _ptr(bias), n,
+                                                    vocab, width, _ptr(lse), _ptr(upstream), *(_ptr(o) for o in outs),
+                                                    _ptr(work), work.numel(), _stream()), "gjx_linear_categorical_grad")
+    return outs
+
+
+def sample_linear_categorical(k, x, weight, bias=None, offset: int = 0) -> torch.Tensor:
+    """One Gumbel-max draw per row of x from softmax(x W^T + b); the noise layout of sample_categorical's per-row form."""
+    x, weight, bias = _linear_args("linear_categorical", x, weight, bias)
+    n, (vocab, width) = x.shape[0], weight.shape
+    out = torch.empty(n, dtype=torch.int32, device=x.device)
+    if n > 0:
+        work = _linear_workspace(x, weight, 0)
+        N.check(N.lib().gjx_random_linear_categorical_i32(_ckey(k), offset, ELEMENT_TYPES[x.dtype], *_linear_head(x, weight),
+                                                          _ptr(bias), n, vocab, width, _ptr(out), _ptr(work), work.numel(),
+                                                          _stream()), "gjx_random_linear_categorical_i32")
+    return out
+
+
 def mvnormal_logpdf(x, mu, cov):
     """x: (n, d); mu: (n, d) or (d,); cov: (n, d, d) or (d, d)."""
     x = _f32(x)

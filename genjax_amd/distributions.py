@@ -115,6 +115,67 @@ class _Categorical(Distribution):
 categorical = _Categorical(None, lambda x, logits: B.categorical_logpdf(x, as_col(logits)), name="categorical")
 
 
+# categorical(logits = x W^T + b) of distributions.py:92-95 without its logits: for vocabularies too large to keep one
+# row of them per particle.  The gradient (x, weight, bias) is the library's, as for the densities above.
+class _LinearCategoricalFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, x, weight, bias):
+        lp, lse = B.linear_categorical_logpdf(y, x, weight, bias)
+        ctx.save_for_backward(y, x, weight, bias, lse)
+        return lp
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        y, x, weight, bias, lse = ctx.saved_tensors
+        return (None, *B.linear_categorical_grad(y, x, weight, bias, lse, g, want=ctx.needs_input_grad[1:4]))
+
+
+class _LinearCategorical(Distribution):
+    """linear_categorical(x, weight, bias=None): a draw from softmax(x W^T + b) per row.  x: (n, width) rows or one
+    (width,) row shared by every particle; weight: (vocab, width); bias: (vocab,).  All float32 or all bfloat16;
+    sums and log-densities are float32.  Differentiable in x, weight and bias."""
+
+    def _param_event_ndims(self, a):
+        return a.dim() if isinstance(a, torch.Tensor) else 0
+
+    @staticmethod
+    def _rows(x, n):
+        if x.dim() not in (1, 2):
+            raise B.GjxError(f"linear_categorical: x {tuple(x.shape)} must be (width,) or (n, width)")
+        return x if x.dim() == 2 and x.shape[0] == n else x.reshape(-1, x.shape[-1]).expand(n, x.shape[-1])
+
+    def sample(self, x, weight, bias=None, **kwargs):
+        from .core import _next_key, batch_size
+
+        x, weight, bias = as_col(x), as_col(weight), None if bias is None else as_col(bias)
+        n = x.shape[0] if x.dim() == 2 else (batch_size() or 1)
+        out = B.sample_linear_categorical(_next_key(), self._rows(x.detach(), n), weight.detach(),
+                                          None if bias is None else bias.detach())
+        return out if (x.dim() == 2 or batch_size()) else out[0]
+
+    def logpdf(self, y, x, weight, bias=None, **kwargs):
+        x, weight, bias = as_col(x), as_col(weight), None if bias is None else as_col(bias)
+        y = torch.as_tensor(y, device=x.device)
+        if y.dim() > 1:
+            raise B.GjxError(f"linear_categorical: y {tuple(y.shape)} must be one value or one per row")
+        n = x.shape[0] if x.dim() == 2 else max(1, y.numel())
+        if y.dim() == 1 and x.dim() == 2 and n == 1:
+            n = y.numel()
+        if y.dim() == 1 and y.numel() not in (1, n):
+            raise B.GjxError(f"linear_categorical: {y.numel()} values against {n} rows of x")
+        scalar = y.dim() == 0 and x.dim() == 1
+        rows, ys = self._rows(x, n), y.reshape(-1).to(torch.int32).expand(n)
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+            out = _LinearCategoricalFn.apply(ys, rows, weight, bias)
+        else:
+            out = B.linear_categorical_logpdf(ys, rows, weight, bias)[0]
+        return out.reshape(()) if scalar else out
+
+
+linear_categorical = _LinearCategorical(None, None, name="linear_categorical")
+
+
 # multivariate_normal(mu, cov)                                 distributions.py:298-301
 class _MvNormal(Distribution):
     def sample(self, mu, cov, **kwargs):

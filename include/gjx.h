@@ -48,6 +48,11 @@ extern "C" {
 #define GJX_MAX_COLS 16
 #define GJX_MAX_PIECES 64   /* ranges per gjx_shard_pack call (= max ranks of a sharded run) */
 #define GJX_MAX_POINTS 64
+#define GJX_MAX_LINCAT (1 << 24)   /* rows and vocabulary entries of the linear-categorical calls */
+
+/* element types of the calls that take more than float */
+#define GJX_F32 0
+#define GJX_BF16 1
 
 typedef struct gjx_ctx gjx_ctx;
 
@@ -134,6 +139,32 @@ int32_t gjx_logpdf_grad_f32(int32_t kind, const float* d_x, const float* d_p1, i
 /* logits: n x k row-major when logits_stride = 1, one shared row of k when 0 */
 int32_t gjx_categorical_logpdf_f32(const int32_t* d_x, const float* d_logits, int32_t logits_stride,
                                    int64_t n, int32_t k, float* d_out, void* stream);
+/* ---- categorical(logits = x W^T + b): the categorical of distributions.py:92-95 whose logits are a linear map of a
+ * feature row, without keeping the n x vocab logits.  x: n rows of `width` (row stride x_ld elements), W: vocab rows
+ * (stride w_ld), bias: vocab or NULL, all of type `dtype` (GJX_F32 or GJX_BF16); sums and outputs lp, lse in f32.
+ * y outside [0, vocab) takes the nearest entry.  A bias of -inf takes its entry out of the distribution; a row with no
+ * entry left is NaN.  The caller owns the workspace (256-byte aligned, gjx_linear_categorical_workspace bytes; grad:
+ * 0 for the log-density, 1 for the gradient, 2 for the gradient without d_dx); its contents need not be kept between calls.
+ *   logpdf: lp_i = l_{i, y_i} - lse_i, lse_i = log sum_v exp(l_iv)
+ *   grad:   outputs (nullable) dx, dW, db of sum_i upstream_i lp_i, contiguous, of type dtype (what jax.grad of
+ *           assess produces inside hmc, mcmc.py:59-88, 508, 523); d_lse is the log-density call's */
+int32_t gjx_linear_categorical_workspace(int32_t dtype, const void* d_x, int64_t x_ld, const void* d_w, int64_t w_ld,
+                                         int64_t n, int64_t vocab, int64_t width, int32_t grad, int64_t* bytes);
+int32_t gjx_linear_categorical_logpdf(int32_t dtype, const int32_t* d_y, const void* d_x, int64_t x_ld,
+                                      const void* d_w, int64_t w_ld, const void* d_bias, int64_t n, int64_t vocab,
+                                      int64_t width, float* d_lp, float* d_lse, void* d_work, int64_t work_bytes,
+                                      void* stream);
+int32_t gjx_linear_categorical_grad(int32_t dtype, const int32_t* d_y, const void* d_x, int64_t x_ld, const void* d_w,
+                                    int64_t w_ld, const void* d_bias, int64_t n, int64_t vocab, int64_t width,
+                                    const float* d_lse, const float* d_upstream, void* d_dx, void* d_dw, void* d_db,
+                                    void* d_work, int64_t work_bytes, void* stream);
+/* its draw: argmax_v (l_iv + Gumbel), the Gumbel of entry v of row i on counter (offset + i) vocab + v of the key (the
+ * layout of gjx_random_categorical_i32 with per-row logits; distributions.py:92-95), ties to the lowest entry;
+ * workspace as for the log-density */
+int32_t gjx_random_linear_categorical_i32(const uint32_t key[2], uint64_t offset, int32_t dtype, const void* d_x,
+                                          int64_t x_ld, const void* d_w, int64_t w_ld, const void* d_bias, int64_t n,
+                                          int64_t vocab, int64_t width, int32_t* d_out, void* d_work,
+                                          int64_t work_bytes, void* stream);
 /* x: n x d; mu: n x d or d (stride 0); cov: n x d x d or d x d (stride 0); d <= 8 */
 int32_t gjx_mvnormal_logpdf_f32(const float* d_x, const float* d_mu, int32_t mu_stride,
                                 const float* d_cov, int32_t cov_stride, int64_t n, int32_t d,
@@ -718,6 +749,7 @@ int32_t gjx_gol_gibbs_pass(const uint32_t* d_pass_keys, int64_t n_chains, int32_
 /* full_gibbs_sweep (core.py:188-204): the nine colour passes; d_pass_keys9 = 9 x n_chains x 2 */
 int32_t gjx_gol_sweep(const uint32_t* d_pass_keys9, int64_t n_chains, int32_t n, float p_flip,
                       const uint8_t* d_future, int64_t future_stride, uint8_t* d_boards, void* stream);
+
 /* The same passes on BIT-PACKED boards (one bit per cell, row pitch gjx_gol_words_per_row(n) = ceil(n / 64)
  * 64-bit words, bit c of word w of a row = column 64 w + c, bits beyond n zero; chains contiguous).  Same
  * conditionals, same draws, same new boards as the byte form bit for bit; the 18 rule outcomes of a cell come

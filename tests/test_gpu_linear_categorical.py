@@ -1,0 +1,312 @@
+"""linear_categorical: log-density, gradients and draws against the definition in 64 bits on the same inputs.
+
+Tolerances (per element, from the arithmetic):
+ * a logit is a sum of `width` products accumulated in f32; whatever the order, it is off by at most
+   2 width 2^-23 sum_k |x_k w_k| (2^-23 a step: the matrix unit may truncate where an addition would round; the factor 2
+   covers the f32 operands' partial products left out, 2^-22 of each product) =: E;
+ * lse: the exponentials' relative errors (2 E and 2^-22 of expf) and at most 256 additions in a chain, 2^-16 in all;
+   the subtraction and the logarithm round once more, 2^-22 of |l| + |lse|;
+ * dl = g (onehot - p): p is off by (2 E + 2^-15) p, and dl is rounded to bf16 (2^-8) or split exactly (f32, 2^-22);
+ * dx, dW, db: the products' sums over m terms in f32 add 2 m 2^-23 sum |terms|; the result is rounded once to its type."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+TYPES = {"bf16": torch.bfloat16, "f32": torch.float32}
+HALF = {torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}
+
+
+@pytest.fixture(scope="module")
+def G():
+    import genjax_amd
+
+    assert torch.cuda.is_available()
+    return genjax_amd
+
+
+def _inputs(n, vocab, width, dtype, seed=0, bias=True, scale=2.0):
+    g = torch.Generator(device="cuda").manual_seed(1000 * n + vocab + width + seed)
+    r = lambda *s: torch.randn(s, generator=g, device="cuda")      # noqa: E731
+    x, w = r(n, width).to(dtype), (r(vocab, width) * scale / width ** 0.5).to(dtype)
+    b = (r(vocab) * 0.5).to(dtype) if bias else None
+    y = torch.randint(0, vocab, (n,), generator=g, device="cuda", dtype=torch.int32)
+    return x, w, b, y, r(n) * 0.1 + 1.0
+
+
+def _truth(x, w, b, y, up):
+    """lp, dx, dW, db in 64 bits and the elementwise bounds of the module's docstring."""
+    X, W, u = x.double(), w.double(), up.double().unsqueeze(1)
+    vocab, width, n = W.shape[0], W.shape[1], X.shape[0]
+    L = X @ W.t() + (0.0 if b is None else b.double())
+    lse = torch.logsumexp(L, 1, keepdim=True)
+    Y = y.long().clamp(0, vocab - 1).unsqueeze(1)
+    lp = (L.gather(1, Y) - lse).squeeze(1)
+    mag = X.abs() @ W.abs().t()
+    E = 2 * width * 2.0 ** -23 * mag.max(1, keepdim=True)[0]
+    lp_tol = (2 * E + 2.0 ** -16 + 2.0 ** -22 * (L.gather(1, Y).abs() + lse.abs())).squeeze(1)
+    P = (L - lse).exp()
+    D = -P * u
+    D.scatter_add_(1, Y, u)
+    half = HALF[x.dtype]
+    dD = D.abs() * (half if x.dtype == torch.bfloat16 else 2.0 ** -22) + u.abs() * P * (2 * E + 2.0 ** -15)
+    out = {"lp": (lp, lp_tol)}
+    dx, dw, db = D @ W, D.t() @ X, D.sum(0)
+    out["dx"] = (dx, dD @ W.abs() + 2 * vocab * 2.0 ** -23 * (D.abs() @ W.abs()) + half * dx.abs() + 1e-30)
+    out["dw"] = (dw, dD.t() @ X.abs() + 2 * n * 2.0 ** -23 * (D.abs().t() @ X.abs()) + half * dw.abs() + 1e-30)
+    out["db"] = (db, dD.sum(0) + 2 * n * 2.0 ** -23 * D.abs().sum(0) + half * db.abs() + 1e-30)
+    return out
+
+
+def _close(name, got, want_tol):
+    want, tol = want_tol
+    err = (got.double() - want).abs()
+    worst = (err / tol).max().item()
+    assert got.shape == want.shape and worst <= 1.0, f"{name}: {worst:.3g} times its bound (error {err.max().item():.3g})"
+
+
+def _grads(G, x, w, b, y, up):
+    leaves = [t.detach().clone().requires_grad_(True) for t in (x, w, b) if t is not None]
+    lp = G.linear_categorical.logpdf(y, *leaves)
+    return (lp.detach(),) + torch.autograd.grad(lp, leaves, up)
+
+
+SIZES = [(1, 1, 1), (1, 2, 7), (3, 5, 64), (5, 257, 65), (64, 256, 64), (65, 300, 128), (130, 70, 1000), (17, 4099, 520),
+         (257, 511, 192), (33, 2560, 8), (300, 33000, 64), (1000, 20011, 72), (4, 1500, 4096)]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("n,vocab,width", SIZES)
+def test_logpdf_and_gradients(G, n, vocab, width, dtype):
+    x, w, b, y, up = _inputs(n, vocab, width, TYPES[dtype])
+    t = _truth(x, w, b, y, up)
+    _close("lp without a gradient", G.linear_categorical.logpdf(y, x, w, b), t["lp"])
+    for name, got in zip(("lp", "dx", "dw", "db"), _grads(G, x, w, b, y, up)):
+        _close(name, got, t[name])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_no_bias_strided_rows_and_partial_gradients(G, dtype):
+    t = TYPES[dtype]
+    n, vocab, width = 70, 900, 128
+    wide_x, wide_w, _, y, up = _inputs(n, vocab, 2 * width + 5, t, bias=False)
+    x, w = wide_x[:, 3:3 + width], wide_w[:, 1:1 + width]                  # spaced, misaligned rows
+    want = _truth(x, w, None, y, up)
+    _close("lp", G.linear_categorical.logpdf(y, x, w), want["lp"])
+    for name, leaf in (("dx", 0), ("dw", 1)):                              # one gradient at a time
+        args = [x.detach(), w.detach()]
+        args[leaf] = args[leaf].clone().requires_grad_(True)
+        lp = G.linear_categorical.logpdf(y, *args)
+        _close(name, torch.autograd.grad(lp, args[leaf], up)[0], want[name])
+    xt = wide_x[:, :width].t().contiguous().t()                            # columns contiguous: copied inside
+    _close("lp of a transposed x", G.linear_categorical.logpdf(y, xt, w), _truth(xt, w, None, y, up)["lp"])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("n", [3, 200])
+def test_masked_entries_and_empty_rows(G, n, dtype):
+    x, w, b, y, up = _inputs(n, 700, 64, TYPES[dtype])
+    b[::3] = -float("inf")
+    y = y // 3 * 3 + 1                                     # an entry that is left
+    y[y >= 700] = 1
+    t = _truth(x, w, b, y, up)
+    for name, got in zip(("lp", "dx", "dw", "db"), _grads(G, x, w, b, y, up)):
+        _close(name, got, t[name])
+        assert torch.isfinite(got).all()
+    y0 = torch.zeros_like(y)                               # a masked entry has density zero
+    assert torch.equal(G.linear_categorical.logpdf(y0, x, w, b), torch.full((n,), -float("inf"), device="cuda"))
+    low = torch.full_like(b, torch.finfo(b.dtype).min)     # masks of the type's lowest value: finite and normalised
+    low[5] = 0.0
+    lp = G.linear_categorical.logpdf(torch.full_like(y, 5), x, w, low)
+    assert torch.equal(lp, torch.zeros_like(lp))
+    none = torch.full_like(b, -float("inf"))               # no entry left
+    assert torch.isnan(G.linear_categorical.logpdf(y, x, w, none)).all()
+
+
+def test_values_outside_the_vocabulary_take_the_nearest_entry(G):
+    from genjax_amd import backend as B
+
+    x, w, b, _, _ = _inputs(6, 40, 64, torch.float32)
+    y = torch.tensor([-5, 0, 39, 40, 2 ** 31 - 1, -2 ** 31], dtype=torch.int32, device="cuda")
+    got = G.linear_categorical.logpdf(y, x, w, b)
+    assert torch.equal(got, G.linear_categorical.logpdf(y.clamp(0, 39), x, w, b))
+    ref = B.categorical_logpdf(y, x @ w.t() + b)           # the same rule as categorical's
+    np.testing.assert_allclose(got.cpu().numpy(), ref.cpu().numpy(), atol=1e-4)
+
+
+def test_shared_rows_scalars_and_empty_batches(G):
+    x, w, b, y, up = _inputs(5, 90, 64, torch.float32)
+    one = G.linear_categorical.logpdf(y[0], x[0], w, b)
+    assert one.dim() == 0
+    _close("one", one.reshape(1), tuple(v[:1] for v in _truth(x, w, b, y, up)["lp"]))
+    same = x[:1].expand(5, 64)
+    _close("shared x", G.linear_categorical.logpdf(y, x[0], w, b), _truth(same, w, b, y, up)["lp"])
+    _close("shared y", G.linear_categorical.logpdf(y[0], x, w, b), _truth(x, w, b, y[:1].expand(5), up)["lp"])
+    leaf = x[0].clone().requires_grad_(True)               # a shared row collects the gradient of every value
+    lp = G.linear_categorical.logpdf(y, leaf, w, b)
+    want, tol = _truth(same, w, b, y, up)["dx"]
+    _close("dx of a shared row", torch.autograd.grad(lp, leaf, up)[0], (want.sum(0), tol.sum(0) + 2.0 ** -20 * want.abs().sum(0)))
+    e = torch.empty(0, 64, device="cuda", requires_grad=True)
+    w2 = w.clone().requires_grad_(True)
+    lp = G.linear_categorical.logpdf(y[:0], e, w2, b)
+    assert lp.shape == (0,)
+    gx, gw = torch.autograd.grad(lp.sum(), (e, w2))
+    assert gx.shape == (0, 64) and torch.equal(gw, torch.zeros_like(w))
+
+
+def test_gradient_against_differences(G):
+    x, w, b, y, up = _inputs(40, 333, 24, torch.float32)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    for i, t in enumerate((x, w, b)):
+        d = torch.randn(t.shape, generator=g, device="cuda")
+        d = d / d.norm()
+        h = 2.0 ** -6
+        args = [x, w, b]
+        f = []
+        for s in (h, -h):
+            args[i] = t + s * d
+            f.append((G.linear_categorical.logpdf(y, *args) * up).sum().double())
+        num = ((f[0] - f[1]) / (2 * h)).item()
+        ana = (_grads(G, x, w, b, y, up)[1 + i].double() * d.double()).sum().item()
+        # forty log-densities of ~2^3, each off by up to 2^-16: 2^-7 of difference quotient at worst; h^2 terms below that
+        assert abs(num - ana) <= 2.0 ** -6 * max(1.0, abs(ana)), (i, num, ana)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("n,vocab,width", [(1, 3, 64), (50, 777, 40), (300, 33000, 64)])
+def test_draws(G, n, vocab, width, dtype):
+    """The draw maximises l + Gumbel over categorical's noise: where the 64-bit runner-up is further away than the
+    logits' error, the entry is that one; with the framework's own logits it is categorical's draw."""
+    from genjax_amd import backend as B
+
+    x, w, b, y, up = _inputs(n, vocab, width, TYPES[dtype])
+    key = G.key(7)
+    got = B.sample_linear_categorical(key, x, w, b)
+    u = B.random_uniform(key, n * vocab, 1.17549435e-38, 1.0).double().reshape(n, vocab)
+    z = x.double() @ w.double().t() + b.double() - (-u.log()).log()
+    top = z.topk(2, dim=1)
+    clear = (top[0][:, 0] - top[0][:, 1]) > 1e-3
+    assert clear.float().mean() > 0.9 and torch.equal(got.long()[clear], top[1][:, 0][clear])
+    assert ((z.gather(1, got.long().unsqueeze(1)).squeeze(1) - top[0][:, 0]).abs() <= 1e-3).all()
+    cat = B.sample_categorical(key, (x.double() @ w.double().t() + b.double()).float())
+    assert torch.equal(cat[clear], got[clear])
+    b2 = torch.full_like(b, -float("inf"))                 # masked entries are never drawn
+    b2[vocab // 2] = 0.0
+    assert (B.sample_linear_categorical(key, x, w, b2) == vocab // 2).all()
+
+
+def test_draw_frequencies_and_gfi(G):
+    from genjax_amd import gen, linear_categorical, seed
+    from genjax_amd.core import batched
+
+    x, w, b, _, _ = _inputs(1, 6, 8, torch.float32)
+
+    @gen
+    def model(x, w, b):
+        return linear_categorical(x, w, b) @ "token"
+
+    n = 20000
+    with batched(n):
+        tr = seed(model.simulate)(G.key(1), x[0], w, b)
+    tok = tr.get_choices()["token"]
+    assert tok.shape == (n,) and tok.dtype == torch.int32
+    p = torch.softmax((x @ w.t() + b)[0], 0)
+    freq = torch.bincount(tok.long(), minlength=6) / n
+    assert ((freq - p).abs() <= 6 * (p * (1 - p) / n).sqrt() + 1e-6).all()      # six standard errors
+    lp, _ = model.assess({"token": tok}, x[0], w, b)
+    np.testing.assert_allclose(tr.get_score().cpu().numpy(), -lp.cpu().numpy(), rtol=0, atol=0)
+
+
+def test_hmc_over_latent_features(G):
+    """The gradient move differentiates through the density: hmc on a latent feature row per chain runs and its
+    log-density gradient is the 64-bit one."""
+    from genjax_amd import gen, linear_categorical, normal, seed, sel
+    from genjax_amd.core import batched
+    from genjax_amd.inference import hmc
+    from genjax_amd.inference.mcmc import _SelectedDensity
+
+    _, w, b, y, _ = _inputs(1, 50, 2, torch.float32)
+
+    @gen
+    def model(w, b):
+        h0 = normal(0.0, 1.0) @ "h0"
+        h1 = normal(0.0, 1.0) @ "h1"
+        linear_categorical(torch.stack([h0, h1], -1), w, b) @ "token"
+
+    n = 64
+    with batched(n):
+        tr, _ = seed(model.generate)(G.key(3), {"token": y[0]}, w, b)
+        d = _SelectedDensity(tr, sel("h0") | sel("h1"))
+        _, grads = d.logp(d.q0, True)
+        x = torch.stack(d.q0, -1)
+        up = torch.ones(n, device="cuda")
+        want, tol = _truth(x, w, b, y[:1].expand(n), up)["dx"]
+        _close("gradient", torch.stack(grads, -1), (want - x.double(), tol + 2.0 ** -20 * (want.abs() + x.abs())))
+        out = seed(lambda t: hmc(t, sel("h0") | sel("h1"), 0.1, 5))(G.key(4), tr)
+    assert torch.isfinite(out.get_choices()["h0"]).all()
+
+
+def test_weights_beyond_32_bit_offsets(G):
+    """vocab x width passes 2^31 elements; the last entries' logits and gradients come from the right rows."""
+    n, vocab, width = 2, (1 << 20) + 300, 2048
+    w = torch.zeros(vocab, width, dtype=torch.bfloat16, device="cuda")
+    w[-300:] = torch.randn(300, width, device="cuda", generator=torch.Generator("cuda").manual_seed(1)).to(torch.bfloat16) * 0.1
+    x = torch.randn(n, width, device="cuda", generator=torch.Generator("cuda").manual_seed(2)).to(torch.bfloat16)
+    y = torch.tensor([vocab - 1, vocab - 150], dtype=torch.int32, device="cuda")
+    tail = x.double() @ w[-300:].double().t()
+    lse = torch.logsumexp(torch.cat([tail, torch.full((n, 1), float(np.log(vocab - 300)), device="cuda", dtype=torch.float64)], 1), 1)
+    want = tail[torch.arange(n), (y - (vocab - 300)).long()] - lse
+    leaf = w.requires_grad_(True)
+    lp = G.linear_categorical.logpdf(y, x, leaf)
+    assert ((lp.double() - want).abs() <= 2.0 ** -10).all()
+    dw = torch.autograd.grad(lp.sum(), leaf)[0]
+    d = -(tail - lse.unsqueeze(1)).exp()
+    d[torch.arange(n), (y - (vocab - 300)).long()] += 1.0
+    err = (dw[-300:].double() - d.t() @ x.double()).abs()
+    assert (err <= 2.0 ** -6 * (d.abs().t() @ x.double().abs()) + 1e-9).all()
+    p = (-lse).exp().unsqueeze(1)                          # every entry with zero weights has this probability
+    zero = (p * x.double()).sum(0)
+    assert ((dw[:1000].double() + zero).abs() <= 2.0 ** -6 * (p * x.double().abs()).sum(0)).all()
+
+
+def test_streams_and_captured_graphs(G):
+    """A call on a side stream; two graphs captured from calls of different sizes, replayed in turn with new inputs,
+    each against the eager result (forward, gradient and draw)."""
+    from genjax_amd import backend as B
+
+    side = torch.cuda.Stream()
+    sets = []
+    for n, vocab, width in ((70, 1000, 96), (33, 2500, 64)):
+        x, w, b, y, up = _inputs(n, vocab, width, torch.bfloat16)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            lp, lse = B.linear_categorical_logpdf(y, x, w, b)
+        side.synchronize()
+        assert torch.equal(lp, B.linear_categorical_logpdf(y, x, w, b)[0])
+
+        def call(x=x, w=w, b=b, y=y, up=up):
+            lp, lse = B.linear_categorical_logpdf(y, x, w, b)
+            return [lp] + B.linear_categorical_grad(y, x, w, b, lse, up) + [B.sample_linear_categorical(G.key(1), x, w, b)]
+
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            call()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = call()
+        sets.append((graph, outs, call, x, up))
+    for turn in range(4):
+        for graph, outs, call, x, up in sets:
+            x.copy_(torch.randn(x.shape, device="cuda", generator=torch.Generator("cuda").manual_seed(turn)).to(x.dtype))
+            graph.replay()
+            want = call()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, c) for a, c in zip(outs, want))
+
+
+def test_same_bits_on_every_call(G):
+    x, w, b, y, up = _inputs(300, 20011, 256, torch.bfloat16)
+    first = _grads(G, x, w, b, y, up)
+    for _ in range(3):
+        assert all(torch.equal(a, c) for a, c in zip(first, _grads(G, x, w, b, y, up)))
