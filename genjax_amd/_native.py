@@ -139,6 +139,18 @@ class ShardBufs(C.Structure):
     ]
 
 
+class DeltaShape(C.Structure):
+    """gjx_delta_shape (include/gjx.h)."""
+
+    _fields_ = [
+        ("dtype", C.c_int32), ("kheads", C.c_int32), ("heads", C.c_int32), ("dk", C.c_int32), ("dv", C.c_int32),
+        ("scale", C.c_float),
+        ("batch", C.c_int64), ("time", C.c_int64),
+        ("q_stride", C.c_int64 * 3), ("k_stride", C.c_int64 * 3), ("v_stride", C.c_int64 * 3),
+        ("g_stride", C.c_int64 * 3), ("b_stride", C.c_int64 * 3),
+    ]
+
+
 _lib = None
 
 _vp, _i32, _i64, _u64, _f32 = C.c_void_p, C.c_int32, C.c_int64, C.c_uint64, C.c_float
@@ -241,6 +253,10 @@ _SIGNATURES = {
     "gjx_comm_all_gather": ([_vp, _vp, _vp, _i64, _vp], _i32),
     "gjx_shard_front": ([_vp, _vp, C.POINTER(LocWorld), _u32p, _i32, _f32p, _f32, C.POINTER(ShardBufs), _i32, _vp,
                          _u32p, _i32, C.POINTER(_vp), _vp, _vp, _vp, _vp], _i32),
+    "gjx_delta_filter_workspace": ([C.POINTER(DeltaShape), _i32, C.POINTER(_i64)], _i32),
+    "gjx_delta_filter": ([C.POINTER(DeltaShape)] + [_vp] * 9 + [_i32, _vp, _i64, _vp], _i32),
+    "gjx_delta_filter_grad": ([C.POINTER(DeltaShape)] + [_vp] * 15 + [_i64, _vp, _i64, _vp], _i32),
+    "gjx_delta_filter_step": ([C.POINTER(DeltaShape)] + [_vp] * 10, _i32),
     "gjx_lgssm_smc_run": ([_vp, C.POINTER(LgssmParams), _u32p, _i32, _f32p, _i64, _i32] + [_vp] * 11
                           + [C.POINTER(C.c_int32), _vp], _i32),
     "gjx_ctx_set_stage_events": ([_vp, C.POINTER(_vp), _i32], _i32),

@@ -557,6 +557,133 @@ def mvnormal_logpdf(x, mu, cov):
 
 
 # --------------------------------------------------------------------------- #
+# gated delta filter
+# --------------------------------------------------------------------------- #
+def _delta_shape(who, q, k, v, log_decay, beta, scale):
+    """Check the tensors of one call against each other and describe them to the library; axes (batch, time, head, ...)."""
+    for name, t in (("q", q), ("k", k), ("v", v), ("log_decay", log_decay), ("beta", beta)):
+        if not isinstance(t, torch.Tensor):
+            raise GjxError(f"{who}: `{name}` must be a tensor")
+    if q.dim() != 4 or k.shape != q.shape or v.dim() != 4 or v.shape[:2] != q.shape[:2]:
+        raise GjxError(f"{who}: q {tuple(q.shape)} and k {tuple(k.shape)} must be (batch, time, key heads, dk) and v "
+                       f"{tuple(v.shape)} (batch, time, heads, dv)")
+    batch, time, kheads, dk = q.shape
+    heads, dv = v.shape[2:]
+    if kheads < 1 or heads < 1 or heads % kheads:
+        raise GjxError(f"{who}: {heads} heads must be a multiple of {kheads} key heads")
+    if not (1 <= dk <= 128 and 1 <= dv <= 1024):
+        raise GjxError(f"{who}: dk = {dk} must be in [1, 128] and dv = {dv} in [1, 1024]")
+    if tuple(log_decay.shape) != (batch, time, heads) or tuple(beta.shape) != (batch, time, heads):
+        raise GjxError(f"{who}: log_decay {tuple(log_decay.shape)} and beta {tuple(beta.shape)} must be {(batch, time, heads)}")
+    if q.dtype not in ELEMENT_TYPES or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise GjxError(f"{who}: q, k and v must all be float32 or all bfloat16 (got {q.dtype}, {k.dtype}, {v.dtype})")
+    if log_decay.dtype != torch.float32 or beta.dtype != torch.float32:
+        raise GjxError(f"{who}: log_decay and beta must be float32 (got {log_decay.dtype}, {beta.dtype})")
+    _on_current_device(who, q=q, k=k, v=v, log_decay=log_decay, beta=beta)
+    s = N.DeltaShape(dtype=ELEMENT_TYPES[q.dtype], kheads=kheads, heads=heads, dk=dk, dv=dv,
+                     scale=float(dk ** -0.5 if scale is None else scale), batch=batch, time=time)
+    tensors = [t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous() for t in (q, k, v)] + [log_decay, beta]
+    for name, t in zip("qkvgb", tensors):
+        setattr(s, f"{name}_stride", (C.c_int64 * 3)(*t.stride()[:3]))
+    return s, tensors
+
+
+def _delta_state(who, name, state, s):
+    """A (batch, heads, dk, dv) float32 state, contiguous."""
+    if state is None:
+        return None
+    if not isinstance(state, torch.Tensor) or tuple(state.shape) != (s.batch, s.heads, s.dk, s.dv) or state.dtype != torch.float32:
+        raise GjxError(f"{who}: `{name}` must be float32 of shape {(s.batch, s.heads, s.dk, s.dv)}")
+    _on_current_device(who, **{name: state})
+    return state.contiguous()
+
+
+def _delta_lengths(who, lengths, s):
+    if lengths is None:
+        return None
+    if not isinstance(lengths, torch.Tensor) or lengths.dtype != torch.int32 or tuple(lengths.shape) != (s.batch,):
+        raise GjxError(f"{who}: `lengths` must be int32 of shape ({s.batch},)")
+    _on_current_device(who, lengths=lengths)
+    return lengths.contiguous()
+
+
+def _delta_workspace(s, keep, device):
+    size = C.c_int64()
+    N.check(N.lib().gjx_delta_filter_workspace(C.byref(s), keep, C.byref(size)), "gjx_delta_filter_workspace")
+    return torch.empty(max(size.value, 256), dtype=torch.uint8, device=device)
+
+
+def _raw(t):
+    return C.c_void_p(0) if t is None else C.c_void_p(t.data_ptr())
+
+
+def delta_filter(q, k, v, log_decay, beta, initial_state=None, scale=None, lengths=None, keep=False):
+    """-> (o (batch, time, heads, dv), last state (batch, heads, dk, dv), the workspace the gradient reads or None)."""
+    who = "delta_filter"
+    s, (q, k, v, g, be) = _delta_shape(who, q, k, v, log_decay, beta, scale)
+    state0, lengths = _delta_state(who, "initial_state", initial_state, s), _delta_lengths(who, lengths, s)
+    o = torch.empty((s.batch, s.time, s.heads, s.dv), dtype=v.dtype, device=v.device)
+    state = torch.empty((s.batch, s.heads, s.dk, s.dv), dtype=torch.float32, device=v.device)
+    work = _delta_workspace(s, int(keep), v.device)
+    N.check(N.lib().gjx_delta_filter(C.byref(s), _raw(q), _raw(k), _raw(v), _raw(g), _raw(be), _raw(state0), _raw(lengths), _raw(o),
+                                     _raw(state), int(keep), _raw(work), work.numel(), _stream()), "gjx_delta_filter")
+    return o, state, work if keep else None
+
+
+def delta_filter_grad(q, k, v, log_decay, beta, d_o, d_state, kept, scale=None, lengths=None, want_state0=True):
+    """Gradients (q, k, v, log_decay, beta, initial state or None) from the upstream ones of o and of the last state."""
+    who = "delta_filter"
+    s, (q, k, v, g, be) = _delta_shape(who, q, k, v, log_decay, beta, scale)
+    lengths = _delta_lengths(who, lengths, s)
+    d_state = _delta_state(who, "d_state", d_state, s)
+    dev = v.device
+    d_o = torch.zeros((s.batch, s.time, s.heads, s.dv), dtype=v.dtype, device=dev) if d_o is None else d_o.contiguous()
+    outs = [torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v, g, be)]
+    state0 = torch.empty((s.batch, s.heads, s.dk, s.dv), dtype=torch.float32, device=dev) if want_state0 else None
+    work = _delta_workspace(s, 2, dev)
+    N.check(N.lib().gjx_delta_filter_grad(C.byref(s), _raw(q), _raw(k), _raw(v), _raw(g), _raw(be), _raw(lengths), _raw(d_o),
+                                          _raw(d_state), *(_raw(t) for t in outs), _raw(state0), _raw(kept), kept.numel(),
+                                          _raw(work), work.numel(), _stream()), "gjx_delta_filter_grad")
+    return outs + [state0]
+
+
+def _overlap(a, b):
+    lo_a, lo_b = a.data_ptr(), b.data_ptr()
+    return lo_a < lo_b + b.numel() * b.element_size() and lo_b < lo_a + a.numel() * a.element_size()
+
+
+def delta_filter_step(state, q, k, v, log_decay, beta, scale=None, ancestors=None, out=None):
+    """One token per batch element: q, k (n, key heads, dk), v (n, heads, dv), gates (n, heads) -> (o (n, heads, dv), state)."""
+    who = "delta_filter_step"
+    for name, t, d in (("q", q, 3), ("k", k, 3), ("v", v, 3), ("log_decay", log_decay, 2), ("beta", beta, 2)):
+        if not isinstance(t, torch.Tensor) or t.dim() != d:
+            raise GjxError(f"{who}: `{name}` must have {d} axes (particle, head{', entry' if d == 3 else ''})")
+    s, (q, k, v, g, be) = _delta_shape(who, *(t.unsqueeze(1) for t in (q, k, v, log_decay, beta)), scale)
+    state = _delta_state(who, "state", state, s)
+    if state is None:
+        raise GjxError(f"{who}: `state` must be float32 of shape {(s.batch, s.heads, s.dk, s.dv)}")
+    if ancestors is not None:
+        if not isinstance(ancestors, torch.Tensor) or ancestors.dtype != torch.int32 or tuple(ancestors.shape) != (s.batch,):
+            raise GjxError(f"{who}: `ancestors` must be int32 of shape ({s.batch},)")
+        _on_current_device(who, ancestors=ancestors)
+        ancestors = ancestors.contiguous()
+    if out is None:
+        out = torch.empty_like(state)
+    else:
+        if not isinstance(out, torch.Tensor) or out.shape != state.shape or out.dtype != torch.float32 or not out.is_contiguous():
+            raise GjxError(f"{who}: `out` must be contiguous float32 of shape {tuple(state.shape)}")
+        _on_current_device(who, out=out)
+        if _overlap(out, state) and (ancestors is not None or out.data_ptr() != state.data_ptr()):
+            raise GjxError(f"{who}: `out` may be the state itself without ancestors and must not overlap it otherwise")
+    if state.data_ptr() % 16 or out.data_ptr() % 16:
+        raise GjxError(f"{who}: states must be aligned to 16 bytes")
+    o = torch.empty((s.batch, s.heads, s.dv), dtype=v.dtype, device=v.device)
+    N.check(N.lib().gjx_delta_filter_step(C.byref(s), _raw(state), _raw(ancestors), _raw(q), _raw(k), _raw(v), _raw(g), _raw(be),
+                                          _raw(o), _raw(out), _stream()), "gjx_delta_filter_step")
+    return o, out
+
+
+# --------------------------------------------------------------------------- #
 # MH accept / select for generic traces
 # --------------------------------------------------------------------------- #
 def mh_accept(k, log_weight: torch.Tensor, n: int, offset: int = 0) -> torch.Tensor:

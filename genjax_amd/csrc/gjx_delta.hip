@@ -1,0 +1,1159 @@
+// gjx_delta.hip -- the gated delta filter: the mean recursion of a Kalman filter over a dk x dv matrix of regression
+// weights S that is observed along k_t with the gain beta_t k_t,
+//   S_t = a_t S_{t-1} + k_t u_t^T,   u_t = beta_t (v_t - a_t S_{t-1}^T k_t),   o_t = scale S_t^T q_t,   a_t = exp(g_t),
+// over whole sequences in chunks of 64 tokens, its gradient, and one token at a time.
+//
+// One chunk with gamma = cumsum(g), D_ij = exp(gamma_i - gamma_j) (i >= j), N_ij = D_ij k_i.k_j (i > j):
+//   r = V - e^gamma K S0,   delta = (I + N beta)^-1 r,   V' = beta delta   (the rows are the u_t),
+//   O = scale e^gamma Q S0 + P V',  P_ij = scale D_ij q_i.k_j (i >= j),   S1 = e^gamma_C S0 + K^T (e^(gamma_C - gamma) V').
+// Everything but the three products with S0 is known before the recursion: k_delta_prepare forms That = (I + N beta)^-1
+// and P for all chunks at once; k_delta_scan walks the chunks with S in registers.
+// Gradient (e = T^T dV', T = (I + beta N)^-1 = I - beta That N):
+//   dV' = P^T dO + e^(gamma_C - gamma) K dS1,  dV = beta e,  dbeta_i = e_i.delta_i,
+//   dS0 = e^gamma_C dS1 + Q^T (scale e^gamma dO) - K^T (beta e^gamma e)            (k_delta_scan_back),
+//   E = scale D (dO V'^T), F = -beta_i D_ij (e_i.V'_j)  (i > j),
+//   dQ = scale e^gamma dO S0^T + E K,  dK as what is read = -beta e^gamma e S0^T + F K,
+//   dK as what is written = E^T Q + F^T K + e^(gamma_C - gamma) V' dS1^T,
+//   dgamma_i = q_i.dq_i + k_i.dk_i(read) - k_i.dk_i(written), + <dS1, S1> at the chunk's end,
+//   dg = reverse cumsum of dgamma within the chunk                               (k_delta_back, all chunks at once).
+//
+// Arithmetic: 16x16x32 bf16 MFMA with f32 accumulators.  Whatever is not an input in bf16 is split into three bf16 planes
+// (8 bits each) and multiplied in the partial products above 2^-23, so that states, gains and gradients keep f32
+// accuracy; only the read-out of bf16 calls takes two planes (2^-16 before the rounding of o to 2^-8).
+// Operands are laid out as matrix fragments: 64 lanes x 8 elements, lane = (index % 16) + 16 q, the eight elements of quad
+// q in slab s being reduction indices 32 s + 4 q + {0..3} and 32 s + 16 + 4 q + {0..3}.  That order is the one in which the
+// accumulators of two stacked 16-row tiles come out, so S, r, delta, ... go from accumulator to operand without moving.
+#include "gjx_common.h"
+
+#include <algorithm>
+
+typedef __bf16 bf16;
+typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+namespace {
+
+constexpr int C = 64;           // tokens per chunk
+constexpr int FRAG = 512;       // elements of one fragment
+constexpr int LD = 68;          // row pitch of the 64 x 64 f32 matrices in LDS
+constexpr float G_MIN = -100.0f;
+
+struct Shape {
+  int kheads, heads, group, dk, dv, dvp;
+  float scale;
+  int64_t batch, time;
+  int64_t qs[3], ks[3], vs[3], gs[3], bs[3];
+  int64_t chunks;
+};
+
+// element offsets (bf16) of the fragment blocks of one chunk
+template <int DKP, int NPI>
+struct KeyBlock {               // per key head
+  static constexpr int KS = DKP / 32, MT = DKP / 16;
+  static constexpr int KA = 0, QA = NPI * 4 * KS * FRAG, KT = 2 * QA, QT = KT + NPI * MT * 2 * FRAG;
+  static constexpr int SIZE = QT, SIZE_KEEP = QT + NPI * MT * 2 * FRAG;
+};
+struct GateBlock {              // per head: That, P, then (keep) T^T, P^T; three planes of six fragments each
+  static constexpr int TA = 0, PA = 18 * FRAG, TT = 36 * FRAG, PT = 54 * FRAG, SIZE = 36 * FRAG, SIZE_KEEP = 72 * FRAG;
+};
+constexpr int ROWS = 3 * C;     // f32 per head and chunk: beta, e^gamma, e^(gamma_C - gamma)
+
+struct Work {
+  bf16 *keys, *gates;
+  int64_t key_size, gate_size;
+  float* rows;
+  float *s0, *delta;            // keep: state before the chunk (DKP x dvp), delta (64 x dvp)
+  float *ds1, *e;               // gradient scratch
+  float *dq, *dk;               // gradient scratch, heads that share a key head: f32 (batch, time, heads, dk)
+};
+
+__device__ __forceinline__ f32x4 mma(bf16x8 a, bf16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// f32 -> bf16 planes, exactly for P = 3 (an h that would round to infinity is cut off; an infinite x keeps h only)
+template <int P>
+__device__ __forceinline__ void split(const float (&x)[8], bf16x8 (&out)[P]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    float r = x[j];
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      bf16 h = (bf16)r;
+      if (p == 0 && __builtin_isinf((float)h)) {
+        h = (bf16)__uint_as_float(__float_as_uint(r) & 0xffff0000u);
+        if (__builtin_isinf(r)) r = (float)h;
+      }
+      out[p][j] = h;
+      r = __builtin_isinf(r) ? 0.0f : r - (float)h;
+    }
+  }
+}
+
+// acc += sum of the partial products a_p b_r with p + r < LIM, smallest first
+template <int PA, int PB, int LIM>
+__device__ __forceinline__ f32x4 mma_planes(const bf16x8 (&a)[PA], const bf16x8 (&b)[PB], f32x4 acc) {
+#pragma unroll
+  for (int s = LIM - 1; s >= 0; --s)
+#pragma unroll
+    for (int p = 0; p < PA; ++p)
+      if (s - p >= 0 && s - p < PB) acc = mma(a[p], b[s - p], acc);
+  return acc;
+}
+
+template <int P>
+__device__ __forceinline__ void load_frag(const bf16* base, int index, int plane, int lane, bf16x8 (&out)[P]) {
+#pragma unroll
+  for (int p = 0; p < P; ++p) out[p] = *(const bf16x8*)(base + p * plane + index * FRAG + lane * 8);
+}
+
+// two accumulator tiles (rows 16 (2 s) .. 16 (2 s + 2)) as the operand of slab s
+template <int P>
+__device__ __forceinline__ void tiles_to_frag(f32x4 lo, f32x4 hi, bf16x8 (&out)[P]) {
+  const float x[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  split<P>(x, out);
+}
+
+// fragments of a lower triangular 64 x 64 matrix: row tile i needs slabs 0 .. i / 2; of its transpose: slabs i / 2 .. 1
+__device__ __forceinline__ constexpr int lower(int i, int s) { return i < 2 ? i : 2 + 2 * (i - 2) + s; }
+__device__ __forceinline__ constexpr int upper(int i, int s) { return i < 2 ? 2 * i + s : 4 + (i - 2); }
+
+__device__ __forceinline__ int perm(int s, int q, int j) { return 32 * s + (j < 4 ? 4 * q + j : 12 + 4 * q + j); }
+
+template <typename T>
+__device__ __forceinline__ float to_f32(T v) { return (float)v; }
+
+__device__ __forceinline__ int64_t length_of(const int32_t* lengths, int64_t b, int64_t time) {
+  return lengths ? std::min<int64_t>(std::max<int64_t>(lengths[b], 0), time) : time;
+}
+
+// ---------------------------------------------------------------------------
+// all chunks at once: fragments of K, Q and their transposes, That, P (keep: T^T, P^T), the row factors
+// ---------------------------------------------------------------------------
+template <typename T, int DKP, int NPI>
+__device__ __forceinline__ void load_rows(const T* src, int64_t token_stride, int tokens, int dk, bool vec, bf16* lds, int tid) {
+  constexpr int PITCH = DKP + 8, PLANE = C * PITCH;
+  for (int i = tid; i < C * (DKP / 8); i += 256) {
+    const int t = i / (DKP / 8), c0 = (i % (DKP / 8)) * 8;
+    float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (t < tokens && c0 < dk) {
+      const T* p = src + t * token_stride + c0;
+      if (vec && c0 + 8 <= dk) {
+        typedef T vec8 __attribute__((ext_vector_type(8)));
+        const vec8 v = *(const vec8*)p;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = (float)v[j];
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (c0 + j < dk) x[j] = (float)p[j];
+      }
+    }
+    bf16x8 out[NPI];
+    split<NPI>(x, out);
+#pragma unroll
+    for (int p = 0; p < NPI; ++p) *(bf16x8*)(lds + p * PLANE + t * PITCH + c0) = out[p];
+  }
+}
+
+template <int DKP, int NPI>
+__device__ __forceinline__ void store_row_frags(const bf16* lds, bf16* dst, int tid) {   // rows are tokens
+  constexpr int PITCH = DKP + 8, PLANE = C * PITCH, KS = DKP / 32;
+  for (int i = tid; i < NPI * 4 * KS * 64; i += 256) {
+    const int lane = i & 63, f = i >> 6, s = f % KS, m = (f / KS) % 4, p = f / (KS * 4), q = lane >> 4;
+    const bf16* row = lds + p * PLANE + (16 * m + (lane & 15)) * PITCH + 32 * s + 4 * q;
+    const bf16x4 lo = *(const bf16x4*)row, hi = *(const bf16x4*)(row + 16);
+    *(bf16x8*)(dst + (int64_t)i * 8) = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+}
+
+template <int DKP, int NPI>
+__device__ __forceinline__ void store_col_frags(const bf16* lds, bf16* dst, int tid) {   // rows are the dk axis
+  constexpr int PITCH = DKP + 8, PLANE = C * PITCH, MT = DKP / 16;
+  for (int i = tid; i < NPI * MT * 2 * 64; i += 256) {
+    const int lane = i & 63, f = i >> 6, s = f % 2, m = (f / 2) % MT, p = f / (2 * MT), q = lane >> 4;
+    bf16x8 v;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = lds[p * PLANE + perm(s, q, j) * PITCH + 16 * m + (lane & 15)];
+    *(bf16x8*)(dst + (int64_t)i * 8) = v;
+  }
+}
+
+// 64 x 64 f32 in LDS -> three planes of the six fragments of a triangle (of its transpose: TRANS)
+template <bool TRANS>
+__device__ __forceinline__ void store_triangle(const float* m, bf16* dst, int tid) {
+  for (int i = tid; i < 6 * 64; i += 256) {
+    const int lane = i & 63, f = i >> 6, q = lane >> 4;
+    int t, s;
+    if (TRANS) {
+      t = f < 4 ? f / 2 : f - 2;
+      s = f < 4 ? f % 2 : 1;
+    } else {
+      t = f < 2 ? f : 2 + (f - 2) / 2;
+      s = f < 2 ? 0 : (f - 2) % 2;
+    }
+    const int a = 16 * t + (lane & 15);
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = TRANS ? m[perm(s, q, j) * LD + a] : m[a * LD + perm(s, q, j)];
+    bf16x8 out[3];
+    split<3>(x, out);
+#pragma unroll
+    for (int p = 0; p < 3; ++p) *(bf16x8*)(dst + ((int64_t)p * 6 + f) * FRAG + lane * 8) = out[p];
+  }
+}
+
+// acc += X(rows i, cols l) Y(rows l, cols j) of 16 x 16 f32 blocks in LDS; X's columns times col_scale (or 1)
+__device__ __forceinline__ f32x4 block_product(const float* x, const float* col_scale, const float* y, int i, int l, int j,
+                                               int lane, f32x4 acc) {
+  const int q = lane >> 4, c = lane & 15;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int kk = 16 * l + 4 * k + q;
+    const float a = x[(16 * i + c) * LD + kk] * (col_scale ? col_scale[kk] : 1.0f);
+    acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a, y[kk * LD + 16 * j + c], acc, 0, 0, 0);
+  }
+  return acc;
+}
+
+template <typename T, int DKP, int NPI, bool KEEP>
+__global__ void __launch_bounds__(256)
+    k_delta_prepare(Shape sh, const T* __restrict__ q, const T* __restrict__ k, const float* __restrict__ g,
+                    const float* __restrict__ beta, const int32_t* __restrict__ lengths, Work w, int vec) {
+  constexpr int KS = DKP / 32, PITCH = DKP + 8, PLANE = C * PITCH;
+  extern __shared__ char smem[];
+  bf16* sk = (bf16*)smem;
+  bf16* sq = sk + NPI * PLANE;
+  float* sn = (float*)(sq + NPI * PLANE);       // N
+  float* st = sn + C * LD;                      // That
+  float* sp = st + C * LD;                      // P, then T
+  float* s_gh = sp + C * LD;
+  float *s_gl = s_gh + C, *s_beta = s_gl + C;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, quad = lane >> 4, c = lane & 15;
+  const int64_t chunk = blockIdx.x % sh.chunks, bh = blockIdx.x / sh.chunks, b = bh / sh.heads;
+  const int h = (int)(bh % sh.heads), kh = h / sh.group;
+  const int64_t len = length_of(lengths, b, sh.time), t0 = chunk * C;
+  if (t0 >= len) return;
+  const int tokens = (int)std::min<int64_t>(C, len - t0);
+  bf16* keys = w.keys + ((b * sh.kheads + kh) * sh.chunks + chunk) * w.key_size;
+  bf16* gates = w.gates + (bh * sh.chunks + chunk) * w.gate_size;
+  float* rows = w.rows + (bh * sh.chunks + chunk) * ROWS;
+
+  load_rows<T, DKP, NPI>(k + b * sh.ks[0] + t0 * sh.ks[1] + kh * sh.ks[2], sh.ks[1], tokens, sh.dk, vec, sk, tid);
+  load_rows<T, DKP, NPI>(q + b * sh.qs[0] + t0 * sh.qs[1] + kh * sh.qs[2], sh.qs[1], tokens, sh.dk, vec, sq, tid);
+  if (wave == 0) {
+    const bool in = lane < tokens;
+    // differences of the cumulative decay keep f32 accuracy whatever its size: 64-bit sum, kept as two floats
+    double gam = in ? (double)fmaxf(g[b * sh.gs[0] + (t0 + lane) * sh.gs[1] + h * sh.gs[2]], G_MIN) : 0.0;
+    if (in && __builtin_isnan(g[b * sh.gs[0] + (t0 + lane) * sh.gs[1] + h * sh.gs[2]])) gam = __builtin_nan("");
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const double up = __shfl_up(gam, o);
+      if (lane >= o) gam += up;
+    }
+    const double last = __shfl(gam, 63);
+    const float be = in ? beta[b * sh.bs[0] + (t0 + lane) * sh.bs[1] + h * sh.bs[2]] : 0.0f;
+    s_gh[lane] = (float)gam;
+    s_gl[lane] = (float)(gam - (double)(float)gam);
+    s_beta[lane] = be;
+    rows[lane] = be;
+    rows[C + lane] = expf((float)gam);
+    rows[2 * C + lane] = expf((float)(last - gam));
+  }
+  for (int i = tid; i < C * LD; i += 256) st[i] = 0.0f;
+  __syncthreads();
+
+  // K K^T and Q K^T, row tile = wave
+  for (int j = 0; j < 4; ++j) {
+    f32x4 kk = {0, 0, 0, 0}, qk = {0, 0, 0, 0};
+    if (j <= wave) {
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        bf16x8 a[NPI], x[NPI], bq[NPI];
+#pragma unroll
+        for (int p = 0; p < NPI; ++p) {
+          a[p] = *(const bf16x8*)(sk + p * PLANE + (16 * j + c) * PITCH + 32 * s + 8 * quad);
+          x[p] = *(const bf16x8*)(sk + p * PLANE + (16 * wave + c) * PITCH + 32 * s + 8 * quad);
+          bq[p] = *(const bf16x8*)(sq + p * PLANE + (16 * wave + c) * PITCH + 32 * s + 8 * quad);
+        }
+        kk = mma_planes<NPI, NPI, NPI>(x, a, kk);
+        qk = mma_planes<NPI, NPI, NPI>(bq, a, qk);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int i = 16 * wave + 4 * quad + r, jj = 16 * j + c;
+      const float d = jj <= i ? expf((s_gh[i] - s_gh[jj]) + (s_gl[i] - s_gl[jj])) : 0.0f;
+      sn[i * LD + jj] = jj < i ? d * kk[r] : 0.0f;
+      sp[i * LD + jj] = jj <= i ? sh.scale * d * qk[r] : 0.0f;
+    }
+  }
+  if (h % sh.group == 0) {
+    typedef KeyBlock<DKP, NPI> KB;
+    store_row_frags<DKP, NPI>(sk, keys + KB::KA, tid);
+    store_row_frags<DKP, NPI>(sq, keys + KB::QA, tid);
+    store_col_frags<DKP, NPI>(sk, keys + KB::KT, tid);
+    if (KEEP) store_col_frags<DKP, NPI>(sq, keys + KB::QT, tid);
+  }
+  __syncthreads();
+  store_triangle<false>(sp, gates + GateBlock::PA, tid);
+  if (KEEP) store_triangle<true>(sp, gates + GateBlock::PT, tid);
+
+  // That = (I + N beta)^-1: the diagonal 16 x 16 blocks by forward substitution, one column per lane ...
+  {
+    float x[16];
+    const float* n = sn + 16 * wave * LD + 16 * wave;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float v = i == c ? 1.0f : 0.0f;
+#pragma unroll
+      for (int j = 0; j < i; ++j) v -= n[i * LD + j] * s_beta[16 * wave + j] * x[j];
+      x[i] = v;
+    }
+    if (quad == 0)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) st[(16 * wave + i) * LD + 16 * wave + c] = x[i];
+  }
+  __syncthreads();
+  // ... the others by block diagonals: That_ij = -That_ii sum_{j <= l < i} (N beta)_il That_lj
+  for (int d = 1; d < 4; ++d) {
+    const int j = wave, i = wave + d;
+    f32x4 out = {0, 0, 0, 0};
+    if (i < 4) {
+      f32x4 tmp = {0, 0, 0, 0};
+      for (int l = j; l < i; ++l) tmp = block_product(sn, s_beta, st, i, l, j, lane, tmp);
+#pragma unroll
+      for (int r = 0; r < 4; ++r)      // the accumulator's register r holds rows 4 q + r: take those columns of That_ii
+        out = __builtin_amdgcn_mfma_f32_16x16x4f32(st[(16 * i + c) * LD + 16 * i + 4 * quad + r], tmp[r], out, 0, 0, 0);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) st[(16 * i + 4 * quad + r) * LD + 16 * j + c] = -out[r];
+    }
+    __syncthreads();
+  }
+  store_triangle<false>(st, gates + GateBlock::TA, tid);
+  if (KEEP) {                          // T = I - beta That N, transposed
+    for (int j = 0; j < 4; ++j) {
+      f32x4 acc = {0, 0, 0, 0};
+      for (int l = j; l <= wave; ++l) acc = block_product(st, nullptr, sn, wave, l, j, lane, acc);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int i = 16 * wave + 4 * quad + r, jj = 16 * j + c;
+        sp[i * LD + jj] = (i == jj ? 1.0f : 0.0f) - s_beta[i] * acc[r];
+      }
+    }
+    __syncthreads();
+    store_triangle<true>(sp, gates + GateBlock::TT, tid);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// the recursion: one wave owns 16 columns of S
+// ---------------------------------------------------------------------------
+// the waves of one head go to one XCD (workgroups go round the eight of them): they read the same fragments
+__device__ __forceinline__ bool scan_place(int64_t block, int tiles, int64_t heads, int64_t& bh, int& tile) {
+  bh = block / (8 * tiles) * 8 + block % 8;
+  tile = (int)(block / 8 % tiles);
+  return bh < heads;
+}
+
+template <typename T, int DKP, int NPI, bool KEEP>
+__global__ void __launch_bounds__(64)
+    k_delta_scan(Shape sh, const T* __restrict__ v, const float* __restrict__ state0, const int32_t* __restrict__ lengths,
+                 T* __restrict__ o, float* __restrict__ state, Work w) {
+  typedef KeyBlock<DKP, NPI> KB;
+  constexpr int KS = DKP / 32, MT = DKP / 16;
+  constexpr int NPO = NPI == 1 ? 2 : 3;          // planes of what only the read-out takes
+  const int lane = threadIdx.x, quad = lane >> 4, c = lane & 15;
+  int64_t bh;
+  int tile;
+  if (!scan_place(blockIdx.x, sh.dvp / 16, sh.batch * sh.heads, bh, tile)) return;
+  const int64_t b = bh / sh.heads;
+  const int h = (int)(bh % sh.heads), kh = h / sh.group;
+  const int col = tile * 16 + c;
+  const bool in = col < sh.dv;
+  const int64_t len = length_of(lengths, b, sh.time), n_chunks = (len + C - 1) / C;
+  const bf16* keys = w.keys + (b * sh.kheads + kh) * sh.chunks * w.key_size;
+  const bf16* gates = w.gates + bh * sh.chunks * w.gate_size;
+  const float* rows = w.rows + bh * sh.chunks * ROWS;
+  const T* vp = v + b * sh.vs[0] + h * sh.vs[2] + col;
+  T* op = o + ((b * sh.time) * sh.heads + h) * sh.dv + col;
+  const int64_t o_stride = (int64_t)sh.heads * sh.dv;
+
+  f32x4 S[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int row = 16 * t + 4 * quad + r;
+      S[t][r] = state0 && in && row < sh.dk ? state0[(bh * sh.dk + row) * sh.dv + col] : 0.0f;
+    }
+
+  for (int64_t ch = 0; ch < n_chunks; ++ch) {
+    const bf16* kb = keys + ch * w.key_size;
+    const bf16* gb = gates + ch * w.gate_size;
+    const float* rb = rows + ch * ROWS;
+    const int64_t t0 = ch * C;
+    if (KEEP) {
+      float* s0 = w.s0 + (bh * sh.chunks + ch) * (int64_t)DKP * sh.dvp + col;
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s0[(int64_t)(16 * t + 4 * quad + r) * sh.dvp] = S[t][r];
+    }
+    bf16x8 sf[KS][3];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) tiles_to_frag<3>(S[2 * s], S[2 * s + 1], sf[s]);
+    f32x4 r[4], qs[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f32x4 acc = {0, 0, 0, 0}, aq = {0, 0, 0, 0};
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        bf16x8 a[NPI], aqf[NPI];
+        load_frag<NPI>(kb + KB::KA, i * KS + s, 4 * KS * FRAG, lane, a);
+        load_frag<NPI>(kb + KB::QA, i * KS + s, 4 * KS * FRAG, lane, aqf);
+        acc = mma_planes<NPI, 3, 3>(a, sf[s], acc);
+        aq = mma_planes<NPI, 3, NPO>(aqf, sf[s], aq);
+      }
+      const f32x4 eg = *(const f32x4*)(rb + C + 16 * i + 4 * quad);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int64_t t = t0 + 16 * i + 4 * quad + e;
+        const float val = in && t < len ? (float)vp[t * sh.vs[1]] : 0.0f;
+        r[i][e] = val - eg[e] * acc[e];
+        qs[i][e] = sh.scale * eg[e] * aq[e];
+      }
+    }
+    bf16x8 rf[2][3];
+    tiles_to_frag<3>(r[0], r[1], rf[0]);
+    tiles_to_frag<3>(r[2], r[3], rf[1]);
+    f32x4 vn[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+      for (int s = 0; s <= i / 2; ++s) {
+        bf16x8 a[3];
+        load_frag<3>(gb + GateBlock::TA, lower(i, s), 6 * FRAG, lane, a);
+        acc = mma_planes<3, 3, 3>(a, rf[s], acc);
+      }
+      if (KEEP) {
+        float* dp = w.delta + ((bh * sh.chunks + ch) * C + 16 * i + 4 * quad) * (int64_t)sh.dvp + col;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dp[(int64_t)e * sh.dvp] = acc[e];
+      }
+      vn[i] = acc * *(const f32x4*)(rb + 16 * i + 4 * quad);
+    }
+    bf16x8 vf[2][NPO];
+    tiles_to_frag<NPO>(vn[0], vn[1], vf[0]);
+    tiles_to_frag<NPO>(vn[2], vn[3], vf[1]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int s = 0; s <= i / 2; ++s) {
+        bf16x8 a[NPO];
+        load_frag<NPO>(gb + GateBlock::PA, lower(i, s), 6 * FRAG, lane, a);
+        qs[i] = mma_planes<NPO, NPO, NPO>(a, vf[s], qs[i]);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int64_t t = t0 + 16 * i + 4 * quad + e;
+        if (in && t < sh.time) op[t * o_stride] = (T)qs[i][e];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) vn[i] *= *(const f32x4*)(rb + 2 * C + 16 * i + 4 * quad);
+    tiles_to_frag<3>(vn[0], vn[1], rf[0]);
+    tiles_to_frag<3>(vn[2], vn[3], rf[1]);
+    const float whole = rb[2 * C - 1];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      f32x4 acc = S[t] * whole;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        bf16x8 a[NPI];
+        load_frag<NPI>(kb + KB::KT, t * 2 + s, MT * 2 * FRAG, lane, a);
+        acc = mma_planes<NPI, 3, 3>(a, rf[s], acc);
+      }
+      S[t] = acc;
+    }
+  }
+  if (in)
+    for (int64_t t = n_chunks * C + quad; t < sh.time; t += 4) op[t * o_stride] = (T)0.0f;
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int row = 16 * t + 4 * quad + r;
+      if (in && row < sh.dk) state[(bh * sh.dk + row) * sh.dv + col] = S[t][r];
+    }
+}
+
+template <typename T, int DKP, int NPI>
+__global__ void __launch_bounds__(64)
+    k_delta_scan_back(Shape sh, const T* __restrict__ d_o, const float* __restrict__ d_state, const int32_t* __restrict__ lengths,
+                      T* __restrict__ dv, float* __restrict__ d_state0, Work w) {
+  typedef KeyBlock<DKP, NPI> KB;
+  constexpr int KS = DKP / 32, MT = DKP / 16;
+  const int lane = threadIdx.x, quad = lane >> 4, c = lane & 15;
+  int64_t bh;
+  int tile;
+  if (!scan_place(blockIdx.x, sh.dvp / 16, sh.batch * sh.heads, bh, tile)) return;
+  const int64_t b = bh / sh.heads;
+  const int h = (int)(bh % sh.heads), kh = h / sh.group;
+  const int col = tile * 16 + c;
+  const bool in = col < sh.dv;
+  const int64_t len = length_of(lengths, b, sh.time), n_chunks = (len + C - 1) / C;
+  const bf16* keys = w.keys + (b * sh.kheads + kh) * sh.chunks * w.key_size;
+  const bf16* gates = w.gates + bh * sh.chunks * w.gate_size;
+  const float* rows = w.rows + bh * sh.chunks * ROWS;
+  const int64_t stride = (int64_t)sh.heads * sh.dv, base = ((b * sh.time) * sh.heads + h) * sh.dv + col;
+
+  f32x4 S[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int row = 16 * t + 4 * quad + r;
+      S[t][r] = d_state && in && row < sh.dk ? d_state[(bh * sh.dk + row) * sh.dv + col] : 0.0f;
+    }
+  if (in)
+    for (int64_t t = n_chunks * C + quad; t < sh.time; t += 4) dv[base + t * stride] = (T)0.0f;
+
+  for (int64_t ch = n_chunks - 1; ch >= 0; --ch) {
+    const bf16* kb = keys + ch * w.key_size;
+    const bf16* gb = gates + ch * w.gate_size;
+    const float* rb = rows + ch * ROWS;
+    const int64_t t0 = ch * C, at = bh * sh.chunks + ch;
+    float* s1 = w.ds1 + at * DKP * sh.dvp + col;
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s1[(int64_t)(16 * t + 4 * quad + r) * sh.dvp] = S[t][r];
+    f32x4 d[4], x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int64_t t = t0 + 16 * i + 4 * quad + e;
+        d[i][e] = in && t < len ? (float)d_o[base + t * stride] : 0.0f;
+      }
+    bf16x8 sf[KS][3];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) tiles_to_frag<3>(S[2 * s], S[2 * s + 1], sf[s]);
+    bf16x8 df[2][NPI];                       // bf16 upstream gradients are one plane
+    tiles_to_frag<NPI>(d[0], d[1], df[0]);
+    tiles_to_frag<NPI>(d[2], d[3], df[1]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        bf16x8 a[NPI];
+        load_frag<NPI>(kb + KB::KA, i * KS + s, 4 * KS * FRAG, lane, a);
+        acc = mma_planes<NPI, 3, 3>(a, sf[s], acc);
+      }
+      acc *= *(const f32x4*)(rb + 2 * C + 16 * i + 4 * quad);
+#pragma unroll
+      for (int s = i / 2; s < 2; ++s) {
+        bf16x8 a[3];
+        load_frag<3>(gb + GateBlock::PT, upper(i, s), 6 * FRAG, lane, a);
+        acc = mma_planes<3, NPI, 3>(a, df[s], acc);
+      }
+      x[i] = acc;
+    }
+    bf16x8 xf[2][3];
+    tiles_to_frag<3>(x[0], x[1], xf[0]);
+    tiles_to_frag<3>(x[2], x[3], xf[1]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+      for (int s = i / 2; s < 2; ++s) {
+        bf16x8 a[3];
+        load_frag<3>(gb + GateBlock::TT, upper(i, s), 6 * FRAG, lane, a);
+        acc = mma_planes<3, 3, 3>(a, xf[s], acc);
+      }
+      float* ep = w.e + (at * C + 16 * i + 4 * quad) * sh.dvp + col;
+      const f32x4 be = *(const f32x4*)(rb + 16 * i + 4 * quad), eg = *(const f32x4*)(rb + C + 16 * i + 4 * quad);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        ep[(int64_t)e * sh.dvp] = acc[e];
+        const int64_t t = t0 + 16 * i + 4 * quad + e;
+        if (in && t < sh.time) dv[base + t * stride] = (T)(t < len ? be[e] * acc[e] : 0.0f);
+        d[i][e] *= sh.scale * eg[e];
+        x[i][e] = -be[e] * eg[e] * acc[e];
+      }
+    }
+    bf16x8 dff[2][3];
+    tiles_to_frag<3>(d[0], d[1], dff[0]);
+    tiles_to_frag<3>(d[2], d[3], dff[1]);
+    tiles_to_frag<3>(x[0], x[1], xf[0]);
+    tiles_to_frag<3>(x[2], x[3], xf[1]);
+    const float whole = rb[2 * C - 1];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      f32x4 acc = S[t] * whole;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        bf16x8 a[NPI], aq[NPI];
+        load_frag<NPI>(kb + KB::KT, t * 2 + s, MT * 2 * FRAG, lane, a);
+        load_frag<NPI>(kb + KB::QT, t * 2 + s, MT * 2 * FRAG, lane, aq);
+        acc = mma_planes<NPI, 3, 3>(aq, dff[s], acc);
+        acc = mma_planes<NPI, 3, 3>(a, xf[s], acc);
+      }
+      S[t] = acc;
+    }
+  }
+  if (d_state0)
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int row = 16 * t + 4 * quad + r;
+        if (in && row < sh.dk) d_state0[(bh * sh.dk + row) * sh.dv + col] = S[t][r];
+      }
+}
+
+// ---------------------------------------------------------------------------
+// gradients of q, k and the gates, all chunks at once; wave = 16 tokens
+// ---------------------------------------------------------------------------
+template <int P>
+__device__ __forceinline__ void load_f32_frag(const float* p, bf16x8 (&out)[P]) {
+  const f32x4 a = *(const f32x4*)p, b = *(const f32x4*)(p + 4);
+  const float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+  split<P>(x, out);
+}
+
+template <typename T, int DKP, int NPI>
+__global__ void __launch_bounds__(256)
+    k_delta_back(Shape sh, const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ d_o,
+                 const float* __restrict__ g, const int32_t* __restrict__ lengths, T* __restrict__ dq, T* __restrict__ dk,
+                 float* __restrict__ dg, float* __restrict__ dbeta, Work w) {
+  typedef KeyBlock<DKP, NPI> KB;
+  constexpr int MT = DKP / 16;
+  __shared__ float se[C * LD], sf[C * LD];
+  __shared__ float s_gh[C], s_gl[C], s_row[C], s_db[C], s_sum[4], s_put[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, quad = lane >> 4, c = lane & 15;
+  const int64_t chunk = blockIdx.x % sh.chunks, bh = blockIdx.x / sh.chunks, b = bh / sh.heads;
+  const int h = (int)(bh % sh.heads), kh = h / sh.group;
+  const int64_t len = length_of(lengths, b, sh.time), t0 = chunk * C, at = bh * sh.chunks + chunk;
+  const bool shared = sh.group > 1;
+  const int64_t g_at = (b * sh.time + t0) * sh.heads + h;
+  if (t0 >= len) {
+    const int tokens = (int)std::min<int64_t>(C, sh.time - t0);
+    for (int i = tid; i < tokens; i += 256) {
+      dg[g_at + (int64_t)i * sh.heads] = 0.0f;
+      dbeta[g_at + (int64_t)i * sh.heads] = 0.0f;
+    }
+    for (int i = tid; i < tokens * sh.dk; i += 256) {
+      const int64_t p = ((b * sh.time + t0 + i / sh.dk) * sh.heads + h) * sh.dk + i % sh.dk;
+      if (shared) {
+        w.dq[p] = 0.0f;
+        w.dk[p] = 0.0f;
+      } else {
+        dq[p] = (T)0.0f;
+        dk[p] = (T)0.0f;
+      }
+    }
+    return;
+  }
+  const float* rb = w.rows + at * ROWS;
+  const float *s0 = w.s0 + at * DKP * sh.dvp, *ds1 = w.ds1 + at * DKP * sh.dvp;
+  const float *dl = w.delta + at * C * sh.dvp, *ee = w.e + at * C * sh.dvp;
+  const bf16* kb = w.keys + ((b * sh.kheads + kh) * sh.chunks + chunk) * w.key_size;
+  if (wave == 0) {
+    double gam = t0 + lane < len ? (double)fmaxf(g[b * sh.gs[0] + (t0 + lane) * sh.gs[1] + h * sh.gs[2]], G_MIN) : 0.0;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const double up = __shfl_up(gam, o);
+      if (lane >= o) gam += up;
+    }
+    s_gh[lane] = (float)gam;
+    s_gl[lane] = (float)(gam - (double)(float)gam);
+  }
+  // <dS1, S0> and dbeta_i = e_i . delta_i
+  {
+    double dot = 0.0;
+    for (int i = tid; i < DKP * sh.dvp; i += 256) dot += (double)s0[i] * (double)ds1[i];
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) dot += __shfl_xor(dot, o);
+    if (lane == 0) s_sum[wave] = (float)dot;
+    const int t = tid >> 2;
+    float db = 0.0f;
+    for (int i = tid & 3; i < sh.dvp; i += 4) db += dl[t * sh.dvp + i] * ee[t * sh.dvp + i];
+    db += __shfl_xor(db, 1);
+    db += __shfl_xor(db, 2);
+    if ((tid & 3) == 0) s_db[t] = db;
+  }
+  __syncthreads();
+
+  const int tok = 16 * wave + c;             // this lane's row of the operands
+  f32x4 m1[MT], m2[MT], m3[MT], pe[4], pf[4];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) m1[t] = m2[t] = m3[t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) pe[j] = pf[j] = f32x4{0, 0, 0, 0};
+  const bool live = t0 + tok < len;
+  const T* dop = d_o + ((b * sh.time + t0 + tok) * sh.heads + h) * sh.dv;
+  for (int s = 0; s < sh.dvp / 32; ++s) {
+    const int c0 = 32 * s + 8 * quad;
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = live && c0 + j < sh.dv ? (float)dop[c0 + j] : 0.0f;
+    bf16x8 fo[NPI], fe[3], fd[3];
+    split<NPI>(x, fo);
+    load_f32_frag<3>(ee + tok * sh.dvp + c0, fe);
+    load_f32_frag<3>(dl + tok * sh.dvp + c0, fd);
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      bf16x8 f0[3], f1[3];
+      load_f32_frag<3>(s0 + (16 * t + c) * sh.dvp + c0, f0);
+      load_f32_frag<3>(ds1 + (16 * t + c) * sh.dvp + c0, f1);
+      m1[t] = mma_planes<NPI, 3, 3>(fo, f0, m1[t]);
+      m2[t] = mma_planes<3, 3, 3>(fe, f0, m2[t]);
+      m3[t] = mma_planes<3, 3, 3>(fd, f1, m3[t]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j <= wave) {
+        bf16x8 fj[3];
+        load_f32_frag<3>(dl + (16 * j + c) * sh.dvp + c0, fj);
+        pe[j] = mma_planes<NPI, 3, 3>(fo, fj, pe[j]);
+        pf[j] = mma_planes<3, 3, 3>(fe, fj, pf[j]);
+      }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int i = 16 * wave + 4 * quad + r, jj = 16 * j + c;
+      const float d = jj <= i ? expf((s_gh[i] - s_gh[jj]) + (s_gl[i] - s_gl[jj])) * rb[jj] : 0.0f;
+      se[i * LD + jj] = jj <= i ? sh.scale * d * pe[j][r] : 0.0f;
+      sf[i * LD + jj] = jj < i ? -rb[i] * d * pf[j][r] : 0.0f;
+    }
+  const f32x4 be = *(const f32x4*)(rb + 16 * wave + 4 * quad), eg = *(const f32x4*)(rb + C + 16 * wave + 4 * quad);
+  const f32x4 rest = *(const f32x4*)(rb + 2 * C + 16 * wave + 4 * quad);
+  __syncthreads();
+
+  bf16x8 fe[2][3], ff[2][3], fet[2][3], fft[2][3];
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    float x[8], y[8], z[8], u[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int p = perm(s, quad, j);
+      x[j] = se[tok * LD + p];
+      y[j] = sf[tok * LD + p];
+      z[j] = se[p * LD + tok];
+      u[j] = sf[p * LD + tok];
+    }
+    split<3>(x, fe[s]);
+    split<3>(y, ff[s]);
+    split<3>(z, fet[s]);
+    split<3>(u, fft[s]);
+  }
+  f32x4 row = {0, 0, 0, 0}, put = {0, 0, 0, 0};
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    f32x4 aq = m1[t] * eg * sh.scale, ar = -(m2[t] * be * eg), aw = m3[t] * be * rest;
+    const f32x4 last = aw;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      bf16x8 kt[NPI], qt[NPI];
+      load_frag<NPI>(kb + KB::KT, t * 2 + s, MT * 2 * FRAG, lane, kt);
+      load_frag<NPI>(kb + KB::QT, t * 2 + s, MT * 2 * FRAG, lane, qt);
+      aq = mma_planes<3, NPI, 3>(fe[s], kt, aq);
+      ar = mma_planes<3, NPI, 3>(ff[s], kt, ar);
+      aw = mma_planes<3, NPI, 3>(fet[s], qt, aw);
+      aw = mma_planes<3, NPI, 3>(fft[s], kt, aw);
+    }
+    const int col = 16 * t + c;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int64_t tt = t0 + 16 * wave + 4 * quad + r;
+      if (col < sh.dk && tt < sh.time) {
+        const float qv = tt < len ? (float)q[b * sh.qs[0] + tt * sh.qs[1] + kh * sh.qs[2] + col] : 0.0f;
+        const float kv = tt < len ? (float)k[b * sh.ks[0] + tt * sh.ks[1] + kh * sh.ks[2] + col] : 0.0f;
+        row[r] += qv * aq[r] + kv * (ar[r] - aw[r]);
+        put[r] += kv * last[r];
+        const int64_t p = ((b * sh.time + tt) * sh.heads + h) * sh.dk + col;
+        const float vq = tt < len ? aq[r] : 0.0f, vk = tt < len ? ar[r] + aw[r] : 0.0f;
+        if (shared) {
+          w.dq[p] = vq;
+          w.dk[p] = vk;
+        } else {
+          dq[p] = (T)vq;
+          dk[p] = (T)vk;
+        }
+      }
+    }
+  }
+  float all = put[0] + put[1] + put[2] + put[3];
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) all += __shfl_xor(all, o);
+  if (lane == 0) s_put[wave] = all;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    float s = row[r];
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) s += __shfl_xor(s, o);
+    if (c == 0) s_row[16 * wave + 4 * quad + r] = s;
+  }
+  __syncthreads();
+  if (wave == 0) {
+    double s = (double)s_row[lane];
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const double down = __shfl_down(s, o);
+      if (lane + o < 64) s += down;
+    }
+    const float whole = rb[2 * C - 1];
+    s += (double)whole * ((double)s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3]) + ((double)s_put[0] + s_put[1] + s_put[2] + s_put[3]);
+    if (t0 + lane < sh.time) {
+      const bool on = t0 + lane < len;
+      dg[g_at + (int64_t)lane * sh.heads] = on ? (float)s : 0.0f;
+      dbeta[g_at + (int64_t)lane * sh.heads] = on ? s_db[lane] : 0.0f;
+    }
+  }
+}
+
+// sum over the heads that share a key head, in order
+template <typename T>
+__global__ void __launch_bounds__(GJX_BLOCK)
+    k_delta_shared_heads(Shape sh, const float* __restrict__ a, const float* __restrict__ b, T* __restrict__ out_a, T* __restrict__ out_b) {
+  const int64_t total = sh.batch * sh.time * sh.kheads * sh.dk;
+  for (int64_t i = (int64_t)blockIdx.x * GJX_BLOCK + threadIdx.x; i < total; i += (int64_t)gridDim.x * GJX_BLOCK) {
+    const int64_t d = i % sh.dk, row = i / sh.dk;
+    const float *pa = a + row * sh.group * sh.dk + d, *pb = b + row * sh.group * sh.dk + d;
+    float sa = 0.0f, sb = 0.0f;
+    for (int j = 0; j < sh.group; ++j) {
+      sa += pa[(int64_t)j * sh.dk];
+      sb += pb[(int64_t)j * sh.dk];
+    }
+    out_a[i] = (T)sa;
+    out_b[i] = (T)sb;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// one token: a workgroup holds a head's state in registers, 4 columns x R rows per lane
+//   u = beta (v - a S^T k), S' = a S + k u^T, o = scale (a S^T q + (q.k) u)
+// ---------------------------------------------------------------------------
+template <typename T, int CG, int R>
+__global__ void __launch_bounds__(256)
+    k_delta_step(Shape sh, const float* __restrict__ state, const int32_t* __restrict__ ancestors, const T* __restrict__ q,
+                 const T* __restrict__ k, const T* __restrict__ v, const float* __restrict__ g, const float* __restrict__ beta,
+                 T* __restrict__ o, float* __restrict__ state_out, int col_tiles) {
+  constexpr int RG = 256 / CG;
+  __shared__ float s_q[128], s_k[128];
+  __shared__ f32x4 s_pk[RG][CG], s_pq[RG][CG];
+  const int tid = threadIdx.x, cg = tid % CG, rg = tid / CG;
+  const int64_t bh = blockIdx.x / col_tiles;
+  const int64_t b = bh / sh.heads;
+  const int h = (int)(bh % sh.heads), kh = h / sh.group;
+  const int col = (int)(blockIdx.x % col_tiles) * CG * 4 + cg * 4;
+  if (tid < 128) {
+    s_q[tid] = tid < sh.dk ? (float)q[b * sh.qs[0] + kh * sh.qs[2] + tid] : 0.0f;
+    s_k[tid] = tid < sh.dk ? (float)k[b * sh.ks[0] + kh * sh.ks[2] + tid] : 0.0f;
+  }
+  int64_t src = b;
+  if (ancestors) src = std::min<int64_t>(std::max<int64_t>(ancestors[b], 0), sh.batch - 1);
+  const float* sp = state + (src * sh.heads + h) * (int64_t)sh.dk * sh.dv;
+  float* op = state_out + bh * (int64_t)sh.dk * sh.dv;
+  const bool vec = (sh.dv & 3) == 0;
+  f32x4 S[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int row = r * RG + rg;
+    S[r] = f32x4{0, 0, 0, 0};
+    if (row < sh.dk) {
+      if (vec && col < sh.dv) S[r] = *(const f32x4*)(sp + (int64_t)row * sh.dv + col);
+      else
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (col + e < sh.dv) S[r][e] = sp[(int64_t)row * sh.dv + col + e];
+    }
+  }
+  const float a = expf(g[b * sh.gs[0] + h * sh.gs[2]]), be = beta[b * sh.bs[0] + h * sh.bs[2]];
+  __syncthreads();
+  f32x4 pk = {0, 0, 0, 0}, pq = {0, 0, 0, 0};
+  float qk = 0.0f;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int row = r * RG + rg;
+    S[r] *= a;
+    pk += S[r] * s_k[row];
+    pq += S[r] * s_q[row];
+  }
+  for (int i = 0; i < sh.dk; ++i) qk += s_q[i] * s_k[i];
+  s_pk[rg][cg] = pk;
+  s_pq[rg][cg] = pq;
+  __syncthreads();
+  pk = pq = f32x4{0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < RG; ++i) {
+    pk += s_pk[i][cg];
+    pq += s_pq[i][cg];
+  }
+  f32x4 u;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    u[e] = col + e < sh.dv ? be * ((float)v[b * sh.vs[0] + h * sh.vs[2] + col + e] - pk[e]) : 0.0f;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int row = r * RG + rg;
+    if (row < sh.dk) {
+      S[r] += u * s_k[row];
+      if (vec && col < sh.dv) *(f32x4*)(op + (int64_t)row * sh.dv + col) = S[r];
+      else
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (col + e < sh.dv) op[(int64_t)row * sh.dv + col + e] = S[r][e];
+    }
+  }
+  if (rg == 0)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (col + e < sh.dv) o[bh * sh.dv + col + e] = (T)(sh.scale * (pq[e] + qk * u[e]));
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
+
+int32_t check_shape(const char* who, const gjx_delta_shape* s) {
+  GJX_REQUIRE(s != nullptr, GJX_EINVAL, "%s: shape is null", who);
+  GJX_REQUIRE(s->dtype == GJX_F32 || s->dtype == GJX_BF16, GJX_EINVAL, "%s: dtype %d is neither GJX_F32 nor GJX_BF16", who, s->dtype);
+  GJX_REQUIRE(s->batch >= 0 && s->time >= 0 && s->kheads >= 1 && s->heads >= 1 && s->heads % s->kheads == 0, GJX_EINVAL,
+              "%s: bad sizes (batch %lld, time %lld, kheads %d, heads %d)", who, (long long)s->batch, (long long)s->time, s->kheads, s->heads);
+  GJX_REQUIRE(s->dk >= 1 && s->dk <= 128 && s->dv >= 1 && s->dv <= 1024, GJX_ELIMIT, "%s: dk=%d not in [1, 128] or dv=%d not in [1, 1024]",
+              who, s->dk, s->dv);
+  GJX_REQUIRE(s->batch <= (1 << 24) && s->heads <= 1024 && s->time <= ((int64_t)1 << 30), GJX_ELIMIT,
+              "%s: batch up to 2^24, heads up to 1024, time up to 2^30", who);
+  const int64_t blocks = s->batch * s->heads * std::max<int64_t>(up(s->time, C) / C, up(s->dv, 32) / 16 + 8);
+  GJX_REQUIRE(blocks < ((int64_t)1 << 31), GJX_ELIMIT, "%s: batch x heads x chunks is too large", who);
+  return GJX_OK;
+}
+
+Shape shape_of(const gjx_delta_shape* s) {
+  Shape r = {};
+  r.kheads = s->kheads;
+  r.heads = s->heads;
+  r.group = s->heads / s->kheads;
+  r.dk = s->dk;
+  r.dv = s->dv;
+  r.dvp = (int)up(s->dv, 32);
+  r.scale = s->scale;
+  r.batch = s->batch;
+  r.time = s->time;
+  for (int i = 0; i < 3; ++i) {
+    r.qs[i] = s->q_stride[i];
+    r.ks[i] = s->k_stride[i];
+    r.vs[i] = s->v_stride[i];
+    r.gs[i] = s->g_stride[i];
+    r.bs[i] = s->b_stride[i];
+  }
+  r.chunks = up(s->time, C) / C;
+  return r;
+}
+
+struct Layout {
+  int dkp, npi;
+  int64_t key_size, gate_size;
+  int64_t keys, gates, rows, s0, delta, bytes;       // the filter's workspace
+  int64_t ds1, e, dq, dk, grad_bytes;                // the gradient's scratch
+};
+
+Layout layout_of(const gjx_delta_shape* s, bool keep) {
+  Layout l = {};
+  const Shape sh = shape_of(s);
+  l.dkp = s->dk <= 64 ? 64 : 128;
+  l.npi = s->dtype == GJX_F32 ? 3 : 1;
+  const int64_t side = (int64_t)l.npi * 4 * (l.dkp / 32) * FRAG;      // K rows = Q rows = K columns = Q columns
+  l.key_size = side * (keep ? 4 : 3);
+  l.gate_size = keep ? GateBlock::SIZE_KEEP : GateBlock::SIZE;
+  const int64_t kc = sh.batch * sh.kheads * sh.chunks, hc = sh.batch * sh.heads * sh.chunks;
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t p = at;
+    at = up(at + bytes, 256);
+    return p;
+  };
+  l.keys = take(kc * l.key_size * 2);
+  l.gates = take(hc * l.gate_size * 2);
+  l.rows = take(hc * ROWS * 4);
+  l.s0 = take(keep ? hc * l.dkp * sh.dvp * 4 : 0);
+  l.delta = take(keep ? hc * C * sh.dvp * 4 : 0);
+  l.bytes = at;
+  at = 0;
+  const int64_t shared = sh.group > 1 ? sh.batch * sh.time * sh.heads * sh.dk * 4 : 0;
+  l.ds1 = take(hc * l.dkp * sh.dvp * 4);
+  l.e = take(hc * C * sh.dvp * 4);
+  l.dq = take(shared);
+  l.dk = take(shared);
+  l.grad_bytes = at;
+  return l;
+}
+
+Work work_of(const Layout& l, char* base, char* scratch) {
+  Work w = {};
+  w.keys = (bf16*)(base + l.keys);
+  w.gates = (bf16*)(base + l.gates);
+  w.key_size = l.key_size;
+  w.gate_size = l.gate_size;
+  w.rows = (float*)(base + l.rows);
+  w.s0 = (float*)(base + l.s0);
+  w.delta = (float*)(base + l.delta);
+  if (scratch) {
+    w.ds1 = (float*)(scratch + l.ds1);
+    w.e = (float*)(scratch + l.e);
+    w.dq = (float*)(scratch + l.dq);
+    w.dk = (float*)(scratch + l.dk);
+  }
+  return w;
+}
+
+template <typename T>
+bool aligned_rows(const T* p, const int64_t (&s)[3]) {
+  const int per16 = 16 / (int)sizeof(T);
+  return ((uintptr_t)p & 15) == 0 && s[0] % per16 == 0 && s[1] % per16 == 0 && s[2] % per16 == 0;
+}
+
+unsigned scan_grid(const Shape& sh) { return (unsigned)(up(sh.batch * sh.heads, 8) * (sh.dvp / 16)); }
+
+template <typename T, int DKP, bool KEEP>
+int32_t run_filter(const Shape& sh, const T* q, const T* k, const T* v, const float* g, const float* beta, const float* state0,
+                   const int32_t* lengths, T* o, float* state, const Work& w, hipStream_t s) {
+  constexpr int NPI = sizeof(T) == 4 ? 3 : 1;
+  if (sh.chunks > 0) {
+    constexpr int lds = 2 * NPI * C * (DKP + 8) * 2 + 3 * C * LD * 4 + 3 * C * 4;
+    GJX_CHECK_HIP(hipFuncSetAttribute((const void*)k_delta_prepare<T, DKP, NPI, KEEP>, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+    k_delta_prepare<T, DKP, NPI, KEEP><<<(unsigned)(sh.batch * sh.heads * sh.chunks), 256, lds, s>>>(
+        sh, q, k, g, beta, lengths, w, aligned_rows(q, sh.qs) && aligned_rows(k, sh.ks));
+    GJX_LAUNCH_CHECK();
+  }
+  k_delta_scan<T, DKP, NPI, KEEP><<<scan_grid(sh), 64, 0, s>>>(sh, v, state0, lengths, o, state, w);
+  GJX_LAUNCH_CHECK();
+  return GJX_OK;
+}
+
+template <typename T, int DKP>
+int32_t run_grad(const Shape& sh, const T* q, const T* k, const float* g, const int32_t* lengths, const T* d_o, const float* d_state,
+                 T* dq, T* dk, T* dv, float* dg, float* dbeta, float* d_state0, const Work& w, hipStream_t s) {
+  constexpr int NPI = sizeof(T) == 4 ? 3 : 1;
+  k_delta_scan_back<T, DKP, NPI><<<scan_grid(sh), 64, 0, s>>>(sh, d_o, d_state, lengths, dv, d_state0, w);
+  GJX_LAUNCH_CHECK();
+  if (sh.chunks == 0) return GJX_OK;
+  k_delta_back<T, DKP, NPI><<<(unsigned)(sh.batch * sh.heads * sh.chunks), 256, 0, s>>>(sh, q, k, d_o, g, lengths, dq, dk, dg, dbeta, w);
+  GJX_LAUNCH_CHECK();
+  if (sh.group > 1) {
+    k_delta_shared_heads<T><<<gjx_grid_for(sh.batch * sh.time * sh.kheads * sh.dk), GJX_BLOCK, 0, s>>>(sh, w.dq, w.dk, dq, dk);
+    GJX_LAUNCH_CHECK();
+  }
+  return GJX_OK;
+}
+
+template <typename T>
+int32_t run_step(const Shape& sh, const float* state, const int32_t* anc, const T* q, const T* k, const T* v, const float* g,
+                 const float* beta, T* o, float* out, hipStream_t s) {
+  const int64_t bh = sh.batch * sh.heads;
+#define GJX_STEP(CG, R)                                                                                                       \
+  k_delta_step<T, CG, R><<<(unsigned)(bh * (up(sh.dv, CG * 4) / (CG * 4))), 256, 0, s>>>(sh, state, anc, q, k, v, g, beta, o, out, \
+                                                                                         (int)(up(sh.dv, CG * 4) / (CG * 4)))
+  if (sh.dv <= 64) {
+    if (sh.dk <= 64) GJX_STEP(16, 4);
+    else GJX_STEP(16, 8);
+  } else {
+    if (sh.dk <= 64) GJX_STEP(32, 8);
+    else GJX_STEP(32, 16);
+  }
+#undef GJX_STEP
+  GJX_LAUNCH_CHECK();
+  return GJX_OK;
+}
+
+}  // namespace
+
+GJX_API int32_t gjx_delta_filter_workspace(const gjx_delta_shape* shape, int32_t keep, int64_t* bytes) {
+  const char* who = "gjx_delta_filter_workspace";
+  const int32_t rc = check_shape(who, shape);
+  if (rc != GJX_OK) return rc;
+  GJX_REQUIRE(bytes != nullptr && keep >= 0 && keep <= 2, GJX_EINVAL, "%s: bytes is null or keep not in [0, 2]", who);
+  const Layout l = layout_of(shape, keep != 0);
+  *bytes = keep == 2 ? l.grad_bytes : l.bytes;
+  return GJX_OK;
+}
+
+GJX_API int32_t gjx_delta_filter(const gjx_delta_shape* shape, const void* d_q, const void* d_k, const void* d_v, const float* d_g,
+                                 const float* d_beta, const float* d_state0, const int32_t* d_lengths, void* d_o, float* d_state,
+                                 int32_t keep, void* d_work, int64_t work_bytes, void* stream) {
+  const char* who = "gjx_delta_filter";
+  const int32_t rc = check_shape(who, shape);
+  if (rc != GJX_OK) return rc;
+  if (shape->batch == 0) return GJX_OK;
+  GJX_REQUIRE(d_state && (shape->time == 0 || (d_q && d_k && d_v && d_g && d_beta && d_o)), GJX_EINVAL, "%s: null argument", who);
+  const Layout l = layout_of(shape, keep != 0);
+  GJX_REQUIRE(l.bytes == 0 || (d_work && ((uintptr_t)d_work & 255) == 0 && work_bytes >= l.bytes), GJX_EINVAL,
+              "%s: the workspace has %lld bytes, needs %lld aligned to 256", who, (long long)work_bytes, (long long)l.bytes);
+  const Shape sh = shape_of(shape);
+  const Work w = work_of(l, (char*)d_work, nullptr);
+  hipStream_t s = (hipStream_t)stream;
+#define GJX_FILTER(T, DKP, KEEP) \
+  run_filter<T, DKP, KEEP>(sh, (const T*)d_q, (const T*)d_k, (const T*)d_v, d_g, d_beta, d_state0, d_lengths, (T*)d_o, d_state, w, s)
+  if (shape->dtype == GJX_F32) {
+    if (l.dkp == 64) return keep ? GJX_FILTER(float, 64, true) : GJX_FILTER(float, 64, false);
+    return keep ? GJX_FILTER(float, 128, true) : GJX_FILTER(float, 128, false);
+  }
+  if (l.dkp == 64) return keep ? GJX_FILTER(bf16, 64, true) : GJX_FILTER(bf16, 64, false);
+  return keep ? GJX_FILTER(bf16, 128, true) : GJX_FILTER(bf16, 128, false);
+#undef GJX_FILTER
+}
+
+GJX_API int32_t gjx_delta_filter_grad(const gjx_delta_shape* shape, const void* d_q, const void* d_k, const void* d_v, const float* d_g,
+                                      const float* d_beta, const int32_t* d_lengths, const void* d_do, const float* d_dstate, void* d_dq,
+                                      void* d_dk, void* d_dv, float* d_dg, float* d_dbeta, float* d_dstate0, const void* d_kept,
+                                      int64_t kept_bytes, void* d_work, int64_t work_bytes, void* stream) {
+  const char* who = "gjx_delta_filter_grad";
+  const int32_t rc = check_shape(who, shape);
+  if (rc != GJX_OK) return rc;
+  if (shape->batch == 0) return GJX_OK;
+  GJX_REQUIRE(shape->time == 0 || (d_q && d_k && d_v && d_g && d_beta && d_do && d_dq && d_dk && d_dv && d_dg && d_dbeta), GJX_EINVAL,
+              "%s: null argument", who);
+  const Layout l = layout_of(shape, true);
+  GJX_REQUIRE(l.bytes == 0 || (d_kept && ((uintptr_t)d_kept & 255) == 0 && kept_bytes >= l.bytes), GJX_EINVAL,
+              "%s: the kept workspace has %lld bytes, needs %lld aligned to 256", who, (long long)kept_bytes, (long long)l.bytes);
+  GJX_REQUIRE(l.grad_bytes == 0 || (d_work && ((uintptr_t)d_work & 255) == 0 && work_bytes >= l.grad_bytes), GJX_EINVAL,
+              "%s: the workspace has %lld bytes, needs %lld aligned to 256", who, (long long)work_bytes, (long long)l.grad_bytes);
+  const Shape sh = shape_of(shape);
+  const Work w = work_of(l, (char*)const_cast<void*>(d_kept), (char*)d_work);
+  hipStream_t s = (hipStream_t)stream;
+#define GJX_GRAD(T, DKP)                                                                                                            \
+  run_grad<T, DKP>(sh, (const T*)d_q, (const T*)d_k, d_g, d_lengths, (const T*)d_do, d_dstate, (T*)d_dq, (T*)d_dk, (T*)d_dv, d_dg, d_dbeta, \
+                   d_dstate0, w, s)
+  if (shape->dtype == GJX_F32) return l.dkp == 64 ? GJX_GRAD(float, 64) : GJX_GRAD(float, 128);
+  return l.dkp == 64 ? GJX_GRAD(bf16, 64) : GJX_GRAD(bf16, 128);
+#undef GJX_GRAD
+}
+
+GJX_API int32_t gjx_delta_filter_step(const gjx_delta_shape* shape, const float* d_state, const int32_t* d_ancestors, const void* d_q,
+                                      const void* d_k, const void* d_v, const float* d_g, const float* d_beta, void* d_o,
+                                      float* d_state_out, void* stream) {
+  const char* who = "gjx_delta_filter_step";
+  const int32_t rc = check_shape(who, shape);
+  if (rc != GJX_OK) return rc;
+  GJX_REQUIRE(shape->time == 1, GJX_EINVAL, "%s: time must be 1", who);
+  if (shape->batch == 0) return GJX_OK;
+  GJX_REQUIRE(d_state && d_q && d_k && d_v && d_g && d_beta && d_o && d_state_out, GJX_EINVAL, "%s: null argument", who);
+  GJX_REQUIRE(!d_ancestors || d_state != d_state_out, GJX_EINVAL, "%s: with ancestors the new state needs a buffer of its own", who);
+  GJX_REQUIRE((((uintptr_t)d_state | (uintptr_t)d_state_out) & 15) == 0, GJX_EINVAL, "%s: states must be aligned to 16 bytes", who);
+  const Shape sh = shape_of(shape);
+  hipStream_t s = (hipStream_t)stream;
+  if (shape->dtype == GJX_F32)
+    return run_step<float>(sh, d_state, d_ancestors, (const float*)d_q, (const float*)d_k, (const float*)d_v, d_g, d_beta, (float*)d_o,
+                           d_state_out, s);
+  return run_step<bf16>(sh, d_state, d_ancestors, (const bf16*)d_q, (const bf16*)d_k, (const bf16*)d_v, d_g, d_beta, (bf16*)d_o,
+                        d_state_out, s);
+}

@@ -238,6 +238,66 @@ def kalman_filter(observations, initial_mean, initial_cov, A, Q, C, R):
 
 
 # --------------------------------------------------------------------------- #
+# gated delta filter: kalman_filter's mean recursion (state_space.py:434-530) for a matrix of regression weights, with
+# the gain beta_t k_t in place of the covariance's -- the memory of a token-sequence model, on the device
+# --------------------------------------------------------------------------- #
+class _DeltaFilterFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, log_decay, beta, initial_state, scale, lengths):
+        o, state, kept = B.delta_filter(q, k, v, log_decay, beta, initial_state, scale, lengths, keep=True)
+        ctx.save_for_backward(q, k, v, log_decay, beta, lengths, kept)
+        ctx.scale, ctx.want_state0 = scale, initial_state is not None and ctx.needs_input_grad[5]
+        ctx.set_materialize_grads(False)
+        return o, state
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_o, d_state):
+        q, k, v, log_decay, beta, lengths, kept = ctx.saved_tensors
+        grads = B.delta_filter_grad(q, k, v, log_decay, beta, d_o, d_state, kept, ctx.scale, lengths, ctx.want_state0)
+        return (*grads, None, None)
+
+
+def delta_filter(q, k, v, log_decay, beta, initial_state=None, scale=None, lengths=None):
+    """The gated delta filter over whole sequences: per batch element and head, with a_t = exp(log_decay_t),
+
+        S_t = a_t S_{t-1} + k_t u_t^T,   u_t = beta_t (v_t - a_t S_{t-1}^T k_t),   o_t = scale S_t^T q_t.
+
+    q, k: (batch, time, key heads, dk); v: (batch, time, heads, dv), heads a multiple of the key heads (consecutive
+    heads share one); log_decay, beta: (batch, time, heads) float32; initial_state: (batch, heads, dk, dv) float32 or
+    None (zeros); scale: dk ** -0.5 unless given; lengths: int32 (batch,) or None -- tokens at and behind a sequence's
+    length are skipped (their outputs are 0, the state passes).  q, k, v are all float32 or all bfloat16; dk <= 128,
+    dv <= 1024.  Keys should keep beta |k|^2 <= 2, beyond which the recursion itself diverges; a log_decay below -100 (a
+    reset: -inf) counts as -100.
+
+    Returns (o (batch, time, heads, dv) of v's type, S_time (batch, heads, dk, dv) float32); differentiable in q, k, v,
+    log_decay, beta and initial_state.  Chunks of 64 tokens run as matrix products; delta_filter_step takes one token."""
+    tensors = (q, k, v, log_decay, beta, initial_state)
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
+        return _DeltaFilterFn.apply(*tensors, scale, lengths)
+    return B.delta_filter(*tensors, scale, lengths)[:2]
+
+
+def delta_filter_step(state, q, k, v, log_decay, beta, scale=None, ancestors=None, out=None):
+    """One token of delta_filter for every particle: state (n, heads, dk, dv) float32, q, k (n, key heads, dk), v
+    (n, heads, dv), log_decay, beta (n, heads) -> (o (n, heads, dv), new state).
+
+    ancestors (int32 (n,), as systematic_resample returns them): particle i continues from the state of ancestors[i];
+    the gather costs no pass of its own.  Indices are clamped to [0, n).  out: buffer for the new state -- the state
+    itself (in place) when there are no ancestors.  Where a gradient is wanted the call is delta_filter over one
+    token."""
+    tensors = (state, q, k, v, log_decay, beta)
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
+        if out is not None:
+            raise GjxError("delta_filter_step: `out` cannot be given where a gradient is wanted")
+        if ancestors is not None:
+            state = state.index_select(0, ancestors.long().clamp(0, state.shape[0] - 1))
+        o, new = delta_filter(*(t.unsqueeze(1) for t in (q, k, v, log_decay, beta)), initial_state=state, scale=scale)
+        return o.squeeze(1), new
+    return B.delta_filter_step(state, q, k, v, log_decay, beta, scale, ancestors, out)
+
+
+# --------------------------------------------------------------------------- #
 # discrete HMM (reference src/genjax/extras/state_space.py:52-100, 103-163, 295-363): the kernel model on the
 # generic column path -- categorical draws and log-densities are library launches, the table look-ups are
 # row gathers -- with the exact forward filter as its test companion (host, f64)

@@ -750,6 +750,42 @@ int32_t gjx_gol_gibbs_pass(const uint32_t* d_pass_keys, int64_t n_chains, int32_
 int32_t gjx_gol_sweep(const uint32_t* d_pass_keys9, int64_t n_chains, int32_t n, float p_flip,
                       const uint8_t* d_future, int64_t future_stride, uint8_t* d_boards, void* stream);
 
+/* ---- gated delta filter: the mean recursion of the Kalman filter (extras/state_space.py:434-530) for a dk x dv
+ * matrix of regression weights S observed along k_t with the gain beta_t k_t,
+ *   S_t = a_t S_{t-1} + k_t u_t^T,  u_t = beta_t (v_t - a_t S_{t-1}^T k_t),  o_t = scale S_t^T q_t,  a_t = exp(g_t),
+ * per batch element and head.  q, k: (batch, time, kheads, dk); v: (batch, time, heads, dv), heads a multiple of
+ * kheads (consecutive heads share a key head); log-decays g and gains beta: (batch, time, heads) f32; states
+ * (batch, heads, dk, dv) f32 contiguous.  q, k, v, o and their gradients are of type dtype.  Strides are in elements
+ * (batch, time, head), the last axis is contiguous.  dk in [1, 128], dv in [1, 1024].  lengths (nullable, int32): the
+ * tokens at and behind lengths[b] are skipped (outputs and gradients 0, the state passes).  log-decays below -100
+ * (-inf among them: a reset) count as -100; the caller's keys keep beta |k|^2 <= 2 (the recursion diverges otherwise,
+ * in any arithmetic). */
+typedef struct gjx_delta_shape {
+  int32_t dtype, kheads, heads, dk, dv;
+  float scale;
+  int64_t batch, time;
+  int64_t q_stride[3], k_stride[3], v_stride[3], g_stride[3], b_stride[3];
+} gjx_delta_shape;
+
+/* workspace bytes (256-byte aligned): keep = 0 for the filter alone, 1 when its gradient follows (the filter then
+ * leaves in the workspace what gjx_delta_filter_grad reads), 2 for the gradient's own scratch */
+int32_t gjx_delta_filter_workspace(const gjx_delta_shape* shape, int32_t keep, int64_t* bytes);
+int32_t gjx_delta_filter(const gjx_delta_shape* shape, const void* d_q, const void* d_k, const void* d_v,
+                         const float* d_g, const float* d_beta, const float* d_state0, const int32_t* d_lengths,
+                         void* d_o, float* d_state, int32_t keep, void* d_work, int64_t work_bytes, void* stream);
+/* d_do (batch, time, heads, dv) contiguous and d_dstate (nullable): upstream gradients of o and of the last state;
+ * outputs contiguous (d_dstate0 nullable); d_kept is the workspace of a keep = 1 call with the same inputs */
+int32_t gjx_delta_filter_grad(const gjx_delta_shape* shape, const void* d_q, const void* d_k, const void* d_v,
+                              const float* d_g, const float* d_beta, const int32_t* d_lengths, const void* d_do,
+                              const float* d_dstate, void* d_dq, void* d_dk, void* d_dv, float* d_dg, float* d_dbeta,
+                              float* d_dstate0, const void* d_kept, int64_t kept_bytes, void* d_work,
+                              int64_t work_bytes, void* stream);
+/* One token for every batch element (time = 1): reads the state of ancestor[i] (nullable: of i; the gather of
+ * smc.py:170-174 fused into the load), writes o and the new state.  d_state_out may be d_state only without ancestors. */
+int32_t gjx_delta_filter_step(const gjx_delta_shape* shape, const float* d_state, const int32_t* d_ancestors,
+                              const void* d_q, const void* d_k, const void* d_v, const float* d_g, const float* d_beta,
+                              void* d_o, float* d_state_out, void* stream);
+
 /* The same passes on BIT-PACKED boards (one bit per cell, row pitch gjx_gol_words_per_row(n) = ceil(n / 64)
  * 64-bit words, bit c of word w of a row = column 64 w + c, bits beyond n zero; chains contiguous).  Same
  * conditionals, same draws, same new boards as the byte form bit for bit; the 18 rule outcomes of a cell come
