@@ -57,7 +57,7 @@ struct KeyBlock {               // per key head
 struct GateBlock {              // per head: That, P, then (keep) T^T, P^T; three planes of six fragments each
   static constexpr int TA = 0, PA = 18 * FRAG, TT = 36 * FRAG, PT = 54 * FRAG, SIZE = 36 * FRAG, SIZE_KEEP = 72 * FRAG;
 };
-constexpr int ROWS = 3 * C;     // f32 per head and chunk: beta, e^gamma, e^(gamma_C - gamma)
+constexpr int ROWS = 4 * C;     // f32 per head and chunk: beta, e^gamma, e^(gamma_C - gamma), e^gamma_C (repeated)
 
 struct Work {
   bf16 *keys, *gates;
@@ -72,22 +72,27 @@ __device__ __forceinline__ f32x4 mma(bf16x8 a, bf16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-// f32 -> bf16 planes, exactly for P = 3 (an h that would round to infinity is cut off; an infinite x keeps h only)
+// f32 -> bf16 planes, exactly for P = 3.  What rounds to infinity in bf16 (above 3.39e38) counts as infinite: h alone.
+template <int P, int N>
+__device__ __forceinline__ void split_planes(float (&x)[N], int p, bf16 (&h)[N]) {
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    h[j] = (bf16)x[j];
+    if (p + 1 < P) x[j] = p == 0 && !(fabsf(x[j]) < 3.389e38f) ? 0.0f : x[j] - (float)h[j];
+  }
+}
+
 template <int P>
 __device__ __forceinline__ void split(const float (&x)[8], bf16x8 (&out)[P]) {
+  float r[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    float r = x[j];
+  for (int j = 0; j < 8; ++j) r[j] = x[j];
 #pragma unroll
-    for (int p = 0; p < P; ++p) {
-      bf16 h = (bf16)r;
-      if (p == 0 && __builtin_isinf((float)h)) {
-        h = (bf16)__uint_as_float(__float_as_uint(r) & 0xffff0000u);
-        if (__builtin_isinf(r)) r = (float)h;
-      }
-      out[p][j] = h;
-      r = __builtin_isinf(r) ? 0.0f : r - (float)h;
-    }
+  for (int p = 0; p < P; ++p) {
+    bf16 h[8];
+    split_planes<P, 8>(r, p, h);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) out[p][j] = h[j];
   }
 }
 
@@ -260,6 +265,7 @@ __global__ void __launch_bounds__(256)
     rows[lane] = be;
     rows[C + lane] = expf((float)gam);
     rows[2 * C + lane] = expf((float)(last - gam));
+    rows[3 * C + lane] = expf((float)last);
   }
   for (int i = tid; i < C * LD; i += 256) st[i] = 0.0f;
   __syncthreads();
@@ -348,272 +354,402 @@ __global__ void __launch_bounds__(256)
 }
 
 // ---------------------------------------------------------------------------
-// the recursion: one wave owns 16 columns of S
+// the recursion: four waves share NC x 16 columns of S
 // ---------------------------------------------------------------------------
-// the waves of one head go to one XCD (workgroups go round the eight of them): they read the same fragments
+// Wave w owns the dk rows [w DKP / 4, (w + 1) DKP / 4) of S and the tokens [16 w, 16 w + 16) of a chunk.  What one wave
+// computes and the others multiply by (S, r, V', ...) goes through LDS in fragment order, three barriers a chunk; what a
+// wave takes from memory (its rows of K, Q, That, P, its rows of K^T) is used by no other wave, so it is loaded straight
+// into registers, each fragment for the next chunk as soon as it has been used for this one.
+constexpr int TEAM = 256;
+
+// the workgroups of one head go to one XCD (workgroups go round the eight of them): they read the same fragments
 __device__ __forceinline__ bool scan_place(int64_t block, int tiles, int64_t heads, int64_t& bh, int& tile) {
   bh = block / (8 * tiles) * 8 + block % 8;
   tile = (int)(block / 8 % tiles);
   return bh < heads;
 }
 
-template <typename T, int DKP, int NPI, bool KEEP>
-__global__ void __launch_bounds__(64)
+// barrier for LDS traffic only: loads and stores of global memory stay in flight
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// four elements per lane of a 16-row tile -> its half of a slab's fragment planes
+template <int P>
+__device__ __forceinline__ void put_half(bf16* frag, int plane, int half, int lane, f32x4 x) {
+  float r[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    bf16 h[4];
+    split_planes<P, 4>(r, p, h);
+    *(bf16x4*)(frag + p * plane + lane * 8 + half * 4) = bf16x4{h[0], h[1], h[2], h[3]};
+  }
+}
+
+template <int P>
+__device__ __forceinline__ void get_frag(const bf16* frag, int plane, int lane, bf16x8 (&out)[P]) {
+#pragma unroll
+  for (int p = 0; p < P; ++p) out[p] = *(const bf16x8*)(frag + p * plane + lane * 8);
+}
+
+template <typename T, int DKP, int NPI, bool KEEP, int NC>
+__global__ void __launch_bounds__(TEAM, 1)
     k_delta_scan(Shape sh, const T* __restrict__ v, const float* __restrict__ state0, const int32_t* __restrict__ lengths,
                  T* __restrict__ o, float* __restrict__ state, Work w) {
   typedef KeyBlock<DKP, NPI> KB;
-  constexpr int KS = DKP / 32, MT = DKP / 16;
-  constexpr int NPO = NPI == 1 ? 2 : 3;          // planes of what only the read-out takes
-  const int lane = threadIdx.x, quad = lane >> 4, c = lane & 15;
+  constexpr int KS = DKP / 32, MT = DKP / 64;     // slabs of S; 16-row tiles of S per wave
+  constexpr int NPO = NPI == 1 ? 2 : 3;           // planes of what only the read-out takes
+  __shared__ bf16 x_s[KS * NC * 3 * FRAG], x_r[2 * NC * 3 * FRAG], x_v[2 * NC * NPO * FRAG], x_w[2 * NC * 3 * FRAG];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quad = lane >> 4, c = lane & 15;
   int64_t bh;
   int tile;
-  if (!scan_place(blockIdx.x, sh.dvp / 16, sh.batch * sh.heads, bh, tile)) return;
+  const int tiles = (sh.dvp / 16 + NC - 1) / NC;
+  if (!scan_place(blockIdx.x, tiles, sh.batch * sh.heads, bh, tile)) return;
   const int64_t b = bh / sh.heads;
   const int h = (int)(bh % sh.heads), kh = h / sh.group;
-  const int col = tile * 16 + c;
-  const bool in = col < sh.dv;
+  const int col0 = tile * 16 * NC + c;
   const int64_t len = length_of(lengths, b, sh.time), n_chunks = (len + C - 1) / C;
   const bf16* keys = w.keys + (b * sh.kheads + kh) * sh.chunks * w.key_size;
   const bf16* gates = w.gates + bh * sh.chunks * w.gate_size;
   const float* rows = w.rows + bh * sh.chunks * ROWS;
-  const T* vp = v + b * sh.vs[0] + h * sh.vs[2] + col;
-  T* op = o + ((b * sh.time) * sh.heads + h) * sh.dv + col;
+  const T* vp = v + b * sh.vs[0] + h * sh.vs[2];
+  T* op = o + ((b * sh.time) * sh.heads + h) * sh.dv;
   const int64_t o_stride = (int64_t)sh.heads * sh.dv;
+  const int row0 = 16 * MT * wave + 4 * quad;     // first of this lane's rows of S
+  const int tok = 16 * wave + 4 * quad;           // ... and tokens of a chunk
+  const int lo = wave / 2;                        // last slab of this wave's rows of That and P
 
-  f32x4 S[MT];
+  f32x4 S[NC][MT];
 #pragma unroll
-  for (int t = 0; t < MT; ++t)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int row = 16 * t + 4 * quad + r;
-      S[t][r] = state0 && in && row < sh.dk ? state0[(bh * sh.dk + row) * sh.dv + col] : 0.0f;
-    }
-
-  for (int64_t ch = 0; ch < n_chunks; ++ch) {
-    const bf16* kb = keys + ch * w.key_size;
-    const bf16* gb = gates + ch * w.gate_size;
-    const float* rb = rows + ch * ROWS;
-    const int64_t t0 = ch * C;
-    if (KEEP) {
-      float* s0 = w.s0 + (bh * sh.chunks + ch) * (int64_t)DKP * sh.dvp + col;
-#pragma unroll
-      for (int t = 0; t < MT; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) s0[(int64_t)(16 * t + 4 * quad + r) * sh.dvp] = S[t][r];
-    }
-    bf16x8 sf[KS][3];
-#pragma unroll
-    for (int s = 0; s < KS; ++s) tiles_to_frag<3>(S[2 * s], S[2 * s + 1], sf[s]);
-    f32x4 r[4], qs[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      f32x4 acc = {0, 0, 0, 0}, aq = {0, 0, 0, 0};
-#pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        bf16x8 a[NPI], aqf[NPI];
-        load_frag<NPI>(kb + KB::KA, i * KS + s, 4 * KS * FRAG, lane, a);
-        load_frag<NPI>(kb + KB::QA, i * KS + s, 4 * KS * FRAG, lane, aqf);
-        acc = mma_planes<NPI, 3, 3>(a, sf[s], acc);
-        aq = mma_planes<NPI, 3, NPO>(aqf, sf[s], aq);
-      }
-      const f32x4 eg = *(const f32x4*)(rb + C + 16 * i + 4 * quad);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int64_t t = t0 + 16 * i + 4 * quad + e;
-        const float val = in && t < len ? (float)vp[t * sh.vs[1]] : 0.0f;
-        r[i][e] = val - eg[e] * acc[e];
-        qs[i][e] = sh.scale * eg[e] * aq[e];
-      }
-    }
-    bf16x8 rf[2][3];
-    tiles_to_frag<3>(r[0], r[1], rf[0]);
-    tiles_to_frag<3>(r[2], r[3], rf[1]);
-    f32x4 vn[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      f32x4 acc = {0, 0, 0, 0};
-#pragma unroll
-      for (int s = 0; s <= i / 2; ++s) {
-        bf16x8 a[3];
-        load_frag<3>(gb + GateBlock::TA, lower(i, s), 6 * FRAG, lane, a);
-        acc = mma_planes<3, 3, 3>(a, rf[s], acc);
-      }
-      if (KEEP) {
-        float* dp = w.delta + ((bh * sh.chunks + ch) * C + 16 * i + 4 * quad) * (int64_t)sh.dvp + col;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) dp[(int64_t)e * sh.dvp] = acc[e];
-      }
-      vn[i] = acc * *(const f32x4*)(rb + 16 * i + 4 * quad);
-    }
-    bf16x8 vf[2][NPO];
-    tiles_to_frag<NPO>(vn[0], vn[1], vf[0]);
-    tiles_to_frag<NPO>(vn[2], vn[3], vf[1]);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-#pragma unroll
-      for (int s = 0; s <= i / 2; ++s) {
-        bf16x8 a[NPO];
-        load_frag<NPO>(gb + GateBlock::PA, lower(i, s), 6 * FRAG, lane, a);
-        qs[i] = mma_planes<NPO, NPO, NPO>(a, vf[s], qs[i]);
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int64_t t = t0 + 16 * i + 4 * quad + e;
-        if (in && t < sh.time) op[t * o_stride] = (T)qs[i][e];
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) vn[i] *= *(const f32x4*)(rb + 2 * C + 16 * i + 4 * quad);
-    tiles_to_frag<3>(vn[0], vn[1], rf[0]);
-    tiles_to_frag<3>(vn[2], vn[3], rf[1]);
-    const float whole = rb[2 * C - 1];
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      f32x4 acc = S[t] * whole;
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        bf16x8 a[NPI];
-        load_frag<NPI>(kb + KB::KT, t * 2 + s, MT * 2 * FRAG, lane, a);
-        acc = mma_planes<NPI, 3, 3>(a, rf[s], acc);
-      }
-      S[t] = acc;
-    }
-  }
-  if (in)
-    for (int64_t t = n_chunks * C + quad; t < sh.time; t += 4) op[t * o_stride] = (T)0.0f;
-#pragma unroll
-  for (int t = 0; t < MT; ++t)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int row = 16 * t + 4 * quad + r;
-      if (in && row < sh.dk) state[(bh * sh.dk + row) * sh.dv + col] = S[t][r];
-    }
-}
-
-template <typename T, int DKP, int NPI>
-__global__ void __launch_bounds__(64)
-    k_delta_scan_back(Shape sh, const T* __restrict__ d_o, const float* __restrict__ d_state, const int32_t* __restrict__ lengths,
-                      T* __restrict__ dv, float* __restrict__ d_state0, Work w) {
-  typedef KeyBlock<DKP, NPI> KB;
-  constexpr int KS = DKP / 32, MT = DKP / 16;
-  const int lane = threadIdx.x, quad = lane >> 4, c = lane & 15;
-  int64_t bh;
-  int tile;
-  if (!scan_place(blockIdx.x, sh.dvp / 16, sh.batch * sh.heads, bh, tile)) return;
-  const int64_t b = bh / sh.heads;
-  const int h = (int)(bh % sh.heads), kh = h / sh.group;
-  const int col = tile * 16 + c;
-  const bool in = col < sh.dv;
-  const int64_t len = length_of(lengths, b, sh.time), n_chunks = (len + C - 1) / C;
-  const bf16* keys = w.keys + (b * sh.kheads + kh) * sh.chunks * w.key_size;
-  const bf16* gates = w.gates + bh * sh.chunks * w.gate_size;
-  const float* rows = w.rows + bh * sh.chunks * ROWS;
-  const int64_t stride = (int64_t)sh.heads * sh.dv, base = ((b * sh.time) * sh.heads + h) * sh.dv + col;
-
-  f32x4 S[MT];
-#pragma unroll
-  for (int t = 0; t < MT; ++t)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int row = 16 * t + 4 * quad + r;
-      S[t][r] = d_state && in && row < sh.dk ? d_state[(bh * sh.dk + row) * sh.dv + col] : 0.0f;
-    }
-  if (in)
-    for (int64_t t = n_chunks * C + quad; t < sh.time; t += 4) dv[base + t * stride] = (T)0.0f;
-
-  for (int64_t ch = n_chunks - 1; ch >= 0; --ch) {
-    const bf16* kb = keys + ch * w.key_size;
-    const bf16* gb = gates + ch * w.gate_size;
-    const float* rb = rows + ch * ROWS;
-    const int64_t t0 = ch * C, at = bh * sh.chunks + ch;
-    float* s1 = w.ds1 + at * DKP * sh.dvp + col;
-#pragma unroll
-    for (int t = 0; t < MT; ++t)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) s1[(int64_t)(16 * t + 4 * quad + r) * sh.dvp] = S[t][r];
-    f32x4 d[4], x[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int64_t t = t0 + 16 * i + 4 * quad + e;
-        d[i][e] = in && t < len ? (float)d_o[base + t * stride] : 0.0f;
-      }
-    bf16x8 sf[KS][3];
-#pragma unroll
-    for (int s = 0; s < KS; ++s) tiles_to_frag<3>(S[2 * s], S[2 * s + 1], sf[s]);
-    bf16x8 df[2][NPI];                       // bf16 upstream gradients are one plane
-    tiles_to_frag<NPI>(d[0], d[1], df[0]);
-    tiles_to_frag<NPI>(d[2], d[3], df[1]);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      f32x4 acc = {0, 0, 0, 0};
-#pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        bf16x8 a[NPI];
-        load_frag<NPI>(kb + KB::KA, i * KS + s, 4 * KS * FRAG, lane, a);
-        acc = mma_planes<NPI, 3, 3>(a, sf[s], acc);
-      }
-      acc *= *(const f32x4*)(rb + 2 * C + 16 * i + 4 * quad);
-#pragma unroll
-      for (int s = i / 2; s < 2; ++s) {
-        bf16x8 a[3];
-        load_frag<3>(gb + GateBlock::PT, upper(i, s), 6 * FRAG, lane, a);
-        acc = mma_planes<3, NPI, 3>(a, df[s], acc);
-      }
-      x[i] = acc;
-    }
-    bf16x8 xf[2][3];
-    tiles_to_frag<3>(x[0], x[1], xf[0]);
-    tiles_to_frag<3>(x[2], x[3], xf[1]);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      f32x4 acc = {0, 0, 0, 0};
-#pragma unroll
-      for (int s = i / 2; s < 2; ++s) {
-        bf16x8 a[3];
-        load_frag<3>(gb + GateBlock::TT, upper(i, s), 6 * FRAG, lane, a);
-        acc = mma_planes<3, 3, 3>(a, xf[s], acc);
-      }
-      float* ep = w.e + (at * C + 16 * i + 4 * quad) * sh.dvp + col;
-      const f32x4 be = *(const f32x4*)(rb + 16 * i + 4 * quad), eg = *(const f32x4*)(rb + C + 16 * i + 4 * quad);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        ep[(int64_t)e * sh.dvp] = acc[e];
-        const int64_t t = t0 + 16 * i + 4 * quad + e;
-        if (in && t < sh.time) dv[base + t * stride] = (T)(t < len ? be[e] * acc[e] : 0.0f);
-        d[i][e] *= sh.scale * eg[e];
-        x[i][e] = -be[e] * eg[e] * acc[e];
-      }
-    }
-    bf16x8 dff[2][3];
-    tiles_to_frag<3>(d[0], d[1], dff[0]);
-    tiles_to_frag<3>(d[2], d[3], dff[1]);
-    tiles_to_frag<3>(x[0], x[1], xf[0]);
-    tiles_to_frag<3>(x[2], x[3], xf[1]);
-    const float whole = rb[2 * C - 1];
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      f32x4 acc = S[t] * whole;
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        bf16x8 a[NPI], aq[NPI];
-        load_frag<NPI>(kb + KB::KT, t * 2 + s, MT * 2 * FRAG, lane, a);
-        load_frag<NPI>(kb + KB::QT, t * 2 + s, MT * 2 * FRAG, lane, aq);
-        acc = mma_planes<NPI, 3, 3>(aq, dff[s], acc);
-        acc = mma_planes<NPI, 3, 3>(a, xf[s], acc);
-      }
-      S[t] = acc;
-    }
-  }
-  if (d_state0)
+  for (int n = 0; n < NC; ++n)
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int row = 16 * t + 4 * quad + r;
-        if (in && row < sh.dk) d_state0[(bh * sh.dk + row) * sh.dv + col] = S[t][r];
+        const int row = row0 + 16 * t + r, col = col0 + 16 * n;
+        S[n][t][r] = state0 && col < sh.dv && row < sh.dk ? state0[(bh * sh.dk + row) * sh.dv + col] : 0.0f;
       }
+
+  bf16x8 ka[KS][NPI], qa[KS][NPI], kt[MT][2][NPI], ta[2][3], pa[2][NPO];
+  f32x4 f_beta, f_eg, f_rest;
+  f32x4 whole;
+  T vals[NC][4];                                  // raw: converted and masked where they are used
+  auto load_kq = [&](int64_t ch) {
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      load_frag<NPI>(keys + ch * w.key_size + KB::KA, wave * KS + s, 4 * KS * FRAG, lane, ka[s]);
+      load_frag<NPI>(keys + ch * w.key_size + KB::QA, wave * KS + s, 4 * KS * FRAG, lane, qa[s]);
+    }
+#pragma unroll
+    for (int n = 0; n < NC; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        vals[n][e] = vp[std::min<int64_t>(ch * C + tok + e, len - 1) * sh.vs[1] + min(col0 + 16 * n, sh.dv - 1)];
+      }
+    f_eg = *(const f32x4*)(rows + ch * ROWS + C + tok);
+  };
+  auto load_t = [&](int64_t ch) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+      load_frag<3>(gates + ch * w.gate_size + GateBlock::TA, lower(wave, min(s, lo)), 6 * FRAG, lane, ta[s]);
+    f_beta = *(const f32x4*)(rows + ch * ROWS + tok);
+    f_rest = *(const f32x4*)(rows + ch * ROWS + 2 * C + tok);
+  };
+  auto load_kt = [&](int64_t ch) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      load_frag<NPO>(gates + ch * w.gate_size + GateBlock::PA, lower(wave, min(s, lo)), 6 * FRAG, lane, pa[s]);
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+        load_frag<NPI>(keys + ch * w.key_size + KB::KT, (wave * MT + t) * 2 + s, 2 * KS * 2 * FRAG, lane, kt[t][s]);
+    }
+    whole = *(const f32x4*)(rows + ch * ROWS + 3 * C + tok);      // a vector load: the scalar kind shares the LDS counter
+  };
+  if (n_chunks > 0) {
+    load_kq(0);
+    load_t(0);
+    load_kt(0);
+  }
+
+  for (int64_t ch = 0; ch < n_chunks; ++ch) {
+    const int64_t next = ch + 1 < n_chunks ? ch + 1 : ch;
+    const int64_t t0 = ch * C;
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        const int row_tile = wave * MT + t;
+        put_half<3>(x_s + ((row_tile / 2) * NC + n) * 3 * FRAG, FRAG, row_tile & 1, lane, S[n][t]);
+        if (KEEP && col0 + 16 * n < sh.dvp) {
+          float* s0 = w.s0 + ((bh * sh.chunks + ch) * DKP + row0 + 16 * t) * sh.dvp + col0 + 16 * n;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s0[(int64_t)r * sh.dvp] = S[n][t][r];
+        }
+      }
+    }
+    lds_barrier();
+    f32x4 qs[NC];
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      f32x4 acc = {0, 0, 0, 0}, aq = {0, 0, 0, 0}, r;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        bf16x8 sf[3];
+        get_frag<3>(x_s + (s * NC + n) * 3 * FRAG, FRAG, lane, sf);
+        acc = mma_planes<NPI, 3, 3>(ka[s], sf, acc);
+        aq = mma_planes<NPI, 3, NPO>(qa[s], sf, aq);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float val = col0 + 16 * n < sh.dv && t0 + tok + e < len ? (float)vals[n][e] : 0.0f;
+        r[e] = val - f_eg[e] * acc[e];
+        qs[n][e] = sh.scale * f_eg[e] * aq[e];
+      }
+      put_half<3>(x_r + (lo * NC + n) * 3 * FRAG, FRAG, wave & 1, lane, r);
+    }
+    load_kq(next);
+    lds_barrier();
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      f32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        if (s <= lo) {
+          bf16x8 rf[3];
+          get_frag<3>(x_r + (s * NC + n) * 3 * FRAG, FRAG, lane, rf);
+          acc = mma_planes<3, 3, 3>(ta[s], rf, acc);
+        }
+      if (KEEP && col0 + 16 * n < sh.dvp) {
+        float* dp = w.delta + ((bh * sh.chunks + ch) * C + tok) * sh.dvp + col0 + 16 * n;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dp[(int64_t)e * sh.dvp] = acc[e];
+      }
+      const f32x4 vn = acc * f_beta;
+      put_half<NPO>(x_v + (lo * NC + n) * NPO * FRAG, FRAG, wave & 1, lane, vn);
+      put_half<3>(x_w + (lo * NC + n) * 3 * FRAG, FRAG, wave & 1, lane, vn * f_rest);
+    }
+    load_t(next);
+    lds_barrier();
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+#pragma unroll
+      for (int t = 0; t < MT; ++t) S[n][t] *= whole;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        bf16x8 wf[3], vf[NPO];
+        get_frag<3>(x_w + (s * NC + n) * 3 * FRAG, FRAG, lane, wf);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) S[n][t] = mma_planes<NPI, 3, 3>(kt[t][s], wf, S[n][t]);
+        if (s <= lo) {
+          get_frag<NPO>(x_v + (s * NC + n) * NPO * FRAG, FRAG, lane, vf);
+          qs[n] = mma_planes<NPO, NPO, NPO>(pa[s], vf, qs[n]);
+        }
+      }
+    }
+    load_kt(next);
+#pragma unroll
+    for (int n = 0; n < NC; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int64_t t = t0 + tok + e;
+        if (col0 + 16 * n < sh.dv && t < sh.time) op[t * o_stride + col0 + 16 * n] = (T)qs[n][e];
+      }
+  }
+#pragma unroll
+  for (int n = 0; n < NC; ++n) {
+    const int col = col0 + 16 * n;
+    if (col >= sh.dv) continue;
+    for (int64_t t = n_chunks * C + wave * 4 + quad; t < sh.time; t += 16) op[t * o_stride + col] = (T)0.0f;
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int row = row0 + 16 * t + r;
+        if (row < sh.dk) state[(bh * sh.dk + row) * sh.dv + col] = S[n][t][r];
+      }
+  }
+}
+
+template <typename T, int DKP, int NPI, int NC>
+__global__ void __launch_bounds__(TEAM, 1)
+    k_delta_scan_back(Shape sh, const T* __restrict__ d_o, const float* __restrict__ d_state, const int32_t* __restrict__ lengths,
+                      T* __restrict__ dv, float* __restrict__ d_state0, Work w) {
+  typedef KeyBlock<DKP, NPI> KB;
+  constexpr int KS = DKP / 32, MT = DKP / 64;
+  __shared__ bf16 x_s[KS * NC * 3 * FRAG], x_d[2 * NC * NPI * FRAG], x_g[2 * NC * 3 * FRAG], x_x[2 * NC * 3 * FRAG], x_e[2 * NC * 3 * FRAG];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quad = lane >> 4, c = lane & 15;
+  int64_t bh;
+  int tile;
+  const int tiles = (sh.dvp / 16 + NC - 1) / NC;
+  if (!scan_place(blockIdx.x, tiles, sh.batch * sh.heads, bh, tile)) return;
+  const int64_t b = bh / sh.heads;
+  const int h = (int)(bh % sh.heads), kh = h / sh.group;
+  const int col0 = tile * 16 * NC + c;
+  const int64_t len = length_of(lengths, b, sh.time), n_chunks = (len + C - 1) / C;
+  const bf16* keys = w.keys + (b * sh.kheads + kh) * sh.chunks * w.key_size;
+  const bf16* gates = w.gates + bh * sh.chunks * w.gate_size;
+  const float* rows = w.rows + bh * sh.chunks * ROWS;
+  const int64_t stride = (int64_t)sh.heads * sh.dv, base = ((b * sh.time) * sh.heads + h) * sh.dv;
+  const int row0 = 16 * MT * wave + 4 * quad, tok = 16 * wave + 4 * quad;
+  const int half = wave / 2;                      // first slab of this wave's rows of T^T and P^T
+
+  f32x4 S[NC][MT];
+#pragma unroll
+  for (int n = 0; n < NC; ++n) {
+    const int col = col0 + 16 * n;
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int row = row0 + 16 * t + r;
+        S[n][t][r] = d_state && col < sh.dv && row < sh.dk ? d_state[(bh * sh.dk + row) * sh.dv + col] : 0.0f;
+      }
+    if (col < sh.dv)
+      for (int64_t t = n_chunks * C + wave * 4 + quad; t < sh.time; t += 16) dv[base + t * stride + col] = (T)0.0f;
+  }
+
+  bf16x8 ka[KS][NPI], kt[MT][2][NPI], qt[MT][2][NPI], tt[2][3], pt[2][3];
+  f32x4 f_beta, f_eg, f_rest;
+  f32x4 whole;
+  T vals[NC][4];                                  // raw: converted and masked where they are used
+  auto load_o = [&](int64_t ch) {
+#pragma unroll
+    for (int n = 0; n < NC; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        vals[n][e] = d_o[base + std::min<int64_t>(ch * C + tok + e, len - 1) * stride + min(col0 + 16 * n, sh.dv - 1)];
+      }
+    f_eg = *(const f32x4*)(rows + ch * ROWS + C + tok);
+  };
+  auto load_k = [&](int64_t ch) {
+#pragma unroll
+    for (int s = 0; s < KS; ++s) load_frag<NPI>(keys + ch * w.key_size + KB::KA, wave * KS + s, 4 * KS * FRAG, lane, ka[s]);
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+      load_frag<3>(gates + ch * w.gate_size + GateBlock::PT, upper(wave, max(s, half)), 6 * FRAG, lane, pt[s]);
+    f_rest = *(const f32x4*)(rows + ch * ROWS + 2 * C + tok);
+  };
+  auto load_t = [&](int64_t ch) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+      load_frag<3>(gates + ch * w.gate_size + GateBlock::TT, upper(wave, max(s, half)), 6 * FRAG, lane, tt[s]);
+    f_beta = *(const f32x4*)(rows + ch * ROWS + tok);
+  };
+  auto load_cols = [&](int64_t ch) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        load_frag<NPI>(keys + ch * w.key_size + KB::KT, (wave * MT + t) * 2 + s, 2 * KS * 2 * FRAG, lane, kt[t][s]);
+        load_frag<NPI>(keys + ch * w.key_size + KB::QT, (wave * MT + t) * 2 + s, 2 * KS * 2 * FRAG, lane, qt[t][s]);
+      }
+    whole = *(const f32x4*)(rows + ch * ROWS + 3 * C + tok);      // a vector load: the scalar kind shares the LDS counter
+  };
+  if (n_chunks > 0) {
+    load_o(n_chunks - 1);
+    load_k(n_chunks - 1);
+    load_t(n_chunks - 1);
+    load_cols(n_chunks - 1);
+  }
+
+  for (int64_t ch = n_chunks - 1; ch >= 0; --ch) {
+    const int64_t next = ch > 0 ? ch - 1 : 0;
+    const int64_t t0 = ch * C, at = bh * sh.chunks + ch;
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        const int row_tile = wave * MT + t;
+        put_half<3>(x_s + ((row_tile / 2) * NC + n) * 3 * FRAG, FRAG, row_tile & 1, lane, S[n][t]);
+        if (col0 + 16 * n < sh.dvp) {
+          float* s1 = w.ds1 + (at * DKP + row0 + 16 * t) * sh.dvp + col0 + 16 * n;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s1[(int64_t)r * sh.dvp] = S[n][t][r];
+        }
+      }
+      f32x4 d;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) d[e] = col0 + 16 * n < sh.dv && t0 + tok + e < len ? (float)vals[n][e] : 0.0f;
+      put_half<NPI>(x_d + (half * NC + n) * NPI * FRAG, FRAG, wave & 1, lane, d);       // bf16 gradients are one plane
+      put_half<3>(x_g + (half * NC + n) * 3 * FRAG, FRAG, wave & 1, lane, d * f_eg * sh.scale);
+    }
+    const f32x4 eg = f_eg;
+    load_o(next);
+    lds_barrier();
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      f32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        bf16x8 sf[3];
+        get_frag<3>(x_s + (s * NC + n) * 3 * FRAG, FRAG, lane, sf);
+        acc = mma_planes<NPI, 3, 3>(ka[s], sf, acc);
+      }
+      acc *= f_rest;
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        if (s >= half) {
+          bf16x8 df[NPI];
+          get_frag<NPI>(x_d + (s * NC + n) * NPI * FRAG, FRAG, lane, df);
+          acc = mma_planes<3, NPI, 3>(pt[s], df, acc);
+        }
+      put_half<3>(x_x + (half * NC + n) * 3 * FRAG, FRAG, wave & 1, lane, acc);
+    }
+    load_k(next);
+    lds_barrier();
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      f32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        if (s >= half) {
+          bf16x8 xf[3];
+          get_frag<3>(x_x + (s * NC + n) * 3 * FRAG, FRAG, lane, xf);
+          acc = mma_planes<3, 3, 3>(tt[s], xf, acc);
+        }
+      const f32x4 be = acc * f_beta;
+      put_half<3>(x_e + (half * NC + n) * 3 * FRAG, FRAG, wave & 1, lane, -(be * eg));
+      const int col = col0 + 16 * n;
+      if (col < sh.dvp) {
+        float* ep = w.e + (at * C + tok) * sh.dvp + col;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ep[(int64_t)e * sh.dvp] = acc[e];
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int64_t t = t0 + tok + e;
+        if (col < sh.dv && t < sh.time) dv[base + t * stride + col] = (T)(t < len ? be[e] : 0.0f);
+      }
+    }
+    load_t(next);
+    lds_barrier();
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+#pragma unroll
+      for (int t = 0; t < MT; ++t) S[n][t] *= whole;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        bf16x8 gf[3], ef[3];
+        get_frag<3>(x_g + (s * NC + n) * 3 * FRAG, FRAG, lane, gf);
+        get_frag<3>(x_e + (s * NC + n) * 3 * FRAG, FRAG, lane, ef);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          S[n][t] = mma_planes<NPI, 3, 3>(qt[t][s], gf, S[n][t]);
+          S[n][t] = mma_planes<NPI, 3, 3>(kt[t][s], ef, S[n][t]);
+        }
+      }
+    }
+    load_cols(next);
+    lds_barrier();      // x_g is written again before the next chunk's first barrier
+  }
+  if (d_state0)
+#pragma unroll
+    for (int n = 0; n < NC; ++n)
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int row = row0 + 16 * t + r, col = col0 + 16 * n;
+          if (col < sh.dv && row < sh.dk) d_state0[(bh * sh.dk + row) * sh.dv + col] = S[n][t][r];
+        }
 }
 
 // ---------------------------------------------------------------------------
@@ -1022,7 +1158,13 @@ bool aligned_rows(const T* p, const int64_t (&s)[3]) {
   return ((uintptr_t)p & 15) == 0 && s[0] % per16 == 0 && s[1] % per16 == 0 && s[2] % per16 == 0;
 }
 
-unsigned scan_grid(const Shape& sh) { return (unsigned)(up(sh.batch * sh.heads, 8) * (sh.dvp / 16)); }
+// columns per workgroup of the scans, in tiles of 16: as few as leave every CU at most one workgroup (the walk over the
+// chunks is a chain, so more workgroups are faster until the 256 CUs are taken; then wider ones read each fragment once)
+int scan_tiles(const Shape& sh) {
+  const int64_t all = sh.batch * sh.heads * (sh.dvp / 16);
+  return all <= 256 ? 1 : (all <= 512 ? 2 : 4);
+}
+unsigned scan_grid(const Shape& sh, int nc) { return (unsigned)(up(sh.batch * sh.heads, 8) * (up(sh.dvp / 16, nc) / nc)); }
 
 template <typename T, int DKP, bool KEEP>
 int32_t run_filter(const Shape& sh, const T* q, const T* k, const T* v, const float* g, const float* beta, const float* state0,
@@ -1035,7 +1177,12 @@ int32_t run_filter(const Shape& sh, const T* q, const T* k, const T* v, const fl
         sh, q, k, g, beta, lengths, w, aligned_rows(q, sh.qs) && aligned_rows(k, sh.ks));
     GJX_LAUNCH_CHECK();
   }
-  k_delta_scan<T, DKP, NPI, KEEP><<<scan_grid(sh), 64, 0, s>>>(sh, v, state0, lengths, o, state, w);
+  const int nc = scan_tiles(sh);
+#define GJX_SCAN(NC) k_delta_scan<T, DKP, NPI, KEEP, NC><<<scan_grid(sh, NC), TEAM, 0, s>>>(sh, v, state0, lengths, o, state, w)
+  if (nc == 1) GJX_SCAN(1);
+  else if (nc == 2) GJX_SCAN(2);
+  else GJX_SCAN(4);
+#undef GJX_SCAN
   GJX_LAUNCH_CHECK();
   return GJX_OK;
 }
@@ -1044,7 +1191,13 @@ template <typename T, int DKP>
 int32_t run_grad(const Shape& sh, const T* q, const T* k, const float* g, const int32_t* lengths, const T* d_o, const float* d_state,
                  T* dq, T* dk, T* dv, float* dg, float* dbeta, float* d_state0, const Work& w, hipStream_t s) {
   constexpr int NPI = sizeof(T) == 4 ? 3 : 1;
-  k_delta_scan_back<T, DKP, NPI><<<scan_grid(sh), 64, 0, s>>>(sh, d_o, d_state, lengths, dv, d_state0, w);
+  const int nc = scan_tiles(sh);
+#define GJX_SCAN(NC) \
+  k_delta_scan_back<T, DKP, NPI, NC><<<scan_grid(sh, NC), TEAM, 0, s>>>(sh, d_o, d_state, lengths, dv, d_state0, w)
+  if (nc == 1) GJX_SCAN(1);
+  else if (nc == 2) GJX_SCAN(2);
+  else GJX_SCAN(4);
+#undef GJX_SCAN
   GJX_LAUNCH_CHECK();
   if (sh.chunks == 0) return GJX_OK;
   k_delta_back<T, DKP, NPI><<<(unsigned)(sh.batch * sh.heads * sh.chunks), 256, 0, s>>>(sh, q, k, d_o, g, lengths, dq, dk, dg, dbeta, w);
