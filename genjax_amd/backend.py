@@ -582,7 +582,8 @@ def _delta_shape(who, q, k, v, log_decay, beta, scale):
     _on_current_device(who, q=q, k=k, v=v, log_decay=log_decay, beta=beta)
     s = N.DeltaShape(dtype=ELEMENT_TYPES[q.dtype], kheads=kheads, heads=heads, dk=dk, dv=dv,
                      scale=float(dk ** -0.5 if scale is None else scale), batch=batch, time=time)
-    tensors = [t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous() for t in (q, k, v)] + [log_decay, beta]
+    fits = lambda t: (t.stride(-1) == 1 or t.shape[-1] <= 1) and t.stride(1) <= 1 << 22       # noqa: E731
+    tensors = [t if fits(t) else t.contiguous() for t in (q, k, v)] + [log_decay, beta]
     for name, t in zip("qkvgb", tensors):
         setattr(s, f"{name}_stride", (C.c_int64 * 3)(*t.stride()[:3]))
     return s, tensors

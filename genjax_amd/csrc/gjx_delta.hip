@@ -72,13 +72,20 @@ __device__ __forceinline__ f32x4 mma(bf16x8 a, bf16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-// f32 -> bf16 planes, exactly for P = 3.  What rounds to infinity in bf16 (above 3.39e38) counts as infinite: h alone.
+// f32 -> bf16 planes by cutting off (8 + 8 + 8 bits: exact for P = 3; nothing can overflow).  Cutting costs two
+// operations a plane where rounding takes four; what it leaves out of a product of two split values is at most 2^-21 of
+// it, 2^-23 on average.
 template <int P, int N>
 __device__ __forceinline__ void split_planes(float (&x)[N], int p, bf16 (&h)[N]) {
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    h[j] = (bf16)x[j];
-    if (p + 1 < P) x[j] = p == 0 && !(fabsf(x[j]) < 3.389e38f) ? 0.0f : x[j] - (float)h[j];
+    if (p + 1 < P || P == 3) {
+      const float top = __uint_as_float(__float_as_uint(x[j]) & 0xffff0000u);
+      h[j] = __builtin_bit_cast(bf16, (uint16_t)(__float_as_uint(x[j]) >> 16));
+      x[j] -= top;
+    } else {
+      h[j] = (bf16)x[j];             // the last of fewer than three planes is rounded
+    }
   }
 }
 
@@ -107,10 +114,40 @@ __device__ __forceinline__ f32x4 mma_planes(const bf16x8 (&a)[PA], const bf16x8 
   return acc;
 }
 
+// the same with one accumulator per order of magnitude: chains of dependent products a third as long
+template <int LIM>
+struct Orders {
+  f32x4 v[LIM];
+  __device__ __forceinline__ Orders() {
+#pragma unroll
+    for (int s = 0; s < LIM; ++s) v[s] = f32x4{0, 0, 0, 0};
+  }
+  template <int PA, int PB>
+  __device__ __forceinline__ void add(const bf16x8 (&a)[PA], const bf16x8 (&b)[PB]) {
+#pragma unroll
+    for (int s = LIM - 1; s >= 0; --s)
+#pragma unroll
+      for (int p = 0; p < PA; ++p)
+        if (s - p >= 0 && s - p < PB) v[s] = mma(a[p], b[s - p], v[s]);
+  }
+  __device__ __forceinline__ f32x4 sum() const {
+    f32x4 t = v[LIM - 1];
+#pragma unroll
+    for (int s = LIM - 2; s >= 0; --s) t += v[s];
+    return t;
+  }
+};
+
+// uniform base + 32-bit lane offset in bytes: one address register
+template <typename V>
+__device__ __forceinline__ V load_at(const void* base, uint32_t offset) { return *(const V*)((const char*)base + offset); }
+template <typename V>
+__device__ __forceinline__ void store_at(void* base, uint32_t offset, V v) { *(V*)((char*)base + offset) = v; }
+
 template <int P>
 __device__ __forceinline__ void load_frag(const bf16* base, int index, int plane, int lane, bf16x8 (&out)[P]) {
 #pragma unroll
-  for (int p = 0; p < P; ++p) out[p] = *(const bf16x8*)(base + p * plane + index * FRAG + lane * 8);
+  for (int p = 0; p < P; ++p) out[p] = load_at<bf16x8>(base + p * plane + index * FRAG, (uint32_t)lane * 16);
 }
 
 // two accumulator tiles (rows 16 (2 s) .. 16 (2 s + 2)) as the operand of slab s
@@ -228,13 +265,15 @@ __global__ void __launch_bounds__(256)
                     const float* __restrict__ beta, const int32_t* __restrict__ lengths, Work w, int vec) {
   constexpr int KS = DKP / 32, PITCH = DKP + 8, PLANE = C * PITCH;
   extern __shared__ char smem[];
-  bf16* sk = (bf16*)smem;
-  bf16* sq = sk + NPI * PLANE;
-  float* sn = (float*)(sq + NPI * PLANE);       // N
-  float* st = sn + C * LD;                      // That
-  float* sp = st + C * LD;                      // P, then T
-  float* s_gh = sp + C * LD;
+  // the rows of K and Q; N and That take their place once the products and the fragments are out, so that three
+  // workgroups fit a CU in bf16 (dk = 128; one at a time: 140 us for 2048 chunks)
+  float* s_gh = (float*)smem;
   float *s_gl = s_gh + C, *s_beta = s_gl + C;
+  float* sp = s_beta + C;                       // P, then T
+  bf16* sk = (bf16*)(sp + C * LD);
+  bf16* sq = sk + NPI * PLANE;
+  float* sn = (float*)sk;                       // N
+  float* st = sn + C * LD;                      // That
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, quad = lane >> 4, c = lane & 15;
   const int64_t chunk = blockIdx.x % sh.chunks, bh = blockIdx.x / sh.chunks, b = bh / sh.heads;
   const int h = (int)(bh % sh.heads), kh = h / sh.group;
@@ -267,10 +306,11 @@ __global__ void __launch_bounds__(256)
     rows[2 * C + lane] = expf((float)(last - gam));
     rows[3 * C + lane] = expf((float)last);
   }
-  for (int i = tid; i < C * LD; i += 256) st[i] = 0.0f;
   __syncthreads();
 
   // K K^T and Q K^T, row tile = wave
+  f32x4 nn[4];
+#pragma unroll
   for (int j = 0; j < 4; ++j) {
     f32x4 kk = {0, 0, 0, 0}, qk = {0, 0, 0, 0};
     if (j <= wave) {
@@ -291,7 +331,7 @@ __global__ void __launch_bounds__(256)
     for (int r = 0; r < 4; ++r) {
       const int i = 16 * wave + 4 * quad + r, jj = 16 * j + c;
       const float d = jj <= i ? expf((s_gh[i] - s_gh[jj]) + (s_gl[i] - s_gl[jj])) : 0.0f;
-      sn[i * LD + jj] = jj < i ? d * kk[r] : 0.0f;
+      nn[j][r] = jj < i ? d * kk[r] : 0.0f;
       sp[i * LD + jj] = jj <= i ? sh.scale * d * qk[r] : 0.0f;
     }
   }
@@ -302,6 +342,12 @@ __global__ void __launch_bounds__(256)
     store_col_frags<DKP, NPI>(sk, keys + KB::KT, tid);
     if (KEEP) store_col_frags<DKP, NPI>(sq, keys + KB::QT, tid);
   }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) sn[(16 * wave + 4 * quad + r) * LD + 16 * j + c] = nn[j][r];
+  for (int i = tid; i < C * LD; i += 256) st[i] = 0.0f;
   __syncthreads();
   store_triangle<false>(sp, gates + GateBlock::PA, tid);
   if (KEEP) store_triangle<true>(sp, gates + GateBlock::PT, tid);
@@ -338,7 +384,7 @@ __global__ void __launch_bounds__(256)
     __syncthreads();
   }
   store_triangle<false>(st, gates + GateBlock::TA, tid);
-  if (KEEP) {                          // T = I - beta That N, transposed
+  if (KEEP) {                          // T = I - beta That N, transposed (the barriers above end all reads of P)
     for (int j = 0; j < 4; ++j) {
       f32x4 acc = {0, 0, 0, 0};
       for (int l = j; l <= wave; ++l) acc = block_product(st, nullptr, sn, wave, l, j, lane, acc);
@@ -354,13 +400,17 @@ __global__ void __launch_bounds__(256)
 }
 
 // ---------------------------------------------------------------------------
-// the recursion: four waves share NC x 16 columns of S
+// the recursion: eight waves share NC x 16 columns of S
 // ---------------------------------------------------------------------------
-// Wave w owns the dk rows [w DKP / 4, (w + 1) DKP / 4) of S and the tokens [16 w, 16 w + 16) of a chunk.  What one wave
-// computes and the others multiply by (S, r, V', ...) goes through LDS in fragment order, three barriers a chunk; what a
-// wave takes from memory (its rows of K, Q, That, P, its rows of K^T) is used by no other wave, so it is loaded straight
-// into registers, each fragment for the next chunk as soon as it has been used for this one.
-constexpr int TEAM = 256;
+// Four waves carry the state, four take what hangs off the chain.  State wave w owns the dk rows [w DKP / 4, (w + 1)
+// DKP / 4) of S and the tokens [16 w, 16 w + 16) of a chunk; read-out wave w forms the outputs of the same tokens (in the
+// gradient: the products with dO alone, one chunk ahead).  What one wave computes and others multiply by (S, r, V', ...)
+// goes through LDS in fragment order, three barriers a chunk; what a wave takes from memory (its rows of K, Q, That, P,
+// its rows of K^T) is used by no other wave, so it is loaded straight into registers, each fragment for the next chunk as
+// soon as it has been used for this one.
+constexpr int TEAM = 512;
+// vmcnt(0) alone: with nothing in flight at the loop's entry, the waits inside it count the loop's own loads only
+constexpr int WAIT_VM = 0x0f70;
 
 // the workgroups of one head go to one XCD (workgroups go round the eight of them): they read the same fragments
 __device__ __forceinline__ bool scan_place(int64_t block, int tiles, int64_t heads, int64_t& bh, int& tile) {
@@ -374,49 +424,205 @@ __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(
 
 // four elements per lane of a 16-row tile -> its half of a slab's fragment planes
 template <int P>
-__device__ __forceinline__ void put_half(bf16* frag, int plane, int half, int lane, f32x4 x) {
+__device__ __forceinline__ void put_half(bf16* frag, int half, int lane, f32x4 x) {
   float r[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
   for (int p = 0; p < P; ++p) {
     bf16 h[4];
     split_planes<P, 4>(r, p, h);
-    *(bf16x4*)(frag + p * plane + lane * 8 + half * 4) = bf16x4{h[0], h[1], h[2], h[3]};
+    *(bf16x4*)(frag + p * FRAG + lane * 8 + half * 4) = bf16x4{h[0], h[1], h[2], h[3]};
   }
 }
 
 template <int P>
-__device__ __forceinline__ void get_frag(const bf16* frag, int plane, int lane, bf16x8 (&out)[P]) {
+__device__ __forceinline__ void get_frag(const bf16* frag, int lane, bf16x8 (&out)[P]) {
 #pragma unroll
-  for (int p = 0; p < P; ++p) out[p] = *(const bf16x8*)(frag + p * plane + lane * 8);
+  for (int p = 0; p < P; ++p) out[p] = *(const bf16x8*)(frag + p * FRAG + lane * 8);
+}
+
+// what every wave of a scan knows of its place
+struct Place {
+  int64_t bh, b, len, n_chunks;
+  int h, kh, tile, lane, wave, quad, c, col0, tok;
+  bool reads;                    // a read-out wave
+};
+
+template <int NC>
+__device__ __forceinline__ bool place_of(const Shape& sh, const int32_t* lengths, Place& p) {
+  p.lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  p.wave = w & 3;
+  p.reads = w >= 4;
+  p.quad = p.lane >> 4;
+  p.c = p.lane & 15;
+  if (!scan_place(blockIdx.x, (sh.dvp / 16 + NC - 1) / NC, sh.batch * sh.heads, p.bh, p.tile)) return false;
+  p.b = p.bh / sh.heads;
+  p.h = (int)(p.bh % sh.heads);
+  p.kh = p.h / sh.group;
+  p.col0 = p.tile * 16 * NC + p.c;
+  p.tok = 16 * p.wave + 4 * p.quad;
+  p.len = length_of(lengths, p.b, sh.time);
+  p.n_chunks = (p.len + C - 1) / C;
+  return true;
+}
+
+// where a chunk's operands lie; step() stays inside the sequence
+struct Cursor {
+  const bf16 *keys, *gates;
+  const float* rows;
+  int64_t ch;
+  __device__ __forceinline__ Cursor(const bf16* k, const bf16* g, const float* r, const Work& w, int64_t c)
+      : keys(k + c * w.key_size), gates(g + c * w.gate_size), rows(r + c * ROWS), ch(c) {}
+  __device__ __forceinline__ int left(const Place& p) const { return (int)std::min<int64_t>(C, p.len - ch * C); }
+  __device__ __forceinline__ Cursor step(const Work& w, int d, const Place& p) const {
+    Cursor n = *this;
+    if (d > 0 ? ch + 1 < p.n_chunks : ch > 0) {
+      n.keys += d * w.key_size;
+      n.gates += d * w.gate_size;
+      n.rows += d * ROWS;
+      n.ch += d;
+    }
+    return n;
+  }
+};
+
+// this lane's four tokens of a (batch, time, head, dv) column block: raw values, converted and masked where they are used
+template <typename T, int NC>
+struct Columns {
+  uint32_t step, row[4], col[NC];
+  T raw[NC][4];
+  __device__ __forceinline__ Columns(const Shape& sh, const Place& p, int64_t token_stride) : step((uint32_t)token_stride * sizeof(T)) {
+#pragma unroll
+    for (int n = 0; n < NC; ++n) col[n] = (uint32_t)min(p.col0 + 16 * n, sh.dv - 1) * sizeof(T);
+  }
+  __device__ __forceinline__ void load(const T* chunk, const Place& p, int left) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) row[e] = (uint32_t)(left < C ? min(p.tok + e, left - 1) : p.tok + e) * step;
+#pragma unroll
+    for (int n = 0; n < NC; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) raw[n][e] = load_at<T>(chunk, row[e] + col[n]);
+  }
+  __device__ __forceinline__ f32x4 get(const Shape& sh, const Place& p, int n, int left) const {
+    f32x4 x;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = p.col0 + 16 * n < sh.dv && p.tok + e < left ? (float)raw[n][e] : 0.0f;
+    return x;
+  }
+};
+
+// f32 rows [row, row + 4) x this lane's column of a (rows, dvp) block
+__device__ __forceinline__ void store_rows(float* block, int row, int col, int pitch, f32x4 x) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r) store_at(block, (uint32_t)((row + r) * pitch + col) * 4, x[r]);
+}
+
+template <typename T>
+__device__ __forceinline__ void store_tokens(T* chunk, const Place& p, int col, uint32_t step, bool all, int dv, int left, f32x4 x) {
+  const uint32_t at = (uint32_t)p.tok * step + (uint32_t)col * sizeof(T);
+  if (all) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) store_at(chunk, at + e * step, (T)x[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (col < dv && p.tok + e < left) store_at(chunk, at + e * step, (T)x[e]);
+  }
 }
 
 template <typename T, int DKP, int NPI, bool KEEP, int NC>
-__global__ void __launch_bounds__(TEAM, 1)
+__global__ void __launch_bounds__(TEAM, 2)
     k_delta_scan(Shape sh, const T* __restrict__ v, const float* __restrict__ state0, const int32_t* __restrict__ lengths,
                  T* __restrict__ o, float* __restrict__ state, Work w) {
   typedef KeyBlock<DKP, NPI> KB;
   constexpr int KS = DKP / 32, MT = DKP / 64;     // slabs of S; 16-row tiles of S per wave
   constexpr int NPO = NPI == 1 ? 2 : 3;           // planes of what only the read-out takes
-  __shared__ bf16 x_s[KS * NC * 3 * FRAG], x_r[2 * NC * 3 * FRAG], x_v[2 * NC * NPO * FRAG], x_w[2 * NC * 3 * FRAG];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quad = lane >> 4, c = lane & 15;
-  int64_t bh;
-  int tile;
-  const int tiles = (sh.dvp / 16 + NC - 1) / NC;
-  if (!scan_place(blockIdx.x, tiles, sh.batch * sh.heads, bh, tile)) return;
-  const int64_t b = bh / sh.heads;
-  const int h = (int)(bh % sh.heads), kh = h / sh.group;
-  const int col0 = tile * 16 * NC + c;
-  const int64_t len = length_of(lengths, b, sh.time), n_chunks = (len + C - 1) / C;
-  const bf16* keys = w.keys + (b * sh.kheads + kh) * sh.chunks * w.key_size;
-  const bf16* gates = w.gates + bh * sh.chunks * w.gate_size;
-  const float* rows = w.rows + bh * sh.chunks * ROWS;
-  const T* vp = v + b * sh.vs[0] + h * sh.vs[2];
-  T* op = o + ((b * sh.time) * sh.heads + h) * sh.dv;
-  const int64_t o_stride = (int64_t)sh.heads * sh.dv;
-  const int row0 = 16 * MT * wave + 4 * quad;     // first of this lane's rows of S
-  const int tok = 16 * wave + 4 * quad;           // ... and tokens of a chunk
+  __shared__ bf16 x_s[KS * NC * 3 * FRAG], x_r[2 * NC * 3 * FRAG], x_v[2][2 * NC * NPO * FRAG], x_w[2 * NC * 3 * FRAG];
+  Place p;
+  if (!place_of<NC>(sh, lengths, p)) return;
+  const int lane = p.lane, wave = p.wave, tok = p.tok;
+  const bf16* keys = w.keys + (p.b * sh.kheads + p.kh) * sh.chunks * w.key_size;
+  const bf16* gates = w.gates + p.bh * sh.chunks * w.gate_size;
+  const float* rows = w.rows + p.bh * sh.chunks * ROWS;
   const int lo = wave / 2;                        // last slab of this wave's rows of That and P
 
+  if (p.reads) {
+    T* op = o + (p.b * sh.time * sh.heads + p.h) * sh.dv;
+    const int64_t o_stride = (int64_t)sh.heads * sh.dv;
+    const bool all_cols = p.tile * 16 * NC + 16 * NC <= sh.dv;
+    bf16x8 qa[KS][NPI], pa[2][NPO];
+    f32x4 f_eg;
+    auto load_q = [&](const Cursor& at) {
+#pragma unroll
+      for (int s = 0; s < KS; ++s) load_frag<NPI>(at.keys + KB::QA, wave * KS + s, 4 * KS * FRAG, lane, qa[s]);
+      f_eg = load_at<f32x4>(at.rows + C, (uint32_t)tok * 4);
+    };
+    auto load_p = [&](const Cursor& at) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        load_frag<NPO>(at.gates + GateBlock::PA, lower(wave, min(s, lo)), 6 * FRAG, lane, pa[s]);
+    };
+    Cursor next(keys, gates, rows, w, 0);
+    if (p.n_chunks > 0) {
+      load_q(next);
+      load_p(next);
+      __builtin_amdgcn_s_waitcnt(WAIT_VM);
+    }
+    // a chunk's outputs are finished while the state waves are at the next chunk's That r: nobody waits for them
+    f32x4 qs[NC];
+    auto finish = [&](int64_t ch) {
+      const int left = (int)std::min<int64_t>(C, sh.time - ch * C);
+#pragma unroll
+      for (int n = 0; n < NC; ++n) {
+        Orders<NPO> acc;
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+          if (s <= lo) {
+            bf16x8 vf[NPO];
+            get_frag<NPO>(x_v[ch & 1] + (s * NC + n) * NPO * FRAG, lane, vf);
+            acc.add(pa[s], vf);
+          }
+        store_tokens(op + ch * C * o_stride, p, p.col0 + 16 * n, (uint32_t)o_stride * sizeof(T), all_cols && left == C, sh.dv, left,
+                     qs[n] + acc.sum());
+      }
+    };
+    for (int64_t ch = 0; ch < p.n_chunks; ++ch) {
+      const Cursor here = next;
+      next = next.step(w, 1, p);
+      lds_barrier();
+      f32x4 now[NC];
+#pragma unroll
+      for (int n = 0; n < NC; ++n) {
+        Orders<NPO> acc;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          bf16x8 sf[NPO];
+          get_frag<NPO>(x_s + (s * NC + n) * 3 * FRAG, lane, sf);
+          acc.add(qa[s], sf);
+        }
+        now[n] = acc.sum() * f_eg * sh.scale;
+      }
+      load_q(next);
+      lds_barrier();
+      if (ch > 0) {
+        finish(ch - 1);
+        load_p(here);
+      }
+#pragma unroll
+      for (int n = 0; n < NC; ++n) qs[n] = now[n];
+      lds_barrier();
+    }
+    if (p.n_chunks > 0) finish(p.n_chunks - 1);
+#pragma unroll
+    for (int n = 0; n < NC; ++n)
+      if (p.col0 + 16 * n < sh.dv)
+        for (int64_t t = p.n_chunks * C + wave * 4 + p.quad; t < sh.time; t += 16) op[t * o_stride + p.col0 + 16 * n] = (T)0.0f;
+    return;
+  }
+
+  __builtin_amdgcn_s_setprio(3);                  // ahead of the read-out wave on the same SIMD
+  const T* vp = v + p.b * sh.vs[0] + p.h * sh.vs[2];
+  const int row0 = 16 * MT * wave + 4 * p.quad;   // first of this lane's rows of S
   f32x4 S[NC][MT];
 #pragma unroll
   for (int n = 0; n < NC; ++n)
@@ -424,321 +630,319 @@ __global__ void __launch_bounds__(TEAM, 1)
     for (int t = 0; t < MT; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int row = row0 + 16 * t + r, col = col0 + 16 * n;
-        S[n][t][r] = state0 && col < sh.dv && row < sh.dk ? state0[(bh * sh.dk + row) * sh.dv + col] : 0.0f;
+        const int row = row0 + 16 * t + r, col = p.col0 + 16 * n;
+        S[n][t][r] = state0 && col < sh.dv && row < sh.dk ? state0[(p.bh * sh.dk + row) * sh.dv + col] : 0.0f;
       }
-
-  bf16x8 ka[KS][NPI], qa[KS][NPI], kt[MT][2][NPI], ta[2][3], pa[2][NPO];
-  f32x4 f_beta, f_eg, f_rest;
-  f32x4 whole;
-  T vals[NC][4];                                  // raw: converted and masked where they are used
-  auto load_kq = [&](int64_t ch) {
+  bf16x8 ka[KS][NPI], kt[MT][2][NPI], ta[2][3];
+  f32x4 f_beta, f_eg, f_rest, whole;
+  Columns<T, NC> vals(sh, p, sh.vs[1]);
+  auto load_k = [&](const Cursor& at) {
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      load_frag<NPI>(keys + ch * w.key_size + KB::KA, wave * KS + s, 4 * KS * FRAG, lane, ka[s]);
-      load_frag<NPI>(keys + ch * w.key_size + KB::QA, wave * KS + s, 4 * KS * FRAG, lane, qa[s]);
-    }
+    for (int s = 0; s < KS; ++s) load_frag<NPI>(at.keys + KB::KA, wave * KS + s, 4 * KS * FRAG, lane, ka[s]);
+    vals.load(vp + at.ch * C * sh.vs[1], p, at.left(p));
+    f_eg = load_at<f32x4>(at.rows + C, (uint32_t)tok * 4);
+  };
+  auto load_t = [&](const Cursor& at) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+      load_frag<3>(at.gates + GateBlock::TA, lower(wave, min(s, lo)), 6 * FRAG, lane, ta[s]);
+    f_beta = load_at<f32x4>(at.rows, (uint32_t)tok * 4);
+    f_rest = load_at<f32x4>(at.rows + 2 * C, (uint32_t)tok * 4);
+  };
+  auto load_kt = [&](const Cursor& at) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+        load_frag<NPI>(at.keys + KB::KT, (wave * MT + t) * 2 + s, 2 * KS * 2 * FRAG, lane, kt[t][s]);
+    whole = load_at<f32x4>(at.rows + 3 * C, (uint32_t)tok * 4);     // a vector load: the scalar kind shares the LDS counter
+  };
+  Cursor next(keys, gates, rows, w, 0);
+  if (p.n_chunks > 0) {
+    load_k(next);
+    load_t(next);
+    load_kt(next);
+    __builtin_amdgcn_s_waitcnt(WAIT_VM);
+  }
+  for (int64_t ch = 0; ch < p.n_chunks; ++ch) {
+    const int left = (int)std::min<int64_t>(C, p.len - ch * C);
+    next = next.step(w, 1, p);
 #pragma unroll
     for (int n = 0; n < NC; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        vals[n][e] = vp[std::min<int64_t>(ch * C + tok + e, len - 1) * sh.vs[1] + min(col0 + 16 * n, sh.dv - 1)];
-      }
-    f_eg = *(const f32x4*)(rows + ch * ROWS + C + tok);
-  };
-  auto load_t = [&](int64_t ch) {
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-      load_frag<3>(gates + ch * w.gate_size + GateBlock::TA, lower(wave, min(s, lo)), 6 * FRAG, lane, ta[s]);
-    f_beta = *(const f32x4*)(rows + ch * ROWS + tok);
-    f_rest = *(const f32x4*)(rows + ch * ROWS + 2 * C + tok);
-  };
-  auto load_kt = [&](int64_t ch) {
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      load_frag<NPO>(gates + ch * w.gate_size + GateBlock::PA, lower(wave, min(s, lo)), 6 * FRAG, lane, pa[s]);
-#pragma unroll
       for (int t = 0; t < MT; ++t)
-        load_frag<NPI>(keys + ch * w.key_size + KB::KT, (wave * MT + t) * 2 + s, 2 * KS * 2 * FRAG, lane, kt[t][s]);
-    }
-    whole = *(const f32x4*)(rows + ch * ROWS + 3 * C + tok);      // a vector load: the scalar kind shares the LDS counter
-  };
-  if (n_chunks > 0) {
-    load_kq(0);
-    load_t(0);
-    load_kt(0);
-  }
-
-  for (int64_t ch = 0; ch < n_chunks; ++ch) {
-    const int64_t next = ch + 1 < n_chunks ? ch + 1 : ch;
-    const int64_t t0 = ch * C;
-#pragma unroll
-    for (int n = 0; n < NC; ++n) {
-#pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        const int row_tile = wave * MT + t;
-        put_half<3>(x_s + ((row_tile / 2) * NC + n) * 3 * FRAG, FRAG, row_tile & 1, lane, S[n][t]);
-        if (KEEP && col0 + 16 * n < sh.dvp) {
-          float* s0 = w.s0 + ((bh * sh.chunks + ch) * DKP + row0 + 16 * t) * sh.dvp + col0 + 16 * n;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) s0[(int64_t)r * sh.dvp] = S[n][t][r];
-        }
-      }
-    }
+        put_half<3>(x_s + (((wave * MT + t) / 2) * NC + n) * 3 * FRAG, (wave * MT + t) & 1, lane, S[n][t]);
     lds_barrier();
-    f32x4 qs[NC];
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
-      f32x4 acc = {0, 0, 0, 0}, aq = {0, 0, 0, 0}, r;
+      Orders<3> acc;
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         bf16x8 sf[3];
-        get_frag<3>(x_s + (s * NC + n) * 3 * FRAG, FRAG, lane, sf);
-        acc = mma_planes<NPI, 3, 3>(ka[s], sf, acc);
-        aq = mma_planes<NPI, 3, NPO>(qa[s], sf, aq);
+        get_frag<3>(x_s + (s * NC + n) * 3 * FRAG, lane, sf);
+        acc.add(ka[s], sf);
       }
+      put_half<3>(x_r + (lo * NC + n) * 3 * FRAG, wave & 1, lane, vals.get(sh, p, n, left) - f_eg * acc.sum());
+      if (KEEP && p.col0 + 16 * n < sh.dvp)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float val = col0 + 16 * n < sh.dv && t0 + tok + e < len ? (float)vals[n][e] : 0.0f;
-        r[e] = val - f_eg[e] * acc[e];
-        qs[n][e] = sh.scale * f_eg[e] * aq[e];
-      }
-      put_half<3>(x_r + (lo * NC + n) * 3 * FRAG, FRAG, wave & 1, lane, r);
+        for (int t = 0; t < MT; ++t)
+          store_rows(w.s0 + (p.bh * sh.chunks + ch) * DKP * sh.dvp, row0 + 16 * t, p.col0 + 16 * n, sh.dvp, S[n][t]);
     }
-    load_kq(next);
     lds_barrier();
+    load_k(next);                // behind the barrier: issued while the first LDS reads are on their way
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
-      f32x4 acc = {0, 0, 0, 0};
+      Orders<3> acc;
 #pragma unroll
       for (int s = 0; s < 2; ++s)
         if (s <= lo) {
           bf16x8 rf[3];
-          get_frag<3>(x_r + (s * NC + n) * 3 * FRAG, FRAG, lane, rf);
-          acc = mma_planes<3, 3, 3>(ta[s], rf, acc);
+          get_frag<3>(x_r + (s * NC + n) * 3 * FRAG, lane, rf);
+          acc.add(ta[s], rf);
         }
-      if (KEEP && col0 + 16 * n < sh.dvp) {
-        float* dp = w.delta + ((bh * sh.chunks + ch) * C + tok) * sh.dvp + col0 + 16 * n;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) dp[(int64_t)e * sh.dvp] = acc[e];
-      }
-      const f32x4 vn = acc * f_beta;
-      put_half<NPO>(x_v + (lo * NC + n) * NPO * FRAG, FRAG, wave & 1, lane, vn);
-      put_half<3>(x_w + (lo * NC + n) * 3 * FRAG, FRAG, wave & 1, lane, vn * f_rest);
+      const f32x4 delta = acc.sum(), vn = delta * f_beta;
+      put_half<3>(x_w + (lo * NC + n) * 3 * FRAG, wave & 1, lane, vn * f_rest);
+      put_half<NPO>(x_v[ch & 1] + (lo * NC + n) * NPO * FRAG, wave & 1, lane, vn);
+      if (KEEP && p.col0 + 16 * n < sh.dvp)
+        store_rows(w.delta + (p.bh * sh.chunks + ch) * C * sh.dvp, tok, p.col0 + 16 * n, sh.dvp, delta);
     }
-    load_t(next);
     lds_barrier();
+    load_t(next);
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
+      Orders<3> acc[MT];
 #pragma unroll
-      for (int t = 0; t < MT; ++t) S[n][t] *= whole;
+      for (int t = 0; t < MT; ++t) acc[t].v[0] = S[n][t] * whole;
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        bf16x8 wf[3], vf[NPO];
-        get_frag<3>(x_w + (s * NC + n) * 3 * FRAG, FRAG, lane, wf);
+        bf16x8 wf[3];
+        get_frag<3>(x_w + (s * NC + n) * 3 * FRAG, lane, wf);
 #pragma unroll
-        for (int t = 0; t < MT; ++t) S[n][t] = mma_planes<NPI, 3, 3>(kt[t][s], wf, S[n][t]);
-        if (s <= lo) {
-          get_frag<NPO>(x_v + (s * NC + n) * NPO * FRAG, FRAG, lane, vf);
-          qs[n] = mma_planes<NPO, NPO, NPO>(pa[s], vf, qs[n]);
-        }
+        for (int t = 0; t < MT; ++t) acc[t].add(kt[t][s], wf);
       }
+#pragma unroll
+      for (int t = 0; t < MT; ++t) S[n][t] = acc[t].sum();
     }
     load_kt(next);
-#pragma unroll
-    for (int n = 0; n < NC; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int64_t t = t0 + tok + e;
-        if (col0 + 16 * n < sh.dv && t < sh.time) op[t * o_stride + col0 + 16 * n] = (T)qs[n][e];
-      }
   }
 #pragma unroll
-  for (int n = 0; n < NC; ++n) {
-    const int col = col0 + 16 * n;
-    if (col >= sh.dv) continue;
-    for (int64_t t = n_chunks * C + wave * 4 + quad; t < sh.time; t += 16) op[t * o_stride + col] = (T)0.0f;
+  for (int n = 0; n < NC; ++n)
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int row = row0 + 16 * t + r;
-        if (row < sh.dk) state[(bh * sh.dk + row) * sh.dv + col] = S[n][t][r];
+        const int row = row0 + 16 * t + r, col = p.col0 + 16 * n;
+        if (col < sh.dv && row < sh.dk) state[(p.bh * sh.dk + row) * sh.dv + col] = S[n][t][r];
       }
-  }
 }
 
 template <typename T, int DKP, int NPI, int NC>
-__global__ void __launch_bounds__(TEAM, 1)
+__global__ void __launch_bounds__(TEAM, 2)
     k_delta_scan_back(Shape sh, const T* __restrict__ d_o, const float* __restrict__ d_state, const int32_t* __restrict__ lengths,
                       T* __restrict__ dv, float* __restrict__ d_state0, Work w) {
   typedef KeyBlock<DKP, NPI> KB;
   constexpr int KS = DKP / 32, MT = DKP / 64;
+  // the read-out waves' P^T dO (x_p) and Q^T (scale e^gamma dO) (x_q) as accumulators of the state waves, in f32
   __shared__ bf16 x_s[KS * NC * 3 * FRAG], x_d[2 * NC * NPI * FRAG], x_g[2 * NC * 3 * FRAG], x_x[2 * NC * 3 * FRAG], x_e[2 * NC * 3 * FRAG];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quad = lane >> 4, c = lane & 15;
-  int64_t bh;
-  int tile;
-  const int tiles = (sh.dvp / 16 + NC - 1) / NC;
-  if (!scan_place(blockIdx.x, tiles, sh.batch * sh.heads, bh, tile)) return;
-  const int64_t b = bh / sh.heads;
-  const int h = (int)(bh % sh.heads), kh = h / sh.group;
-  const int col0 = tile * 16 * NC + c;
-  const int64_t len = length_of(lengths, b, sh.time), n_chunks = (len + C - 1) / C;
-  const bf16* keys = w.keys + (b * sh.kheads + kh) * sh.chunks * w.key_size;
-  const bf16* gates = w.gates + bh * sh.chunks * w.gate_size;
-  const float* rows = w.rows + bh * sh.chunks * ROWS;
-  const int64_t stride = (int64_t)sh.heads * sh.dv, base = ((b * sh.time) * sh.heads + h) * sh.dv;
-  const int row0 = 16 * MT * wave + 4 * quad, tok = 16 * wave + 4 * quad;
+  __shared__ f32x4 x_p[4 * NC * 64], x_q[4 * MT * NC * 64];
+  Place p;
+  if (!place_of<NC>(sh, lengths, p)) return;
+  const int lane = p.lane, wave = p.wave, tok = p.tok;
+  const bf16* keys = w.keys + (p.b * sh.kheads + p.kh) * sh.chunks * w.key_size;
+  const bf16* gates = w.gates + p.bh * sh.chunks * w.gate_size;
+  const float* rows = w.rows + p.bh * sh.chunks * ROWS;
+  const int64_t stride = (int64_t)sh.heads * sh.dv, base = (p.b * sh.time * sh.heads + p.h) * sh.dv;
   const int half = wave / 2;                      // first slab of this wave's rows of T^T and P^T
 
+  if (p.reads) {
+    bf16x8 qt[MT][2][NPI], pt[2][3];
+    f32x4 f_eg;
+    Columns<T, NC> vals(sh, p, stride);
+    auto load_o = [&](const Cursor& at) {
+      vals.load(d_o + base + at.ch * C * stride, p, at.left(p));
+      f_eg = load_at<f32x4>(at.rows + C, (uint32_t)tok * 4);
+    };
+    auto load_qp = [&](const Cursor& at) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        load_frag<3>(at.gates + GateBlock::PT, upper(wave, max(s, half)), 6 * FRAG, lane, pt[s]);
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+          load_frag<NPI>(at.keys + KB::QT, (wave * MT + t) * 2 + s, 2 * KS * 2 * FRAG, lane, qt[t][s]);
+      }
+    };
+    // a chunk's dO into fragments, then the two products: step `ch` runs between the state waves' barriers of chunk ch + 1
+    auto put_o = [&](const Cursor& at) {
+      const int left = at.left(p);
+#pragma unroll
+      for (int n = 0; n < NC; ++n) {
+        const f32x4 d = vals.get(sh, p, n, left);
+        put_half<NPI>(x_d + (half * NC + n) * NPI * FRAG, wave & 1, lane, d);       // bf16 gradients are one plane
+        put_half<3>(x_g + (half * NC + n) * 3 * FRAG, wave & 1, lane, d * f_eg * sh.scale);
+      }
+      load_o(at.step(w, -1, p));
+    };
+    f32x4 rp[NC], rq[NC][MT];
+    auto products = [&](const Cursor& at) {
+#pragma unroll
+      for (int n = 0; n < NC; ++n) {
+        Orders<3> acc, aq[MT];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          bf16x8 df[NPI], gf[3];
+          get_frag<NPI>(x_d + (s * NC + n) * NPI * FRAG, lane, df);
+          get_frag<3>(x_g + (s * NC + n) * 3 * FRAG, lane, gf);
+          if (s >= half) acc.add(pt[s], df);
+#pragma unroll
+          for (int t = 0; t < MT; ++t) aq[t].add(qt[t][s], gf);
+        }
+        rp[n] = acc.sum();
+#pragma unroll
+        for (int t = 0; t < MT; ++t) rq[n][t] = aq[t].sum();
+      }
+      load_qp(at.step(w, -1, p));
+    };
+    auto hand_over = [&]() {
+#pragma unroll
+      for (int n = 0; n < NC; ++n) {
+        x_p[(wave * NC + n) * 64 + lane] = rp[n];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) x_q[((wave * MT + t) * NC + n) * 64 + lane] = rq[n][t];
+      }
+    };
+    Cursor now(keys, gates, rows, w, std::max<int64_t>(p.n_chunks, 1) - 1);
+    if (p.n_chunks > 0) {
+      load_o(now);
+      load_qp(now);
+      __builtin_amdgcn_s_waitcnt(WAIT_VM);
+      put_o(now);
+    }
+    lds_barrier();
+    if (p.n_chunks > 0) products(now);
+    for (int64_t ch = p.n_chunks - 1; ch >= 0; --ch) {
+      hand_over();               // read by the state waves between barriers one and two (x_p) and behind three (x_q)
+      now = now.step(w, -1, p);
+      lds_barrier();
+      if (ch > 0) put_o(now);
+      lds_barrier();
+      if (ch > 0) products(now);
+      lds_barrier();
+      lds_barrier();
+    }
+    return;
+  }
+
+  __builtin_amdgcn_s_setprio(3);
+  const int row0 = 16 * MT * wave + 4 * p.quad;
+  const bool all_cols = p.tile * 16 * NC + 16 * NC <= sh.dv;
   f32x4 S[NC][MT];
 #pragma unroll
   for (int n = 0; n < NC; ++n) {
-    const int col = col0 + 16 * n;
+    const int col = p.col0 + 16 * n;
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int row = row0 + 16 * t + r;
-        S[n][t][r] = d_state && col < sh.dv && row < sh.dk ? d_state[(bh * sh.dk + row) * sh.dv + col] : 0.0f;
+        S[n][t][r] = d_state && col < sh.dv && row < sh.dk ? d_state[(p.bh * sh.dk + row) * sh.dv + col] : 0.0f;
       }
     if (col < sh.dv)
-      for (int64_t t = n_chunks * C + wave * 4 + quad; t < sh.time; t += 16) dv[base + t * stride + col] = (T)0.0f;
+      for (int64_t t = p.n_chunks * C + wave * 4 + p.quad; t < sh.time; t += 16) dv[base + t * stride + col] = (T)0.0f;
   }
-
-  bf16x8 ka[KS][NPI], kt[MT][2][NPI], qt[MT][2][NPI], tt[2][3], pt[2][3];
-  f32x4 f_beta, f_eg, f_rest;
-  f32x4 whole;
-  T vals[NC][4];                                  // raw: converted and masked where they are used
-  auto load_o = [&](int64_t ch) {
+  bf16x8 ka[KS][NPI], kt[MT][2][NPI], tt[2][3];
+  f32x4 f_beta, f_eg, f_rest, whole;
+  auto load_k = [&](const Cursor& at) {
+#pragma unroll
+    for (int s = 0; s < KS; ++s) load_frag<NPI>(at.keys + KB::KA, wave * KS + s, 4 * KS * FRAG, lane, ka[s]);
+    f_rest = load_at<f32x4>(at.rows + 2 * C, (uint32_t)tok * 4);
+  };
+  auto load_t = [&](const Cursor& at) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+      load_frag<3>(at.gates + GateBlock::TT, upper(wave, max(s, half)), 6 * FRAG, lane, tt[s]);
+    f_beta = load_at<f32x4>(at.rows, (uint32_t)tok * 4);
+    f_eg = load_at<f32x4>(at.rows + C, (uint32_t)tok * 4);
+  };
+  auto load_kt = [&](const Cursor& at) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+        load_frag<NPI>(at.keys + KB::KT, (wave * MT + t) * 2 + s, 2 * KS * 2 * FRAG, lane, kt[t][s]);
+    whole = load_at<f32x4>(at.rows + 3 * C, (uint32_t)tok * 4);
+  };
+  Cursor next(keys, gates, rows, w, std::max<int64_t>(p.n_chunks, 1) - 1);
+  if (p.n_chunks > 0) {
+    load_k(next);
+    load_t(next);
+    load_kt(next);
+    __builtin_amdgcn_s_waitcnt(WAIT_VM);
+  }
+  lds_barrier();
+  for (int64_t ch = p.n_chunks - 1; ch >= 0; --ch) {
+    const int64_t at = p.bh * sh.chunks + ch;
+    const int left = (int)std::min<int64_t>(C, p.len - ch * C), left_o = (int)std::min<int64_t>(C, sh.time - ch * C);
+    next = next.step(w, -1, p);
 #pragma unroll
     for (int n = 0; n < NC; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        vals[n][e] = d_o[base + std::min<int64_t>(ch * C + tok + e, len - 1) * stride + min(col0 + 16 * n, sh.dv - 1)];
-      }
-    f_eg = *(const f32x4*)(rows + ch * ROWS + C + tok);
-  };
-  auto load_k = [&](int64_t ch) {
-#pragma unroll
-    for (int s = 0; s < KS; ++s) load_frag<NPI>(keys + ch * w.key_size + KB::KA, wave * KS + s, 4 * KS * FRAG, lane, ka[s]);
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-      load_frag<3>(gates + ch * w.gate_size + GateBlock::PT, upper(wave, max(s, half)), 6 * FRAG, lane, pt[s]);
-    f_rest = *(const f32x4*)(rows + ch * ROWS + 2 * C + tok);
-  };
-  auto load_t = [&](int64_t ch) {
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-      load_frag<3>(gates + ch * w.gate_size + GateBlock::TT, upper(wave, max(s, half)), 6 * FRAG, lane, tt[s]);
-    f_beta = *(const f32x4*)(rows + ch * ROWS + tok);
-  };
-  auto load_cols = [&](int64_t ch) {
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        load_frag<NPI>(keys + ch * w.key_size + KB::KT, (wave * MT + t) * 2 + s, 2 * KS * 2 * FRAG, lane, kt[t][s]);
-        load_frag<NPI>(keys + ch * w.key_size + KB::QT, (wave * MT + t) * 2 + s, 2 * KS * 2 * FRAG, lane, qt[t][s]);
-      }
-    whole = *(const f32x4*)(rows + ch * ROWS + 3 * C + tok);      // a vector load: the scalar kind shares the LDS counter
-  };
-  if (n_chunks > 0) {
-    load_o(n_chunks - 1);
-    load_k(n_chunks - 1);
-    load_t(n_chunks - 1);
-    load_cols(n_chunks - 1);
-  }
-
-  for (int64_t ch = n_chunks - 1; ch >= 0; --ch) {
-    const int64_t next = ch > 0 ? ch - 1 : 0;
-    const int64_t t0 = ch * C, at = bh * sh.chunks + ch;
-#pragma unroll
-    for (int n = 0; n < NC; ++n) {
-#pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        const int row_tile = wave * MT + t;
-        put_half<3>(x_s + ((row_tile / 2) * NC + n) * 3 * FRAG, FRAG, row_tile & 1, lane, S[n][t]);
-        if (col0 + 16 * n < sh.dvp) {
-          float* s1 = w.ds1 + (at * DKP + row0 + 16 * t) * sh.dvp + col0 + 16 * n;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) s1[(int64_t)r * sh.dvp] = S[n][t][r];
-        }
-      }
-      f32x4 d;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) d[e] = col0 + 16 * n < sh.dv && t0 + tok + e < len ? (float)vals[n][e] : 0.0f;
-      put_half<NPI>(x_d + (half * NC + n) * NPI * FRAG, FRAG, wave & 1, lane, d);       // bf16 gradients are one plane
-      put_half<3>(x_g + (half * NC + n) * 3 * FRAG, FRAG, wave & 1, lane, d * f_eg * sh.scale);
-    }
-    const f32x4 eg = f_eg;
-    load_o(next);
+      for (int t = 0; t < MT; ++t)
+        put_half<3>(x_s + (((wave * MT + t) / 2) * NC + n) * 3 * FRAG, (wave * MT + t) & 1, lane, S[n][t]);
     lds_barrier();
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
-      f32x4 acc = {0, 0, 0, 0};
+      Orders<3> acc;
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         bf16x8 sf[3];
-        get_frag<3>(x_s + (s * NC + n) * 3 * FRAG, FRAG, lane, sf);
-        acc = mma_planes<NPI, 3, 3>(ka[s], sf, acc);
+        get_frag<3>(x_s + (s * NC + n) * 3 * FRAG, lane, sf);
+        acc.add(ka[s], sf);
       }
-      acc *= f_rest;
+      put_half<3>(x_x + (half * NC + n) * 3 * FRAG, wave & 1, lane, acc.sum() * f_rest + x_p[(wave * NC + n) * 64 + lane]);
+      if (p.col0 + 16 * n < sh.dvp)
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
-        if (s >= half) {
-          bf16x8 df[NPI];
-          get_frag<NPI>(x_d + (s * NC + n) * NPI * FRAG, FRAG, lane, df);
-          acc = mma_planes<3, NPI, 3>(pt[s], df, acc);
-        }
-      put_half<3>(x_x + (half * NC + n) * 3 * FRAG, FRAG, wave & 1, lane, acc);
+        for (int t = 0; t < MT; ++t) store_rows(w.ds1 + at * DKP * sh.dvp, row0 + 16 * t, p.col0 + 16 * n, sh.dvp, S[n][t]);
     }
-    load_k(next);
     lds_barrier();
+    load_k(next);                // behind the barrier: issued while the first LDS reads are on their way
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
-      f32x4 acc = {0, 0, 0, 0};
+      Orders<3> acc;
 #pragma unroll
       for (int s = 0; s < 2; ++s)
         if (s >= half) {
           bf16x8 xf[3];
-          get_frag<3>(x_x + (s * NC + n) * 3 * FRAG, FRAG, lane, xf);
-          acc = mma_planes<3, 3, 3>(tt[s], xf, acc);
+          get_frag<3>(x_x + (s * NC + n) * 3 * FRAG, lane, xf);
+          acc.add(tt[s], xf);
         }
-      const f32x4 be = acc * f_beta;
-      put_half<3>(x_e + (half * NC + n) * 3 * FRAG, FRAG, wave & 1, lane, -(be * eg));
-      const int col = col0 + 16 * n;
-      if (col < sh.dvp) {
-        float* ep = w.e + (at * C + tok) * sh.dvp + col;
+      const f32x4 e = acc.sum(), be = e * f_beta;
+      put_half<3>(x_e + (half * NC + n) * 3 * FRAG, wave & 1, lane, -(be * f_eg));
+      if (p.col0 + 16 * n < sh.dvp) store_rows(w.e + at * C * sh.dvp, tok, p.col0 + 16 * n, sh.dvp, e);
+      f32x4 out = be;
+      if (left < C)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) ep[(int64_t)e * sh.dvp] = acc[e];
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int64_t t = t0 + tok + e;
-        if (col < sh.dv && t < sh.time) dv[base + t * stride + col] = (T)(t < len ? be[e] : 0.0f);
-      }
+        for (int r = 0; r < 4; ++r) out[r] = tok + r < left ? be[r] : 0.0f;
+      store_tokens(dv + base + ch * C * stride, p, p.col0 + 16 * n, (uint32_t)stride * sizeof(T), all_cols && left_o == C, sh.dv, left_o, out);
     }
-    load_t(next);
     lds_barrier();
+    load_t(next);
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
+      Orders<3> acc[MT];
 #pragma unroll
-      for (int t = 0; t < MT; ++t) S[n][t] *= whole;
+      for (int t = 0; t < MT; ++t) acc[t].v[0] = S[n][t] * whole + x_q[((wave * MT + t) * NC + n) * 64 + lane];
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        bf16x8 gf[3], ef[3];
-        get_frag<3>(x_g + (s * NC + n) * 3 * FRAG, FRAG, lane, gf);
-        get_frag<3>(x_e + (s * NC + n) * 3 * FRAG, FRAG, lane, ef);
+        bf16x8 ef[3];
+        get_frag<3>(x_e + (s * NC + n) * 3 * FRAG, lane, ef);
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
-          S[n][t] = mma_planes<NPI, 3, 3>(qt[t][s], gf, S[n][t]);
-          S[n][t] = mma_planes<NPI, 3, 3>(kt[t][s], ef, S[n][t]);
-        }
+        for (int t = 0; t < MT; ++t) acc[t].add(kt[t][s], ef);
       }
+#pragma unroll
+      for (int t = 0; t < MT; ++t) S[n][t] = acc[t].sum();
     }
-    load_cols(next);
-    lds_barrier();      // x_g is written again before the next chunk's first barrier
+    load_kt(next);
+    lds_barrier();               // x_p and x_q are written again in front of the next chunk's first barrier
   }
   if (d_state0)
 #pragma unroll
@@ -747,8 +951,8 @@ __global__ void __launch_bounds__(TEAM, 1)
       for (int t = 0; t < MT; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int row = row0 + 16 * t + r, col = col0 + 16 * n;
-          if (col < sh.dv && row < sh.dk) d_state0[(bh * sh.dk + row) * sh.dv + col] = S[n][t][r];
+          const int row = row0 + 16 * t + r, col = p.col0 + 16 * n;
+          if (col < sh.dv && row < sh.dk) d_state0[(p.bh * sh.dk + row) * sh.dv + col] = S[n][t][r];
         }
 }
 
@@ -1069,6 +1273,7 @@ int32_t check_shape(const char* who, const gjx_delta_shape* s) {
               who, s->dk, s->dv);
   GJX_REQUIRE(s->batch <= (1 << 24) && s->heads <= 1024 && s->time <= ((int64_t)1 << 30), GJX_ELIMIT,
               "%s: batch up to 2^24, heads up to 1024, time up to 2^30", who);
+  GJX_REQUIRE(s->v_stride[1] <= (1 << 22), GJX_ELIMIT, "%s: v's token stride is above 2^22 elements", who);
   const int64_t blocks = s->batch * s->heads * std::max<int64_t>(up(s->time, C) / C, up(s->dv, 32) / 16 + 8);
   GJX_REQUIRE(blocks < ((int64_t)1 << 31), GJX_ELIMIT, "%s: batch x heads x chunks is too large", who);
   return GJX_OK;
@@ -1158,12 +1363,10 @@ bool aligned_rows(const T* p, const int64_t (&s)[3]) {
   return ((uintptr_t)p & 15) == 0 && s[0] % per16 == 0 && s[1] % per16 == 0 && s[2] % per16 == 0;
 }
 
-// columns per workgroup of the scans, in tiles of 16: as few as leave every CU at most one workgroup (the walk over the
-// chunks is a chain, so more workgroups are faster until the 256 CUs are taken; then wider ones read each fragment once)
-int scan_tiles(const Shape& sh) {
-  const int64_t all = sh.batch * sh.heads * (sh.dvp / 16);
-  return all <= 256 ? 1 : (all <= 512 ? 2 : 4);
-}
+// columns per workgroup of the scans, in tiles of 16: the walk over the chunks is a chain, so narrow workgroups are faster
+// until the 256 CUs are taken; wider ones then read each fragment once for twice the columns
+constexpr int wide_tiles(int dkp, int npi) { return dkp == 128 && npi == 3 ? 1 : 2; }      // f32 at dk > 64: registers for one
+bool scan_wide(const Shape& sh) { return sh.batch * sh.heads * (sh.dvp / 16) > 256; }
 unsigned scan_grid(const Shape& sh, int nc) { return (unsigned)(up(sh.batch * sh.heads, 8) * (up(sh.dvp / 16, nc) / nc)); }
 
 template <typename T, int DKP, bool KEEP>
@@ -1171,18 +1374,17 @@ int32_t run_filter(const Shape& sh, const T* q, const T* k, const T* v, const fl
                    const int32_t* lengths, T* o, float* state, const Work& w, hipStream_t s) {
   constexpr int NPI = sizeof(T) == 4 ? 3 : 1;
   if (sh.chunks > 0) {
-    constexpr int lds = 2 * NPI * C * (DKP + 8) * 2 + 3 * C * LD * 4 + 3 * C * 4;
+    constexpr int lds = std::max(2 * NPI * C * (DKP + 8) * 2, 2 * C * LD * 4) + C * LD * 4 + 3 * C * 4;
     GJX_CHECK_HIP(hipFuncSetAttribute((const void*)k_delta_prepare<T, DKP, NPI, KEEP>, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
     k_delta_prepare<T, DKP, NPI, KEEP><<<(unsigned)(sh.batch * sh.heads * sh.chunks), 256, lds, s>>>(
         sh, q, k, g, beta, lengths, w, aligned_rows(q, sh.qs) && aligned_rows(k, sh.ks));
     GJX_LAUNCH_CHECK();
   }
-  const int nc = scan_tiles(sh);
-#define GJX_SCAN(NC) k_delta_scan<T, DKP, NPI, KEEP, NC><<<scan_grid(sh, NC), TEAM, 0, s>>>(sh, v, state0, lengths, o, state, w)
-  if (nc == 1) GJX_SCAN(1);
-  else if (nc == 2) GJX_SCAN(2);
-  else GJX_SCAN(4);
-#undef GJX_SCAN
+  constexpr int NC = wide_tiles(DKP, NPI);
+  if (scan_wide(sh))
+    k_delta_scan<T, DKP, NPI, KEEP, NC><<<scan_grid(sh, NC), TEAM, 0, s>>>(sh, v, state0, lengths, o, state, w);
+  else
+    k_delta_scan<T, DKP, NPI, KEEP, 1><<<scan_grid(sh, 1), TEAM, 0, s>>>(sh, v, state0, lengths, o, state, w);
   GJX_LAUNCH_CHECK();
   return GJX_OK;
 }
@@ -1191,13 +1393,11 @@ template <typename T, int DKP>
 int32_t run_grad(const Shape& sh, const T* q, const T* k, const float* g, const int32_t* lengths, const T* d_o, const float* d_state,
                  T* dq, T* dk, T* dv, float* dg, float* dbeta, float* d_state0, const Work& w, hipStream_t s) {
   constexpr int NPI = sizeof(T) == 4 ? 3 : 1;
-  const int nc = scan_tiles(sh);
-#define GJX_SCAN(NC) \
-  k_delta_scan_back<T, DKP, NPI, NC><<<scan_grid(sh, NC), TEAM, 0, s>>>(sh, d_o, d_state, lengths, dv, d_state0, w)
-  if (nc == 1) GJX_SCAN(1);
-  else if (nc == 2) GJX_SCAN(2);
-  else GJX_SCAN(4);
-#undef GJX_SCAN
+  constexpr int NC = wide_tiles(DKP, NPI);
+  if (scan_wide(sh))
+    k_delta_scan_back<T, DKP, NPI, NC><<<scan_grid(sh, NC), TEAM, 0, s>>>(sh, d_o, d_state, lengths, dv, d_state0, w);
+  else
+    k_delta_scan_back<T, DKP, NPI, 1><<<scan_grid(sh, 1), TEAM, 0, s>>>(sh, d_o, d_state, lengths, dv, d_state0, w);
   GJX_LAUNCH_CHECK();
   if (sh.chunks == 0) return GJX_OK;
   k_delta_back<T, DKP, NPI><<<(unsigned)(sh.batch * sh.heads * sh.chunks), 256, 0, s>>>(sh, q, k, d_o, g, lengths, dq, dk, dg, dbeta, w);
