@@ -957,37 +957,42 @@ __global__ void __launch_bounds__(TEAM, 2)
 }
 
 // ---------------------------------------------------------------------------
-// gradients of q, k and the gates, all chunks at once; wave = 16 tokens
+// gradients of q, k and the gates, all chunks at once
 // ---------------------------------------------------------------------------
-template <int P>
-__device__ __forceinline__ void load_f32_frag(const float* p, bf16x8 (&out)[P]) {
-  const f32x4 a = *(const f32x4*)p, b = *(const f32x4*)(p + 4);
-  const float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-  split<P>(x, out);
-}
+// Eight waves: wave w forms the rows of tokens [16 (w % 4), + 16) and the dk half w / 4.  Per 32 columns of dv, S0, dS1, e,
+// delta and dO become fragment planes in LDS once, for all waves (each wave splitting its own operands: 380 us for 1024
+// chunks of 64 x 128 x 128), while the next columns are on their way to registers; the row sums <dS1, S0> and e.delta
+// fall out of the same registers.
+constexpr int BACK = 512;
 
 template <typename T, int DKP, int NPI>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(BACK, 2)
     k_delta_back(Shape sh, const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ d_o,
                  const float* __restrict__ g, const int32_t* __restrict__ lengths, T* __restrict__ dq, T* __restrict__ dk,
-                 float* __restrict__ dg, float* __restrict__ dbeta, Work w) {
+                 float* __restrict__ dg, float* __restrict__ dbeta, Work w, int vec_o) {
   typedef KeyBlock<DKP, NPI> KB;
-  constexpr int MT = DKP / 16;
-  __shared__ float se[C * LD], sf[C * LD];
-  __shared__ float s_gh[C], s_gl[C], s_row[C], s_db[C], s_sum[4], s_put[4];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, quad = lane >> 4, c = lane & 15;
+  constexpr int MT = DKP / 16, MH = MT / 2;               // tiles of dk; of one wave
+  constexpr int F_S0 = 0, F_S1 = MT * 3 * FRAG, F_E = 2 * F_S1, F_D = F_E + 12 * FRAG, F_O = F_D + 12 * FRAG, F_ALL = F_O + 4 * NPI * FRAG;
+  constexpr int MATRICES = 2 * C * LD * 4;
+  __shared__ __attribute__((aligned(16))) char buffer[F_ALL * 2 > MATRICES ? F_ALL * 2 : MATRICES];
+  __shared__ float s_gh[C], s_gl[C], s_row[2][C], s_db[C], s_put[8];
+  __shared__ double s_sum[8];
+  bf16* frag = (bf16*)buffer;
+  float *se = (float*)buffer, *sf = se + C * LD;          // E and F, once the fragments are used up
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quad = lane >> 4, c = lane & 15;
+  const int wt = wave & 3, wh = wave >> 2;
   const int64_t chunk = blockIdx.x % sh.chunks, bh = blockIdx.x / sh.chunks, b = bh / sh.heads;
   const int h = (int)(bh % sh.heads), kh = h / sh.group;
   const int64_t len = length_of(lengths, b, sh.time), t0 = chunk * C, at = bh * sh.chunks + chunk;
   const bool shared = sh.group > 1;
   const int64_t g_at = (b * sh.time + t0) * sh.heads + h;
-  if (t0 >= len) {
-    const int tokens = (int)std::min<int64_t>(C, sh.time - t0);
-    for (int i = tid; i < tokens; i += 256) {
+  const int left_o = (int)std::min<int64_t>(C, sh.time - t0), left = (int)std::min<int64_t>(C, len - t0);
+  if (left <= 0) {
+    for (int i = tid; i < left_o; i += BACK) {
       dg[g_at + (int64_t)i * sh.heads] = 0.0f;
       dbeta[g_at + (int64_t)i * sh.heads] = 0.0f;
     }
-    for (int i = tid; i < tokens * sh.dk; i += 256) {
+    for (int i = tid; i < left_o * sh.dk; i += BACK) {
       const int64_t p = ((b * sh.time + t0 + i / sh.dk) * sh.heads + h) * sh.dk + i % sh.dk;
       if (shared) {
         w.dq[p] = 0.0f;
@@ -1000,11 +1005,9 @@ __global__ void __launch_bounds__(256)
     return;
   }
   const float* rb = w.rows + at * ROWS;
-  const float *s0 = w.s0 + at * DKP * sh.dvp, *ds1 = w.ds1 + at * DKP * sh.dvp;
-  const float *dl = w.delta + at * C * sh.dvp, *ee = w.e + at * C * sh.dvp;
   const bf16* kb = w.keys + ((b * sh.kheads + kh) * sh.chunks + chunk) * w.key_size;
   if (wave == 0) {
-    double gam = t0 + lane < len ? (double)fmaxf(g[b * sh.gs[0] + (t0 + lane) * sh.gs[1] + h * sh.gs[2]], G_MIN) : 0.0;
+    double gam = lane < left ? (double)fmaxf(g[b * sh.gs[0] + (t0 + lane) * sh.gs[1] + h * sh.gs[2]], G_MIN) : 0.0;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
       const double up = __shfl_up(gam, o);
@@ -1013,113 +1016,194 @@ __global__ void __launch_bounds__(256)
     s_gh[lane] = (float)gam;
     s_gl[lane] = (float)(gam - (double)(float)gam);
   }
-  // <dS1, S0> and dbeta_i = e_i . delta_i
-  {
-    double dot = 0.0;
-    for (int i = tid; i < DKP * sh.dvp; i += 256) dot += (double)s0[i] * (double)ds1[i];
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) dot += __shfl_xor(dot, o);
-    if (lane == 0) s_sum[wave] = (float)dot;
-    const int t = tid >> 2;
-    float db = 0.0f;
-    for (int i = tid & 3; i < sh.dvp; i += 4) db += dl[t * sh.dvp + i] * ee[t * sh.dvp + i];
-    db += __shfl_xor(db, 1);
-    db += __shfl_xor(db, 2);
-    if ((tid & 3) == 0) s_db[t] = db;
-  }
-  __syncthreads();
 
-  const int tok = 16 * wave + c;             // this lane's row of the operands
-  f32x4 m1[MT], m2[MT], m3[MT], pe[4], pf[4];
+  // this thread's pieces of a slab: eight columns of one row of S0 and dS1, and of e and delta (first half) or dO
+  const int row = tid >> 2, sub = tid & 3;                // 128 rows
+  const bool has_state = row < DKP;
+  const bool first = tid < 256;
+  const int trow = row & 63;
+  const float *p_s0 = w.s0 + (at * DKP + min(row, DKP - 1)) * sh.dvp + 8 * sub, *p_s1 = w.ds1 + (at * DKP + min(row, DKP - 1)) * sh.dvp + 8 * sub;
+  const float *p_e = w.e + (at * C + trow) * sh.dvp + 8 * sub, *p_d = w.delta + (at * C + trow) * sh.dvp + 8 * sub;
+  const T* p_o = d_o + ((b * sh.time + t0 + min(trow, left - 1)) * sh.heads + h) * sh.dv;
+  float x0[8], x1[8], x2[8], x3[8];
+  auto load8 = [](const float* p, float (&x)[8]) {
+    const f32x4 a = *(const f32x4*)p, z = *(const f32x4*)(p + 4);
 #pragma unroll
-  for (int t = 0; t < MT; ++t) m1[t] = m2[t] = m3[t] = f32x4{0, 0, 0, 0};
+    for (int j = 0; j < 4; ++j) {
+      x[j] = a[j];
+      x[4 + j] = z[j];
+    }
+  };
+  auto load = [&](int s) {
+    load8(p_s0 + 32 * s, x0);
+    load8(p_s1 + 32 * s, x1);
+    if (first) {
+      load8(p_e + 32 * s, x2);
+      load8(p_d + 32 * s, x3);
+    } else {
+      const int c0 = 32 * s + 8 * sub;
+      if (vec_o && c0 + 8 <= sh.dv) {
+        typedef T vec8 __attribute__((ext_vector_type(8)));
+        const vec8 v = *(const vec8*)(p_o + c0);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) pe[j] = pf[j] = f32x4{0, 0, 0, 0};
-  const bool live = t0 + tok < len;
-  const T* dop = d_o + ((b * sh.time + t0 + tok) * sh.heads + h) * sh.dv;
-  for (int s = 0; s < sh.dvp / 32; ++s) {
-    const int c0 = 32 * s + 8 * quad;
-    float x[8];
+        for (int j = 0; j < 8; ++j) x2[j] = (float)v[j];
+      } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = live && c0 + j < sh.dv ? (float)dop[c0 + j] : 0.0f;
+        for (int j = 0; j < 8; ++j) x2[j] = c0 + j < sh.dv ? (float)p_o[c0 + j] : 0.0f;
+      }
+    }
+  };
+  auto put8 = [&](int base, int planes, int r, const float (&x)[8]) {
+    bf16* f = frag + base + (r >> 4) * planes * FRAG + ((r & 15) + 16 * sub) * 8;
+    if (planes == 3) {
+      bf16x8 o3[3];
+      split<3>(x, o3);
+#pragma unroll
+      for (int p = 0; p < 3; ++p) *(bf16x8*)(f + p * FRAG) = o3[p];
+    } else {
+      bf16x8 o1[1];
+      split<1>(x, o1);
+      *(bf16x8*)f = o1[0];
+    }
+  };
+
+  f32x4 m1[MH], m2[MH], m3[MH], pe[2], pf[2];
+#pragma unroll
+  for (int t = 0; t < MH; ++t) m1[t] = m2[t] = m3[t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+  for (int j = 0; j < 2; ++j) pe[j] = pf[j] = f32x4{0, 0, 0, 0};
+  float dot = 0.0f, db = 0.0f;
+  const int slabs = sh.dvp / 32;
+  load(0);
+  for (int s = 0; s < slabs; ++s) {
+    if (has_state) {
+      put8(F_S0, 3, row, x0);
+      put8(F_S1, 3, row, x1);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) dot += x0[j] * x1[j];
+    }
+    if (first) {
+      put8(F_E, 3, trow, x2);
+      put8(F_D, 3, trow, x3);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) db += x2[j] * x3[j];
+    } else {
+      if (trow >= left)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x2[j] = 0.0f;
+      put8(F_O, NPI, trow, x2);
+    }
+    __syncthreads();
+    if (s + 1 < slabs) load(s + 1);
     bf16x8 fo[NPI], fe[3], fd[3];
-    split<NPI>(x, fo);
-    load_f32_frag<3>(ee + tok * sh.dvp + c0, fe);
-    load_f32_frag<3>(dl + tok * sh.dvp + c0, fd);
+    get_frag<NPI>(frag + F_O + wt * NPI * FRAG, lane, fo);
+    get_frag<3>(frag + F_E + wt * 3 * FRAG, lane, fe);
+    get_frag<3>(frag + F_D + wt * 3 * FRAG, lane, fd);
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
+    for (int t = 0; t < MH; ++t) {
       bf16x8 f0[3], f1[3];
-      load_f32_frag<3>(s0 + (16 * t + c) * sh.dvp + c0, f0);
-      load_f32_frag<3>(ds1 + (16 * t + c) * sh.dvp + c0, f1);
+      get_frag<3>(frag + F_S0 + (wh * MH + t) * 3 * FRAG, lane, f0);
+      get_frag<3>(frag + F_S1 + (wh * MH + t) * 3 * FRAG, lane, f1);
       m1[t] = mma_planes<NPI, 3, 3>(fo, f0, m1[t]);
       m2[t] = mma_planes<3, 3, 3>(fe, f0, m2[t]);
       m3[t] = mma_planes<3, 3, 3>(fd, f1, m3[t]);
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (j <= wave) {
+    for (int j = 0; j < 2; ++j)
+      if (2 * wh + j <= wt) {
         bf16x8 fj[3];
-        load_f32_frag<3>(dl + (16 * j + c) * sh.dvp + c0, fj);
+        get_frag<3>(frag + F_D + (2 * wh + j) * 3 * FRAG, lane, fj);
         pe[j] = mma_planes<NPI, 3, 3>(fo, fj, pe[j]);
         pf[j] = mma_planes<3, 3, 3>(fe, fj, pf[j]);
       }
+    __syncthreads();
+  }
+  {
+    double d = has_state ? (double)dot : 0.0;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) d += __shfl_xor(d, o);
+    if (lane == 0) s_sum[wave] = d;
+    db += __shfl_xor(db, 1);
+    db += __shfl_xor(db, 2);
+    if (first && sub == 0) s_db[trow] = db;
   }
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
+  for (int j = 0; j < 2; ++j)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int i = 16 * wave + 4 * quad + r, jj = 16 * j + c;
+      const int i = 16 * wt + 4 * quad + r, jj = 16 * (2 * wh + j) + c;
       const float d = jj <= i ? expf((s_gh[i] - s_gh[jj]) + (s_gl[i] - s_gl[jj])) * rb[jj] : 0.0f;
       se[i * LD + jj] = jj <= i ? sh.scale * d * pe[j][r] : 0.0f;
       sf[i * LD + jj] = jj < i ? -rb[i] * d * pf[j][r] : 0.0f;
     }
-  const f32x4 be = *(const f32x4*)(rb + 16 * wave + 4 * quad), eg = *(const f32x4*)(rb + C + 16 * wave + 4 * quad);
-  const f32x4 rest = *(const f32x4*)(rb + 2 * C + 16 * wave + 4 * quad);
+  const f32x4 be = *(const f32x4*)(rb + 16 * wt + 4 * quad), eg = *(const f32x4*)(rb + C + 16 * wt + 4 * quad);
+  const f32x4 rest = *(const f32x4*)(rb + 2 * C + 16 * wt + 4 * quad);
   __syncthreads();
 
-  bf16x8 fe[2][3], ff[2][3], fet[2][3], fft[2][3];
+  const int tok = 16 * wt + c;                            // this lane's row of the operands E, F (column: their transposes)
+  // E and F as rows, then as columns: half the fragments live at a time
+  auto rows_of = [&](const float* m, bool trans, bf16x8 (&out)[2][3]) {
 #pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    float x[8], y[8], z[8], u[8];
+    for (int s = 0; s < 2; ++s) {
+      float x[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int p = perm(s, quad, j);
-      x[j] = se[tok * LD + p];
-      y[j] = sf[tok * LD + p];
-      z[j] = se[p * LD + tok];
-      u[j] = sf[p * LD + tok];
+      for (int j = 0; j < 8; ++j) x[j] = trans ? m[perm(s, quad, j) * LD + tok] : m[tok * LD + perm(s, quad, j)];
+      split<3>(x, out[s]);
     }
-    split<3>(x, fe[s]);
-    split<3>(y, ff[s]);
-    split<3>(z, fet[s]);
-    split<3>(u, fft[s]);
-  }
-  f32x4 row = {0, 0, 0, 0}, put = {0, 0, 0, 0};
+  };
+  {
+    bf16x8 fe[2][3], ff[2][3];
+    rows_of(se, false, fe);
+    rows_of(sf, false, ff);
 #pragma unroll
-  for (int t = 0; t < MT; ++t) {
-    f32x4 aq = m1[t] * eg * sh.scale, ar = -(m2[t] * be * eg), aw = m3[t] * be * rest;
-    const f32x4 last = aw;
+    for (int t = 0; t < MH; ++t) {
+      m1[t] *= eg * sh.scale;
+      m2[t] *= -(be * eg);
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        bf16x8 kt[NPI];
+        load_frag<NPI>(kb + KB::KT, (wh * MH + t) * 2 + s, MT * 2 * FRAG, lane, kt);
+        m1[t] = mma_planes<3, NPI, 3>(fe[s], kt, m1[t]);
+        m2[t] = mma_planes<3, NPI, 3>(ff[s], kt, m2[t]);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  bf16x8 fe[2][3], ff[2][3];
+  rows_of(se, true, fe);
+  rows_of(sf, true, ff);
+  f32x4 sum = {0, 0, 0, 0}, put = {0, 0, 0, 0};
+#pragma unroll
+  for (int t = 0; t < MH; ++t) {
+    const int tile = wh * MH + t, col = 16 * tile + c;
+    T qv[4], kv[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int64_t tt = t0 + min(16 * wt + 4 * quad + r, left - 1);
+      qv[r] = q[b * sh.qs[0] + tt * sh.qs[1] + kh * sh.qs[2] + min(col, sh.dk - 1)];
+      kv[r] = k[b * sh.ks[0] + tt * sh.ks[1] + kh * sh.ks[2] + min(col, sh.dk - 1)];
+    }
+    f32x4 aw = m3[t] * be * rest;
+    const f32x4 last = aw, aq = m1[t], ar = m2[t];
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       bf16x8 kt[NPI], qt[NPI];
-      load_frag<NPI>(kb + KB::KT, t * 2 + s, MT * 2 * FRAG, lane, kt);
-      load_frag<NPI>(kb + KB::QT, t * 2 + s, MT * 2 * FRAG, lane, qt);
-      aq = mma_planes<3, NPI, 3>(fe[s], kt, aq);
-      ar = mma_planes<3, NPI, 3>(ff[s], kt, ar);
-      aw = mma_planes<3, NPI, 3>(fet[s], qt, aw);
-      aw = mma_planes<3, NPI, 3>(fft[s], kt, aw);
+      load_frag<NPI>(kb + KB::KT, tile * 2 + s, MT * 2 * FRAG, lane, kt);
+      load_frag<NPI>(kb + KB::QT, tile * 2 + s, MT * 2 * FRAG, lane, qt);
+      aw = mma_planes<3, NPI, 3>(fe[s], qt, aw);
+      aw = mma_planes<3, NPI, 3>(ff[s], kt, aw);
     }
-    const int col = 16 * t + c;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int64_t tt = t0 + 16 * wave + 4 * quad + r;
-      if (col < sh.dk && tt < sh.time) {
-        const float qv = tt < len ? (float)q[b * sh.qs[0] + tt * sh.qs[1] + kh * sh.qs[2] + col] : 0.0f;
-        const float kv = tt < len ? (float)k[b * sh.ks[0] + tt * sh.ks[1] + kh * sh.ks[2] + col] : 0.0f;
-        row[r] += qv * aq[r] + kv * (ar[r] - aw[r]);
-        put[r] += kv * last[r];
-        const int64_t p = ((b * sh.time + tt) * sh.heads + h) * sh.dk + col;
-        const float vq = tt < len ? aq[r] : 0.0f, vk = tt < len ? ar[r] + aw[r] : 0.0f;
+      const int i = 16 * wt + 4 * quad + r;
+      if (col < sh.dk && i < left_o) {
+        const bool on = i < left;
+        const float vq = on ? aq[r] : 0.0f, vk = on ? ar[r] + aw[r] : 0.0f;
+        if (on) {
+          sum[r] += (float)qv[r] * aq[r] + (float)kv[r] * (ar[r] - aw[r]);
+          put[r] += (float)kv[r] * last[r];
+        }
+        const int64_t p = ((b * sh.time + t0 + i) * sh.heads + h) * sh.dk + col;
         if (shared) {
           w.dq[p] = vq;
           w.dk[p] = vk;
@@ -1136,25 +1220,29 @@ __global__ void __launch_bounds__(256)
   if (lane == 0) s_put[wave] = all;
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
-    float s = row[r];
+    float s = sum[r];
 #pragma unroll
     for (int o = 1; o < 16; o <<= 1) s += __shfl_xor(s, o);
-    if (c == 0) s_row[16 * wave + 4 * quad + r] = s;
+    if (c == 0) s_row[wh][16 * wt + 4 * quad + r] = s;
   }
   __syncthreads();
   if (wave == 0) {
-    double s = (double)s_row[lane];
+    double s = (double)s_row[0][lane] + (double)s_row[1][lane];
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
       const double down = __shfl_down(s, o);
       if (lane + o < 64) s += down;
     }
-    const float whole = rb[2 * C - 1];
-    s += (double)whole * ((double)s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3]) + ((double)s_put[0] + s_put[1] + s_put[2] + s_put[3]);
-    if (t0 + lane < sh.time) {
-      const bool on = t0 + lane < len;
-      dg[g_at + (int64_t)lane * sh.heads] = on ? (float)s : 0.0f;
-      dbeta[g_at + (int64_t)lane * sh.heads] = on ? s_db[lane] : 0.0f;
+    double end = 0.0, written = 0.0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      end += s_sum[i];
+      written += (double)s_put[i];
+    }
+    s += (double)rb[3 * C] * end + written;
+    if (lane < left_o) {
+      dg[g_at + (int64_t)lane * sh.heads] = lane < left ? (float)s : 0.0f;
+      dbeta[g_at + (int64_t)lane * sh.heads] = lane < left ? s_db[lane] : 0.0f;
     }
   }
 }
@@ -1400,7 +1488,8 @@ int32_t run_grad(const Shape& sh, const T* q, const T* k, const float* g, const 
     k_delta_scan_back<T, DKP, NPI, 1><<<scan_grid(sh, 1), TEAM, 0, s>>>(sh, d_o, d_state, lengths, dv, d_state0, w);
   GJX_LAUNCH_CHECK();
   if (sh.chunks == 0) return GJX_OK;
-  k_delta_back<T, DKP, NPI><<<(unsigned)(sh.batch * sh.heads * sh.chunks), 256, 0, s>>>(sh, q, k, d_o, g, lengths, dq, dk, dg, dbeta, w);
+  const int vec_o = ((uintptr_t)d_o & 15) == 0 && sh.dv % 8 == 0;
+  k_delta_back<T, DKP, NPI><<<(unsigned)(sh.batch * sh.heads * sh.chunks), BACK, 0, s>>>(sh, q, k, d_o, g, lengths, dq, dk, dg, dbeta, w, vec_o);
   GJX_LAUNCH_CHECK();
   if (sh.group > 1) {
     k_delta_shared_heads<T><<<gjx_grid_for(sh.batch * sh.time * sh.kheads * sh.dk), GJX_BLOCK, 0, s>>>(sh, w.dq, w.dk, dq, dk);
