@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import collections
 import ctypes as C
+import functools
 import math
 from typing import Sequence
 
@@ -437,101 +438,119 @@ def categorical_logpdf(x, logits):
 ELEMENT_TYPES = {torch.float32: 0, torch.bfloat16: 1}       # GJX_F32, GJX_BF16
 
 
-def _on_current_device(who, **tensors):
-    """Refuse tensors that are not on the current device (launches go to its current stream)."""
-    cur = torch.cuda.current_device() if torch.cuda.is_available() else None
-    for name, t in tensors.items():
+def _on_current_device(who, *tensors):
+    """Refuse (name, tensor) pairs that are not on the current device (launches go to its current stream)."""
+    cur = None
+    for name, t in tensors:
         if t is None:
             continue
         if not isinstance(t, torch.Tensor) or not t.is_cuda:
             raise GjxError(f"{who}: `{name}` must be a device tensor")
-        if t.device.index != cur:
-            raise GjxError(f"{who}: `{name}` lives on cuda:{t.device.index} but the current device is cuda:{cur}: launches "
+        if cur is None:
+            cur = torch.cuda.current_device()
+        if t.get_device() != cur:
+            raise GjxError(f"{who}: `{name}` lives on {t.device} but the current device is cuda:{cur}: launches "
                            "go to the current device's stream (use torch.cuda.set_device / torch.cuda.device)")
+
+
+def _address(t):
+    return 0 if t is None else t.data_ptr()
 
 
 def _unit_stride(t):
     """`t` itself when its last axis is contiguous and its rows do not overlap, else a contiguous copy."""
-    ok = t.stride(-1) == 1 or t.shape[-1] == 1
-    if t.dim() > 1:
-        ok = ok and t.stride(0) >= t.shape[-1]
-    return t if ok else t.contiguous()
+    width, (step, unit) = t.shape[1], t.stride()
+    return t if (unit == 1 or width == 1) and step >= width else t.contiguous()
 
 
-def _linear_args(who, x, weight, bias):
-    for name, t in (("x", x), ("weight", weight), ("bias", bias)):
-        if t is not None and not isinstance(t, torch.Tensor):
-            raise GjxError(f"{who}: `{name}` must be a tensor")
-    if x.dim() != 2 or weight.dim() != 2 or x.shape[1] != weight.shape[1] or weight.shape[0] < 1 or weight.shape[1] < 1:
-        raise GjxError(f"{who}: x {tuple(x.shape)} and weight {tuple(weight.shape)} must be (n, width) and (vocab, width)")
-    if bias is not None and tuple(bias.shape) != (weight.shape[0],):
-        raise GjxError(f"{who}: bias {tuple(bias.shape)} must be ({weight.shape[0]},)")
-    if x.dtype not in ELEMENT_TYPES or any(t is not None and t.dtype != x.dtype for t in (weight, bias)):
-        raise GjxError(f"{who}: x, weight and bias must all be float32 or all bfloat16 (got {x.dtype}, {weight.dtype}"
-                       f"{'' if bias is None else f', {bias.dtype}'})")
-    _on_current_device(who, x=x, weight=weight, bias=bias)
-    return _unit_stride(x), _unit_stride(weight), None if bias is None else bias.contiguous()
-
-
-def _linear_head(x, weight):
-    return (C.c_void_p(x.data_ptr()), max(x.stride(0), x.shape[1]), C.c_void_p(weight.data_ptr()),
-            max(weight.stride(0), weight.shape[1]))
-
-
-def _linear_workspace(x, weight, grad):
-    n, (vocab, width) = x.shape[0], weight.shape
+@functools.lru_cache(maxsize=1024)
+def _linear_workspace_bytes(dtype, x_low, x_ld, w_low, w_ld, n, vocab, width, grad):
+    """Workspace of a call: depends on the sizes, the row strides and the pointers' alignment (their low bits)."""
     size = C.c_int64()
-    N.check(N.lib().gjx_linear_categorical_workspace(ELEMENT_TYPES[x.dtype], *_linear_head(x, weight), n, vocab, width, grad,
-                                                     C.byref(size)), "gjx_linear_categorical_workspace")
-    return torch.empty(max(size.value, 256), dtype=torch.uint8, device=x.device)
+    N.check(N.lib().gjx_linear_categorical_workspace(dtype, 16 + x_low, x_ld, 16 + w_low, w_ld, n, vocab, width, grad, C.byref(size)),
+            "gjx_linear_categorical_workspace")
+    return max(size.value, 256)
 
 
-def linear_categorical_logpdf(y, x, weight, bias=None):
+class _Linear:
+    """The checked inputs of a linear-categorical call as the library takes them."""
+
+    __slots__ = ("x", "weight", "bias", "n", "vocab", "width", "head")
+
+    def __init__(self, x, weight, bias):
+        who = "linear_categorical"
+        for name, t in (("x", x), ("weight", weight), ("bias", bias)):
+            if t is not None and not isinstance(t, torch.Tensor):
+                raise GjxError(f"{who}: `{name}` must be a tensor")
+        if x.dim() != 2 or weight.dim() != 2 or x.shape[1] != weight.shape[1] or weight.shape[0] < 1 or weight.shape[1] < 1:
+            raise GjxError(f"{who}: x {tuple(x.shape)} and weight {tuple(weight.shape)} must be (n, width) and (vocab, width)")
+        self.n, (self.vocab, self.width) = x.shape[0], weight.shape
+        if bias is not None and bias.shape != (self.vocab,):
+            raise GjxError(f"{who}: bias {tuple(bias.shape)} must be ({self.vocab},)")
+        dtype = ELEMENT_TYPES.get(x.dtype)
+        if dtype is None or weight.dtype != x.dtype or (bias is not None and bias.dtype != x.dtype):
+            raise GjxError(f"{who}: x, weight and bias must all be float32 or all bfloat16 (got {x.dtype}, {weight.dtype}"
+                           f"{'' if bias is None else f', {bias.dtype}'})")
+        _on_current_device(who, ("x", x), ("weight", weight), ("bias", bias))
+        self.x, self.weight, self.bias = _unit_stride(x), _unit_stride(weight), None if bias is None else bias.contiguous()
+        self.head = (dtype, self.x.data_ptr(), max(self.x.stride(0), self.width), self.weight.data_ptr(),
+                     max(self.weight.stride(0), self.width))
+
+    def workspace(self, grad):
+        dtype, xp, x_ld, wp, w_ld = self.head
+        size = _linear_workspace_bytes(dtype, xp & 15, x_ld, wp & 15, w_ld, self.n, self.vocab, self.width, grad)
+        return torch.empty(size, dtype=torch.uint8, device=self.x.device)
+
+
+def _linear_values(y, n):
+    if y.dtype != torch.int32 or y.shape != (n,):
+        raise GjxError(f"linear_categorical: y must be int32 of shape ({n},), got {y.dtype} {tuple(y.shape)}")
+    _on_current_device("linear_categorical", ("y", y))
+    return y.contiguous()
+
+
+def linear_categorical_logpdf(y, x, weight, bias=None, want_lse=True):
     """y: (n,) int32; x: (n, width), weight: (vocab, width), bias: (vocab,) or None -> (log p(y) (n,), logsumexp (n,))."""
-    who = "linear_categorical"
-    x, weight, bias = _linear_args(who, x, weight, bias)
-    n, (vocab, width) = x.shape[0], weight.shape
-    if y.dtype != torch.int32 or tuple(y.shape) != (n,):
-        raise GjxError(f"{who}: y must be int32 of shape ({n},), got {y.dtype} {tuple(y.shape)}")
-    _on_current_device(who, y=y)
-    lp = torch.empty(n, dtype=torch.float32, device=x.device)
-    lse = torch.empty(n, dtype=torch.float32, device=x.device)
-    if n > 0:
-        y = y.contiguous()
-        work = _linear_workspace(x, weight, 0)
-        N.check(N.lib().gjx_linear_categorical_logpdf(ELEMENT_TYPES[x.dtype], _ptr(y), *_linear_head(x, weight), _ptr(bias), n,
-                                                      vocab, width, _ptr(lp), _ptr(lse), _ptr(work), work.numel(), _stream()),
-                "gjx_linear_categorical_logpdf")
+    a = _Linear(x, weight, bias)
+    y = _linear_values(y, a.n)
+    lp = torch.empty(a.n, dtype=torch.float32, device=a.x.device)
+    lse = torch.empty_like(lp) if want_lse else None
+    if a.n > 0:
+        dtype, xp, x_ld, wp, w_ld = a.head
+        work = a.workspace(0)
+        N.check(N.lib().gjx_linear_categorical_logpdf(dtype, y.data_ptr(), xp, x_ld, wp, w_ld, _address(a.bias), a.n, a.vocab,
+                                                      a.width, lp.data_ptr(), _address(lse), work.data_ptr(), work.numel(),
+                                                      _raw_stream()), "gjx_linear_categorical_logpdf")
     return lp, lse
 
 
 def linear_categorical_grad(y, x, weight, bias, lse, upstream, want=(True, True, True)):
     """upstream x d log p / d(x, weight, bias), summed over the rows for weight and bias (entries not wanted: None)."""
-    x, weight, bias = _linear_args("linear_categorical", x, weight, bias)
-    n, (vocab, width) = x.shape[0], weight.shape
-    like = (x, weight, bias)
-    outs = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if w and t is not None else None for w, t in zip(want, like)]
-    if n == 0:
+    a = _Linear(x, weight, bias)
+    y = _linear_values(y, a.n)
+    outs = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if w and t is not None else None
+            for w, t in zip(want, (a.x, a.weight, a.bias))]
+    if a.n == 0:
         return [None if o is None else o.zero_() for o in outs]
     if any(o is not None for o in outs):
-        y, upstream = y.contiguous(), _f32(upstream).contiguous()
-        work = _linear_workspace(x, weight, 1 if outs[0] is not None else 2)
-        N.check(N.lib().gjx_linear_categorical_grad(ELEMENT_TYPES[x.dtype], _ptr(y), *_linear_head(x, weight), _ptr(bias), n,
-                                                    vocab, width, _ptr(lse), _ptr(upstream), *(_ptr(o) for o in outs),
-                                                    _ptr(work), work.numel(), _stream()), "gjx_linear_categorical_grad")
+        upstream = _f32(upstream).contiguous()
+        dtype, xp, x_ld, wp, w_ld = a.head
+        work = a.workspace(1 if outs[0] is not None else 2)
+        N.check(N.lib().gjx_linear_categorical_grad(dtype, y.data_ptr(), xp, x_ld, wp, w_ld, _address(a.bias), a.n, a.vocab, a.width,
+                                                    lse.data_ptr(), upstream.data_ptr(), *map(_address, outs), work.data_ptr(),
+                                                    work.numel(), _raw_stream()), "gjx_linear_categorical_grad")
     return outs
 
 
 def sample_linear_categorical(k, x, weight, bias=None, offset: int = 0) -> torch.Tensor:
     """One Gumbel-max draw per row of x from softmax(x W^T + b); the noise layout of sample_categorical's per-row form."""
-    x, weight, bias = _linear_args("linear_categorical", x, weight, bias)
-    n, (vocab, width) = x.shape[0], weight.shape
-    out = torch.empty(n, dtype=torch.int32, device=x.device)
-    if n > 0:
-        work = _linear_workspace(x, weight, 0)
-        N.check(N.lib().gjx_random_linear_categorical_i32(_ckey(k), offset, ELEMENT_TYPES[x.dtype], *_linear_head(x, weight),
-                                                          _ptr(bias), n, vocab, width, _ptr(out), _ptr(work), work.numel(),
-                                                          _stream()), "gjx_random_linear_categorical_i32")
+    a = _Linear(x, weight, bias)
+    out = torch.empty(a.n, dtype=torch.int32, device=a.x.device)
+    if a.n > 0:
+        work = a.workspace(0)
+        N.check(N.lib().gjx_random_linear_categorical_i32(_ckey(k), offset, *a.head, _address(a.bias), a.n, a.vocab, a.width,
+                                                          out.data_ptr(), work.data_ptr(), work.numel(), _raw_stream()),
+                "gjx_random_linear_categorical_i32")
     return out
 
 
@@ -559,92 +578,110 @@ def mvnormal_logpdf(x, mu, cov):
 # --------------------------------------------------------------------------- #
 # gated delta filter
 # --------------------------------------------------------------------------- #
-def _delta_shape(who, q, k, v, log_decay, beta, scale):
-    """Check the tensors of one call against each other and describe them to the library; axes (batch, time, head, ...)."""
-    for name, t in (("q", q), ("k", k), ("v", v), ("log_decay", log_decay), ("beta", beta)):
-        if not isinstance(t, torch.Tensor):
-            raise GjxError(f"{who}: `{name}` must be a tensor")
-    if q.dim() != 4 or k.shape != q.shape or v.dim() != 4 or v.shape[:2] != q.shape[:2]:
-        raise GjxError(f"{who}: q {tuple(q.shape)} and k {tuple(k.shape)} must be (batch, time, key heads, dk) and v "
-                       f"{tuple(v.shape)} (batch, time, heads, dv)")
-    batch, time, kheads, dk = q.shape
-    heads, dv = v.shape[2:]
+class _DeltaPlan:
+    """A checked set of shapes and strides as the library takes it, with its workspace sizes."""
+
+    __slots__ = ("shape", "ref", "batch", "time", "heads", "dk", "dv", "_bytes")
+
+    def __init__(self, shape):
+        self.shape, self.ref = shape, C.byref(shape)
+        self.batch, self.time, self.heads, self.dk, self.dv = shape.batch, shape.time, shape.heads, shape.dk, shape.dv
+        self._bytes = {}
+
+    def workspace(self, kind, device):
+        size = self._bytes.get(kind)
+        if size is None:
+            out = C.c_int64()
+            N.check(N.lib().gjx_delta_filter_workspace(self.ref, kind, C.byref(out)), "gjx_delta_filter_workspace")
+            size = self._bytes[kind] = max(out.value, 256)
+        return torch.empty(size, dtype=torch.uint8, device=device)
+
+
+@functools.lru_cache(maxsize=1024)
+def _delta_plan(who, dtypes, q_shape, k_shape, v_shape, g_shape, b_shape, q_stride, k_stride, v_stride, g_stride, b_stride, scale):
+    if len(q_shape) != 4 or k_shape != q_shape or len(v_shape) != 4 or v_shape[:2] != q_shape[:2]:
+        raise GjxError(f"{who}: q {tuple(q_shape)} and k {tuple(k_shape)} must be (batch, time, key heads, dk) and v "
+                       f"{tuple(v_shape)} (batch, time, heads, dv)")
+    batch, time, kheads, dk = q_shape
+    heads, dv = v_shape[2:]
     if kheads < 1 or heads < 1 or heads % kheads:
         raise GjxError(f"{who}: {heads} heads must be a multiple of {kheads} key heads")
     if not (1 <= dk <= 128 and 1 <= dv <= 1024):
         raise GjxError(f"{who}: dk = {dk} must be in [1, 128] and dv = {dv} in [1, 1024]")
-    if tuple(log_decay.shape) != (batch, time, heads) or tuple(beta.shape) != (batch, time, heads):
-        raise GjxError(f"{who}: log_decay {tuple(log_decay.shape)} and beta {tuple(beta.shape)} must be {(batch, time, heads)}")
-    if q.dtype not in ELEMENT_TYPES or k.dtype != q.dtype or v.dtype != q.dtype:
-        raise GjxError(f"{who}: q, k and v must all be float32 or all bfloat16 (got {q.dtype}, {k.dtype}, {v.dtype})")
-    if log_decay.dtype != torch.float32 or beta.dtype != torch.float32:
-        raise GjxError(f"{who}: log_decay and beta must be float32 (got {log_decay.dtype}, {beta.dtype})")
-    _on_current_device(who, q=q, k=k, v=v, log_decay=log_decay, beta=beta)
-    s = N.DeltaShape(dtype=ELEMENT_TYPES[q.dtype], kheads=kheads, heads=heads, dk=dk, dv=dv,
-                     scale=float(dk ** -0.5 if scale is None else scale), batch=batch, time=time)
-    fits = lambda t: (t.stride(-1) == 1 or t.shape[-1] <= 1) and t.stride(1) <= 1 << 22       # noqa: E731
-    tensors = [t if fits(t) else t.contiguous() for t in (q, k, v)] + [log_decay, beta]
-    for name, t in zip("qkvgb", tensors):
-        setattr(s, f"{name}_stride", (C.c_int64 * 3)(*t.stride()[:3]))
-    return s, tensors
+    if g_shape != (batch, time, heads) or b_shape != (batch, time, heads):
+        raise GjxError(f"{who}: log_decay {tuple(g_shape)} and beta {tuple(b_shape)} must be {(batch, time, heads)}")
+    if dtypes[0] not in ELEMENT_TYPES or dtypes[1] != dtypes[0] or dtypes[2] != dtypes[0]:
+        raise GjxError(f"{who}: q, k and v must all be float32 or all bfloat16 (got {dtypes[0]}, {dtypes[1]}, {dtypes[2]})")
+    if dtypes[3] != torch.float32 or dtypes[4] != torch.float32:
+        raise GjxError(f"{who}: log_decay and beta must be float32 (got {dtypes[3]}, {dtypes[4]})")
+    three = C.c_int64 * 3
+    return _DeltaPlan(N.DeltaShape(ELEMENT_TYPES[dtypes[0]], kheads, heads, dk, dv, float(dk ** -0.5 if scale is None else scale),
+                                   batch, time, three(*q_stride[:3]), three(*k_stride[:3]), three(*v_stride[:3]),
+                                   three(*g_stride), three(*b_stride)))
 
 
-def _delta_state(who, name, state, s):
+def _delta_inputs(who, q, k, v, log_decay, beta, scale):
+    """Check the tensors of one call against each other; axes (batch, time, head, ...) -> (plan, tensors)."""
+    names = ("q", "k", "v", "log_decay", "beta")
+    for name, t in zip(names, (q, k, v, log_decay, beta)):
+        if not isinstance(t, torch.Tensor):
+            raise GjxError(f"{who}: `{name}` must be a tensor")
+    fits = lambda t: t.dim() != 4 or ((t.stride(3) == 1 or t.shape[3] <= 1) and t.stride(1) <= 1 << 22)      # noqa: E731
+    t = (q if fits(q) else q.contiguous(), k if fits(k) else k.contiguous(), v if fits(v) else v.contiguous(), log_decay, beta)
+    plan = _delta_plan(who, tuple(a.dtype for a in t), *(a.shape for a in t), *(a.stride() for a in t), scale)
+    _on_current_device(who, *zip(names, t))
+    return plan, t
+
+
+def _delta_state(who, name, state, p):
     """A (batch, heads, dk, dv) float32 state, contiguous."""
     if state is None:
         return None
-    if not isinstance(state, torch.Tensor) or tuple(state.shape) != (s.batch, s.heads, s.dk, s.dv) or state.dtype != torch.float32:
-        raise GjxError(f"{who}: `{name}` must be float32 of shape {(s.batch, s.heads, s.dk, s.dv)}")
-    _on_current_device(who, **{name: state})
+    if not isinstance(state, torch.Tensor) or state.shape != (p.batch, p.heads, p.dk, p.dv) or state.dtype != torch.float32:
+        raise GjxError(f"{who}: `{name}` must be float32 of shape {(p.batch, p.heads, p.dk, p.dv)}")
+    _on_current_device(who, (name, state))
     return state.contiguous()
 
 
-def _delta_lengths(who, lengths, s):
-    if lengths is None:
+def _delta_indices(who, name, t, p):
+    if t is None:
         return None
-    if not isinstance(lengths, torch.Tensor) or lengths.dtype != torch.int32 or tuple(lengths.shape) != (s.batch,):
-        raise GjxError(f"{who}: `lengths` must be int32 of shape ({s.batch},)")
-    _on_current_device(who, lengths=lengths)
-    return lengths.contiguous()
-
-
-def _delta_workspace(s, keep, device):
-    size = C.c_int64()
-    N.check(N.lib().gjx_delta_filter_workspace(C.byref(s), keep, C.byref(size)), "gjx_delta_filter_workspace")
-    return torch.empty(max(size.value, 256), dtype=torch.uint8, device=device)
-
-
-def _raw(t):
-    return C.c_void_p(0) if t is None else C.c_void_p(t.data_ptr())
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.shape != (p.batch,):
+        raise GjxError(f"{who}: `{name}` must be int32 of shape ({p.batch},)")
+    _on_current_device(who, (name, t))
+    return t.contiguous()
 
 
 def delta_filter(q, k, v, log_decay, beta, initial_state=None, scale=None, lengths=None, keep=False):
     """-> (o (batch, time, heads, dv), last state (batch, heads, dk, dv), the workspace the gradient reads or None)."""
     who = "delta_filter"
-    s, (q, k, v, g, be) = _delta_shape(who, q, k, v, log_decay, beta, scale)
-    state0, lengths = _delta_state(who, "initial_state", initial_state, s), _delta_lengths(who, lengths, s)
-    o = torch.empty((s.batch, s.time, s.heads, s.dv), dtype=v.dtype, device=v.device)
-    state = torch.empty((s.batch, s.heads, s.dk, s.dv), dtype=torch.float32, device=v.device)
-    work = _delta_workspace(s, int(keep), v.device)
-    N.check(N.lib().gjx_delta_filter(C.byref(s), _raw(q), _raw(k), _raw(v), _raw(g), _raw(be), _raw(state0), _raw(lengths), _raw(o),
-                                     _raw(state), int(keep), _raw(work), work.numel(), _stream()), "gjx_delta_filter")
+    p, (q, k, v, g, be) = _delta_inputs(who, q, k, v, log_decay, beta, scale)
+    state0, lengths = _delta_state(who, "initial_state", initial_state, p), _delta_indices(who, "lengths", lengths, p)
+    dev = v.device
+    o = torch.empty((p.batch, p.time, p.heads, p.dv), dtype=v.dtype, device=dev)
+    state = torch.empty((p.batch, p.heads, p.dk, p.dv), dtype=torch.float32, device=dev)
+    work = p.workspace(int(keep), dev)
+    N.check(N.lib().gjx_delta_filter(p.ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), be.data_ptr(), _address(state0),
+                                     _address(lengths), o.data_ptr(), state.data_ptr(), int(keep), work.data_ptr(), work.numel(),
+                                     _raw_stream()), "gjx_delta_filter")
     return o, state, work if keep else None
 
 
 def delta_filter_grad(q, k, v, log_decay, beta, d_o, d_state, kept, scale=None, lengths=None, want_state0=True):
     """Gradients (q, k, v, log_decay, beta, initial state or None) from the upstream ones of o and of the last state."""
     who = "delta_filter"
-    s, (q, k, v, g, be) = _delta_shape(who, q, k, v, log_decay, beta, scale)
-    lengths = _delta_lengths(who, lengths, s)
-    d_state = _delta_state(who, "d_state", d_state, s)
+    p, (q, k, v, g, be) = _delta_inputs(who, q, k, v, log_decay, beta, scale)
+    lengths = _delta_indices(who, "lengths", lengths, p)
+    d_state = _delta_state(who, "d_state", d_state, p)
     dev = v.device
-    d_o = torch.zeros((s.batch, s.time, s.heads, s.dv), dtype=v.dtype, device=dev) if d_o is None else d_o.contiguous()
+    d_o = torch.zeros((p.batch, p.time, p.heads, p.dv), dtype=v.dtype, device=dev) if d_o is None else d_o.contiguous()
     outs = [torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v, g, be)]
-    state0 = torch.empty((s.batch, s.heads, s.dk, s.dv), dtype=torch.float32, device=dev) if want_state0 else None
-    work = _delta_workspace(s, 2, dev)
-    N.check(N.lib().gjx_delta_filter_grad(C.byref(s), _raw(q), _raw(k), _raw(v), _raw(g), _raw(be), _raw(lengths), _raw(d_o),
-                                          _raw(d_state), *(_raw(t) for t in outs), _raw(state0), _raw(kept), kept.numel(),
-                                          _raw(work), work.numel(), _stream()), "gjx_delta_filter_grad")
+    state0 = torch.empty((p.batch, p.heads, p.dk, p.dv), dtype=torch.float32, device=dev) if want_state0 else None
+    work = p.workspace(2, dev)
+    N.check(N.lib().gjx_delta_filter_grad(p.ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), be.data_ptr(),
+                                          _address(lengths), d_o.data_ptr(), _address(d_state), *(t.data_ptr() for t in outs),
+                                          _address(state0), kept.data_ptr(), kept.numel(), work.data_ptr(), work.numel(),
+                                          _raw_stream()), "gjx_delta_filter_grad")
     return outs + [state0]
 
 
@@ -653,34 +690,45 @@ def _overlap(a, b):
     return lo_a < lo_b + b.numel() * b.element_size() and lo_b < lo_a + a.numel() * a.element_size()
 
 
+@functools.lru_cache(maxsize=1024)
+def _delta_step_plan(dtypes, q_shape, k_shape, v_shape, g_shape, b_shape, q_stride, k_stride, v_stride, g_stride, b_stride, scale):
+    who = "delta_filter_step"
+    for name, shape, d in (("q", q_shape, 3), ("k", k_shape, 3), ("v", v_shape, 3), ("log_decay", g_shape, 2), ("beta", b_shape, 2)):
+        if len(shape) != d:
+            raise GjxError(f"{who}: `{name}` must have {d} axes (particle, head{', entry' if d == 3 else ''})")
+    one = lambda t: (t[0], 1, *t[1:])                           # noqa: E731  a time axis of one token
+    return _delta_plan(who, dtypes, *map(one, (q_shape, k_shape, v_shape, g_shape, b_shape)),
+                       *map(one, (q_stride, k_stride, v_stride, g_stride, b_stride)), scale)
+
+
 def delta_filter_step(state, q, k, v, log_decay, beta, scale=None, ancestors=None, out=None):
     """One token per batch element: q, k (n, key heads, dk), v (n, heads, dv), gates (n, heads) -> (o (n, heads, dv), state)."""
     who = "delta_filter_step"
-    for name, t, d in (("q", q, 3), ("k", k, 3), ("v", v, 3), ("log_decay", log_decay, 2), ("beta", beta, 2)):
-        if not isinstance(t, torch.Tensor) or t.dim() != d:
-            raise GjxError(f"{who}: `{name}` must have {d} axes (particle, head{', entry' if d == 3 else ''})")
-    s, (q, k, v, g, be) = _delta_shape(who, *(t.unsqueeze(1) for t in (q, k, v, log_decay, beta)), scale)
-    state = _delta_state(who, "state", state, s)
+    names = ("q", "k", "v", "log_decay", "beta")
+    t = [q, k, v, log_decay, beta]
+    for i, name in enumerate(names):
+        if not isinstance(t[i], torch.Tensor):
+            raise GjxError(f"{who}: `{name}` must be a tensor")
+        if i < 3 and t[i].dim() > 0 and t[i].stride(-1) != 1 and t[i].shape[-1] > 1:
+            t[i] = t[i].contiguous()
+    p = _delta_step_plan(tuple(a.dtype for a in t), *(a.shape for a in t), *(a.stride() for a in t), scale)
     if state is None:
-        raise GjxError(f"{who}: `state` must be float32 of shape {(s.batch, s.heads, s.dk, s.dv)}")
-    if ancestors is not None:
-        if not isinstance(ancestors, torch.Tensor) or ancestors.dtype != torch.int32 or tuple(ancestors.shape) != (s.batch,):
-            raise GjxError(f"{who}: `ancestors` must be int32 of shape ({s.batch},)")
-        _on_current_device(who, ancestors=ancestors)
-        ancestors = ancestors.contiguous()
+        raise GjxError(f"{who}: `state` must be float32 of shape {(p.batch, p.heads, p.dk, p.dv)}")
+    state, ancestors = _delta_state(who, "state", state, p), _delta_indices(who, "ancestors", ancestors, p)
+    _on_current_device(who, *zip(names, t))
     if out is None:
         out = torch.empty_like(state)
     else:
         if not isinstance(out, torch.Tensor) or out.shape != state.shape or out.dtype != torch.float32 or not out.is_contiguous():
             raise GjxError(f"{who}: `out` must be contiguous float32 of shape {tuple(state.shape)}")
-        _on_current_device(who, out=out)
+        _on_current_device(who, ("out", out))
         if _overlap(out, state) and (ancestors is not None or out.data_ptr() != state.data_ptr()):
             raise GjxError(f"{who}: `out` may be the state itself without ancestors and must not overlap it otherwise")
     if state.data_ptr() % 16 or out.data_ptr() % 16:
         raise GjxError(f"{who}: states must be aligned to 16 bytes")
-    o = torch.empty((s.batch, s.heads, s.dv), dtype=v.dtype, device=v.device)
-    N.check(N.lib().gjx_delta_filter_step(C.byref(s), _raw(state), _raw(ancestors), _raw(q), _raw(k), _raw(v), _raw(g), _raw(be),
-                                          _raw(o), _raw(out), _stream()), "gjx_delta_filter_step")
+    o = torch.empty((p.batch, p.heads, p.dv), dtype=v.dtype, device=v.device)
+    N.check(N.lib().gjx_delta_filter_step(p.ref, state.data_ptr(), _address(ancestors), *(a.data_ptr() for a in t), o.data_ptr(),
+                                          out.data_ptr(), _raw_stream()), "gjx_delta_filter_step")
     return o, out
 
 

@@ -4,11 +4,15 @@
 // them to (max, sum exp) in the product's epilogue, the gradient forms them again piece by piece of the vocabulary,
 // turns them into d l = g (onehot(y) - exp(l - lse)) in that product's epilogue and feeds two more products,
 //   dx = dl W,   dW = dl^T x,   db = sum_i dl_i.
-// The products are 16x16x32 bf16 MFMA tiles with f32 accumulators.  f32 operands are split exactly into three
-// bf16 planes (8 + 8 + 8 bits) and the six partial products above 2^-24 are summed smallest first.
+// The products are 16x16x32 bf16 MFMA tiles with f32 accumulators.  f32 operands are split exactly into three bf16 planes
+// (8 bits each) and the six partial products above 2^-23 are summed.
+//
+// Three kernels: k_lincat_rows for few rows (the weights go once from memory to the matrix unit), k_lincat_gemm for bf16
+// (tiles straight into LDS), k_lincat_gemm32 for f32 (tiles split into planes on their way to LDS).
 #include "gjx_common.h"
 
 #include <algorithm>
+#include <atomic>
 
 typedef __bf16 bf16;
 typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -29,14 +33,21 @@ enum { EPI_SCORE = 0, EPI_DL = 1, EPI_STORE = 2, EPI_DRAW = 3 };
 // multiple of 8).  Indices beyond the end are clamped: what they add is discarded or multiplied by a zero.
 struct Operand {
   const bf16* p;
-  int64_t ld, plane;
+  int64_t ld;
   int rows, cols;
+};
+
+// an f32 operand: `rows` memory rows of `cols` valid entries
+struct OperandF {
+  const float* p;
+  int64_t ld;
+  int rows, cols, vec;   // vec: rows are aligned to 16 bytes
 };
 
 struct GemmArgs {
   Operand a, b;
-  int pairs;           // 1, or 6 partial products of three planes each
-  int ktiles;          // reduction length / 64
+  OperandF fa, fb;
+  int ktiles;          // reduction length / 64 (bf16), / 32 rounded up (f32)
   int mt, nt, splits;  // tiles along m and n, parts of the reduction
   // EPI_SCORE / EPI_DL: m = vocabulary entry (v0 = first of this piece), n = row
   int64_t v0, vocab, n;
@@ -50,10 +61,10 @@ struct GemmArgs {
   uint32_t key0, key1;
   uint64_t offset;
   const float *lse, *g;
-  bf16* dl;            // [planes][n_pad][dl_ld]
+  void* dl;            // [n_pad][dl_ld] of the operands' type
   float* resid;        // [n]: dl of the row's value less its bf16 rounding (bf16 only)
   const float* resid_in;   // EPI_STORE of dW: the same, added to the value's row
-  int64_t dl_ld, dl_plane;
+  int64_t dl_ld;
   float* db_part;      // [tile n][dl_ld]
   // EPI_STORE: out[n][m] (+ split * out_split), f32 or bf16
   void* out;
@@ -66,14 +77,29 @@ __device__ __forceinline__ float load_any(const void* p, int f32, int64_t i) {
 }
 
 // x = h + m + l exactly, each rounded to nearest (8 bits of the 24 apiece, signed): |m| <= 2^-8 |x|, |l| <= 2^-16 |x|, so the
-// partial products left out are at most 2^-23 |x| |w| each.  An h that would round to infinity is cut off instead; an
-// infinite x keeps h only.
-__device__ __forceinline__ void split3(float x, bf16& h, bf16& m, bf16& l) {
-  h = (bf16)x;
-  if (__builtin_isinf((float)h) && !__builtin_isinf(x)) h = (bf16)__uint_as_float(__float_as_uint(x) & 0xffff0000u);
-  const float r = __builtin_isinf(x) ? 0.0f : x - (float)h;
-  m = (bf16)r;
-  l = (bf16)(r - (float)m);
+// partial products left out are at most 2^-23 |x| |w| each.  What rounds to infinity in bf16 (above 3.389e38) counts as
+// infinite and keeps h only.
+__device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&out)[3]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const bf16 h = (bf16)x[j];
+    const float r = fabsf(x[j]) < 3.389e38f ? x[j] - (float)h : 0.0f;
+    const bf16 m = (bf16)r;
+    out[0][j] = h;
+    out[1][j] = m;
+    out[2][j] = (bf16)(r - (float)m);
+  }
+}
+
+__device__ __forceinline__ f32x4 mma(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+
+__device__ __forceinline__ f32x4 mma3(const bf16x8 (&a)[3], const bf16x8 (&b)[3], f32x4 c) {
+  c = mma(a[0], b[2], c);
+  c = mma(a[1], b[1], c);
+  c = mma(a[2], b[0], c);
+  c = mma(a[0], b[1], c);
+  c = mma(a[1], b[0], c);
+  return mma(a[0], b[0], c);
 }
 
 __device__ __forceinline__ int tr_swizzle(int k) { return (k & 3) | (((k >> 3) & 3) << 2); }
@@ -119,76 +145,50 @@ struct TileLoader {
   }
 };
 
-// C[m][n] = sum over plane pairs and k of A(m, k) B(n, k); BM x BN per workgroup of eight waves.  Two LDS buffers of
-// one 64-deep tile each: the loads of tile i + 1 run under the products of tile i, one barrier per tile.
-template <int BN, bool TA, bool TB, int EPI>
-__global__ void __launch_bounds__(GEMM_THREADS)
-    k_lincat_gemm(GemmArgs g) {
-  constexpr int WN = BN == 256 ? 4 : 2, WM = 8 / WN;       // waves along n and m
-  constexpr int MT = BM / WM / 16, NT = BN / WN / 16;
-  constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2, STAGE = A_BYTES + B_BYTES;
-  extern __shared__ char smem_raw[];
-  LDS_AS char* smem = (LDS_AS char*)smem_raw;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+// (max, sum exp) of two sets of logits; (largest value, its entry), ties to the lower entry
+__device__ __forceinline__ void merge_lse(float& top, float& sum, float top2, float sum2) {
+  const float nt = fmaxf(top, top2), b = nt == -__builtin_inff() ? 0.0f : nt;
+  sum = sum * expf(top - b) + sum2 * expf(top2 - b);
+  top = nt;
+}
+__device__ __forceinline__ void merge_best(float& best, int& arg, float best2, int arg2) {
+  if (arg2 != 0x7fffffff && (best2 > best || arg == 0x7fffffff || (best2 == best && arg2 < arg))) {
+    best = best2;
+    arg = arg2;
+  }
+}
 
-  // neighbouring tiles to one XCD (workgroups go round the eight of them), eight m-tiles by all n-tiles at a time
+// where a workgroup's tile lies
+struct Tile {
+  int split, tm, tn, m0, n0;
+};
+
+// neighbouring tiles to one XCD (workgroups go round the eight of them), eight m-tiles by all n-tiles at a time
+template <int BN>
+__device__ __forceinline__ Tile tile_of(const GemmArgs& g) {
   int id = blockIdx.x;
-  const int total = g.mt * g.nt * g.splits;
-  {
-    const int per = total / 8, extra = total % 8, xcd = id % 8;
-    id = xcd * per + min(xcd, extra) + id / 8;
-  }
-  const int split = id / (g.mt * g.nt);
-  id -= split * g.mt * g.nt;
+  const int total = g.mt * g.nt * g.splits, per = total / 8, extra = total % 8, xcd = id % 8;
+  id = xcd * per + min(xcd, extra) + id / 8;
+  Tile t;
+  t.split = id / (g.mt * g.nt);
+  id -= t.split * g.mt * g.nt;
   const int group = id / (8 * g.nt), in = id - group * 8 * g.nt, height = min(8, g.mt - group * 8);
-  const int tm = group * 8 + in % height, tn = in / height;
-  const int m0 = tm * BM, n0 = tn * BN;
+  t.tm = group * 8 + in % height;
+  t.tn = in / height;
+  t.m0 = t.tm * BM;
+  t.n0 = t.tn * BN;
+  return t;
+}
 
-  const int all = g.ktiles;
-  const int kt0 = (int)((int64_t)all * split / g.splits), kt1 = (int)((int64_t)all * (split + 1) / g.splits);
-  const int per_pair = kt1 - kt0, iters = per_pair * g.pairs;
-
-  f32x4 acc[MT][NT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-
-  auto issue = [&](int it, int buf) {
-    const int pair = it / per_pair, kt = kt0 + (it - pair * per_pair);
-    // (h l) (m m) (l h) (h m) (m h) (h h)
-    const int pa = g.pairs == 1 ? 0 : (0x010210 >> (4 * pair)) & 3;
-    const int pb = g.pairs == 1 ? 0 : (0x001012 >> (4 * pair)) & 3;
-    TileLoader<BM, TA>::load(g.a, g.a.p + pa * g.a.plane, m0, kt * BK, smem + buf * STAGE, tid);
-    TileLoader<BN, TB>::load(g.b, g.b.p + pb * g.b.plane, n0, kt * BK, smem + buf * STAGE + A_BYTES, tid);
-  };
-
+// what becomes of a tile's accumulators (rows m0 + wm + 16 i + 4 q + r, columns n0 + wn + 16 j + lane % 16); T: the operands' type
+template <typename T, int BN, int WM, int WN, int MT, int NT, bool TB, int EPI>
+__device__ __forceinline__ void epilogue(const GemmArgs& g, const Tile& tile, f32x4 (&acc)[MT][NT], char* smem_raw) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int split = tile.split, tm = tile.tm, tn = tile.tn, m0 = tile.m0, n0 = tile.n0;
   const int wm = (wave / WN) * (MT * 16), wn = (wave % WN) * (NT * 16);
-  if (iters > 0) issue(0, 0);
-  for (int it = 0; it < iters; ++it) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (it + 1 < iters) issue(it + 1, (it + 1) & 1);
-    LDS_AS char* sa = smem + (it & 1) * STAGE;
-    LDS_AS char* sb = sa + A_BYTES;
-#pragma unroll
-    for (int s = 0; s < BK / 32; ++s) {
-      bf16x8 fb[NT];
-#pragma unroll
-      for (int j = 0; j < NT; ++j) fb[j] = TileLoader<BN, TB>::frag(sb, wn + j * 16, s, lane);
-#pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        const bf16x8 fa = TileLoader<BM, TA>::frag(sa, wm + i * 16, s, lane);
-#pragma unroll
-        for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa, fb[j], acc[i][j], 0, 0, 0);
-      }
-    }
-  }
-  __syncthreads();
-
   const int q = lane >> 4, c = lane & 15;
   if (EPI == EPI_STORE) {
-    if (TB && g.resid_in) {
+    if (sizeof(T) == 2 && TB && g.resid_in) {
       // dW of the rows' own values: += resid_i x_i, in ascending i (every wave looks for its own columns)
       for (int64_t i0 = 0; i0 < g.n; i0 += 64) {
         const int64_t row = min(i0 + lane, g.n - 1);
@@ -290,10 +290,7 @@ __global__ void __launch_bounds__(GEMM_THREADS)
         for (int r = 0; r < 4; ++r) sum += expf(acc[i][j][r] - base);
 #pragma unroll
       for (int o = 16; o <= 32; o <<= 1) {
-        const float t2 = __shfl_xor(top, o), s2 = __shfl_xor(sum, o), nt = fmaxf(top, t2);
-        const float b2 = nt == -__builtin_inff() ? 0.0f : nt;
-        sum = sum * expf(top - b2) + s2 * expf(t2 - b2);
-        top = nt;
+        merge_lse(top, sum, __shfl_xor(top, o), __shfl_xor(sum, o));
       }
       if (q == 0) {
         s_red[((wave / WN) * BN + wn + j * 16 + c) * 2] = top;
@@ -305,10 +302,7 @@ __global__ void __launch_bounds__(GEMM_THREADS)
       float top = s_red[tid * 2], sum = s_red[tid * 2 + 1];
 #pragma unroll
       for (int w = 1; w < WM; ++w) {
-        const float t2 = s_red[(w * BN + tid) * 2], s2 = s_red[(w * BN + tid) * 2 + 1], nt = fmaxf(top, t2);
-        const float b2 = nt == -__builtin_inff() ? 0.0f : nt;
-        sum = sum * expf(top - b2) + s2 * expf(t2 - b2);
-        top = nt;
+        merge_lse(top, sum, s_red[(w * BN + tid) * 2], s_red[(w * BN + tid) * 2 + 1]);
       }
       g.part[(int64_t)(g.part_tile0 + tm) * g.n_pad + n0 + tid] = make_float2(top, sum);
     }
@@ -341,12 +335,7 @@ __global__ void __launch_bounds__(GEMM_THREADS)
           }
 #pragma unroll
       for (int o = 16; o <= 32; o <<= 1) {
-        const float b2 = __shfl_xor(best, o);
-        const int a2 = __shfl_xor(arg, o);
-        if (a2 != 0x7fffffff && (b2 > best || arg == 0x7fffffff || (b2 == best && a2 < arg))) {
-          best = b2;
-          arg = a2;
-        }
+        merge_best(best, arg, __shfl_xor(best, o), __shfl_xor(arg, o));
       }
       if (q == 0) {
         s_red[((wave / WN) * BN + wn + j * 16 + c) * 2] = best;
@@ -359,12 +348,7 @@ __global__ void __launch_bounds__(GEMM_THREADS)
       int arg = __float_as_int(s_red[tid * 2 + 1]);
 #pragma unroll
       for (int w = 1; w < WM; ++w) {
-        const float b2 = s_red[(w * BN + tid) * 2];
-        const int a2 = __float_as_int(s_red[(w * BN + tid) * 2 + 1]);
-        if (a2 != 0x7fffffff && (b2 > best || arg == 0x7fffffff)) {      // later waves hold later entries
-          best = b2;
-          arg = a2;
-        }
+        merge_best(best, arg, s_red[(w * BN + tid) * 2], __float_as_int(s_red[(w * BN + tid) * 2 + 1]));
       }
       g.part[(int64_t)(g.part_tile0 + tm) * g.n_pad + n0 + tid] = make_float2(best, __int_as_float(arg));
     }
@@ -393,8 +377,8 @@ __global__ void __launch_bounds__(GEMM_THREADS)
         d[r] = in ? up * ((y == i * 16 + r ? 1.0f : 0.0f) - expf(l - lse)) : 0.0f;
         dbs[i][r] += d[r];
       }
-      bf16* o = g.dl + n * g.dl_ld + (m0 + wm + i * 16 + 4 * q);
-      if (g.pairs == 1) {
+      T* o = (T*)g.dl + n * g.dl_ld + (m0 + wm + i * 16 + 4 * q);
+      if (sizeof(T) == 2) {
         // rounded to bf16 (the products that follow take bf16 operands): each entry is off by at most 2^-9 of it,
         // independently of its neighbours.  The value's own entry is usually far larger than the others, so that ONE
         // rounding would show in whole rows of the gradients: what it loses is kept apart and added in f32.
@@ -406,16 +390,7 @@ __global__ void __launch_bounds__(GEMM_THREADS)
         }
         *(bf16x4*)o = h;
       } else {
-        bf16x4 h, m, l;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          bf16 hh, mm, ll;
-          split3(d[r], hh, mm, ll);
-          h[r] = hh; m[r] = mm; l[r] = ll;
-        }
-        *(bf16x4*)o = h;
-        *(bf16x4*)(o + g.dl_plane) = m;
-        *(bf16x4*)(o + 2 * g.dl_plane) = l;
+        *(f32x4*)o = f32x4{d[0], d[1], d[2], d[3]};
       }
     }
   }
@@ -439,30 +414,296 @@ __global__ void __launch_bounds__(GEMM_THREADS)
   }
 }
 
-// rows x width of f32 or bf16 (row stride ld) -> planes of bf16 rows of width_pad, zeros behind the width
+// C[m][n] = sum_k A(m, k) B(n, k) in bf16; BM x BN per workgroup of eight waves.  Two LDS buffers of one 64-deep tile each:
+// the loads of tile i + 1 run under the products of tile i, one barrier per tile.
+template <int BN, bool TA, bool TB, int EPI>
+__global__ void __launch_bounds__(GEMM_THREADS)
+    k_lincat_gemm(GemmArgs g) {
+  constexpr int WN = BN == 256 ? 4 : 2, WM = 8 / WN;       // waves along n and m
+  constexpr int MT = BM / WM / 16, NT = BN / WN / 16;
+  constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2, STAGE = A_BYTES + B_BYTES;
+  extern __shared__ char smem_raw[];
+  LDS_AS char* smem = (LDS_AS char*)smem_raw;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const Tile tile = tile_of<BN>(g);
+  const int kt0 = (int)((int64_t)g.ktiles * tile.split / g.splits), kt1 = (int)((int64_t)g.ktiles * (tile.split + 1) / g.splits);
+
+  f32x4 acc[MT][NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+  auto issue = [&](int kt, int buf) {
+    TileLoader<BM, TA>::load(g.a, g.a.p, tile.m0, kt * BK, smem + buf * STAGE, tid);
+    TileLoader<BN, TB>::load(g.b, g.b.p, tile.n0, kt * BK, smem + buf * STAGE + A_BYTES, tid);
+  };
+
+  const int wm = (wave / WN) * (MT * 16), wn = (wave % WN) * (NT * 16);
+  if (kt0 < kt1) issue(kt0, 0);
+  for (int kt = kt0; kt < kt1; ++kt) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (kt + 1 < kt1) issue(kt + 1, (kt + 1 - kt0) & 1);
+    LDS_AS char* sa = smem + ((kt - kt0) & 1) * STAGE;
+    LDS_AS char* sb = sa + A_BYTES;
+#pragma unroll
+    for (int s = 0; s < BK / 32; ++s) {
+      bf16x8 fb[NT];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) fb[j] = TileLoader<BN, TB>::frag(sb, wn + j * 16, s, lane);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const bf16x8 fa = TileLoader<BM, TA>::frag(sa, wm + i * 16, s, lane);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = mma(fa, fb[j], acc[i][j]);
+      }
+    }
+  }
+  __syncthreads();
+  epilogue<bf16, BN, WM, WN, MT, NT, TB, EPI>(g, tile, acc, smem_raw);
+}
+
+// one 32-deep slab of an f32 operand, R output indices wide: pieces of eight reduction entries of one output index, loaded
+// into registers, split and written to LDS as fragments (16 indices x 3 planes x 64 lanes x 16 bytes)
+template <int R, bool T>
+struct SlabLoader {
+  static constexpr int PIECES = (R * 4 + GEMM_THREADS - 1) / GEMM_THREADS;
+  float x[PIECES][8];
+
+  static __device__ __forceinline__ void where(int u, int& index, int& group) {
+    if (T) {
+      index = u % R;          // neighbouring lanes take neighbouring columns
+      group = u / R;
+    } else {
+      index = u >> 2;         // four lanes take a row's 128 bytes
+      group = u & 3;
+    }
+  }
+  __device__ __forceinline__ void load(const OperandF& o, int out0, int k0, int tid) {
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      const int u = i * GEMM_THREADS + tid;
+      int index, group;
+      where(min(u, R * 4 - 1), index, group);
+      const int k = k0 + 8 * group;
+      if (T) {
+        const float* p = o.p + min(out0 + index, o.cols - 1);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[i][j] = k + j < o.rows ? p[(int64_t)(k + j) * o.ld] : 0.0f;
+      } else {
+        const float* p = o.p + (int64_t)min(out0 + index, o.rows - 1) * o.ld + k;
+        if (o.vec && k + 8 <= o.cols) {
+          const f32x4 lo = *(const f32x4*)p, hi = *(const f32x4*)(p + 4);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            x[i][j] = lo[j];
+            x[i][4 + j] = hi[j];
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[i][j] = k + j < o.cols ? p[j] : 0.0f;
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void store(char* lds, int tid) const {
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      const int u = i * GEMM_THREADS + tid;
+      if (R * 4 % GEMM_THREADS && u >= R * 4) continue;
+      int index, group;
+      where(u, index, group);
+      bf16x8 o[3];
+      split8(x[i], o);
+      char* f = lds + (index >> 4) * 3072 + ((index & 15) + 16 * group) * 16;
+#pragma unroll
+      for (int p = 0; p < 3; ++p) *(bf16x8*)(f + p * 1024) = o[p];
+    }
+  }
+  static __device__ __forceinline__ void frag(const char* lds, int i0, int lane, bf16x8 (&out)[3]) {
+#pragma unroll
+    for (int p = 0; p < 3; ++p) out[p] = *(const bf16x8*)(lds + (i0 >> 4) * 3072 + p * 1024 + lane * 16);
+  }
+};
+
+// the same product of f32 operands: six matrix instructions per fragment pair, so the splitting (once per tile) and the
+// LDS traffic are small beside them and no packed copy of the operands is needed (packing to bf16 planes first: pack and
+// product 328 us for 200 x 50001 x 768).  Two LDS buffers of one 32-deep slab, the slab after that in registers.
+template <int BN, bool TA, bool TB, int EPI>
+__global__ void __launch_bounds__(GEMM_THREADS, 2)
+    k_lincat_gemm32(GemmArgs g) {
+  constexpr int WN = 2, WM = 4, MT = BM / WM / 16, NT = BN / WN / 16;
+  constexpr int A_BYTES = BM / 16 * 3072, STAGE = A_BYTES + BN / 16 * 3072;
+  extern __shared__ char smem_raw[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const Tile tile = tile_of<BN>(g);
+  const int kt0 = (int)((int64_t)g.ktiles * tile.split / g.splits), kt1 = (int)((int64_t)g.ktiles * (tile.split + 1) / g.splits);
+  f32x4 acc[MT][NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  const int wm = (wave / WN) * (MT * 16), wn = (wave % WN) * (NT * 16);
+  SlabLoader<BM, TA> la;
+  SlabLoader<BN, TB> lb;
+  if (kt0 < kt1) {
+    la.load(g.fa, tile.m0, kt0 * 32, tid);
+    lb.load(g.fb, tile.n0, kt0 * 32, tid);
+  }
+  for (int kt = kt0; kt < kt1; ++kt) {
+    char* sa = smem_raw + ((kt - kt0) & 1) * STAGE;
+    char* sb = sa + A_BYTES;
+    la.store(sa, tid);
+    lb.store(sb, tid);
+    __syncthreads();           // this buffer is written; the other one is written again only behind the next barrier
+    if (kt + 1 < kt1) {
+      la.load(g.fa, tile.m0, (kt + 1) * 32, tid);
+      lb.load(g.fb, tile.n0, (kt + 1) * 32, tid);
+    }
+    bf16x8 fb[NT][3];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) SlabLoader<BN, TB>::frag(sb, wn + j * 16, lane, fb[j]);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      bf16x8 fa[3];
+      SlabLoader<BM, TA>::frag(sa, wm + i * 16, lane, fa);
+#pragma unroll
+      for (int j = 0; j < NT; ++j) acc[i][j] = mma3(fa, fb[j], acc[i][j]);
+    }
+  }
+  __syncthreads();
+  epilogue<float, BN, WM, WN, MT, NT, TB, EPI>(g, tile, acc, smem_raw);
+}
+
+// few rows (n <= 16 NT): a wave takes 16 entries of the vocabulary, the weights go from memory to the matrix unit without
+// a stop, the rows of x (a few KB) come from the caches.  Partial results per 64 entries.
+template <typename T, int NT, int EPI>
 __global__ void __launch_bounds__(GJX_BLOCK)
-    k_lincat_pack(const void* __restrict__ src, int f32, int64_t ld, int64_t rows, int width, int width_pad,
-                  bf16* __restrict__ dst, int64_t plane) {
+    k_lincat_rows(GemmArgs g, const T* __restrict__ x, int64_t x_ld, const T* __restrict__ w, int64_t w_ld, int width, int vec) {
+  constexpr int P = sizeof(T) == 4 ? 3 : 1, U = sizeof(T) == 4 ? 4 : 8;      // planes; slabs in flight
+  __shared__ float s_red[4][16 * NT][2];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, c = lane & 15;
+  const int v0 = blockIdx.x * 64 + wave * 16;
+  const T* wp = w + min((int64_t)v0 + c, g.vocab - 1) * w_ld;
+  const T* xp[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) xp[j] = x + min((int64_t)(j * 16 + c), g.n - 1) * x_ld;
+  auto load = [&](const T* p, int k, float (&f)[8], bf16x8& h) {       // eight entries from k (a multiple of 8) on, zeros behind the end
+    if (vec && k + 8 <= width) {
+      if (P == 1) {
+        h = *(const bf16x8*)(p + k);
+      } else {
+        const f32x4 lo = *(const f32x4*)(p + k), hi = *(const f32x4*)(p + k + 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          f[e] = lo[e];
+          f[4 + e] = hi[e];
+        }
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const T t = k + e < width ? p[k + e] : (T)0.0f;
+        if (P == 1) h[e] = (bf16)t;
+        else f[e] = (float)t;
+      }
+    }
+  };
+  f32x4 acc[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int k0 = 0; k0 < width; k0 += 32 * U) {
+    float fw[U][8];
+    bf16x8 hw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) load(wp, k0 + 32 * u + 8 * q, fw[u], hw[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      bf16x8 a[3];
+      if (P == 3) split8(fw[u], a);
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        float fx[8];
+        bf16x8 hx, b[3];
+        load(xp[j], k0 + 32 * u + 8 * q, fx, hx);
+        if (P == 1) {
+          acc[j] = mma(hw[u], hx, acc[j]);
+        } else {
+          split8(fx, b);
+          acc[j] = mma3(a, b, acc[j]);
+        }
+      }
+    }
+  }
+  float bias[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int64_t v = v0 + 4 * q + r;
+    bias[r] = v < g.vocab ? (g.bias ? load_any(g.bias, g.bias_f32, v) : 0.0f) : -__builtin_inff();
+  }
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const int64_t n = j * 16 + c;
+    float top = -__builtin_inff(), sum = 0.0f;
+    int arg = 0x7fffffff;
+    if (EPI == EPI_SCORE) {
+      const int64_t y = n < g.n ? min(max((int64_t)g.y[n], (int64_t)0), g.vocab - 1) - v0 - 4 * q : -1;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        acc[j][r] = bias[r] == -__builtin_inff() ? bias[r] : acc[j][r] + bias[r];
+        top = fmaxf(top, acc[j][r]);
+        if (y == r) g.target[n] = acc[j][r];
+      }
+      const float base = top == -__builtin_inff() ? 0.0f : top;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) sum += expf(acc[j][r] - base);
+    } else if (n < g.n) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int v = v0 + 4 * q + r;
+        const float u = gjx_uniform_at(g.key0, g.key1, (g.offset + (uint64_t)n) * (uint64_t)g.vocab + (uint64_t)v, 1.17549435e-38f, 1.0f);
+        const float val = bias[r] == -__builtin_inff() ? bias[r] : acc[j][r] + bias[r] + (-logf(-logf(u)));
+        if (v < g.vocab && (val > top || arg == 0x7fffffff)) {
+          top = val;
+          arg = v;
+        }
+      }
+    }
+#pragma unroll
+    for (int o = 16; o <= 32; o <<= 1) {
+      if (EPI == EPI_SCORE) merge_lse(top, sum, __shfl_xor(top, o), __shfl_xor(sum, o));
+      else merge_best(top, arg, __shfl_xor(top, o), __shfl_xor(arg, o));
+    }
+    if (q == 0) {
+      s_red[wave][j * 16 + c][0] = top;
+      s_red[wave][j * 16 + c][1] = EPI == EPI_SCORE ? sum : __int_as_float(arg);
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x < 16 * NT) {
+    float top = s_red[0][threadIdx.x][0], sum = s_red[0][threadIdx.x][1];
+    int arg = __float_as_int(sum);
+#pragma unroll
+    for (int i = 1; i < 4; ++i) {
+      if (EPI == EPI_SCORE) merge_lse(top, sum, s_red[i][threadIdx.x][0], s_red[i][threadIdx.x][1]);
+      else merge_best(top, arg, s_red[i][threadIdx.x][0], __float_as_int(s_red[i][threadIdx.x][1]));
+    }
+    g.part[(int64_t)blockIdx.x * g.n_pad + threadIdx.x] = make_float2(top, EPI == EPI_SCORE ? sum : __int_as_float(arg));
+  }
+}
+
+// bf16 rows of any stride and width -> rows of width_pad, zeros behind the width
+__global__ void __launch_bounds__(GJX_BLOCK)
+    k_lincat_pack(const bf16* __restrict__ src, int64_t ld, int64_t rows, int width, int width_pad, bf16* __restrict__ dst) {
   const int64_t total = rows * (width_pad / 8);
   for (int64_t i = (int64_t)blockIdx.x * GJX_BLOCK + threadIdx.x; i < total; i += (int64_t)gridDim.x * GJX_BLOCK) {
     const int64_t row = i / (width_pad / 8);
     const int c0 = (int)(i - row * (width_pad / 8)) * 8;
-    bf16x8 h, m, l;
+    bf16x8 h;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      bf16 hh = (bf16)0.0f, mm = (bf16)0.0f, ll = (bf16)0.0f;
-      if (c0 + k < width) {
-        if (f32) split3(((const float*)src)[row * ld + c0 + k], hh, mm, ll);
-        else hh = ((const bf16*)src)[row * ld + c0 + k];
-      }
-      h[k] = hh; m[k] = mm; l[k] = ll;
-    }
-    bf16* o = dst + row * width_pad + c0;
-    *(bf16x8*)o = h;
-    if (f32) {
-      *(bf16x8*)(o + plane) = m;
-      *(bf16x8*)(o + 2 * plane) = l;
-    }
+    for (int k = 0; k < 8; ++k) h[k] = c0 + k < width ? src[row * ld + c0 + k] : (bf16)0.0f;
+    *(bf16x8*)(dst + row * width_pad + c0) = h;
   }
 }
 
@@ -474,11 +715,7 @@ __global__ void __launch_bounds__(GJX_BLOCK)
   const int col = threadIdx.x % width, grp = threadIdx.x / width, groups = GJX_BLOCK / width;
   const int64_t i = (int64_t)blockIdx.x * width + col;
   float top = -__builtin_inff(), sum = 0.0f;
-  auto merge = [&](float2 p) {
-    const float nt = fmaxf(top, p.x), b = nt == -__builtin_inff() ? 0.0f : nt;
-    sum = sum * expf(top - b) + p.y * expf(p.x - b);
-    top = nt;
-  };
+  auto merge = [&](float2 p) { merge_lse(top, sum, p.x, p.y); };
   if (i < n)
     for (int t = grp; t < tiles; t += groups) merge(part[(int64_t)t * n_pad + i]);
   sm[threadIdx.x] = make_float2(top, sum);
@@ -492,7 +729,7 @@ __global__ void __launch_bounds__(GJX_BLOCK)
   }
   if (grp == 0 && i < n) {
     const float l = top + logf(sum);
-    lse[i] = l;
+    if (lse) lse[i] = l;
     lp[i] = target[i] - l;
   }
 }
@@ -546,16 +783,37 @@ __global__ void __launch_bounds__(GJX_BLOCK)
 // ---------------------------------------------------------------------------
 constexpr int64_t DL_BYTES = (int64_t)512 << 20;      // dl of one piece of the vocabulary (any size is right)
 constexpr int64_t PACK_BYTES = (int64_t)512 << 20;    // packed weights of one piece
+constexpr int ROWS_MAX = 32;                          // rows up to which k_lincat_rows is used
 
 int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 
+// a call's inputs
+struct Call {
+  const char* who;
+  int dtype;
+  const int32_t* y;
+  const void* x;
+  int64_t x_ld;
+  const void* w;
+  int64_t w_ld;
+  const void* bias;
+  int64_t n, vocab, width;
+  bool f32() const { return dtype == GJX_F32; }
+  const char* w_row(int64_t v) const { return (const char*)w + v * w_ld * (f32() ? 4 : 2); }
+};
+
+// rows a tile loader can take as they are: aligned to 16 bytes, whole 64-deep tiles
+bool direct(const void* p, int64_t ld, int64_t width) { return ((uintptr_t)p & 15) == 0 && ld % 8 == 0 && width % 64 == 0; }
+// ... a vector load can take: aligned to 16 bytes
+bool vector_rows(const Call& c, const void* p, int64_t ld) { return ((uintptr_t)p & 15) == 0 && ld % (c.f32() ? 4 : 8) == 0; }
+
 struct Plan {
-  int planes, pairs;
+  bool rows;                    // k_lincat_rows
   int bn;                       // rows per tile
   int64_t kp, n_pad, n_tiles;
-  int pack_x, pack_w;
+  bool pack_x, pack_w;
   int64_t piece;                // vocabulary entries per piece (multiple of 256)
-  int64_t tiles;                // tiles of 256 over the whole vocabulary
+  int64_t tiles;                // partial results per row
   int splits;                   // parts of dx's reduction
   int64_t o_x, o_w, o_part, o_target, o_dl, o_db, o_dx, o_resid, bytes;
 };
@@ -569,75 +827,208 @@ struct Carver {
   }
 };
 
-bool direct(const void* p, int64_t ld, int64_t width) {
-  return ((uintptr_t)p & 15) == 0 && ld % 8 == 0 && width % 64 == 0;
-}
-
-Plan plan_of(int dtype, int64_t n, int64_t vocab, int64_t width, int pack_x, int pack_w, bool grad, bool want_dx) {
+Plan plan_of(const Call& c, bool grad, bool want_dx) {
   Plan p = {};
-  p.planes = dtype == GJX_F32 ? 3 : 1;
-  p.pairs = dtype == GJX_F32 ? 6 : 1;
-  p.kp = up(width, 64);
-  p.pack_x = pack_x;
-  p.pack_w = pack_w;
-  p.tiles = up(vocab, BM) / BM;
-  p.bn = (n > 64 && up(n, 256) / 256 * p.tiles >= 256) ? 256 : 64;
-  p.n_pad = up(n, p.bn);
+  const int64_t vt = up(c.vocab, BM) / BM;
+  p.rows = !grad && c.n <= ROWS_MAX;
+  p.kp = c.f32() ? c.width : up(c.width, 64);
+  p.pack_x = !c.f32() && !p.rows && !direct(c.x, c.x_ld, c.width);
+  p.pack_w = !c.f32() && !p.rows && !direct(c.w, c.w_ld, c.width);
+  // wide tiles where there are enough of them to fill the 256 CUs; f32 tiles are half as wide (three planes in LDS)
+  const int wide = c.f32() ? 128 : 256;
+  p.bn = (c.n > 64 && up(c.n, wide) / wide * vt >= 256) ? wide : 64;
+  p.n_pad = p.rows ? up(c.n, 16) : up(c.n, p.bn);
   p.n_tiles = p.n_pad / p.bn;
-  int64_t piece = p.tiles * BM;
-  if (pack_w) piece = std::min(piece, std::max<int64_t>(BM, PACK_BYTES / (p.kp * 2 * p.planes) / BM * BM));
-  if (grad) piece = std::min(piece, std::max<int64_t>(BM, DL_BYTES / (p.n_pad * 2 * p.planes) / BM * BM));
-  const int64_t pieces = up(p.tiles * BM, piece) / piece;
-  p.piece = up(up(p.tiles, pieces) / pieces * BM, BM);      // equal pieces
-  Carver c;
-  p.o_x = c.take(pack_x ? n * p.kp * 2 * p.planes : 0);
-  p.o_w = c.take(pack_w ? p.piece * p.kp * 2 * p.planes : 0);
+  p.tiles = p.rows ? up(c.vocab, 64) / 64 : vt;
+  const int64_t e = c.f32() ? 4 : 2;
+  int64_t piece = vt * BM;
+  if (p.pack_w) piece = std::min(piece, std::max<int64_t>(BM, PACK_BYTES / (p.kp * 2) / BM * BM));
+  if (grad) piece = std::min(piece, std::max<int64_t>(BM, DL_BYTES / (p.n_pad * e) / BM * BM));
+  const int64_t pieces = up(vt * BM, piece) / piece;
+  p.piece = up(up(vt, pieces) / pieces * BM, BM);           // equal pieces
+  Carver k;
+  p.o_x = k.take(p.pack_x ? c.n * p.kp * 2 : 0);
+  p.o_w = k.take(p.pack_w ? p.piece * p.kp * 2 : 0);
   if (grad) {
-    p.o_dl = c.take(p.n_pad * p.piece * 2 * p.planes);
-    p.o_db = c.take(p.n_tiles * p.piece * 4);
-    p.o_resid = c.take(n * 4);
-    const int64_t tiles = up(width, BM) / BM * p.n_tiles;
+    p.o_dl = k.take(p.n_pad * p.piece * e);
+    p.o_db = k.take(p.n_tiles * p.piece * 4);
+    p.o_resid = k.take(c.n * 4);
+    const int64_t tiles = up(c.width, BM) / BM * p.n_tiles;
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(512 / tiles, p.piece / BK / 8));
-    p.o_dx = c.take(want_dx ? (int64_t)p.splits * n * p.kp * 4 : 0);
+    p.o_dx = k.take(want_dx ? (int64_t)p.splits * c.n * up(p.kp, 4) * 4 : 0);
   } else {
-    p.o_part = c.take(p.tiles * p.n_pad * 8);
-    p.o_target = c.take(n * 4);
+    p.o_part = k.take(p.tiles * p.n_pad * 8);
+    p.o_target = k.take(c.n * 4);
   }
-  p.bytes = c.at;
+  p.bytes = k.at;
   return p;
 }
 
+// a kernel's dynamic LDS limit, raised once per device
+template <typename K>
+int32_t allow_lds(K* kernel, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  GJX_CHECK_HIP(hipGetDevice(&dev));
+  if (dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1)) return GJX_OK;
+  GJX_CHECK_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  if (dev < 64) done.fetch_or((uint64_t)1 << dev, std::memory_order_relaxed);
+  return GJX_OK;
+}
+
 template <int BN, bool TA, bool TB, int EPI>
-int32_t launch_gemm(const GemmArgs& a, hipStream_t s) {
-  const int64_t blocks = (int64_t)a.mt * a.nt * a.splits;
-  GJX_REQUIRE(blocks < ((int64_t)1 << 31), GJX_ELIMIT, "linear_categorical: %lld tiles", (long long)blocks);
+int32_t launch16(const GemmArgs& a, unsigned blocks, hipStream_t s) {
+  static std::atomic<uint64_t> done{0};
   constexpr int lds = 2 * (BM + BN) * BK * 2;
-  GJX_CHECK_HIP(hipFuncSetAttribute((const void*)k_lincat_gemm<BN, TA, TB, EPI>, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-  k_lincat_gemm<BN, TA, TB, EPI><<<(unsigned)blocks, GEMM_THREADS, lds, s>>>(a);
+  const int32_t rc = allow_lds(k_lincat_gemm<BN, TA, TB, EPI>, lds, done);
+  if (rc != GJX_OK) return rc;
+  k_lincat_gemm<BN, TA, TB, EPI><<<blocks, GEMM_THREADS, lds, s>>>(a);
   GJX_LAUNCH_CHECK();
   return GJX_OK;
 }
 
-int32_t pack(const void* src, int dtype, int64_t ld, int64_t rows, int64_t width, int64_t kp, bf16* dst, int64_t plane,
-             hipStream_t s) {
-  k_lincat_pack<<<gjx_grid_for(rows * (kp / 8)), GJX_BLOCK, 0, s>>>(src, dtype == GJX_F32, ld, rows, (int)width, (int)kp, dst, plane);
+template <int BN, bool TA, bool TB, int EPI>
+int32_t launch32(const GemmArgs& a, unsigned blocks, hipStream_t s) {
+  static std::atomic<uint64_t> done{0};
+  constexpr int lds = 2 * (BM + BN) / 16 * 3072;
+  const int32_t rc = allow_lds(k_lincat_gemm32<BN, TA, TB, EPI>, lds, done);
+  if (rc != GJX_OK) return rc;
+  k_lincat_gemm32<BN, TA, TB, EPI><<<blocks, GEMM_THREADS, lds, s>>>(a);
   GJX_LAUNCH_CHECK();
   return GJX_OK;
 }
 
-const char* at_row(const void* p, int dtype, int64_t elements) {
-  return (const char*)p + elements * (dtype == GJX_F32 ? 4 : 2);
+// wide: the larger of the two row tiles
+template <bool TA, bool TB, int EPI>
+int32_t launch(const Call& c, bool wide, const GemmArgs& a, hipStream_t s) {
+  const int64_t blocks = (int64_t)a.mt * a.nt * a.splits;
+  GJX_REQUIRE(blocks < ((int64_t)1 << 31), GJX_ELIMIT, "%s: %lld tiles", c.who, (long long)blocks);
+  if constexpr (TB) {           // dW: n is the vocabulary, always wide
+    return c.f32() ? launch32<128, TA, TB, EPI>(a, (unsigned)blocks, s) : launch16<256, TA, TB, EPI>(a, (unsigned)blocks, s);
+  } else {
+    if (c.f32()) return wide ? launch32<128, TA, TB, EPI>(a, (unsigned)blocks, s) : launch32<64, TA, TB, EPI>(a, (unsigned)blocks, s);
+    return wide ? launch16<256, TA, TB, EPI>(a, (unsigned)blocks, s) : launch16<64, TA, TB, EPI>(a, (unsigned)blocks, s);
+  }
 }
 
-int32_t check_args(const char* who, const int32_t* y, const void* x, int64_t x_ld, const void* w, int64_t w_ld, int dtype,
-                   int64_t n, int64_t vocab, int64_t width) {
-  GJX_REQUIRE(dtype == GJX_F32 || dtype == GJX_BF16, GJX_EINVAL, "%s: dtype %d is neither GJX_F32 nor GJX_BF16", who, dtype);
-  GJX_REQUIRE(n >= 0 && vocab >= 1 && width >= 1, GJX_EINVAL, "%s: bad sizes (n %lld, vocab %lld, width %lld)", who,
-              (long long)n, (long long)vocab, (long long)width);
-  GJX_REQUIRE(n == 0 || (y && x && w), GJX_EINVAL, "%s: null input", who);
-  GJX_REQUIRE(x_ld >= width && w_ld >= width, GJX_EINVAL, "%s: a row stride is smaller than the width", who);
-  GJX_REQUIRE(n <= GJX_MAX_LINCAT && vocab <= GJX_MAX_LINCAT && width <= 65536, GJX_ELIMIT,
-              "%s: n and vocab go up to 2^24, width up to 65536", who);
+int32_t pack(const void* src, int64_t ld, int64_t rows, int64_t width, int64_t kp, bf16* dst, hipStream_t s) {
+  k_lincat_pack<<<gjx_grid_for(rows * (kp / 8)), GJX_BLOCK, 0, s>>>((const bf16*)src, ld, rows, (int)width, (int)kp, dst);
+  GJX_LAUNCH_CHECK();
+  return GJX_OK;
+}
+
+int32_t check_args(const Call& c) {
+  GJX_REQUIRE(c.dtype == GJX_F32 || c.dtype == GJX_BF16, GJX_EINVAL, "%s: dtype %d is neither GJX_F32 nor GJX_BF16", c.who, c.dtype);
+  GJX_REQUIRE(c.n >= 0 && c.vocab >= 1 && c.width >= 1, GJX_EINVAL, "%s: bad sizes (n %lld, vocab %lld, width %lld)", c.who,
+              (long long)c.n, (long long)c.vocab, (long long)c.width);
+  GJX_REQUIRE(c.n == 0 || (c.y && c.x && c.w), GJX_EINVAL, "%s: null input", c.who);
+  GJX_REQUIRE(c.x_ld >= c.width && c.w_ld >= c.width, GJX_EINVAL, "%s: a row stride is smaller than the width", c.who);
+  GJX_REQUIRE(c.n <= GJX_MAX_LINCAT && c.vocab <= GJX_MAX_LINCAT && c.width <= 65536, GJX_ELIMIT,
+              "%s: n and vocab go up to 2^24, width up to 65536", c.who);
+  return GJX_OK;
+}
+
+int32_t check_work(const Call& c, const Plan& p, const void* work, int64_t bytes) {
+  GJX_REQUIRE(work && ((uintptr_t)work & 255) == 0 && bytes >= p.bytes, GJX_EINVAL,
+              "%s: the workspace has %lld bytes, needs %lld aligned to 256", c.who, (long long)bytes, (long long)p.bytes);
+  return GJX_OK;
+}
+
+GemmArgs common_args(const Call& c, const Plan& p) {
+  GemmArgs a = {};
+  a.splits = 1;
+  a.vocab = c.vocab;
+  a.n = c.n;
+  a.n_pad = p.n_pad;
+  a.bias = c.bias;
+  a.bias_f32 = c.f32();
+  a.y = c.y;
+  return a;
+}
+
+// x and `rows` rows of W from v0 on as operands, packed where the tile loader needs it
+struct Inputs {
+  Operand x, w;
+  OperandF fx, fw;
+};
+
+int32_t take_x(const Call& c, const Plan& p, char* ws, Inputs& in, hipStream_t s) {
+  in.fx = {(const float*)c.x, c.x_ld, (int)c.n, (int)c.width, vector_rows(c, c.x, c.x_ld)};
+  in.x = {(const bf16*)c.x, c.x_ld, (int)c.n, (int)p.kp};
+  if (!p.pack_x) return GJX_OK;
+  in.x = {(const bf16*)(ws + p.o_x), p.kp, (int)c.n, (int)p.kp};
+  return pack(c.x, c.x_ld, c.n, c.width, p.kp, (bf16*)(ws + p.o_x), s);
+}
+
+int32_t take_w(const Call& c, const Plan& p, char* ws, int64_t v0, int64_t rows, Inputs& in, hipStream_t s) {
+  const char* w = c.w_row(v0);
+  in.fw = {(const float*)w, c.w_ld, (int)rows, (int)c.width, vector_rows(c, w, c.w_ld)};
+  in.w = {(const bf16*)w, c.w_ld, (int)rows, (int)p.kp};
+  if (!p.pack_w) return GJX_OK;
+  in.w = {(const bf16*)(ws + p.o_w), p.kp, (int)rows, (int)p.kp};
+  return pack(w, c.w_ld, rows, c.width, p.kp, (bf16*)(ws + p.o_w), s);
+}
+
+int depth_tiles(const Call& c, int64_t depth) { return (int)(c.f32() ? up(depth, 32) / 32 : up(depth, BK) / BK); }
+
+// the forward product, reduced to log-densities (EPI_SCORE) or draws (EPI_DRAW)
+struct Forward {
+  float *lp, *lse;
+  uint32_t key0, key1;
+  uint64_t offset;
+  int32_t* out;
+};
+
+template <typename T, int EPI>
+int32_t launch_rows(const Call& c, const Plan& p, const GemmArgs& a, hipStream_t s) {
+  const int vec = vector_rows(c, c.x, c.x_ld) && vector_rows(c, c.w, c.w_ld);
+  const unsigned blocks = (unsigned)p.tiles;
+  if (p.n_pad == 16) k_lincat_rows<T, 1, EPI><<<blocks, GJX_BLOCK, 0, s>>>(a, (const T*)c.x, c.x_ld, (const T*)c.w, c.w_ld, (int)c.width, vec);
+  else k_lincat_rows<T, 2, EPI><<<blocks, GJX_BLOCK, 0, s>>>(a, (const T*)c.x, c.x_ld, (const T*)c.w, c.w_ld, (int)c.width, vec);
+  GJX_LAUNCH_CHECK();
+  return GJX_OK;
+}
+
+template <int EPI>
+int32_t forward(const Call& c, const Forward& f, void* d_work, int64_t work_bytes, hipStream_t s) {
+  const Plan p = plan_of(c, false, false);
+  int32_t rc = check_work(c, p, d_work, work_bytes);
+  if (rc != GJX_OK) return rc;
+  char* ws = (char*)d_work;
+  GemmArgs a = common_args(c, p);
+  a.key0 = f.key0;
+  a.key1 = f.key1;
+  a.offset = f.offset;
+  a.part = (float2*)(ws + p.o_part);
+  a.target = (float*)(ws + p.o_target);
+  if (p.rows) {
+    rc = c.f32() ? launch_rows<float, EPI>(c, p, a, s) : launch_rows<bf16, EPI>(c, p, a, s);
+    if (rc != GJX_OK) return rc;
+  } else {
+    Inputs in = {};
+    if ((rc = take_x(c, p, ws, in, s)) != GJX_OK) return rc;
+    a.b = in.x;
+    a.fb = in.fx;
+    a.ktiles = depth_tiles(c, p.kp);
+    a.nt = (int)p.n_tiles;
+    for (int64_t v0 = 0; v0 < c.vocab; v0 += p.piece) {
+      const int64_t rows = std::min(p.piece, c.vocab - v0);
+      if ((rc = take_w(c, p, ws, v0, rows, in, s)) != GJX_OK) return rc;
+      a.a = in.w;
+      a.fa = in.fw;
+      a.v0 = v0;
+      a.part_tile0 = (int)(v0 / BM);
+      a.mt = (int)(up(rows, BM) / BM);
+      if ((rc = launch<false, false, EPI>(c, p.bn > 64, a, s)) != GJX_OK) return rc;
+    }
+  }
+  if (EPI == EPI_SCORE) {
+    int cols = 1;
+    while (cols < 64 && cols < c.n) cols *= 2;
+    k_lincat_combine<<<(unsigned)(up(c.n, cols) / cols), GJX_BLOCK, 0, s>>>(a.part, (int)p.tiles, p.n_pad, c.n, cols, a.target, f.lp, f.lse);
+  } else {
+    k_lincat_pick<<<(unsigned)(up(c.n, GJX_BLOCK / 64) / (GJX_BLOCK / 64)), GJX_BLOCK, 0, s>>>(a.part, (int)p.tiles, p.n_pad, c.n, f.out);
+  }
+  GJX_LAUNCH_CHECK();
   return GJX_OK;
 }
 
@@ -645,176 +1036,88 @@ int32_t check_args(const char* who, const int32_t* y, const void* x, int64_t x_l
 
 GJX_API int32_t gjx_linear_categorical_workspace(int32_t dtype, const void* d_x, int64_t x_ld, const void* d_w, int64_t w_ld,
                                                  int64_t n, int64_t vocab, int64_t width, int32_t grad, int64_t* bytes) {
-  GJX_REQUIRE(bytes != nullptr, GJX_EINVAL, "gjx_linear_categorical_workspace: bytes is null");
   static const int32_t some_y = 0;
-  int32_t rc = check_args("gjx_linear_categorical_workspace", &some_y, d_x, x_ld, d_w, w_ld, dtype, n, vocab, width);
+  const Call c = {"gjx_linear_categorical_workspace", dtype, &some_y, d_x, x_ld, d_w, w_ld, nullptr, n, vocab, width};
+  GJX_REQUIRE(bytes != nullptr && grad >= 0 && grad <= 2, GJX_EINVAL, "%s: bytes is null or grad not in [0, 2]", c.who);
+  const int32_t rc = check_args(c);
   if (rc != GJX_OK) return rc;
-  if (n == 0) {
-    *bytes = 0;
-    return GJX_OK;
-  }
-  const bool f32 = dtype == GJX_F32;
-  *bytes = plan_of(dtype, n, vocab, width, f32 || !direct(d_x, x_ld, width), f32 || !direct(d_w, w_ld, width), grad != 0,
-                   (grad & 1) != 0).bytes;
+  *bytes = n == 0 ? 0 : plan_of(c, grad != 0, grad == 1).bytes;
   return GJX_OK;
 }
-
-namespace {
-
-// the forward product, reduced to log-densities (EPI_SCORE) or draws (EPI_DRAW)
-struct Forward {
-  const char* who;
-  int epi;
-  const int32_t* y;
-  float *lp, *lse;
-  uint32_t key0, key1;
-  uint64_t offset;
-  int32_t* out;
-};
-
-template <int EPI>
-int32_t launch_rows(int bn, const GemmArgs& a, hipStream_t s) {
-  return bn == 256 ? launch_gemm<256, false, false, EPI>(a, s) : launch_gemm<64, false, false, EPI>(a, s);
-}
-
-int32_t forward(const Forward& f, int dtype, const void* d_x, int64_t x_ld, const void* d_w, int64_t w_ld, const void* d_bias,
-                int64_t n, int64_t vocab, int64_t width, void* d_work, int64_t work_bytes, hipStream_t s) {
-  const bool f32 = dtype == GJX_F32;
-  const Plan p = plan_of(dtype, n, vocab, width, f32 || !direct(d_x, x_ld, width), f32 || !direct(d_w, w_ld, width), false, false);
-  GJX_REQUIRE(d_work && ((uintptr_t)d_work & 255) == 0 && work_bytes >= p.bytes, GJX_EINVAL,
-              "%s: the workspace has %lld bytes, needs %lld aligned to 256", f.who, (long long)work_bytes, (long long)p.bytes);
-  int32_t rc;
-  char* ws = (char*)d_work;
-  GemmArgs a = {};
-  a.pairs = p.pairs;
-  a.ktiles = (int)(p.kp / BK);
-  a.splits = 1;
-  a.nt = (int)p.n_tiles;
-  a.b = {(const bf16*)d_x, x_ld, 0, (int)n, 0};
-  if (p.pack_x) {
-    if ((rc = pack(d_x, dtype, x_ld, n, width, p.kp, (bf16*)(ws + p.o_x), n * p.kp, s)) != GJX_OK) return rc;
-    a.b = {(const bf16*)(ws + p.o_x), p.kp, n * p.kp, (int)n, 0};
-  }
-  a.vocab = vocab;
-  a.n = n;
-  a.n_pad = p.n_pad;
-  a.bias = d_bias;
-  a.bias_f32 = f32;
-  a.y = f.y;
-  a.key0 = f.key0;
-  a.key1 = f.key1;
-  a.offset = f.offset;
-  a.part = (float2*)(ws + p.o_part);
-  a.target = (float*)(ws + p.o_target);
-  for (int64_t v0 = 0; v0 < vocab; v0 += p.piece) {
-    const int64_t rows = std::min(p.piece, vocab - v0);
-    a.a = {(const bf16*)at_row(d_w, dtype, v0 * w_ld), w_ld, 0, (int)rows, 0};
-    if (p.pack_w) {
-      if ((rc = pack(at_row(d_w, dtype, v0 * w_ld), dtype, w_ld, rows, width, p.kp, (bf16*)(ws + p.o_w), p.piece * p.kp, s)) != GJX_OK)
-        return rc;
-      a.a = {(const bf16*)(ws + p.o_w), p.kp, p.piece * p.kp, (int)rows, 0};
-    }
-    a.v0 = v0;
-    a.part_tile0 = (int)(v0 / BM);
-    a.mt = (int)(up(rows, BM) / BM);
-    rc = f.epi == EPI_SCORE ? launch_rows<EPI_SCORE>(p.bn, a, s) : launch_rows<EPI_DRAW>(p.bn, a, s);
-    if (rc != GJX_OK) return rc;
-  }
-  if (f.epi == EPI_SCORE) {
-    int cols = 1;
-    while (cols < 64 && cols < n) cols *= 2;
-    k_lincat_combine<<<(unsigned)(up(n, cols) / cols), GJX_BLOCK, 0, s>>>(a.part, (int)p.tiles, p.n_pad, n, cols, a.target, f.lp, f.lse);
-  } else {
-    k_lincat_pick<<<(unsigned)(up(n, GJX_BLOCK / 64) / (GJX_BLOCK / 64)), GJX_BLOCK, 0, s>>>(a.part, (int)p.tiles, p.n_pad, n, f.out);
-  }
-  GJX_LAUNCH_CHECK();
-  return GJX_OK;
-}
-
-}  // namespace
 
 GJX_API int32_t gjx_linear_categorical_logpdf(int32_t dtype, const int32_t* d_y, const void* d_x, int64_t x_ld,
                                               const void* d_w, int64_t w_ld, const void* d_bias, int64_t n, int64_t vocab,
                                               int64_t width, float* d_lp, float* d_lse, void* d_work, int64_t work_bytes,
                                               void* stream) {
-  Forward f = {"gjx_linear_categorical_logpdf", EPI_SCORE, d_y, d_lp, d_lse, 0, 0, 0, nullptr};
-  const int32_t rc = check_args(f.who, d_y, d_x, x_ld, d_w, w_ld, dtype, n, vocab, width);
+  const Call c = {"gjx_linear_categorical_logpdf", dtype, d_y, d_x, x_ld, d_w, w_ld, d_bias, n, vocab, width};
+  const int32_t rc = check_args(c);
   if (rc != GJX_OK || n == 0) return rc;
-  GJX_REQUIRE(d_lp && d_lse, GJX_EINVAL, "%s: null output", f.who);
-  return forward(f, dtype, d_x, x_ld, d_w, w_ld, d_bias, n, vocab, width, d_work, work_bytes, (hipStream_t)stream);
+  GJX_REQUIRE(d_lp, GJX_EINVAL, "%s: null output", c.who);
+  Forward f = {};
+  f.lp = d_lp;
+  f.lse = d_lse;
+  return forward<EPI_SCORE>(c, f, d_work, work_bytes, (hipStream_t)stream);
 }
 
 GJX_API int32_t gjx_random_linear_categorical_i32(const uint32_t key[2], uint64_t offset, int32_t dtype, const void* d_x,
                                                   int64_t x_ld, const void* d_w, int64_t w_ld, const void* d_bias, int64_t n,
                                                   int64_t vocab, int64_t width, int32_t* d_out, void* d_work,
                                                   int64_t work_bytes, void* stream) {
-  const char* who = "gjx_random_linear_categorical_i32";
   static const int32_t some_y = 0;
-  const int32_t rc = check_args(who, &some_y, d_x, x_ld, d_w, w_ld, dtype, n, vocab, width);
+  const Call c = {"gjx_random_linear_categorical_i32", dtype, &some_y, d_x, x_ld, d_w, w_ld, d_bias, n, vocab, width};
+  const int32_t rc = check_args(c);
   if (rc != GJX_OK || n == 0) return rc;
-  GJX_REQUIRE(key && d_out, GJX_EINVAL, "%s: null key or output", who);
-  Forward f = {who, EPI_DRAW, nullptr, nullptr, nullptr, key[0], key[1], offset, d_out};
-  return forward(f, dtype, d_x, x_ld, d_w, w_ld, d_bias, n, vocab, width, d_work, work_bytes, (hipStream_t)stream);
+  GJX_REQUIRE(key && d_out, GJX_EINVAL, "%s: null key or output", c.who);
+  Forward f = {};
+  f.key0 = key[0];
+  f.key1 = key[1];
+  f.offset = offset;
+  f.out = d_out;
+  return forward<EPI_DRAW>(c, f, d_work, work_bytes, (hipStream_t)stream);
 }
 
 GJX_API int32_t gjx_linear_categorical_grad(int32_t dtype, const int32_t* d_y, const void* d_x, int64_t x_ld, const void* d_w,
                                             int64_t w_ld, const void* d_bias, int64_t n, int64_t vocab, int64_t width,
                                             const float* d_lse, const float* d_upstream, void* d_dx, void* d_dw, void* d_db,
                                             void* d_work, int64_t work_bytes, void* stream) {
-  const char* who = "gjx_linear_categorical_grad";
-  int32_t rc = check_args(who, d_y, d_x, x_ld, d_w, w_ld, dtype, n, vocab, width);
+  const Call c = {"gjx_linear_categorical_grad", dtype, d_y, d_x, x_ld, d_w, w_ld, d_bias, n, vocab, width};
+  int32_t rc = check_args(c);
   if (rc != GJX_OK) return rc;
-  GJX_REQUIRE(n >= 1, GJX_EINVAL, "%s: no rows (the gradients are zero; the caller fills them)", who);
-  const bool f32 = dtype == GJX_F32;
-  const Plan p = plan_of(dtype, n, vocab, width, f32 || !direct(d_x, x_ld, width), f32 || !direct(d_w, w_ld, width), true,
-                         d_dx != nullptr);
-  GJX_REQUIRE(d_lse && d_upstream, GJX_EINVAL, "%s: null input", who);
-  GJX_REQUIRE(d_work && ((uintptr_t)d_work & 255) == 0 && work_bytes >= p.bytes, GJX_EINVAL,
-              "%s: the workspace has %lld bytes, needs %lld aligned to 256", who, (long long)work_bytes, (long long)p.bytes);
+  GJX_REQUIRE(n >= 1, GJX_EINVAL, "%s: no rows (the gradients are zero; the caller fills them)", c.who);
+  GJX_REQUIRE(d_lse && d_upstream, GJX_EINVAL, "%s: null input", c.who);
+  const bool f32 = c.f32();
+  const Plan p = plan_of(c, true, d_dx != nullptr);
+  if ((rc = check_work(c, p, d_work, work_bytes)) != GJX_OK) return rc;
   if (!d_dx && !d_dw && !d_db) return GJX_OK;
   hipStream_t s = (hipStream_t)stream;
   char* ws = (char*)d_work;
-  Operand x = {(const bf16*)d_x, x_ld, 0, (int)n, (int)p.kp};
-  if (p.pack_x) {
-    if ((rc = pack(d_x, dtype, x_ld, n, width, p.kp, (bf16*)(ws + p.o_x), n * p.kp, s)) != GJX_OK) return rc;
-    x = {(const bf16*)(ws + p.o_x), p.kp, n * p.kp, (int)n, (int)p.kp};
-  }
-  const Operand dl_rows = {(const bf16*)(ws + p.o_dl), p.piece, p.n_pad * p.piece, (int)p.n_pad, (int)p.piece};
+  Inputs in = {};
+  if ((rc = take_x(c, p, ws, in, s)) != GJX_OK) return rc;
+  const bool wide = p.bn > 64;
   const int mk = (int)(up(width, BM) / BM);
-  float* dx_part = (float*)(ws + p.o_dx);
-  float* resid = (float*)(ws + p.o_resid);
+  const int64_t part_ld = up(p.kp, 4);
+  float *dx_part = (float*)(ws + p.o_dx), *resid = f32 ? nullptr : (float*)(ws + p.o_resid);
   for (int64_t v0 = 0; v0 < vocab; v0 += p.piece) {
     const int64_t rows = std::min(p.piece, vocab - v0), rows_pad = up(rows, BM);
-    Operand w = {(const bf16*)at_row(d_w, dtype, v0 * w_ld), w_ld, 0, (int)rows, (int)p.kp};
-    if (p.pack_w) {
-      if ((rc = pack(at_row(d_w, dtype, v0 * w_ld), dtype, w_ld, rows, width, p.kp, (bf16*)(ws + p.o_w), p.piece * p.kp, s)) != GJX_OK)
-        return rc;
-      w = {(const bf16*)(ws + p.o_w), p.kp, p.piece * p.kp, (int)rows, (int)p.kp};
-    }
-    GemmArgs a = {};                                         // logits of the piece -> dl
-    a.pairs = p.pairs;
-    a.splits = 1;
-    a.a = w;
-    a.b = x;
-    a.ktiles = (int)(p.kp / BK);
+    if ((rc = take_w(c, p, ws, v0, rows, in, s)) != GJX_OK) return rc;
+    const Operand dl = {(const bf16*)(ws + p.o_dl), p.piece, (int)p.n_pad, (int)p.piece};
+    const OperandF fdl = {(const float*)(ws + p.o_dl), p.piece, (int)p.n_pad, (int)rows_pad, 1};
+    GemmArgs a = common_args(c, p);                          // logits of the piece -> dl
+    a.a = in.w;
+    a.fa = in.fw;
+    a.b = in.x;
+    a.fb = in.fx;
+    a.ktiles = depth_tiles(c, p.kp);
     a.mt = (int)(rows_pad / BM);
     a.nt = (int)p.n_tiles;
     a.v0 = v0;
-    a.vocab = vocab;
-    a.n = n;
-    a.n_pad = p.n_pad;
-    a.bias = d_bias;
-    a.bias_f32 = f32;
-    a.y = d_y;
     a.lse = d_lse;
     a.g = d_upstream;
-    a.dl = (bf16*)(ws + p.o_dl);
+    a.dl = ws + p.o_dl;
     a.resid = resid;
     a.dl_ld = p.piece;
-    a.dl_plane = p.n_pad * p.piece;
     a.db_part = d_db ? (float*)(ws + p.o_db) : nullptr;
-    rc = p.bn == 256 ? launch_gemm<256, false, false, EPI_DL>(a, s) : launch_gemm<64, false, false, EPI_DL>(a, s);
-    if (rc != GJX_OK) return rc;
+    if ((rc = launch<false, false, EPI_DL>(c, wide, a, s)) != GJX_OK) return rc;
     if (d_db) {
       k_lincat_fold<<<gjx_grid_for(rows), GJX_BLOCK, 0, s>>>((const float*)(ws + p.o_db), (int)p.n_tiles, p.piece, 1, rows, rows,
                                                            f32 ? (void*)((float*)d_db + v0) : (void*)((bf16*)d_db + v0), !f32,
@@ -822,49 +1125,45 @@ GJX_API int32_t gjx_linear_categorical_grad(int32_t dtype, const int32_t* d_y, c
       GJX_LAUNCH_CHECK();
     }
     if (d_dx) {                                              // dx^T = W^T dl^T: m = feature, n = row, over the piece
-      GemmArgs b = {};
-      b.pairs = p.pairs;
-      b.a = w;
-      b.b = dl_rows;
-      b.ktiles = (int)(rows_pad / BK);
+      GemmArgs b = common_args(c, p);
+      b.a = in.w;
+      b.fa = in.fw;
+      b.b = dl;
+      b.fb = fdl;
+      b.ktiles = depth_tiles(c, rows_pad);
       b.mt = mk;
       b.nt = (int)p.n_tiles;
       b.splits = p.splits;
       b.out = dx_part;
-      b.out_ld = p.kp;
-      b.out_split = n * p.kp;
+      b.out_ld = part_ld;
+      b.out_split = n * part_ld;
       b.out_m = (int)p.kp;
       b.out_n = (int)n;
       b.accumulate = v0 > 0;
-      rc = p.bn == 256 ? launch_gemm<256, true, false, EPI_STORE>(b, s) : launch_gemm<64, true, false, EPI_STORE>(b, s);
-      if (rc != GJX_OK) return rc;
+      if ((rc = launch<true, false, EPI_STORE>(c, wide, b, s)) != GJX_OK) return rc;
     }
     if (d_dw) {                                              // dW^T = x^T dl: m = feature, n = entry, over the rows
-      GemmArgs b = {};
-      b.pairs = p.pairs;
-      b.a = x;
-      b.b = dl_rows;
-      b.ktiles = (int)(p.n_pad / BK);
+      GemmArgs b = common_args(c, p);
+      b.a = in.x;
+      b.fa = in.fx;
+      b.b = dl;
+      b.fb = fdl;
+      b.ktiles = depth_tiles(c, f32 ? n : p.n_pad);
       b.mt = mk;
-      b.nt = (int)(rows_pad / BM);
-      b.splits = 1;
+      b.nt = (int)(f32 ? up(rows, 128) / 128 : rows_pad / 256);
       b.out = f32 ? (void*)((float*)d_dw + v0 * width) : (void*)((bf16*)d_dw + v0 * width);
       b.out_ld = width;
       b.out_m = (int)width;
       b.out_n = (int)rows;
       b.out_bf16 = !f32;
-      b.resid_in = f32 ? nullptr : resid;
-      b.y = d_y;
-      b.n = n;
+      b.resid_in = resid;
       b.v0 = v0;
-      b.vocab = vocab;
-      rc = launch_gemm<256, true, true, EPI_STORE>(b, s);
-      if (rc != GJX_OK) return rc;
+      if ((rc = launch<true, true, EPI_STORE>(c, true, b, s)) != GJX_OK) return rc;
     }
   }
   if (d_dx) {
-    k_lincat_fold<<<gjx_grid_for(n * width), GJX_BLOCK, 0, s>>>(dx_part, p.splits, n * p.kp, n, p.kp, width, d_dx, !f32,
-                                                                    f32 ? nullptr : resid, d_y, (const bf16*)d_w, w_ld, vocab);
+    k_lincat_fold<<<gjx_grid_for(n * width), GJX_BLOCK, 0, s>>>(dx_part, p.splits, n * part_ld, n, part_ld, width, d_dx, !f32, resid,
+                                                                d_y, (const bf16*)d_w, w_ld, vocab);
     GJX_LAUNCH_CHECK();
   }
   return GJX_OK;

@@ -156,7 +156,7 @@ class _LinearCategorical(Distribution):
 
     def logpdf(self, y, x, weight, bias=None, **kwargs):
         x, weight, bias = as_col(x), as_col(weight), None if bias is None else as_col(bias)
-        y = torch.as_tensor(y, device=x.device)
+        y = y if isinstance(y, torch.Tensor) and y.is_cuda else torch.as_tensor(y, device=x.device)
         if y.dim() > 1:
             raise B.GjxError(f"linear_categorical: y {tuple(y.shape)} must be one value or one per row")
         n = x.shape[0] if x.dim() == 2 else max(1, y.numel())
@@ -165,11 +165,13 @@ class _LinearCategorical(Distribution):
         if y.dim() == 1 and y.numel() not in (1, n):
             raise B.GjxError(f"linear_categorical: {y.numel()} values against {n} rows of x")
         scalar = y.dim() == 0 and x.dim() == 1
-        rows, ys = self._rows(x, n), y.reshape(-1).to(torch.int32).expand(n)
+        rows, ys = self._rows(x, n), y.to(torch.int32)
+        if ys.shape != (n,):
+            ys = ys.reshape(-1).expand(n)
         if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
             out = _LinearCategoricalFn.apply(ys, rows, weight, bias)
         else:
-            out = B.linear_categorical_logpdf(ys, rows, weight, bias)[0]
+            out = B.linear_categorical_logpdf(ys, rows, weight, bias, want_lse=False)[0]
         return out.reshape(()) if scalar else out
 
 

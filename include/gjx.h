@@ -145,7 +145,7 @@ int32_t gjx_categorical_logpdf_f32(const int32_t* d_x, const float* d_logits, in
  * y outside [0, vocab) takes the nearest entry.  A bias of -inf takes its entry out of the distribution; a row with no
  * entry left is NaN.  The caller owns the workspace (256-byte aligned, gjx_linear_categorical_workspace bytes; grad:
  * 0 for the log-density, 1 for the gradient, 2 for the gradient without d_dx); its contents need not be kept between calls.
- *   logpdf: lp_i = l_{i, y_i} - lse_i, lse_i = log sum_v exp(l_iv)
+ *   logpdf: lp_i = l_{i, y_i} - lse_i, lse_i = log sum_v exp(l_iv) (d_lse nullable)
  *   grad:   outputs (nullable) dx, dW, db of sum_i upstream_i lp_i, contiguous, of type dtype (what jax.grad of
  *           assess produces inside hmc, mcmc.py:59-88, 508, 523); d_lse is the log-density call's */
 int32_t gjx_linear_categorical_workspace(int32_t dtype, const void* d_x, int64_t x_ld, const void* d_w, int64_t w_ld,

@@ -44,7 +44,7 @@ def test_linear_categorical_abi_refusals():
     assert L.gjx_linear_categorical_workspace(0, p, 8, p, 8, 3, 5, 8, 1, None) == -1
     assert code(dtype=2) == -1 and b"dtype" in L.gjx_last_error()
     assert code(n=-1) == -1 and code(vocab=0) == -1 and code(width=0) == -1
-    assert code(x=None) == -1 and code(w=None) == -1 and code(y=None) == -1 and code(lp=None) == -1 and code(lse=None) == -1
+    assert code(x=None) == -1 and code(w=None) == -1 and code(y=None) == -1 and code(lp=None) == -1
     assert code(x_ld=7) == -1 and code(w_ld=7) == -1 and b"stride" in L.gjx_last_error()
     assert code(work=None) == -1 and code(work_bytes=16) == -1 and b"workspace" in L.gjx_last_error()
     assert code(work=C.c_void_p((1 << 20) + 8)) == -1
