@@ -5,7 +5,7 @@
 // turns them into d l = g (onehot(y) - exp(l - lse)) in that product's epilogue and feeds two more products,
 //   dx = dl W,   dW = dl^T x,   db = sum_i dl_i.
 // The products are 16x16x32 bf16 MFMA tiles with f32 accumulators.  f32 operands are split exactly into three bf16 planes
-// (8 bits each) and the six partial products above 2^-23 are summed.
+// (8 bits each) and the six largest partial products are summed.
 //
 // Three kernels: k_lincat_rows for few rows (the weights go once from memory to the matrix unit), k_lincat_gemm for bf16
 // (tiles straight into LDS), k_lincat_gemm32 for f32 (tiles split into planes on their way to LDS).
@@ -24,7 +24,8 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 namespace {
 
-constexpr int BM = 256, BK = 64, GEMM_THREADS = 512;
+constexpr int BM = 256, BK = 64, GEMM_THREADS = 512;         // bf16 tiles: BM entries of m, 64 deep, eight waves
+constexpr int BM32 = 128, GEMM32_THREADS = 256;              // f32 tiles: 32 deep, four waves
 
 enum { EPI_SCORE = 0, EPI_DL = 1, EPI_STORE = 2, EPI_DRAW = 3 };
 
@@ -76,18 +77,18 @@ __device__ __forceinline__ float load_any(const void* p, int f32, int64_t i) {
   return f32 ? ((const float*)p)[i] : (float)((const bf16*)p)[i];
 }
 
-// x = h + m + l exactly, each rounded to nearest (8 bits of the 24 apiece, signed): |m| <= 2^-8 |x|, |l| <= 2^-16 |x|, so the
-// partial products left out are at most 2^-23 |x| |w| each.  What rounds to infinity in bf16 (above 3.389e38) counts as
-// infinite and keeps h only.
+// x = h + m + l exactly by cutting off 8 bits at a time (half the operations of rounding, and nothing can overflow):
+// |m| < 2^-7 |x|, |l| < 2^-15 |x|, so the partial products left out are below 2^-21 |x| |w|, 2^-23 on average.
 __device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&out)[3]) {
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const bf16 h = (bf16)x[j];
-    const float r = fabsf(x[j]) < 3.389e38f ? x[j] - (float)h : 0.0f;
-    const bf16 m = (bf16)r;
-    out[0][j] = h;
-    out[1][j] = m;
-    out[2][j] = (bf16)(r - (float)m);
+    const uint32_t u = __float_as_uint(x[j]);
+    const float r = x[j] - __uint_as_float(u & 0xffff0000u);
+    const uint32_t v = __float_as_uint(r);
+    const uint32_t t = __float_as_uint(r - __uint_as_float(v & 0xffff0000u));
+    out[0][j] = __builtin_bit_cast(bf16, (uint16_t)(u >> 16));
+    out[1][j] = __builtin_bit_cast(bf16, (uint16_t)(v >> 16));
+    out[2][j] = __builtin_bit_cast(bf16, (uint16_t)(t >> 16));
   }
 }
 
@@ -164,7 +165,7 @@ struct Tile {
 };
 
 // neighbouring tiles to one XCD (workgroups go round the eight of them), eight m-tiles by all n-tiles at a time
-template <int BN>
+template <int BM, int BN>
 __device__ __forceinline__ Tile tile_of(const GemmArgs& g) {
   int id = blockIdx.x;
   const int total = g.mt * g.nt * g.splits, per = total / 8, extra = total % 8, xcd = id % 8;
@@ -181,7 +182,7 @@ __device__ __forceinline__ Tile tile_of(const GemmArgs& g) {
 }
 
 // what becomes of a tile's accumulators (rows m0 + wm + 16 i + 4 q + r, columns n0 + wn + 16 j + lane % 16); T: the operands' type
-template <typename T, int BN, int WM, int WN, int MT, int NT, bool TB, int EPI>
+template <typename T, int BM, int BN, int WM, int WN, int MT, int NT, bool TB, int EPI>
 __device__ __forceinline__ void epilogue(const GemmArgs& g, const Tile& tile, f32x4 (&acc)[MT][NT], char* smem_raw) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int split = tile.split, tm = tile.tm, tn = tile.tn, m0 = tile.m0, n0 = tile.n0;
@@ -425,7 +426,7 @@ __global__ void __launch_bounds__(GEMM_THREADS)
   extern __shared__ char smem_raw[];
   LDS_AS char* smem = (LDS_AS char*)smem_raw;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const Tile tile = tile_of<BN>(g);
+  const Tile tile = tile_of<BM, BN>(g);
   const int kt0 = (int)((int64_t)g.ktiles * tile.split / g.splits), kt1 = (int)((int64_t)g.ktiles * (tile.split + 1) / g.splits);
 
   f32x4 acc[MT][NT];
@@ -461,14 +462,14 @@ __global__ void __launch_bounds__(GEMM_THREADS)
     }
   }
   __syncthreads();
-  epilogue<bf16, BN, WM, WN, MT, NT, TB, EPI>(g, tile, acc, smem_raw);
+  epilogue<bf16, BM, BN, WM, WN, MT, NT, TB, EPI>(g, tile, acc, smem_raw);
 }
 
 // one 32-deep slab of an f32 operand, R output indices wide: pieces of eight reduction entries of one output index, loaded
 // into registers, split and written to LDS as fragments (16 indices x 3 planes x 64 lanes x 16 bytes)
 template <int R, bool T>
 struct SlabLoader {
-  static constexpr int PIECES = (R * 4 + GEMM_THREADS - 1) / GEMM_THREADS;
+  static constexpr int PIECES = (R * 4 + GEMM32_THREADS - 1) / GEMM32_THREADS;
   float x[PIECES][8];
 
   static __device__ __forceinline__ void where(int u, int& index, int& group) {
@@ -483,18 +484,20 @@ struct SlabLoader {
   __device__ __forceinline__ void load(const OperandF& o, int out0, int k0, int tid) {
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
-      const int u = i * GEMM_THREADS + tid;
+      const int u = i * GEMM32_THREADS + tid;
       int index, group;
       where(min(u, R * 4 - 1), index, group);
       const int k = k0 + 8 * group;
       if (T) {
         const float* p = o.p + min(out0 + index, o.cols - 1);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[i][j] = k + j < o.rows ? p[(int64_t)(k + j) * o.ld] : 0.0f;
+        for (int j = 0; j < 8; ++j) x[i][j] = p[(int64_t)min(k + j, o.rows - 1) * o.ld];       // all eight in flight, then masked
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[i][j] = k + j < o.rows ? x[i][j] : 0.0f;
       } else {
-        const float* p = o.p + (int64_t)min(out0 + index, o.rows - 1) * o.ld + k;
+        const float* p = o.p + (int64_t)min(out0 + index, o.rows - 1) * o.ld;
         if (o.vec && k + 8 <= o.cols) {
-          const f32x4 lo = *(const f32x4*)p, hi = *(const f32x4*)(p + 4);
+          const f32x4 lo = *(const f32x4*)(p + k), hi = *(const f32x4*)(p + k + 4);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             x[i][j] = lo[j];
@@ -502,7 +505,9 @@ struct SlabLoader {
           }
         } else {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) x[i][j] = k + j < o.cols ? p[j] : 0.0f;
+          for (int j = 0; j < 8; ++j) x[i][j] = p[min(k + j, o.cols - 1)];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[i][j] = k + j < o.cols ? x[i][j] : 0.0f;
         }
       }
     }
@@ -510,8 +515,8 @@ struct SlabLoader {
   __device__ __forceinline__ void store(char* lds, int tid) const {
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
-      const int u = i * GEMM_THREADS + tid;
-      if (R * 4 % GEMM_THREADS && u >= R * 4) continue;
+      const int u = i * GEMM32_THREADS + tid;
+      if (R * 4 % GEMM32_THREADS && u >= R * 4) continue;
       int index, group;
       where(u, index, group);
       bf16x8 o[3];
@@ -529,15 +534,16 @@ struct SlabLoader {
 
 // the same product of f32 operands: six matrix instructions per fragment pair, so the splitting (once per tile) and the
 // LDS traffic are small beside them and no packed copy of the operands is needed (packing to bf16 planes first: pack and
-// product 328 us for 200 x 50001 x 768).  Two LDS buffers of one 32-deep slab, the slab after that in registers.
+// product 328 us for 200 x 50001 x 768).  One 32-deep slab in LDS, the next one in registers; three workgroups a CU
+// cover each other's splitting and barriers and leave less idle at the end than one of twice the size.
 template <int BN, bool TA, bool TB, int EPI>
-__global__ void __launch_bounds__(GEMM_THREADS, 2)
+__global__ void __launch_bounds__(GEMM32_THREADS, 3)
     k_lincat_gemm32(GemmArgs g) {
-  constexpr int WN = 2, WM = 4, MT = BM / WM / 16, NT = BN / WN / 16;
-  constexpr int A_BYTES = BM / 16 * 3072, STAGE = A_BYTES + BN / 16 * 3072;
+  constexpr int BM = BM32, WN = 2, WM = 2, MT = BM / WM / 16, NT = BN / WN / 16;
+  constexpr int A_BYTES = BM / 16 * 3072;
   extern __shared__ char smem_raw[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const Tile tile = tile_of<BN>(g);
+  const Tile tile = tile_of<BM, BN>(g);
   const int kt0 = (int)((int64_t)g.ktiles * tile.split / g.splits), kt1 = (int)((int64_t)g.ktiles * (tile.split + 1) / g.splits);
   f32x4 acc[MT][NT];
 #pragma unroll
@@ -551,12 +557,11 @@ __global__ void __launch_bounds__(GEMM_THREADS, 2)
     la.load(g.fa, tile.m0, kt0 * 32, tid);
     lb.load(g.fb, tile.n0, kt0 * 32, tid);
   }
+  char *sa = smem_raw, *sb = sa + A_BYTES;
   for (int kt = kt0; kt < kt1; ++kt) {
-    char* sa = smem_raw + ((kt - kt0) & 1) * STAGE;
-    char* sb = sa + A_BYTES;
     la.store(sa, tid);
     lb.store(sb, tid);
-    __syncthreads();           // this buffer is written; the other one is written again only behind the next barrier
+    __syncthreads();
     if (kt + 1 < kt1) {
       la.load(g.fa, tile.m0, (kt + 1) * 32, tid);
       lb.load(g.fb, tile.n0, (kt + 1) * 32, tid);
@@ -571,9 +576,9 @@ __global__ void __launch_bounds__(GEMM_THREADS, 2)
 #pragma unroll
       for (int j = 0; j < NT; ++j) acc[i][j] = mma3(fa, fb[j], acc[i][j]);
     }
+    __syncthreads();
   }
-  __syncthreads();
-  epilogue<float, BN, WM, WN, MT, NT, TB, EPI>(g, tile, acc, smem_raw);
+  epilogue<float, BM, BN, WM, WN, MT, NT, TB, EPI>(g, tile, acc, smem_raw);
 }
 
 // few rows (n <= 16 NT): a wave takes 16 entries of the vocabulary, the weights go from memory to the matrix unit without
@@ -581,7 +586,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 2)
 template <typename T, int NT, int EPI>
 __global__ void __launch_bounds__(GJX_BLOCK)
     k_lincat_rows(GemmArgs g, const T* __restrict__ x, int64_t x_ld, const T* __restrict__ w, int64_t w_ld, int width, int vec) {
-  constexpr int P = sizeof(T) == 4 ? 3 : 1, U = sizeof(T) == 4 ? 4 : 8;      // planes; slabs in flight
+  constexpr int P = sizeof(T) == 4 ? 3 : 1, U = (sizeof(T) == 4 ? 8 : 16) / NT;      // planes; slabs in flight
   __shared__ float s_red[4][16 * NT][2];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, c = lane & 15;
   const int v0 = blockIdx.x * 64 + wave * 16;
@@ -602,11 +607,14 @@ __global__ void __launch_bounds__(GJX_BLOCK)
         }
       }
     } else {
+      T t[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) t[e] = p[min(k + e, width - 1)];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const T t = k + e < width ? p[k + e] : (T)0.0f;
-        if (P == 1) h[e] = (bf16)t;
-        else f[e] = (float)t;
+        if (k + e >= width) t[e] = (T)0.0f;
+        if (P == 1) h[e] = (bf16)t[e];
+        else f[e] = (float)t[e];
       }
     }
   };
@@ -809,7 +817,7 @@ bool vector_rows(const Call& c, const void* p, int64_t ld) { return ((uintptr_t)
 
 struct Plan {
   bool rows;                    // k_lincat_rows
-  int bn;                       // rows per tile
+  int bm, bn;                       // rows per tile
   int64_t kp, n_pad, n_tiles;
   bool pack_x, pack_w;
   int64_t piece;                // vocabulary entries per piece (multiple of 256)
@@ -829,8 +837,9 @@ struct Carver {
 
 Plan plan_of(const Call& c, bool grad, bool want_dx) {
   Plan p = {};
-  const int64_t vt = up(c.vocab, BM) / BM;
+  const int64_t bm = c.f32() ? BM32 : BM, vt = up(c.vocab, bm) / bm;
   p.rows = !grad && c.n <= ROWS_MAX;
+  p.bm = (int)bm;
   p.kp = c.f32() ? c.width : up(c.width, 64);
   p.pack_x = !c.f32() && !p.rows && !direct(c.x, c.x_ld, c.width);
   p.pack_w = !c.f32() && !p.rows && !direct(c.w, c.w_ld, c.width);
@@ -841,11 +850,11 @@ Plan plan_of(const Call& c, bool grad, bool want_dx) {
   p.n_tiles = p.n_pad / p.bn;
   p.tiles = p.rows ? up(c.vocab, 64) / 64 : vt;
   const int64_t e = c.f32() ? 4 : 2;
-  int64_t piece = vt * BM;
+  int64_t piece = up(c.vocab, BM);
   if (p.pack_w) piece = std::min(piece, std::max<int64_t>(BM, PACK_BYTES / (p.kp * 2) / BM * BM));
   if (grad) piece = std::min(piece, std::max<int64_t>(BM, DL_BYTES / (p.n_pad * e) / BM * BM));
-  const int64_t pieces = up(vt * BM, piece) / piece;
-  p.piece = up(up(vt, pieces) / pieces * BM, BM);           // equal pieces
+  const int64_t pieces = up(c.vocab, piece) / piece;
+  p.piece = up(up(c.vocab, pieces) / pieces, BM);           // equal pieces
   Carver k;
   p.o_x = k.take(p.pack_x ? c.n * p.kp * 2 : 0);
   p.o_w = k.take(p.pack_w ? p.piece * p.kp * 2 : 0);
@@ -853,8 +862,8 @@ Plan plan_of(const Call& c, bool grad, bool want_dx) {
     p.o_dl = k.take(p.n_pad * p.piece * e);
     p.o_db = k.take(p.n_tiles * p.piece * 4);
     p.o_resid = k.take(c.n * 4);
-    const int64_t tiles = up(c.width, BM) / BM * p.n_tiles;
-    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(512 / tiles, p.piece / BK / 8));
+    const int64_t tiles = up(c.width, bm) / bm * p.n_tiles;
+    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>((c.f32() ? 768 : 512) / tiles, p.piece / BK / 8));
     p.o_dx = k.take(want_dx ? (int64_t)p.splits * c.n * up(p.kp, 4) * 4 : 0);
   } else {
     p.o_part = k.take(p.tiles * p.n_pad * 8);
@@ -889,10 +898,10 @@ int32_t launch16(const GemmArgs& a, unsigned blocks, hipStream_t s) {
 template <int BN, bool TA, bool TB, int EPI>
 int32_t launch32(const GemmArgs& a, unsigned blocks, hipStream_t s) {
   static std::atomic<uint64_t> done{0};
-  constexpr int lds = 2 * (BM + BN) / 16 * 3072;
+  constexpr int lds = (BM32 + BN) / 16 * 3072;
   const int32_t rc = allow_lds(k_lincat_gemm32<BN, TA, TB, EPI>, lds, done);
   if (rc != GJX_OK) return rc;
-  k_lincat_gemm32<BN, TA, TB, EPI><<<blocks, GEMM_THREADS, lds, s>>>(a);
+  k_lincat_gemm32<BN, TA, TB, EPI><<<blocks, GEMM32_THREADS, lds, s>>>(a);
   GJX_LAUNCH_CHECK();
   return GJX_OK;
 }
@@ -1016,14 +1025,14 @@ int32_t forward(const Call& c, const Forward& f, void* d_work, int64_t work_byte
       a.a = in.w;
       a.fa = in.fw;
       a.v0 = v0;
-      a.part_tile0 = (int)(v0 / BM);
-      a.mt = (int)(up(rows, BM) / BM);
+      a.part_tile0 = (int)(v0 / p.bm);
+      a.mt = (int)(up(rows, p.bm) / p.bm);
       if ((rc = launch<false, false, EPI>(c, p.bn > 64, a, s)) != GJX_OK) return rc;
     }
   }
   if (EPI == EPI_SCORE) {
-    int cols = 1;
-    while (cols < 64 && cols < c.n) cols *= 2;
+    int cols = 1;                                            // 16 rows x 16 parts of the tiles per workgroup
+    while (cols < 16 && cols < c.n) cols *= 2;
     k_lincat_combine<<<(unsigned)(up(c.n, cols) / cols), GJX_BLOCK, 0, s>>>(a.part, (int)p.tiles, p.n_pad, c.n, cols, a.target, f.lp, f.lse);
   } else {
     k_lincat_pick<<<(unsigned)(up(c.n, GJX_BLOCK / 64) / (GJX_BLOCK / 64)), GJX_BLOCK, 0, s>>>(a.part, (int)p.tiles, p.n_pad, c.n, f.out);
@@ -1094,7 +1103,7 @@ GJX_API int32_t gjx_linear_categorical_grad(int32_t dtype, const int32_t* d_y, c
   Inputs in = {};
   if ((rc = take_x(c, p, ws, in, s)) != GJX_OK) return rc;
   const bool wide = p.bn > 64;
-  const int mk = (int)(up(width, BM) / BM);
+  const int mk = (int)(up(width, p.bm) / p.bm);
   const int64_t part_ld = up(p.kp, 4);
   float *dx_part = (float*)(ws + p.o_dx), *resid = f32 ? nullptr : (float*)(ws + p.o_resid);
   for (int64_t v0 = 0; v0 < vocab; v0 += p.piece) {
@@ -1108,7 +1117,7 @@ GJX_API int32_t gjx_linear_categorical_grad(int32_t dtype, const int32_t* d_y, c
     a.b = in.x;
     a.fb = in.fx;
     a.ktiles = depth_tiles(c, p.kp);
-    a.mt = (int)(rows_pad / BM);
+    a.mt = (int)(rows_pad / p.bm);
     a.nt = (int)p.n_tiles;
     a.v0 = v0;
     a.lse = d_lse;

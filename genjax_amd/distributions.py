@@ -125,8 +125,9 @@ class _LinearCategoricalFn(torch.autograd.Function):
         return lp
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g):
+        if torch.is_grad_enabled():
+            raise B.GjxError("linear_categorical: its gradient cannot be differentiated again (create_graph=True)")
         y, x, weight, bias, lse = ctx.saved_tensors
         return (None, *B.linear_categorical_grad(y, x, weight, bias, lse, g, want=ctx.needs_input_grad[1:4]))
 

@@ -251,8 +251,9 @@ class _DeltaFilterFn(torch.autograd.Function):
         return o, state
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, d_o, d_state):
+        if torch.is_grad_enabled():
+            raise GjxError("delta_filter: its gradient cannot be differentiated again (create_graph=True)")
         q, k, v, log_decay, beta, lengths, kept = ctx.saved_tensors
         grads = B.delta_filter_grad(q, k, v, log_decay, beta, d_o, d_state, kept, ctx.scale, lengths, ctx.want_state0)
         return (*grads, None, None)
