@@ -458,9 +458,9 @@ def _address(t):
 
 
 def _unit_stride(t):
-    """`t` itself when its last axis is contiguous and its rows do not overlap, else a contiguous copy."""
+    """`t` itself when its last axis is contiguous and its rows neither overlap nor lie too far apart, else a copy."""
     width, (step, unit) = t.shape[1], t.stride()
-    return t if (unit == 1 or width == 1) and step >= width else t.contiguous()
+    return t if (unit == 1 or width == 1) and width <= step <= 1 << 22 else t.contiguous()
 
 
 @functools.lru_cache(maxsize=1024)

@@ -105,44 +105,61 @@ __device__ __forceinline__ f32x4 mma3(const bf16x8 (&a)[3], const bf16x8 (&b)[3]
 
 __device__ __forceinline__ int tr_swizzle(int k) { return (k & 3) | (((k >> 3) & 3) << 2); }
 
+// One BK-deep tile of an operand, R output indices wide: R * 8 chunks of 16 bytes straight into LDS.  The offsets of a
+// lane's chunks from the tile's first byte are kept (32 bits), so a step along the reduction costs one scalar addition;
+// the fragments' LDS addresses are one or two lane addresses plus constants.
 template <int R, bool T>
 struct TileLoader {
-  // one BK-deep tile of an operand, R output indices wide: R * 8 chunks of 16 bytes straight into LDS
-  static constexpr int LOADS = R * 8 / GEMM_THREADS;
+  static constexpr int LOADS = R * 8 / GEMM_THREADS, WAVES = GEMM_THREADS / 64, FRAGS = T ? R / 16 : 2;
+  uint32_t off[LOADS];
+  uint32_t at[2];                       // lane addresses of the fragments (T: of the row, swizzle apart)
+  int out0, lane, wave;
+  const char* base;                     // uniform
+  int64_t step;
 
-  static __device__ __forceinline__ void load(const Operand& o, const bf16* plane, int out0, int k0, LDS_AS char* lds,
-                                              int tid) {
-    const int wave = tid >> 6;
+  __device__ __forceinline__ TileLoader(const Operand& o, int out, int k0, int lane_, int wave_) : out0(out), lane(lane_), wave(wave_) {
+    base = (const char*)o.p + (T ? (int64_t)k0 * o.ld : (int64_t)out0 * o.ld + k0) * 2;
+    step = T ? BK * o.ld * 2 : BK * 2;
 #pragma unroll
-    for (int j = 0; j < LOADS; ++j) {
-      const int c = (j * (GEMM_THREADS / 64) + wave) * 64 + (tid & 63);
-      const bf16* src;
-      if (T) {
-        const int row = c / (R / 8), ch = c % (R / 8);
-        const int mem = min(k0 + row, o.rows - 1);
-        const int col = min(out0 + ((((ch >> 1) ^ tr_swizzle(row)) << 1) | (ch & 1)) * 8, o.cols - 8);
-        src = plane + (int64_t)mem * o.ld + col;
-      } else {
-        const int row = c >> 3, ch = (c & 7) ^ ((row >> 1) & 7);
-        src = plane + (int64_t)min(out0 + row, o.rows - 1) * o.ld + (k0 + ch * 8);
-      }
-      __builtin_amdgcn_global_load_lds((const GLB_AS void*)src, (LDS_AS void*)(lds + (j * (GEMM_THREADS / 64) + wave) * 1024),
-                                       16, 0, 0);
-    }
-  }
-
-  // the 8 reduction elements 8 q .. 8 q + 7 of slab s (32 deep) for output index i0 + lane % 16
-  static __device__ __forceinline__ bf16x8 frag(LDS_AS char* lds, int i0, int s, int lane) {
+    for (int j = 0; j < LOADS; ++j) off[j] = offset(o, j, BK);
     const int q = lane >> 4, i = lane & 15;
     if (T) {
-      const int k = 32 * s + 8 * q + (i >> 2);
-      LDS_AS char* p = lds + k * (R * 2) + (((i0 >> 4) ^ tr_swizzle(k)) << 5) + ((i & 3) << 3);
+      at[0] = (uint32_t)((8 * q + (i >> 2)) * (R * 2) + ((i & 3) << 3));
+      at[1] = (uint32_t)tr_swizzle(8 * q + (i >> 2));
+    } else {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) at[s] = (uint32_t)(i * 128 + (((s * 4 + q) ^ (i >> 1)) << 4));
+    }
+  }
+  // left: rows of the reduction left from the tile on (T), at least one
+  __device__ __forceinline__ uint32_t offset(const Operand& o, int j, int left) const {
+    const int c = (j * WAVES + wave) * 64 + lane;
+    if (T) {
+      const int row = c / (R / 8), ch = c % (R / 8);
+      const int col = min(out0 + ((((ch >> 1) ^ tr_swizzle(row)) << 1) | (ch & 1)) * 8, o.cols - 8);
+      return ((uint32_t)min(row, left - 1) * (uint32_t)o.ld + (uint32_t)col) * 2u;
+    }
+    const int row = c >> 3, ch = (c & 7) ^ ((row >> 1) & 7);
+    return ((uint32_t)min(row, o.rows - 1 - out0) * (uint32_t)o.ld + (uint32_t)ch * 8u) * 2u;
+  }
+  __device__ __forceinline__ void load(const Operand& o, int k0, LDS_AS char* lds) {
+    const bool ragged = T && k0 + BK > o.rows;
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) {
+      const uint32_t f = ragged ? offset(o, j, o.rows - k0) : off[j];
+      __builtin_amdgcn_global_load_lds((const GLB_AS void*)(base + f), (LDS_AS void*)(lds + (j * WAVES + wave) * 1024), 16, 0, 0);
+    }
+    base += step;
+  }
+  // the 8 reduction elements 8 q .. 8 q + 7 of slab s (32 deep) for output index i0 + lane % 16
+  __device__ __forceinline__ bf16x8 frag(LDS_AS char* lds, int i0, int s) const {
+    if (T) {
+      LDS_AS char* p = lds + at[0] + s * 32 * (R * 2) + (((uint32_t)(i0 >> 4) ^ at[1]) << 5);
       const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((LDS_AS bf16x4*)p);
       const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((LDS_AS bf16x4*)(p + 4 * R * 2));
       return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     }
-    const int row = i0 + i, ch = (s * 4 + q) ^ ((row >> 1) & 7);
-    return *(LDS_AS bf16x8*)(lds + row * 128 + ch * 16);
+    return *(LDS_AS bf16x8*)(lds + at[s] + i0 * 128);
   }
 };
 
@@ -157,6 +174,17 @@ __device__ __forceinline__ void merge_best(float& best, int& arg, float best2, i
     best = best2;
     arg = arg2;
   }
+}
+
+// exp(x) for x <= 0 by the hardware's exp2: the product's rounding moves it by at most 2^-24 |x| log2 e of itself, small
+// where the term is not
+__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504f); }
+
+// the row's value relative to this lane's first entry (first + v0 of the piece), negative where there is none
+__device__ __forceinline__ int value_of(const GemmArgs& g, int64_t n, int first) {
+  if (n >= g.n) return -1;
+  const int64_t y = min(max((int64_t)g.y[n], (int64_t)0), g.vocab - 1) - g.v0 - first;    // outside the vocabulary: the nearest
+  return y < 0 || y > (1 << 20) ? -1 : (int)y;
 }
 
 // where a workgroup's tile lies
@@ -270,25 +298,29 @@ __device__ __forceinline__ void epilogue(const GemmArgs& g, const Tile& tile, f3
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       const int64_t n = n0 + wn + j * 16 + c;
-      const bool live = n < g.n;
       float top = -__builtin_inff();
-      // y outside [0, vocab) takes the nearest entry, as categorical does
-      const int64_t y = live ? min(max((int64_t)g.y[n], (int64_t)0), g.vocab - 1) - g.v0 - m0 - wm - 4 * q : -1;
 #pragma unroll
       for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           acc[i][j][r] += bias[i][r];
-          if (s_bias[wm + i * 16 + 4 * q + r] == -__builtin_inff()) acc[i][j][r] = bias[i][r];
           top = fmaxf(top, acc[i][j][r]);
-          if (y == i * 16 + r) g.target[n] = acc[i][j][r];
         }
+      // the row's value, if its logit is among this lane's (rare: one entry of the vocabulary per row)
+      const int y = value_of(g, n, m0 + wm + 4 * q);
+      if (__ballot(y >= 0 && y < MT * 16 && (y & 15) < 4)) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (y == i * 16 + r) g.target[n] = acc[i][j][r];
+      }
       const float base = top == -__builtin_inff() ? 0.0f : top;
       float sum = 0.0f;
 #pragma unroll
       for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) sum += expf(acc[i][j][r] - base);
+        for (int r = 0; r < 4; ++r) sum += exp_of(acc[i][j][r] - base);
 #pragma unroll
       for (int o = 16; o <= 32; o <<= 1) {
         merge_lse(top, sum, __shfl_xor(top, o), __shfl_xor(sum, o));
@@ -366,32 +398,43 @@ __device__ __forceinline__ void epilogue(const GemmArgs& g, const Tile& tile, f3
   for (int j = 0; j < NT; ++j) {
     const int64_t n = n0 + wn + j * 16 + c;
     const bool live = n < g.n;
-    const float lse = live ? g.lse[n] : 0.0f, up = live ? g.g[n] : 0.0f;
-    const int64_t y = live ? min(max((int64_t)g.y[n], (int64_t)0), g.vocab - 1) - g.v0 - m0 - wm - 4 * q : -1;
+    const float lse = live ? g.lse[n] : 0.0f, up = live ? g.g[n] : 0.0f;      // rows behind the last: up = 0 and finite logits
+    // -up exp(l - lse); entries behind the vocabulary have the bias -inf
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[i][j][r] = -up * exp_of(acc[i][j][r] + bias[i][r] - lse);
+    if (!live)
+#pragma unroll
+      for (int i = 0; i < MT; ++i) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    const int y = value_of(g, n, m0 + wm + 4 * q);
+    const bool here = __ballot(y >= 0 && y < MT * 16 && (y & 15) < 4) != 0;
+    if (here) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (y == i * 16 + r) acc[i][j][r] += up;
+    }
+    T* o = (T*)g.dl + n * g.dl_ld + (m0 + wm + 4 * q);
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-      float d[4];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const bool in = live && g.v0 + m0 + wm + i * 16 + 4 * q + r < g.vocab;
-        const float l = bias[i][r] == -__builtin_inff() ? bias[i][r] : acc[i][j][r] + bias[i][r];
-        d[r] = in ? up * ((y == i * 16 + r ? 1.0f : 0.0f) - expf(l - lse)) : 0.0f;
-        dbs[i][r] += d[r];
-      }
-      T* o = (T*)g.dl + n * g.dl_ld + (m0 + wm + i * 16 + 4 * q);
+      for (int r = 0; r < 4; ++r) dbs[i][r] += acc[i][j][r];
       if (sizeof(T) == 2) {
         // rounded to bf16 (the products that follow take bf16 operands): each entry is off by at most 2^-9 of it,
         // independently of its neighbours.  The value's own entry is usually far larger than the others, so that ONE
         // rounding would show in whole rows of the gradients: what it loses is kept apart and added in f32.
         bf16x4 h;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          h[r] = (bf16)d[r];
-          if (y == i * 16 + r) g.resid[n] = d[r] - (float)h[r];
-        }
-        *(bf16x4*)o = h;
+        for (int r = 0; r < 4; ++r) h[r] = (bf16)acc[i][j][r];
+        *(bf16x4*)(o + i * 16) = h;
+        if (here)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (y == i * 16 + r) g.resid[n] = acc[i][j][r] - (float)h[r];
       } else {
-        *(f32x4*)o = f32x4{d[0], d[1], d[2], d[3]};
+        *(f32x4*)(o + i * 16) = acc[i][j];
       }
     }
   }
@@ -422,7 +465,7 @@ __global__ void __launch_bounds__(GEMM_THREADS)
     k_lincat_gemm(GemmArgs g) {
   constexpr int WN = BN == 256 ? 4 : 2, WM = 8 / WN;       // waves along n and m
   constexpr int MT = BM / WM / 16, NT = BN / WN / 16;
-  constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2, STAGE = A_BYTES + B_BYTES;
+  constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2;
   extern __shared__ char smem_raw[];
   LDS_AS char* smem = (LDS_AS char*)smem_raw;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -435,31 +478,38 @@ __global__ void __launch_bounds__(GEMM_THREADS)
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-  auto issue = [&](int kt, int buf) {
-    TileLoader<BM, TA>::load(g.a, g.a.p, tile.m0, kt * BK, smem + buf * STAGE, tid);
-    TileLoader<BN, TB>::load(g.b, g.b.p, tile.n0, kt * BK, smem + buf * STAGE + A_BYTES, tid);
-  };
-
   const int wm = (wave / WN) * (MT * 16), wn = (wave % WN) * (NT * 16);
-  if (kt0 < kt1) issue(kt0, 0);
-  for (int kt = kt0; kt < kt1; ++kt) {
+  TileLoader<BM, TA> la(g.a, tile.m0, kt0 * BK, lane, wave);
+  TileLoader<BN, TB> lb(g.b, tile.n0, kt0 * BK, lane, wave);
+  if (kt0 < kt1) {
+    la.load(g.a, kt0 * BK, smem);
+    lb.load(g.b, kt0 * BK, smem + 2 * A_BYTES);
+  }
+  auto step = [&](int kt, int buf) {       // buf: a constant where it is called
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    if (kt + 1 < kt1) issue(kt + 1, (kt + 1 - kt0) & 1);
-    LDS_AS char* sa = smem + ((kt - kt0) & 1) * STAGE;
-    LDS_AS char* sb = sa + A_BYTES;
+    if (kt + 1 < kt1) {
+      la.load(g.a, (kt + 1) * BK, smem + (buf ^ 1) * A_BYTES);
+      lb.load(g.b, (kt + 1) * BK, smem + 2 * A_BYTES + (buf ^ 1) * B_BYTES);
+    }
+    LDS_AS char* sa = smem + buf * A_BYTES;
+    LDS_AS char* sb = smem + 2 * A_BYTES + buf * B_BYTES;
 #pragma unroll
     for (int s = 0; s < BK / 32; ++s) {
       bf16x8 fb[NT];
 #pragma unroll
-      for (int j = 0; j < NT; ++j) fb[j] = TileLoader<BN, TB>::frag(sb, wn + j * 16, s, lane);
+      for (int j = 0; j < NT; ++j) fb[j] = lb.frag(sb, wn + j * 16, s);
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
-        const bf16x8 fa = TileLoader<BM, TA>::frag(sa, wm + i * 16, s, lane);
+        const bf16x8 fa = la.frag(sa, wm + i * 16, s);
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = mma(fa, fb[j], acc[i][j]);
       }
     }
+  };
+  for (int kt = kt0; kt < kt1; kt += 2) {
+    step(kt, 0);
+    if (kt + 1 < kt1) step(kt + 1, 1);
   }
   __syncthreads();
   epilogue<bf16, BM, BN, WM, WN, MT, NT, TB, EPI>(g, tile, acc, smem_raw);
@@ -665,7 +715,7 @@ __global__ void __launch_bounds__(GJX_BLOCK)
       }
       const float base = top == -__builtin_inff() ? 0.0f : top;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) sum += expf(acc[j][r] - base);
+      for (int r = 0; r < 4; ++r) sum += exp_of(acc[j][r] - base);
     } else if (n < g.n) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -791,6 +841,7 @@ __global__ void __launch_bounds__(GJX_BLOCK)
 // ---------------------------------------------------------------------------
 constexpr int64_t DL_BYTES = (int64_t)512 << 20;      // dl of one piece of the vocabulary (any size is right)
 constexpr int64_t PACK_BYTES = (int64_t)512 << 20;    // packed weights of one piece
+constexpr int64_t MAX_LD = 1 << 22;                   // 256 rows stay within 32-bit byte offsets
 constexpr int ROWS_MAX = 32;                          // rows up to which k_lincat_rows is used
 
 int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
@@ -931,6 +982,7 @@ int32_t check_args(const Call& c) {
               (long long)c.n, (long long)c.vocab, (long long)c.width);
   GJX_REQUIRE(c.n == 0 || (c.y && c.x && c.w), GJX_EINVAL, "%s: null input", c.who);
   GJX_REQUIRE(c.x_ld >= c.width && c.w_ld >= c.width, GJX_EINVAL, "%s: a row stride is smaller than the width", c.who);
+  GJX_REQUIRE(c.x_ld <= MAX_LD && c.w_ld <= MAX_LD, GJX_ELIMIT, "%s: a row stride is above 2^22 elements", c.who);
   GJX_REQUIRE(c.n <= GJX_MAX_LINCAT && c.vocab <= GJX_MAX_LINCAT && c.width <= 65536, GJX_ELIMIT,
               "%s: n and vocab go up to 2^24, width up to 65536", c.who);
   return GJX_OK;
@@ -1139,7 +1191,7 @@ GJX_API int32_t gjx_linear_categorical_grad(int32_t dtype, const int32_t* d_y, c
       b.fa = in.fw;
       b.b = dl;
       b.fb = fdl;
-      b.ktiles = depth_tiles(c, rows_pad);
+      b.ktiles = depth_tiles(c, rows);                       // no tile lies wholly behind the last row of W
       b.mt = mk;
       b.nt = (int)p.n_tiles;
       b.splits = p.splits;
@@ -1157,7 +1209,7 @@ GJX_API int32_t gjx_linear_categorical_grad(int32_t dtype, const int32_t* d_y, c
       b.fa = in.fx;
       b.b = dl;
       b.fb = fdl;
-      b.ktiles = depth_tiles(c, f32 ? n : p.n_pad);
+      b.ktiles = depth_tiles(c, n);
       b.mt = mk;
       b.nt = (int)(f32 ? up(rows, 128) / 128 : rows_pad / 256);
       b.out = f32 ? (void*)((float*)d_dw + v0 * width) : (void*)((bf16*)d_dw + v0 * width);
