@@ -458,8 +458,10 @@ __device__ __forceinline__ void epilogue(const GemmArgs& g, const Tile& tile, f3
   }
 }
 
-// C[m][n] = sum_k A(m, k) B(n, k) in bf16; BM x BN per workgroup of eight waves.  Two LDS buffers of one 64-deep tile each:
-// the loads of tile i + 1 run under the products of tile i, one barrier per tile.
+// C[m][n] = sum_k A(m, k) B(n, k) in bf16; BM x BN per workgroup of eight waves.  Two LDS buffers of one 64-deep tile each
+// and two register sets of fragments: while the products of one 32-deep slab run, the next slab is read (across the tile's
+// end: the one barrier of a tile stands between its two slabs, when its last slab is in registers), and the tile after the
+// next one is on its way into the buffer just emptied.
 template <int BN, bool TA, bool TB, int EPI>
 __global__ void __launch_bounds__(GEMM_THREADS)
     k_lincat_gemm(GemmArgs g) {
@@ -485,28 +487,52 @@ __global__ void __launch_bounds__(GEMM_THREADS)
     la.load(g.a, kt0 * BK, smem);
     lb.load(g.b, kt0 * BK, smem + 2 * A_BYTES);
   }
-  auto step = [&](int kt, int buf) {       // buf: a constant where it is called
+  if (kt0 + 1 < kt1) {
+    la.load(g.a, (kt0 + 1) * BK, smem + A_BYTES);
+    lb.load(g.b, (kt0 + 1) * BK, smem + 2 * A_BYTES + B_BYTES);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(la.LOADS + lb.LOADS) : "memory");
+  } else {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (kt + 1 < kt1) {
-      la.load(g.a, (kt + 1) * BK, smem + (buf ^ 1) * A_BYTES);
-      lb.load(g.b, (kt + 1) * BK, smem + 2 * A_BYTES + (buf ^ 1) * B_BYTES);
-    }
+  }
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  struct Frags {
+    bf16x8 a[MT], b[NT];
+  } f0, f1;
+  auto read = [&](int buf, int s, Frags& f) {
     LDS_AS char* sa = smem + buf * A_BYTES;
     LDS_AS char* sb = smem + 2 * A_BYTES + buf * B_BYTES;
 #pragma unroll
-    for (int s = 0; s < BK / 32; ++s) {
-      bf16x8 fb[NT];
+    for (int j = 0; j < NT; ++j) f.b[j] = lb.frag(sb, wn + j * 16, s);
 #pragma unroll
-      for (int j = 0; j < NT; ++j) fb[j] = lb.frag(sb, wn + j * 16, s);
+    for (int i = 0; i < MT; ++i) f.a[i] = la.frag(sa, wm + i * 16, s);
+  };
+  auto multiply = [&](const Frags& f) {
 #pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        const bf16x8 fa = la.frag(sa, wm + i * 16, s);
+    for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int j = 0; j < NT; ++j) acc[i][j] = mma(fa, fb[j], acc[i][j]);
-      }
+      for (int j = 0; j < NT; ++j) acc[i][j] = mma(f.a[i], f.b[j], acc[i][j]);
+    // the reads that stand in front of the products go between them
+    constexpr int READS = MT * (TA ? 2 : 1) + NT * (TB ? 2 : 1), EACH = MT * NT / READS > 0 ? MT * NT / READS : 1;
+#pragma unroll
+    for (int r = 0; r < READS; ++r) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);       // one LDS read
+      __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);    // EACH matrix instructions
     }
   };
+  auto step = [&](int kt, int buf) {       // buf: a constant where it is called
+    read(buf, 1, f1);
+    multiply(f0);
+    // this wave's reads of the tile are done and its loads of the next tile have arrived; behind the barrier: everyone's
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (kt + 2 < kt1) {
+      la.load(g.a, (kt + 2) * BK, smem + buf * A_BYTES);
+      lb.load(g.b, (kt + 2) * BK, smem + 2 * A_BYTES + buf * B_BYTES);
+    }
+    read(buf ^ 1, 0, f0);                  // behind the last tile: the other buffer's old contents, not used
+    multiply(f1);
+  };
+  if (kt0 < kt1) read(0, 0, f0);
   for (int kt = kt0; kt < kt1; kt += 2) {
     step(kt, 0);
     if (kt + 1 < kt1) step(kt + 1, 1);
