@@ -105,6 +105,15 @@ __device__ __forceinline__ f32x4 mma3(const bf16x8 (&a)[3], const bf16x8 (&b)[3]
 
 __device__ __forceinline__ int tr_swizzle(int k) { return (k & 3) | (((k >> 3) & 3) << 2); }
 
+// Two transposing reads of four reduction entries each.  `other` (unused) and the restrict qualifiers give the reads alias
+// information: without any, the compiler takes them to read what the loads into LDS in flight are writing and waits for
+// those first.  (What is read was loaded, waited for and fenced by a barrier a tile earlier.)
+__device__ __forceinline__ bf16x8 read_transposed(LDS_AS char* __restrict__ p, LDS_AS char* __restrict__ other, int four_rows) {
+  const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((LDS_AS bf16x4*)p);
+  const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((LDS_AS bf16x4*)(p + four_rows));
+  return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
 // One BK-deep tile of an operand, R output indices wide: R * 8 chunks of 16 bytes straight into LDS.  The offsets of a
 // lane's chunks from the tile's first byte are kept (32 bits), so a step along the reduction costs one scalar addition;
 // the fragments' LDS addresses are one or two lane addresses plus constants.
@@ -155,9 +164,7 @@ struct TileLoader {
   __device__ __forceinline__ bf16x8 frag(LDS_AS char* lds, int i0, int s) const {
     if (T) {
       LDS_AS char* p = lds + at[0] + s * 32 * (R * 2) + (((uint32_t)(i0 >> 4) ^ at[1]) << 5);
-      const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((LDS_AS bf16x4*)p);
-      const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((LDS_AS bf16x4*)(p + 4 * R * 2));
-      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+      return read_transposed(p, lds, 4 * R * 2);
     }
     return *(LDS_AS bf16x8*)(lds + at[s] + i0 * 128);
   }
@@ -218,18 +225,27 @@ __device__ __forceinline__ void epilogue(const GemmArgs& g, const Tile& tile, f3
   const int q = lane >> 4, c = lane & 15;
   if (EPI == EPI_STORE) {
     if (sizeof(T) == 2 && TB && g.resid_in) {
-      // dW of the rows' own values: += resid_i x_i, in ascending i (every wave looks for its own columns)
-      for (int64_t i0 = 0; i0 < g.n; i0 += 64) {
-        const int64_t row = min(i0 + lane, g.n - 1);
-        const int64_t v = min(max((int64_t)g.y[row], (int64_t)0), g.vocab - 1) - g.v0 - n0 - wn;
-        const float res = g.resid_in[row];
-        uint64_t hits = __ballot(i0 + lane < g.n && v >= 0 && v < NT * 16);
-        while (hits) {
-          const int l = __builtin_ctzll(hits);
-          hits &= hits - 1;
-          const int vl = __builtin_amdgcn_readlane((int)v, l);
-          const float rl = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(res), l));
-          if ((vl & 15) == c) {
+      // dW of the rows' own values: += resid_i x_i, in ascending i (every wave looks for its own columns, 512 rows at a time)
+      for (int64_t i8 = 0; i8 < g.n; i8 += 512) {
+        int v8[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v8[u] = g.y[min(i8 + 64 * u + lane, g.n - 1)];
+#pragma unroll 1
+        for (int u = 0; u < 8; ++u) {
+          const int64_t i0 = i8 + 64 * u;
+          int yv = v8[0];
+#pragma unroll
+          for (int e = 1; e < 8; ++e) yv = u == e ? v8[e] : yv;
+          const int64_t v = min(max((int64_t)yv, (int64_t)0), g.vocab - 1) - g.v0 - n0 - wn;
+          uint64_t hits = __ballot(i0 + lane < g.n && v >= 0 && v < NT * 16);
+          if (!hits) continue;
+          const float res = g.resid_in[min(i0 + lane, g.n - 1)];
+          while (hits) {
+            const int l = __builtin_ctzll(hits);
+            hits &= hits - 1;
+            const int vl = __builtin_amdgcn_readlane((int)v, l);
+            const float rl = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(res), l));
+            if ((vl & 15) != c) continue;
             const bf16* xr = g.a.p + (i0 + l) * g.a.ld;
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
