@@ -127,7 +127,7 @@ struct TileLoader {
   int64_t step;
 
   __device__ __forceinline__ TileLoader(const Operand& o, int out, int k0, int lane_, int wave_) : out0(out), lane(lane_), wave(wave_) {
-    base = (const char*)o.p + (T ? (int64_t)k0 * o.ld : (int64_t)out0 * o.ld + k0) * 2;
+    base = (const char*)o.p + (T ? (int64_t)k0 * o.ld : (int64_t)min(out0, o.rows - 1) * o.ld + k0) * 2;
     step = T ? BK * o.ld * 2 : BK * 2;
 #pragma unroll
     for (int j = 0; j < LOADS; ++j) off[j] = offset(o, j, BK);
@@ -146,10 +146,10 @@ struct TileLoader {
     if (T) {
       const int row = c / (R / 8), ch = c % (R / 8);
       const int col = min(out0 + ((((ch >> 1) ^ tr_swizzle(row)) << 1) | (ch & 1)) * 8, o.cols - 8);
-      return ((uint32_t)min(row, left - 1) * (uint32_t)o.ld + (uint32_t)col) * 2u;
+      return ((uint32_t)min(row, max(left, 1) - 1) * (uint32_t)o.ld + (uint32_t)col) * 2u;
     }
     const int row = c >> 3, ch = (c & 7) ^ ((row >> 1) & 7);
-    return ((uint32_t)min(row, o.rows - 1 - out0) * (uint32_t)o.ld + (uint32_t)ch * 8u) * 2u;
+    return ((uint32_t)(min(out0 + row, o.rows - 1) - min(out0, o.rows - 1)) * (uint32_t)o.ld + (uint32_t)ch * 8u) * 2u;
   }
   __device__ __forceinline__ void load(const Operand& o, int k0, LDS_AS char* lds) {
     const bool ragged = T && k0 + BK > o.rows;
@@ -557,14 +557,21 @@ __global__ void __launch_bounds__(GEMM_THREADS)
   epilogue<bf16, BM, BN, WM, WN, MT, NT, TB, EPI>(g, tile, acc, smem_raw);
 }
 
-// one 32-deep slab of an f32 operand, R output indices wide: pieces of eight reduction entries of one output index, loaded
-// into registers, split and written to LDS as fragments (16 indices x 3 planes x 64 lanes x 16 bytes)
+// One 32-deep slab of an f32 operand, R output indices wide: pieces of eight reduction entries of one output index, loaded
+// into registers, split and written to LDS as fragments (16 indices x 3 planes x 64 slots of 16 bytes).  Whole slabs of
+// aligned rows are read at a uniform base plus a kept 32-bit offset; others entry by entry, clamped and masked.
+// Slot (index, group) lies at 16 group + (index + 2 group) % 16: neither the four lanes that write a row's groups nor the
+// sixteen that read a group meet in a bank (without the rotation 60 % of the LDS cycles were conflicts).
 template <int R, bool T>
 struct SlabLoader {
   static constexpr int PIECES = (R * 4 + GEMM32_THREADS - 1) / GEMM32_THREADS;
   float x[PIECES][8];
+  uint32_t off[PIECES];
+  const char* base;                    // uniform
+  int out0, tid;
 
-  static __device__ __forceinline__ void where(int u, int& index, int& group) {
+  __device__ __forceinline__ void where(int i, int& index, int& group) const {
+    const int u = min(i * GEMM32_THREADS + tid, R * 4 - 1);
     if (T) {
       index = u % R;          // neighbouring lanes take neighbouring columns
       group = u / R;
@@ -573,54 +580,67 @@ struct SlabLoader {
       group = u & 3;
     }
   }
-  __device__ __forceinline__ void load(const OperandF& o, int out0, int k0, int tid) {
+  __device__ __forceinline__ SlabLoader(const OperandF& o, int out, int k0, int tid_) : out0(out), tid(tid_) {
+    const int row0 = min(out0, o.rows - 1);       // a tile may lie wholly behind the last row (the vocabulary is padded)
+    base = (const char*)(o.p + (T ? (int64_t)k0 * o.ld : (int64_t)row0 * o.ld + k0));
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
-      const int u = i * GEMM32_THREADS + tid;
       int index, group;
-      where(min(u, R * 4 - 1), index, group);
-      const int k = k0 + 8 * group;
-      if (T) {
-        const float* p = o.p + min(out0 + index, o.cols - 1);
+      where(i, index, group);
+      off[i] = T ? ((uint32_t)(8 * group) * (uint32_t)o.ld + (uint32_t)min(out0 + index, o.cols - 1)) * 4u
+                 : ((uint32_t)(min(out0 + index, o.rows - 1) - row0) * (uint32_t)o.ld + (uint32_t)(8 * group)) * 4u;
+    }
+  }
+  __device__ __forceinline__ void load(const OperandF& o, int k0) {
+    if (T ? k0 + 32 <= o.rows : o.vec && k0 + 32 <= o.cols) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[i][j] = p[(int64_t)min(k + j, o.rows - 1) * o.ld];       // all eight in flight, then masked
+      for (int i = 0; i < PIECES; ++i) {
+        if (T) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[i][j] = k + j < o.rows ? x[i][j] : 0.0f;
-      } else {
-        const float* p = o.p + (int64_t)min(out0 + index, o.rows - 1) * o.ld;
-        if (o.vec && k + 8 <= o.cols) {
-          const f32x4 lo = *(const f32x4*)(p + k), hi = *(const f32x4*)(p + k + 4);
+          for (int j = 0; j < 8; ++j) x[i][j] = *(const float*)(base + (int64_t)j * o.ld * 4 + off[i]);
+        } else {
+          const f32x4 lo = *(const f32x4*)(base + off[i]), hi = *(const f32x4*)(base + 16 + off[i]);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             x[i][j] = lo[j];
             x[i][4 + j] = hi[j];
           }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) x[i][j] = p[min(k + j, o.cols - 1)];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) x[i][j] = k + j < o.cols ? x[i][j] : 0.0f;
         }
       }
+    } else {
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) {
+        int index, group;
+        where(i, index, group);
+        const int k = k0 + 8 * group;
+        const float* p = T ? o.p + min(out0 + index, o.cols - 1) : o.p + (int64_t)min(out0 + index, o.rows - 1) * o.ld;
+        const int64_t step = T ? o.ld : 1;
+        const int end = T ? o.rows : o.cols;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[i][j] = p[min(k + j, end - 1) * step];       // all eight in flight, then masked
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[i][j] = k + j < end ? x[i][j] : 0.0f;
+      }
     }
+    base += T ? 32 * o.ld * 4 : 128;
   }
-  __device__ __forceinline__ void store(char* lds, int tid) const {
+  __device__ __forceinline__ void store(char* lds) const {
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
-      const int u = i * GEMM32_THREADS + tid;
-      if (R * 4 % GEMM32_THREADS && u >= R * 4) continue;
+      if (R * 4 % GEMM32_THREADS && i * GEMM32_THREADS + tid >= R * 4) continue;
       int index, group;
-      where(u, index, group);
+      where(i, index, group);
       bf16x8 o[3];
       split8(x[i], o);
-      char* f = lds + (index >> 4) * 3072 + ((index & 15) + 16 * group) * 16;
+      char* f = lds + (index >> 4) * 3072 + (16 * group + ((index + 2 * group) & 15)) * 16;
 #pragma unroll
       for (int p = 0; p < 3; ++p) *(bf16x8*)(f + p * 1024) = o[p];
     }
   }
   static __device__ __forceinline__ void frag(const char* lds, int i0, int lane, bf16x8 (&out)[3]) {
+    const int q = lane >> 4;
 #pragma unroll
-    for (int p = 0; p < 3; ++p) out[p] = *(const bf16x8*)(lds + (i0 >> 4) * 3072 + p * 1024 + lane * 16);
+    for (int p = 0; p < 3; ++p) out[p] = *(const bf16x8*)(lds + (i0 >> 4) * 3072 + p * 1024 + (16 * q + ((lane + 2 * q) & 15)) * 16);
   }
 };
 
@@ -643,30 +663,34 @@ __global__ void __launch_bounds__(GEMM32_THREADS, 3)
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   const int wm = (wave / WN) * (MT * 16), wn = (wave % WN) * (NT * 16);
-  SlabLoader<BM, TA> la;
-  SlabLoader<BN, TB> lb;
+  SlabLoader<BM, TA> la(g.fa, tile.m0, kt0 * 32, tid);
+  SlabLoader<BN, TB> lb(g.fb, tile.n0, kt0 * 32, tid);
   if (kt0 < kt1) {
-    la.load(g.fa, tile.m0, kt0 * 32, tid);
-    lb.load(g.fb, tile.n0, kt0 * 32, tid);
+    la.load(g.fa, kt0 * 32);
+    lb.load(g.fb, kt0 * 32);
   }
   char *sa = smem_raw, *sb = sa + A_BYTES;
   for (int kt = kt0; kt < kt1; ++kt) {
-    la.store(sa, tid);
-    lb.store(sb, tid);
+    la.store(sa);
+    lb.store(sb);
     __syncthreads();
     if (kt + 1 < kt1) {
-      la.load(g.fa, tile.m0, (kt + 1) * 32, tid);
-      lb.load(g.fb, tile.n0, (kt + 1) * 32, tid);
+      la.load(g.fa, (kt + 1) * 32);
+      lb.load(g.fb, (kt + 1) * 32);
     }
-    bf16x8 fb[NT][3];
 #pragma unroll
-    for (int j = 0; j < NT; ++j) SlabLoader<BN, TB>::frag(sb, wn + j * 16, lane, fb[j]);
+    for (int j = 0; j < NT; j += 2) {          // two column tiles at a time: with all four, registers spill
+      bf16x8 fb[2][3];
+      SlabLoader<BN, TB>::frag(sb, wn + j * 16, lane, fb[0]);
+      SlabLoader<BN, TB>::frag(sb, wn + j * 16 + 16, lane, fb[1]);
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      bf16x8 fa[3];
-      SlabLoader<BM, TA>::frag(sa, wm + i * 16, lane, fa);
-#pragma unroll
-      for (int j = 0; j < NT; ++j) acc[i][j] = mma3(fa, fb[j], acc[i][j]);
+      for (int i = 0; i < MT; ++i) {
+        bf16x8 fa[3];
+        SlabLoader<BM, TA>::frag(sa, wm + i * 16, lane, fa);
+        acc[i][j] = mma3(fa, fb[0], acc[i][j]);
+        acc[i][j + 1] = mma3(fa, fb[1], acc[i][j + 1]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
     __syncthreads();
   }
