@@ -704,18 +704,17 @@ def _delta_step_plan(dtypes, q_shape, k_shape, v_shape, g_shape, b_shape, q_stri
 def delta_filter_step(state, q, k, v, log_decay, beta, scale=None, ancestors=None, out=None):
     """One token per batch element: q, k (n, key heads, dk), v (n, heads, dv), gates (n, heads) -> (o (n, heads, dv), state)."""
     who = "delta_filter_step"
-    names = ("q", "k", "v", "log_decay", "beta")
-    t = [q, k, v, log_decay, beta]
-    for i, name in enumerate(names):
-        if not isinstance(t[i], torch.Tensor):
+    for name, t in (("q", q), ("k", k), ("v", v), ("log_decay", log_decay), ("beta", beta)):
+        if not isinstance(t, torch.Tensor):
             raise GjxError(f"{who}: `{name}` must be a tensor")
-        if i < 3 and t[i].dim() > 0 and t[i].stride(-1) != 1 and t[i].shape[-1] > 1:
-            t[i] = t[i].contiguous()
-    p = _delta_step_plan(tuple(a.dtype for a in t), *(a.shape for a in t), *(a.stride() for a in t), scale)
+    unit = lambda t: t if t.dim() == 0 or t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()       # noqa: E731
+    q, k, v = unit(q), unit(k), unit(v)
+    p = _delta_step_plan((q.dtype, k.dtype, v.dtype, log_decay.dtype, beta.dtype), q.shape, k.shape, v.shape, log_decay.shape,
+                         beta.shape, q.stride(), k.stride(), v.stride(), log_decay.stride(), beta.stride(), scale)
     if state is None:
         raise GjxError(f"{who}: `state` must be float32 of shape {(p.batch, p.heads, p.dk, p.dv)}")
     state, ancestors = _delta_state(who, "state", state, p), _delta_indices(who, "ancestors", ancestors, p)
-    _on_current_device(who, *zip(names, t))
+    _on_current_device(who, ("q", q), ("k", k), ("v", v), ("log_decay", log_decay), ("beta", beta))
     if out is None:
         out = torch.empty_like(state)
     else:
@@ -724,11 +723,13 @@ def delta_filter_step(state, q, k, v, log_decay, beta, scale=None, ancestors=Non
         _on_current_device(who, ("out", out))
         if _overlap(out, state) and (ancestors is not None or out.data_ptr() != state.data_ptr()):
             raise GjxError(f"{who}: `out` may be the state itself without ancestors and must not overlap it otherwise")
-    if state.data_ptr() % 16 or out.data_ptr() % 16:
+    from_, to = state.data_ptr(), out.data_ptr()
+    if (from_ | to) & 15:
         raise GjxError(f"{who}: states must be aligned to 16 bytes")
     o = torch.empty((p.batch, p.heads, p.dv), dtype=v.dtype, device=v.device)
-    N.check(N.lib().gjx_delta_filter_step(p.ref, state.data_ptr(), _address(ancestors), *(a.data_ptr() for a in t), o.data_ptr(),
-                                          out.data_ptr(), _raw_stream()), "gjx_delta_filter_step")
+    N.check(N.lib().gjx_delta_filter_step(p.ref, from_, _address(ancestors), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                                          log_decay.data_ptr(), beta.data_ptr(), o.data_ptr(), to, _raw_stream()),
+            "gjx_delta_filter_step")
     return o, out
 
 

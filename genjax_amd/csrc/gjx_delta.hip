@@ -173,31 +173,39 @@ __device__ __forceinline__ int64_t length_of(const int32_t* lengths, int64_t b, 
 // ---------------------------------------------------------------------------
 // all chunks at once: fragments of K, Q and their transposes, That, P (keep: T^T, P^T), the row factors
 // ---------------------------------------------------------------------------
+// 64 rows of K or Q: into registers (all loads in flight at once), then split and into LDS
 template <typename T, int DKP, int NPI>
-__device__ __forceinline__ void load_rows(const T* src, int64_t token_stride, int tokens, int dk, bool vec, bf16* lds, int tid) {
-  constexpr int PITCH = DKP + 8, PLANE = C * PITCH;
-  for (int i = tid; i < C * (DKP / 8); i += 256) {
-    const int t = i / (DKP / 8), c0 = (i % (DKP / 8)) * 8;
-    float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (t < tokens && c0 < dk) {
-      const T* p = src + t * token_stride + c0;
-      if (vec && c0 + 8 <= dk) {
-        typedef T vec8 __attribute__((ext_vector_type(8)));
-        const vec8 v = *(const vec8*)p;
+struct RowLoader {
+  static constexpr int PIECES = C * (DKP / 8) / 256, PITCH = DKP + 8, PLANE = C * PITCH;
+  typedef T vec8 __attribute__((ext_vector_type(8)));
+  vec8 x[PIECES];
+  __device__ __forceinline__ void load(const T* src, int64_t token_stride, int tokens, int dk, bool vec, int tid) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = (float)v[j];
+    for (int i = 0; i < PIECES; ++i) {
+      const int u = i * 256 + tid, t = min(u / (DKP / 8), tokens - 1), c0 = (u % (DKP / 8)) * 8;
+      const T* p = src + t * token_stride;
+      if (vec) {
+        x[i] = *(const vec8*)(p + min(c0, dk - 8));
       } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (c0 + j < dk) x[j] = (float)p[j];
+        for (int j = 0; j < 8; ++j) x[i][j] = p[min(c0 + j, dk - 1)];
       }
     }
-    bf16x8 out[NPI];
-    split<NPI>(x, out);
-#pragma unroll
-    for (int p = 0; p < NPI; ++p) *(bf16x8*)(lds + p * PLANE + t * PITCH + c0) = out[p];
   }
-}
+  __device__ __forceinline__ void store(int tokens, int dk, bf16* lds, int tid) const {
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      const int u = i * 256 + tid, t = u / (DKP / 8), c0 = (u % (DKP / 8)) * 8;
+      float f[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = t < tokens && c0 + j < dk ? (float)x[i][j] : 0.0f;
+      bf16x8 out[NPI];
+      split<NPI>(f, out);
+#pragma unroll
+      for (int p = 0; p < NPI; ++p) *(bf16x8*)(lds + p * PLANE + t * PITCH + c0) = out[p];
+    }
+  }
+};
 
 template <int DKP, int NPI>
 __device__ __forceinline__ void store_row_frags(const bf16* lds, bf16* dst, int tid) {   // rows are tokens
@@ -284,8 +292,9 @@ __global__ void __launch_bounds__(256)
   bf16* gates = w.gates + (bh * sh.chunks + chunk) * w.gate_size;
   float* rows = w.rows + (bh * sh.chunks + chunk) * ROWS;
 
-  load_rows<T, DKP, NPI>(k + b * sh.ks[0] + t0 * sh.ks[1] + kh * sh.ks[2], sh.ks[1], tokens, sh.dk, vec, sk, tid);
-  load_rows<T, DKP, NPI>(q + b * sh.qs[0] + t0 * sh.qs[1] + kh * sh.qs[2], sh.qs[1], tokens, sh.dk, vec, sq, tid);
+  RowLoader<T, DKP, NPI> lk, lq;
+  lk.load(k + b * sh.ks[0] + t0 * sh.ks[1] + kh * sh.ks[2], sh.ks[1], tokens, sh.dk, vec, tid);
+  lq.load(q + b * sh.qs[0] + t0 * sh.qs[1] + kh * sh.qs[2], sh.qs[1], tokens, sh.dk, vec, tid);
   if (wave == 0) {
     const bool in = lane < tokens;
     // differences of the cumulative decay keep f32 accuracy whatever its size: 64-bit sum, kept as two floats
@@ -306,6 +315,8 @@ __global__ void __launch_bounds__(256)
     rows[2 * C + lane] = expf((float)(last - gam));
     rows[3 * C + lane] = expf((float)last);
   }
+  lk.store(tokens, sh.dk, sk, tid);
+  lq.store(tokens, sh.dk, sq, tid);
   __syncthreads();
 
   // K K^T and Q K^T, row tile = wave
@@ -486,6 +497,15 @@ struct Cursor {
   }
 };
 
+// Touch a chunk's operands, one load of four bytes per 128-byte line, so that they are in this XCD's L2 when the waves load
+// them a chunk later.  The workgroups of a head share the lines out: `first` of `waves` waves.  The loads go to LDS that
+// nobody reads.
+__device__ __forceinline__ void touch(const void* block, int bytes, int first, int waves, int lane, char* sink) {
+  for (int i = first; i * 8192 < bytes; i += waves)
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)((const char*)block + min(i * 8192 + lane * 128, bytes - 4)),
+                                     (__attribute__((address_space(3))) void*)sink, 4, 0, 0);
+}
+
 // this lane's four tokens of a (batch, time, head, dv) column block: raw values, converted and masked where they are used
 template <typename T, int NC>
 struct Columns {
@@ -517,6 +537,20 @@ __device__ __forceinline__ void store_rows(float* block, int row, int col, int p
   for (int r = 0; r < 4; ++r) store_at(block, (uint32_t)((row + r) * pitch + col) * 4, x[r]);
 }
 
+// a slab of S from its three planes (their sum is exact) to rows of an f32 block
+__device__ __forceinline__ void store_slab(const bf16* frag, float* block, int s, const Place& p, int col, int pitch) {
+  bf16x8 f[3];
+  get_frag<3>(frag, p.lane, f);
+  f32x4 lo, hi;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    lo[j] = (float)f[0][j] + ((float)f[1][j] + (float)f[2][j]);
+    hi[j] = (float)f[0][4 + j] + ((float)f[1][4 + j] + (float)f[2][4 + j]);
+  }
+  store_rows(block, 32 * s + 4 * p.quad, col, pitch, lo);
+  store_rows(block, 32 * s + 16 + 4 * p.quad, col, pitch, hi);
+}
+
 template <typename T>
 __device__ __forceinline__ void store_tokens(T* chunk, const Place& p, int col, uint32_t step, bool all, int dv, int left, f32x4 x) {
   const uint32_t at = (uint32_t)p.tok * step + (uint32_t)col * sizeof(T);
@@ -538,6 +572,9 @@ __global__ void __launch_bounds__(TEAM, 2)
   constexpr int KS = DKP / 32, MT = DKP / 64;     // slabs of S; 16-row tiles of S per wave
   constexpr int NPO = NPI == 1 ? 2 : 3;           // planes of what only the read-out takes
   __shared__ bf16 x_s[KS * NC * 3 * FRAG], x_r[2 * NC * 3 * FRAG], x_v[2][2 * NC * NPO * FRAG], x_w[2 * NC * 3 * FRAG];
+  __shared__ f32x4 x_d[KEEP ? 2 * 4 * NC * 64 : 1];        // delta, for the read-out waves to keep
+  __shared__ char sink[4][256];
+  const int tiles = (sh.dvp / 16 + NC - 1) / NC;
   Place p;
   if (!place_of<NC>(sh, lengths, p)) return;
   const int lane = p.lane, wave = p.wave, tok = p.tok;
@@ -574,6 +611,9 @@ __global__ void __launch_bounds__(TEAM, 2)
       const int left = (int)std::min<int64_t>(C, sh.time - ch * C);
 #pragma unroll
       for (int n = 0; n < NC; ++n) {
+        if (KEEP && p.col0 + 16 * n < sh.dvp)
+          store_rows(w.delta + (p.bh * sh.chunks + ch) * C * sh.dvp, tok, p.col0 + 16 * n, sh.dvp,
+                     x_d[(((int)(ch & 1) * 4 + wave) * NC + n) * 64 + lane]);
         Orders<NPO> acc;
 #pragma unroll
         for (int s = 0; s < 2; ++s)
@@ -589,6 +629,11 @@ __global__ void __launch_bounds__(TEAM, 2)
     for (int64_t ch = 0; ch < p.n_chunks; ++ch) {
       const Cursor here = next;
       next = next.step(w, 1, p);
+      const Cursor later = next.step(w, 1, p);
+      if (KEEP) {              // (without the stores of what is kept the loads are fast enough)
+        touch(later.keys, KB::SIZE * 2, p.tile * 4 + wave, tiles * 4, lane, sink[wave]);
+        touch(later.gates, (18 + 6 * NPO) * FRAG * 2, tiles * 4 - 1 - p.tile * 4 - wave, tiles * 4, lane, sink[wave]);
+      }
       lds_barrier();
       f32x4 now[NC];
 #pragma unroll
@@ -601,6 +646,9 @@ __global__ void __launch_bounds__(TEAM, 2)
           acc.add(qa[s], sf);
         }
         now[n] = acc.sum() * f_eg * sh.scale;
+        // what the gradient needs is stored from here: loads of the state waves would wait behind their own stores
+        if (KEEP && wave < KS && p.col0 + 16 * n < sh.dvp)
+          store_slab(x_s + (wave * NC + n) * 3 * FRAG, w.s0 + (p.bh * sh.chunks + ch) * DKP * sh.dvp, wave, p, p.col0 + 16 * n, sh.dvp);
       }
       load_q(next);
       lds_barrier();
@@ -683,10 +731,6 @@ __global__ void __launch_bounds__(TEAM, 2)
         acc.add(ka[s], sf);
       }
       put_half<3>(x_r + (lo * NC + n) * 3 * FRAG, wave & 1, lane, vals.get(sh, p, n, left) - f_eg * acc.sum());
-      if (KEEP && p.col0 + 16 * n < sh.dvp)
-#pragma unroll
-        for (int t = 0; t < MT; ++t)
-          store_rows(w.s0 + (p.bh * sh.chunks + ch) * DKP * sh.dvp, row0 + 16 * t, p.col0 + 16 * n, sh.dvp, S[n][t]);
     }
     lds_barrier();
     load_k(next);                // behind the barrier: issued while the first LDS reads are on their way
@@ -703,8 +747,7 @@ __global__ void __launch_bounds__(TEAM, 2)
       const f32x4 delta = acc.sum(), vn = delta * f_beta;
       put_half<3>(x_w + (lo * NC + n) * 3 * FRAG, wave & 1, lane, vn * f_rest);
       put_half<NPO>(x_v[ch & 1] + (lo * NC + n) * NPO * FRAG, wave & 1, lane, vn);
-      if (KEEP && p.col0 + 16 * n < sh.dvp)
-        store_rows(w.delta + (p.bh * sh.chunks + ch) * C * sh.dvp, tok, p.col0 + 16 * n, sh.dvp, delta);
+      if (KEEP) x_d[(((int)(ch & 1) * 4 + wave) * NC + n) * 64 + lane] = delta;
     }
     lds_barrier();
     load_t(next);
@@ -744,7 +787,9 @@ __global__ void __launch_bounds__(TEAM, 2)
   constexpr int KS = DKP / 32, MT = DKP / 64;
   // the read-out waves' P^T dO (x_p) and Q^T (scale e^gamma dO) (x_q) as accumulators of the state waves, in f32
   __shared__ bf16 x_s[KS * NC * 3 * FRAG], x_d[2 * NC * NPI * FRAG], x_g[2 * NC * 3 * FRAG], x_x[2 * NC * 3 * FRAG], x_e[2 * NC * 3 * FRAG];
-  __shared__ f32x4 x_p[4 * NC * 64], x_q[4 * MT * NC * 64];
+  __shared__ f32x4 x_p[4 * NC * 64], x_q[4 * MT * NC * 64], x_l[4 * NC * 64];      // x_l: e, for the read-out waves to store
+  __shared__ char sink[4][256];
+  const int tiles = (sh.dvp / 16 + NC - 1) / NC;
   Place p;
   if (!place_of<NC>(sh, lengths, p)) return;
   const int lane = p.lane, wave = p.wave, tok = p.tok;
@@ -755,6 +800,7 @@ __global__ void __launch_bounds__(TEAM, 2)
   const int half = wave / 2;                      // first slab of this wave's rows of T^T and P^T
 
   if (p.reads) {
+    const bool all_cols = p.tile * 16 * NC + 16 * NC <= sh.dv;
     bf16x8 qt[MT][2][NPI], pt[2][3];
     f32x4 f_eg;
     Columns<T, NC> vals(sh, p, stride);
@@ -821,12 +867,33 @@ __global__ void __launch_bounds__(TEAM, 2)
     if (p.n_chunks > 0) products(now);
     for (int64_t ch = p.n_chunks - 1; ch >= 0; --ch) {
       hand_over();               // read by the state waves between barriers one and two (x_p) and behind three (x_q)
+      const int64_t at = p.bh * sh.chunks + ch;
+      const int left = now.left(p), left_o = (int)std::min<int64_t>(C, sh.time - ch * C);
+      const f32x4 f_beta = load_at<f32x4>(now.rows, (uint32_t)tok * 4);
       now = now.step(w, -1, p);
+      const Cursor later = now.step(w, -1, p);
+      touch(later.keys, KB::SIZE_KEEP * 2, p.tile * 4 + wave, tiles * 4, lane, sink[wave]);
+      touch(later.gates + GateBlock::TT, 36 * FRAG * 2, tiles * 4 - 1 - p.tile * 4 - wave, tiles * 4, lane, sink[wave]);
       lds_barrier();
+      if (wave < KS)
+#pragma unroll
+        for (int n = 0; n < NC; ++n)
+          if (p.col0 + 16 * n < sh.dvp)
+            store_slab(x_s + (wave * NC + n) * 3 * FRAG, w.ds1 + at * DKP * sh.dvp, wave, p, p.col0 + 16 * n, sh.dvp);
       if (ch > 0) put_o(now);
       lds_barrier();
       if (ch > 0) products(now);
       lds_barrier();
+#pragma unroll
+      for (int n = 0; n < NC; ++n) {
+        const f32x4 e = x_l[(wave * NC + n) * 64 + lane];
+        if (p.col0 + 16 * n < sh.dvp) store_rows(w.e + at * C * sh.dvp, tok, p.col0 + 16 * n, sh.dvp, e);
+        f32x4 out = e * f_beta;
+        if (left < C)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) out[r] = tok + r < left ? out[r] : 0.0f;
+        store_tokens(dv + base + ch * C * stride, p, p.col0 + 16 * n, (uint32_t)stride * sizeof(T), all_cols && left_o == C, sh.dv, left_o, out);
+      }
       lds_barrier();
     }
     return;
@@ -834,7 +901,6 @@ __global__ void __launch_bounds__(TEAM, 2)
 
   __builtin_amdgcn_s_setprio(3);
   const int row0 = 16 * MT * wave + 4 * p.quad;
-  const bool all_cols = p.tile * 16 * NC + 16 * NC <= sh.dv;
   f32x4 S[NC][MT];
 #pragma unroll
   for (int n = 0; n < NC; ++n) {
@@ -880,8 +946,6 @@ __global__ void __launch_bounds__(TEAM, 2)
   }
   lds_barrier();
   for (int64_t ch = p.n_chunks - 1; ch >= 0; --ch) {
-    const int64_t at = p.bh * sh.chunks + ch;
-    const int left = (int)std::min<int64_t>(C, p.len - ch * C), left_o = (int)std::min<int64_t>(C, sh.time - ch * C);
     next = next.step(w, -1, p);
 #pragma unroll
     for (int n = 0; n < NC; ++n)
@@ -899,9 +963,6 @@ __global__ void __launch_bounds__(TEAM, 2)
         acc.add(ka[s], sf);
       }
       put_half<3>(x_x + (half * NC + n) * 3 * FRAG, wave & 1, lane, acc.sum() * f_rest + x_p[(wave * NC + n) * 64 + lane]);
-      if (p.col0 + 16 * n < sh.dvp)
-#pragma unroll
-        for (int t = 0; t < MT; ++t) store_rows(w.ds1 + at * DKP * sh.dvp, row0 + 16 * t, p.col0 + 16 * n, sh.dvp, S[n][t]);
     }
     lds_barrier();
     load_k(next);                // behind the barrier: issued while the first LDS reads are on their way
@@ -917,12 +978,7 @@ __global__ void __launch_bounds__(TEAM, 2)
         }
       const f32x4 e = acc.sum(), be = e * f_beta;
       put_half<3>(x_e + (half * NC + n) * 3 * FRAG, wave & 1, lane, -(be * f_eg));
-      if (p.col0 + 16 * n < sh.dvp) store_rows(w.e + at * C * sh.dvp, tok, p.col0 + 16 * n, sh.dvp, e);
-      f32x4 out = be;
-      if (left < C)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) out[r] = tok + r < left ? be[r] : 0.0f;
-      store_tokens(dv + base + ch * C * stride, p, p.col0 + 16 * n, (uint32_t)stride * sizeof(T), all_cols && left_o == C, sh.dv, left_o, out);
+      x_l[(wave * NC + n) * 64 + lane] = e;
     }
     lds_barrier();
     load_t(next);
@@ -1465,7 +1521,7 @@ int32_t run_filter(const Shape& sh, const T* q, const T* k, const T* v, const fl
     constexpr int lds = std::max(2 * NPI * C * (DKP + 8) * 2, 2 * C * LD * 4) + C * LD * 4 + 3 * C * 4;
     GJX_CHECK_HIP(hipFuncSetAttribute((const void*)k_delta_prepare<T, DKP, NPI, KEEP>, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
     k_delta_prepare<T, DKP, NPI, KEEP><<<(unsigned)(sh.batch * sh.heads * sh.chunks), 256, lds, s>>>(
-        sh, q, k, g, beta, lengths, w, aligned_rows(q, sh.qs) && aligned_rows(k, sh.ks));
+        sh, q, k, g, beta, lengths, w, aligned_rows(q, sh.qs) && aligned_rows(k, sh.ks) && sh.dk % 8 == 0);
     GJX_LAUNCH_CHECK();
   }
   constexpr int NC = wide_tiles(DKP, NPI);

@@ -241,6 +241,14 @@ def kalman_filter(observations, initial_mean, initial_cov, A, Q, C, R):
 # gated delta filter: kalman_filter's mean recursion (state_space.py:434-530) for a matrix of regression weights, with
 # the gain beta_t k_t in place of the covariance's -- the memory of a token-sequence model, on the device
 # --------------------------------------------------------------------------- #
+def _wants_gradient(*tensors) -> bool:
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if getattr(t, "requires_grad", False):
+                return True
+    return False
+
+
 class _DeltaFilterFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, log_decay, beta, initial_state, scale, lengths):
@@ -273,10 +281,9 @@ def delta_filter(q, k, v, log_decay, beta, initial_state=None, scale=None, lengt
 
     Returns (o (batch, time, heads, dv) of v's type, S_time (batch, heads, dk, dv) float32); differentiable in q, k, v,
     log_decay, beta and initial_state.  Chunks of 64 tokens run as matrix products; delta_filter_step takes one token."""
-    tensors = (q, k, v, log_decay, beta, initial_state)
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
-        return _DeltaFilterFn.apply(*tensors, scale, lengths)
-    return B.delta_filter(*tensors, scale, lengths)[:2]
+    if _wants_gradient(q, k, v, log_decay, beta, initial_state):
+        return _DeltaFilterFn.apply(q, k, v, log_decay, beta, initial_state, scale, lengths)
+    return B.delta_filter(q, k, v, log_decay, beta, initial_state, scale, lengths)[:2]
 
 
 def delta_filter_step(state, q, k, v, log_decay, beta, scale=None, ancestors=None, out=None):
@@ -287,8 +294,7 @@ def delta_filter_step(state, q, k, v, log_decay, beta, scale=None, ancestors=Non
     the gather costs no pass of its own.  Indices are clamped to [0, n).  out: buffer for the new state -- the state
     itself (in place) when there are no ancestors.  Where a gradient is wanted the call is delta_filter over one
     token."""
-    tensors = (state, q, k, v, log_decay, beta)
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
+    if _wants_gradient(state, q, k, v, log_decay, beta):
         if out is not None:
             raise GjxError("delta_filter_step: `out` cannot be given where a gradient is wanted")
         if ancestors is not None:
