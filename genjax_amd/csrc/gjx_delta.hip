@@ -367,11 +367,19 @@ __global__ void __launch_bounds__(256)
   {
     float x[16];
     const float* n = sn + 16 * wave * LD + 16 * wave;
+    f32x4 bt[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) bt[j] = *(const f32x4*)(s_beta + 16 * wave + 4 * j);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       float v = i == c ? 1.0f : 0.0f;
 #pragma unroll
-      for (int j = 0; j < i; ++j) v -= n[i * LD + j] * s_beta[16 * wave + j] * x[j];
+      for (int j = 0; j < i; j += 4) {         // N is zero on and above the diagonal: whole groups of four
+        const f32x4 row = *(const f32x4*)(n + i * LD + j) * bt[j / 4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (j + e < i) v -= row[e] * x[j + e];
+      }
       x[i] = v;
     }
     if (quad == 0)
