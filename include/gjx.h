@@ -733,23 +733,6 @@ int32_t gjx_outlier_gibbs_hmc_diag(const gjx_outlier_model* model, float step_si
                                    uint32_t* d_chain_keys, float* d_a, float* d_b, float* d_c, float* d_rate,
                                    uint64_t* d_outliers, float* d_diag, int64_t* d_accept_count, void* stream);
 
-/* ---- Game-of-Life inversion by single-site Gibbs sweeps (examples/gol/core.py) ----
- * Boards: n_chains x n x n cells, one byte (0 / 1) per cell, row-major, square (the
- * reference's range mask, core.py:141-149, mixes the axes; all its boards are square).
- * d_future: the observed next state, shared by all chains (future_stride = 0) or per chain
- * (future_stride = n * n).  Keys: n_chains x 2 uint32 on the device, one key per chain. */
-/* proposal.simulate (core.py:240-249): cell c = uniform(key)[c] < 0.5 */
-int32_t gjx_gol_init(const uint32_t* d_keys, int64_t n_chains, int32_t n, uint8_t* d_boards,
-                     void* stream);
-/* gibbs_move_on_all_cells_at_offset (core.py:108-185): cells (oy + 3a, ox + 3b) in place;
- * draw of cell (a, b) = uniform(pass key, (ny', nx'))[a, b] < 1 - softmax(scores)[0] */
-int32_t gjx_gol_gibbs_pass(const uint32_t* d_pass_keys, int64_t n_chains, int32_t n, int32_t oy,
-                           int32_t ox, float p_flip, const uint8_t* d_future, int64_t future_stride,
-                           uint8_t* d_boards, void* stream);
-/* full_gibbs_sweep (core.py:188-204): the nine colour passes; d_pass_keys9 = 9 x n_chains x 2 */
-int32_t gjx_gol_sweep(const uint32_t* d_pass_keys9, int64_t n_chains, int32_t n, float p_flip,
-                      const uint8_t* d_future, int64_t future_stride, uint8_t* d_boards, void* stream);
-
 /* ---- gated delta filter: the mean recursion of the Kalman filter (extras/state_space.py:434-530) for a dk x dv
  * matrix of regression weights S observed along k_t with the gain beta_t k_t,
  *   S_t = a_t S_{t-1} + k_t u_t^T,  u_t = beta_t (v_t - a_t S_{t-1}^T k_t),  o_t = scale S_t^T q_t,  a_t = exp(g_t),
@@ -785,6 +768,23 @@ int32_t gjx_delta_filter_grad(const gjx_delta_shape* shape, const void* d_q, con
 int32_t gjx_delta_filter_step(const gjx_delta_shape* shape, const float* d_state, const int32_t* d_ancestors,
                               const void* d_q, const void* d_k, const void* d_v, const float* d_g, const float* d_beta,
                               void* d_o, float* d_state_out, void* stream);
+
+/* ---- Game-of-Life inversion by single-site Gibbs sweeps (examples/gol/core.py) ----
+ * Boards: n_chains x n x n cells, one byte (0 / 1) per cell, row-major, square (the
+ * reference's range mask, core.py:141-149, mixes the axes; all its boards are square).
+ * d_future: the observed next state, shared by all chains (future_stride = 0) or per chain
+ * (future_stride = n * n).  Keys: n_chains x 2 uint32 on the device, one key per chain. */
+/* proposal.simulate (core.py:240-249): cell c = uniform(key)[c] < 0.5 */
+int32_t gjx_gol_init(const uint32_t* d_keys, int64_t n_chains, int32_t n, uint8_t* d_boards,
+                     void* stream);
+/* gibbs_move_on_all_cells_at_offset (core.py:108-185): cells (oy + 3a, ox + 3b) in place;
+ * draw of cell (a, b) = uniform(pass key, (ny', nx'))[a, b] < 1 - softmax(scores)[0] */
+int32_t gjx_gol_gibbs_pass(const uint32_t* d_pass_keys, int64_t n_chains, int32_t n, int32_t oy,
+                           int32_t ox, float p_flip, const uint8_t* d_future, int64_t future_stride,
+                           uint8_t* d_boards, void* stream);
+/* full_gibbs_sweep (core.py:188-204): the nine colour passes; d_pass_keys9 = 9 x n_chains x 2 */
+int32_t gjx_gol_sweep(const uint32_t* d_pass_keys9, int64_t n_chains, int32_t n, float p_flip,
+                      const uint8_t* d_future, int64_t future_stride, uint8_t* d_boards, void* stream);
 
 /* The same passes on BIT-PACKED boards (one bit per cell, row pitch gjx_gol_words_per_row(n) = ceil(n / 64)
  * 64-bit words, bit c of word w of a row = column 64 w + c, bits beyond n zero; chains contiguous).  Same
