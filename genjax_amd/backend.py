@@ -9,6 +9,7 @@ import collections
 import ctypes as C
 import functools
 import math
+import numbers
 from typing import Sequence
 
 import numpy as np
@@ -457,6 +458,19 @@ def _address(t):
     return 0 if t is None else t.data_ptr()
 
 
+def _note_leaves(who, out):
+    """Refuse, while a graph is being captured, a differentiable call whose leaves an eager autograd graph still holds: a
+    leaf's node keeps the stream it was made on, and a captured backward that reaches such a node waits across the capture
+    border, which ends the process.  (Leaves seen by this call are noted on their nodes, which live as long as the graph.)"""
+    stream = _raw_stream()
+    for node, _ in out.grad_fn.next_functions:
+        if node is not None and hasattr(node, "variable"):
+            first = node.metadata.setdefault("gjx_stream", stream)
+            if first != stream and torch.cuda.is_current_stream_capturing():
+                raise GjxError(f"{who}: a leaf of this captured call belongs to an autograd graph that was built on another "
+                               "stream and still lives: drop that graph (its outputs) first, or capture with fresh leaves")
+
+
 def _unit_stride(t):
     """`t` itself when its last axis is contiguous and its rows neither overlap nor lie too far apart, else a copy."""
     width, (step, unit) = t.shape[1], t.stride()
@@ -626,9 +640,12 @@ def _delta_inputs(who, q, k, v, log_decay, beta, scale):
     for name, t in zip(names, (q, k, v, log_decay, beta)):
         if not isinstance(t, torch.Tensor):
             raise GjxError(f"{who}: `{name}` must be a tensor")
+    if scale is not None and not isinstance(scale, numbers.Real):
+        raise GjxError(f"{who}: `scale` must be a number")
     fits = lambda t: t.dim() != 4 or ((t.stride(3) == 1 or t.shape[3] <= 1) and t.stride(1) <= 1 << 22)      # noqa: E731
     t = (q if fits(q) else q.contiguous(), k if fits(k) else k.contiguous(), v if fits(v) else v.contiguous(), log_decay, beta)
-    plan = _delta_plan(who, tuple(a.dtype for a in t), *(a.shape for a in t), *(a.stride() for a in t), scale)
+    plan = _delta_plan(who, tuple(a.dtype for a in t), *(a.shape for a in t), *(a.stride() for a in t),
+                       None if scale is None else float(scale))
     _on_current_device(who, *zip(names, t))
     return plan, t
 
@@ -686,8 +703,11 @@ def delta_filter_grad(q, k, v, log_decay, beta, d_o, d_state, kept, scale=None, 
 
 
 def _overlap(a, b):
-    lo_a, lo_b = a.data_ptr(), b.data_ptr()
-    return lo_a < lo_b + b.numel() * b.element_size() and lo_b < lo_a + a.numel() * a.element_size()
+    """Whether the address ranges of two tensors meet (strided ones count from their first entry to their last)."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    end = lambda t: t.data_ptr() + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()     # noqa: E731
+    return a.data_ptr() < end(b) and b.data_ptr() < end(a)
 
 
 @functools.lru_cache(maxsize=1024)
@@ -707,15 +727,20 @@ def delta_filter_step(state, q, k, v, log_decay, beta, scale=None, ancestors=Non
     for name, t in (("q", q), ("k", k), ("v", v), ("log_decay", log_decay), ("beta", beta)):
         if not isinstance(t, torch.Tensor):
             raise GjxError(f"{who}: `{name}` must be a tensor")
+    if scale is not None and not isinstance(scale, numbers.Real):
+        raise GjxError(f"{who}: `scale` must be a number")
     unit = lambda t: t if t.dim() == 0 or t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()       # noqa: E731
     q, k, v = unit(q), unit(k), unit(v)
     p = _delta_step_plan((q.dtype, k.dtype, v.dtype, log_decay.dtype, beta.dtype), q.shape, k.shape, v.shape, log_decay.shape,
-                         beta.shape, q.stride(), k.stride(), v.stride(), log_decay.stride(), beta.stride(), scale)
+                         beta.shape, q.stride(), k.stride(), v.stride(), log_decay.stride(), beta.stride(),
+                         None if scale is None else float(scale))
     if state is None:
         raise GjxError(f"{who}: `state` must be float32 of shape {(p.batch, p.heads, p.dk, p.dv)}")
     state, ancestors = _delta_state(who, "state", state, p), _delta_indices(who, "ancestors", ancestors, p)
     _on_current_device(who, ("q", q), ("k", k), ("v", v), ("log_decay", log_decay), ("beta", beta))
     if out is None:
+        if state.data_ptr() & 15:                               # a view into the middle of a buffer
+            state = state.clone()
         out = torch.empty_like(state)
     else:
         if not isinstance(out, torch.Tensor) or out.shape != state.shape or out.dtype != torch.float32 or not out.is_contiguous():
@@ -723,9 +748,12 @@ def delta_filter_step(state, q, k, v, log_decay, beta, scale=None, ancestors=Non
         _on_current_device(who, ("out", out))
         if _overlap(out, state) and (ancestors is not None or out.data_ptr() != state.data_ptr()):
             raise GjxError(f"{who}: `out` may be the state itself without ancestors and must not overlap it otherwise")
+        for name, t in (("q", q), ("k", k), ("v", v), ("log_decay", log_decay), ("beta", beta), ("ancestors", ancestors)):
+            if t is not None and _overlap(out, t):
+                raise GjxError(f"{who}: `out` must not overlap `{name}`")
     from_, to = state.data_ptr(), out.data_ptr()
     if (from_ | to) & 15:
-        raise GjxError(f"{who}: states must be aligned to 16 bytes")
+        raise GjxError(f"{who}: `state` and `out` must be aligned to 16 bytes")
     o = torch.empty((p.batch, p.heads, p.dv), dtype=v.dtype, device=v.device)
     N.check(N.lib().gjx_delta_filter_step(p.ref, from_, _address(ancestors), q.data_ptr(), k.data_ptr(), v.data_ptr(),
                                           log_decay.data_ptr(), beta.data_ptr(), o.data_ptr(), to, _raw_stream()),

@@ -171,6 +171,7 @@ class _LinearCategorical(Distribution):
             ys = ys.reshape(-1).expand(n)
         if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
             out = _LinearCategoricalFn.apply(ys, rows, weight, bias)
+            B._note_leaves("linear_categorical", out)
         else:
             out = B.linear_categorical_logpdf(ys, rows, weight, bias, want_lse=False)[0]
         return out.reshape(()) if scalar else out

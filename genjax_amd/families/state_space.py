@@ -282,7 +282,9 @@ def delta_filter(q, k, v, log_decay, beta, initial_state=None, scale=None, lengt
     Returns (o (batch, time, heads, dv) of v's type, S_time (batch, heads, dk, dv) float32); differentiable in q, k, v,
     log_decay, beta and initial_state.  Chunks of 64 tokens run as matrix products; delta_filter_step takes one token."""
     if _wants_gradient(q, k, v, log_decay, beta, initial_state):
-        return _DeltaFilterFn.apply(q, k, v, log_decay, beta, initial_state, scale, lengths)
+        out = _DeltaFilterFn.apply(q, k, v, log_decay, beta, initial_state, scale, lengths)
+        B._note_leaves("delta_filter", out[0])
+        return out
     return B.delta_filter(q, k, v, log_decay, beta, initial_state, scale, lengths)[:2]
 
 
@@ -297,8 +299,15 @@ def delta_filter_step(state, q, k, v, log_decay, beta, scale=None, ancestors=Non
     if _wants_gradient(state, q, k, v, log_decay, beta):
         if out is not None:
             raise GjxError("delta_filter_step: `out` cannot be given where a gradient is wanted")
+        for name, t in (("state", state), ("q", q), ("k", k), ("v", v), ("log_decay", log_decay), ("beta", beta)):
+            if not isinstance(t, torch.Tensor) or t.dim() < 1:
+                raise GjxError(f"delta_filter_step: `{name}` must be a tensor with a particle axis")
         if ancestors is not None:
-            state = state.index_select(0, ancestors.long().clamp(0, state.shape[0] - 1))
+            n = state.shape[0]
+            if not isinstance(ancestors, torch.Tensor) or ancestors.dtype != torch.int32 or ancestors.shape != (n,):
+                raise GjxError(f"delta_filter_step: `ancestors` must be int32 of shape ({n},)")
+            if n > 0:
+                state = state.index_select(0, ancestors.long().clamp(0, n - 1))
         o, new = delta_filter(*(t.unsqueeze(1) for t in (q, k, v, log_decay, beta)), initial_state=state, scale=scale)
         return o.squeeze(1), new
     return B.delta_filter_step(state, q, k, v, log_decay, beta, scale, ancestors, out)

@@ -55,3 +55,158 @@ def test_linear_categorical_abi_refusals():
     assert L.gjx_linear_categorical_grad(0, p, p, 8, p, 8, None, 3, 5, 8, p, p, p, p, p, p, 16, None) == -1
     key = (C.c_uint32 * 2)(0, 1)
     assert L.gjx_random_linear_categorical_i32(key, 0, 0, p, 8, p, 8, None, 3, 5, 8, None, p, 1 << 30, None) == -1
+
+
+def _delta_args(batch=2, time=3, kheads=1, heads=2, dk=8, dv=4, dtype=torch.float32):
+    return [torch.zeros(batch, time, kheads, dk, dtype=dtype), torch.zeros(batch, time, kheads, dk, dtype=dtype),
+            torch.zeros(batch, time, heads, dv, dtype=dtype), torch.zeros(batch, time, heads), torch.zeros(batch, time, heads)]
+
+
+DELTA_BAD = [
+    (0, lambda t: t[..., 0], "must be"),                                    # q without its last axis
+    (1, lambda t: t[:, :2], "must be"),                                     # k shorter than q
+    (2, lambda t: t[:1], "must be"),                                        # v of another batch
+    (2, lambda t: torch.zeros(2, 3, 0, 4), "multiple"),
+    (0, lambda t: None, "`q` must be a tensor"),
+    (3, lambda t: t[..., :1], "log_decay"),
+    (4, lambda t: t[:, :2], "beta"),
+    (0, lambda t: t.double(), "float32 or all bfloat16"),
+    (1, lambda t: t.bfloat16(), "float32 or all bfloat16"),
+    (2, lambda t: t.half(), "float32 or all bfloat16"),
+    (3, lambda t: t.bfloat16(), "must be float32"),
+    (4, lambda t: t.double(), "must be float32"),
+    (0, lambda t: t, "device tensor"),                                      # good shapes, but host tensors
+]
+
+
+@pytest.mark.parametrize("which,change,message", DELTA_BAD)
+def test_delta_filter_front_end_refusals(which, change, message):
+    from genjax_amd.families import state_space as S
+
+    B = _B()
+    args = _delta_args()
+    args[which] = change(args[which])
+    with pytest.raises(B.GjxError, match=message):
+        S.delta_filter(*args)
+    if args[which] is not None and args[which].dim() >= 3:                  # the single-token form, and the same with a gradient
+        step = [t[:, 0] for t in args]
+        state = torch.zeros(2, 2, 8, 4)
+        if message == "beta" or (message == "must be" and which < 2):       # (good single tokens, or a q without its axes)
+            return
+        with pytest.raises(B.GjxError, match=message):
+            S.delta_filter_step(state, *step)
+        with pytest.raises(B.GjxError, match=message):
+            S.delta_filter_step(state.requires_grad_(True), *step)
+
+
+def test_delta_filter_sizes_heads_and_options():
+    from genjax_amd.families import state_space as S
+
+    B = _B()
+    for sizes, message in (({"dk": 129}, "dk = 129"), ({"dv": 1025}, "dv = 1025"), ({"dk": 0}, "dk = 0"), ({"dv": 0}, "dv = 0"),
+                           ({"kheads": 2, "heads": 3}, "multiple"), ({"kheads": 2, "heads": 1}, "multiple")):
+        with pytest.raises(B.GjxError, match=message):
+            S.delta_filter(*_delta_args(**sizes))
+    for scale in (torch.tensor(0.5), "0.5", 1j):                             # a tensor would be read at an unknown time
+        with pytest.raises(B.GjxError, match="`scale` must be a number"):
+            S.delta_filter(*_delta_args(), scale=scale)
+        with pytest.raises(B.GjxError, match="`scale` must be a number"):
+            S.delta_filter_step(torch.zeros(2, 2, 8, 4), *(t[:, 0] for t in _delta_args()), scale=scale)
+
+
+def test_delta_filter_step_refusals():
+    from genjax_amd.families import state_space as S
+
+    B = _B()
+    args = [t[:, 0] for t in _delta_args()]
+    state = torch.zeros(2, 2, 8, 4)
+    four = [t.unsqueeze(1) for t in args]
+    with pytest.raises(B.GjxError, match="axes"):
+        S.delta_filter_step(state, *four)
+    with pytest.raises(B.GjxError, match="`state` must be"):
+        S.delta_filter_step(None, *args)
+    for bad in (state[:1], state.double(), state[..., :3], [0.0]):
+        with pytest.raises(B.GjxError, match="`state` must be"):
+            S.delta_filter_step(bad, *args)
+    grad = state.clone().requires_grad_(True)
+    with pytest.raises(B.GjxError, match="`out` cannot be given"):
+        S.delta_filter_step(grad, *args, out=state)
+    with pytest.raises(B.GjxError, match="`state` must be a tensor"):
+        S.delta_filter_step(None, args[0].requires_grad_(True), *args[1:])
+    args[0].requires_grad_(False)
+    for ancestors in (torch.zeros(2, dtype=torch.int64), torch.zeros(3, dtype=torch.int32), [0, 1]):
+        with pytest.raises(B.GjxError, match="`ancestors` must be int32"):
+            S.delta_filter_step(grad, *args, ancestors=ancestors)
+
+
+def test_overlap_of_strided_tensors():
+    B = _B()
+    base = torch.zeros(64)
+    assert B._overlap(base[:8], base[7:9]) and not B._overlap(base[:8], base[8:9])
+    assert B._overlap(base[0:20:10], base[10:12]) and not B._overlap(base[0:20:10], base[11:12])
+    assert not B._overlap(base[:0], base) and B._overlap(base[3].expand(5), base[:4])
+
+
+def _shape(dtype=0, kheads=1, heads=2, dk=8, dv=4, batch=2, time=3, v_token=8):
+    from genjax_amd import _native as N
+
+    three = C.c_int64 * 3
+    kv, gate = three(time * kheads * dk, kheads * dk, dk), three(time * heads, heads, 1)
+    return N.DeltaShape(dtype, kheads, heads, dk, dv, 0.5, batch, time, kv, kv, three(time * heads * dv, v_token, dv), gate, gate)
+
+
+def test_delta_filter_abi_refusals():
+    from genjax_amd import _native as N
+
+    L = N.lib()
+    p = C.c_void_p(1 << 20)                      # never dereferenced: each call is refused on the host
+    size = C.c_int64()
+
+    def sizes(shape, keep=0, out=C.byref(size)):
+        return L.gjx_delta_filter_workspace(None if shape is None else C.byref(shape), keep, out)
+
+    need = []
+    for keep in (0, 1, 2):
+        assert sizes(_shape(), keep) == 0 and size.value > 0 and size.value % 256 == 0
+        need.append(size.value)
+    assert sizes(_shape(), 3) == -1 and sizes(_shape(), -1) == -1 and sizes(_shape(), 0, None) == -1 and sizes(None) == -1
+    for bad in (dict(dtype=2), dict(dtype=-1), dict(kheads=0), dict(heads=0), dict(kheads=2, heads=3), dict(batch=-1), dict(time=-1)):
+        assert sizes(_shape(**bad)) == -1, bad
+    for bad in (dict(dk=0), dict(dk=129), dict(dv=0), dict(dv=1025), dict(batch=(1 << 24) + 1), dict(heads=1025), dict(time=(1 << 30) + 1),
+                dict(v_token=(1 << 22) + 1), dict(batch=1 << 20, time=1 << 24)):
+        assert sizes(_shape(**bad)) == -4, bad
+
+    def run(shape=None, q=p, g=p, o=p, state=p, keep=0, work=p, work_bytes=1 << 40):
+        return L.gjx_delta_filter(C.byref(shape or _shape()), q, p, p, g, p, None, None, o, state, keep, work, work_bytes, None)
+
+    assert run(q=None) == -1 and run(g=None) == -1 and run(o=None) == -1 and run(state=None) == -1
+    assert run(work=None) == -1 and run(work_bytes=need[0] - 1) == -1 and run(keep=1, work_bytes=need[1] - 1) == -1
+    assert run(work=C.c_void_p((1 << 20) + 128)) == -1 and b"workspace" in L.gjx_last_error()
+    assert run(shape=_shape(batch=0), q=None, g=None, o=None, state=None, work=None, work_bytes=0) == 0       # nothing to do
+
+    def grad(do=p, dq=p, kept=p, kept_bytes=1 << 40, work=p, work_bytes=1 << 40):
+        return L.gjx_delta_filter_grad(C.byref(_shape()), p, p, p, p, p, None, do, None, dq, p, p, p, p, None, kept, kept_bytes, work,
+                                       work_bytes, None)
+
+    assert grad(do=None) == -1 and grad(dq=None) == -1 and grad(kept=None) == -1 and grad(work=None) == -1
+    assert grad(kept_bytes=need[1] - 1) == -1 and b"kept" in L.gjx_last_error()
+    assert grad(work_bytes=need[2] - 1) == -1 and grad(work=C.c_void_p((1 << 20) + 16)) == -1
+
+    def step(shape, state=p, ancestors=None, o=p, out=C.c_void_p(1 << 21)):
+        return L.gjx_delta_filter_step(C.byref(shape), state, ancestors, p, p, p, p, p, o, out, None)
+
+    assert step(_shape()) == -1 and b"time must be 1" in L.gjx_last_error()
+    one = _shape(time=1)
+    assert step(one, state=None) == -1 and step(one, o=None) == -1 and step(one, out=None) == -1
+    assert step(one, ancestors=p, out=p) == -1 and b"ancestors" in L.gjx_last_error()
+    assert step(one, state=C.c_void_p((1 << 20) + 4)) == -1 and step(one, out=C.c_void_p((1 << 21) + 8)) == -1
+    assert step(_shape(time=1, batch=0), state=None, o=None, out=None) == 0
+
+
+def test_linear_categorical_far_rows():
+    from genjax_amd import _native as N
+
+    L, p, size = N.lib(), C.c_void_p(1 << 20), C.c_int64()
+    assert L.gjx_linear_categorical_workspace(0, p, (1 << 22) + 1, p, 8, 3, 5, 8, 0, C.byref(size)) == -4
+    assert L.gjx_linear_categorical_workspace(0, p, 8, p, (1 << 22) + 1, 3, 5, 8, 0, C.byref(size)) == -4
+    assert L.gjx_linear_categorical_workspace(0, p, 8, p, 8, 3, 5, 8, 3, C.byref(size)) == -1
