@@ -188,8 +188,10 @@ _SIGNATURES = {
     "gjx_beta_logpdf_f32": ([_vp, _vp, _i32, _vp, _i32, _i64, _vp, _vp], _i32),
     "gjx_categorical_logpdf_f32": ([_vp, _vp, _i32, _i64, _i32, _vp, _vp], _i32),
     "gjx_linear_categorical_workspace": ([_i32, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i32, C.POINTER(_i64)], _i32),
-    "gjx_linear_categorical_logpdf": ([_i32, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _vp], _i32),
-    "gjx_linear_categorical_grad": ([_i32, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64] + [_vp] * 6 + [_i64, _vp], _i32),
+    "gjx_linear_categorical_logpdf": ([_i32, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _vp],
+                                      _i32),
+    "gjx_linear_categorical_grad": ([_i32, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64] + [_vp] * 3 + [_i64] + [_vp] * 4 +
+                                    [_i64, _vp], _i32),
     "gjx_random_linear_categorical_i32": ([_u32p, _u64, _i32, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _vp],
                                           _i32),
     "gjx_mvnormal_logpdf_f32": ([_vp, _vp, _i32, _vp, _i32, _i64, _i32, _vp, _vp], _i32),

@@ -478,12 +478,12 @@ def _unit_stride(t):
 
 
 @functools.lru_cache(maxsize=1024)
-def _linear_workspace_bytes(dtype, x_low, x_ld, w_low, w_ld, n, vocab, width, grad):
+def _linear_workspace_bytes(dtype, x_low, x_ld, w_low, w_ld, n, vocab, width, kind):
     """Workspace of a call: depends on the sizes, the row strides and the pointers' alignment (their low bits)."""
     size = C.c_int64()
-    N.check(N.lib().gjx_linear_categorical_workspace(dtype, 16 + x_low, x_ld, 16 + w_low, w_ld, n, vocab, width, grad, C.byref(size)),
+    N.check(N.lib().gjx_linear_categorical_workspace(dtype, 16 + x_low, x_ld, 16 + w_low, w_ld, n, vocab, width, kind, C.byref(size)),
             "gjx_linear_categorical_workspace")
-    return max(size.value, 256)
+    return max(size.value, 256) if kind < 3 else size.value
 
 
 class _Linear:
@@ -510,10 +510,11 @@ class _Linear:
         self.head = (dtype, self.x.data_ptr(), max(self.x.stride(0), self.width), self.weight.data_ptr(),
                      max(self.weight.stride(0), self.width))
 
-    def workspace(self, grad):
+    def workspace(self, kind):
+        """kind: 0 log-density or draw, 1 gradient, 2 gradient without x's, 3 what the first leaves for the second (or None)."""
         dtype, xp, x_ld, wp, w_ld = self.head
-        size = _linear_workspace_bytes(dtype, xp & 15, x_ld, wp & 15, w_ld, self.n, self.vocab, self.width, grad)
-        return torch.empty(size, dtype=torch.uint8, device=self.x.device)
+        size = _linear_workspace_bytes(dtype, xp & 15, x_ld, wp & 15, w_ld, self.n, self.vocab, self.width, kind)
+        return torch.empty(size, dtype=torch.uint8, device=self.x.device) if size else None
 
 
 def _linear_values(y, n):
@@ -523,22 +524,26 @@ def _linear_values(y, n):
     return y.contiguous()
 
 
-def linear_categorical_logpdf(y, x, weight, bias=None, want_lse=True):
-    """y: (n,) int32; x: (n, width), weight: (vocab, width), bias: (vocab,) or None -> (log p(y) (n,), logsumexp (n,))."""
+def linear_categorical_logpdf(y, x, weight, bias=None, want_lse=True, keep=False):
+    """y: (n,) int32; x: (n, width), weight: (vocab, width), bias: (vocab,) or None -> (log p(y) (n,), logsumexp (n,)); with
+    keep also what linear_categorical_grad takes as `kept` (None where it forms the logits again)."""
     a = _Linear(x, weight, bias)
     y = _linear_values(y, a.n)
     lp = torch.empty(a.n, dtype=torch.float32, device=a.x.device)
     lse = torch.empty_like(lp) if want_lse else None
+    kept = None
     if a.n > 0:
         dtype, xp, x_ld, wp, w_ld = a.head
+        kept = a.workspace(3) if keep else None
         work = a.workspace(0)
         N.check(N.lib().gjx_linear_categorical_logpdf(dtype, y.data_ptr(), xp, x_ld, wp, w_ld, _address(a.bias), a.n, a.vocab,
-                                                      a.width, lp.data_ptr(), _address(lse), work.data_ptr(), work.numel(),
+                                                      a.width, lp.data_ptr(), _address(lse), _address(kept),
+                                                      0 if kept is None else kept.numel(), work.data_ptr(), work.numel(),
                                                       _raw_stream()), "gjx_linear_categorical_logpdf")
-    return lp, lse
+    return (lp, lse, kept) if keep else (lp, lse)
 
 
-def linear_categorical_grad(y, x, weight, bias, lse, upstream, want=(True, True, True)):
+def linear_categorical_grad(y, x, weight, bias, lse, upstream, want=(True, True, True), kept=None):
     """upstream x d log p / d(x, weight, bias), summed over the rows for weight and bias (entries not wanted: None)."""
     a = _Linear(x, weight, bias)
     y = _linear_values(y, a.n)
@@ -551,7 +556,8 @@ def linear_categorical_grad(y, x, weight, bias, lse, upstream, want=(True, True,
         dtype, xp, x_ld, wp, w_ld = a.head
         work = a.workspace(1 if outs[0] is not None else 2)
         N.check(N.lib().gjx_linear_categorical_grad(dtype, y.data_ptr(), xp, x_ld, wp, w_ld, _address(a.bias), a.n, a.vocab, a.width,
-                                                    lse.data_ptr(), upstream.data_ptr(), *map(_address, outs), work.data_ptr(),
+                                                    lse.data_ptr(), upstream.data_ptr(), _address(kept),
+                                                    0 if kept is None else kept.numel(), *map(_address, outs), work.data_ptr(),
                                                     work.numel(), _raw_stream()), "gjx_linear_categorical_grad")
     return outs
 

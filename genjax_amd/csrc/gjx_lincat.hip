@@ -18,6 +18,8 @@ typedef __bf16 bf16;
 typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 #define LDS_AS __attribute__((address_space(3)))
 #define GLB_AS __attribute__((address_space(1)))
@@ -27,7 +29,7 @@ namespace {
 constexpr int BM = 256, BK = 64, GEMM_THREADS = 512;         // bf16 tiles: BM entries of m, 64 deep, eight waves
 constexpr int BM32 = 128, GEMM32_THREADS = 256;              // f32 tiles: 32 deep, four waves
 
-enum { EPI_SCORE = 0, EPI_DL = 1, EPI_STORE = 2, EPI_DRAW = 3 };
+enum { EPI_SCORE = 0, EPI_DL = 1, EPI_STORE = 2, EPI_DRAW = 3, EPI_KEEP = 4 };   // KEEP: SCORE that leaves what dl is formed from
 
 // one operand of a product: `rows` memory rows of `ld` elements.  Not transposed: a row is one output index with the
 // reduction along it; transposed: a row is one reduction index with the output index along it (`cols` of them, a
@@ -57,6 +59,9 @@ struct GemmArgs {
   const int32_t* y;
   float2* part;        // [tile m][n_pad]: (max, sum exp) of a row over one tile; drawing: (largest l + Gumbel, its entry)
   float* target;       // logit of y
+  void* keep;          // EPI_KEEP: [n][keep_ld] exp(l - base), f32 or f16 x 2^15, base the row's largest l of a wave's block of entries
+  float* keep_base;    // [v / block][n_pad]
+  int64_t keep_ld;
   int64_t n_pad;
   int part_tile0;
   uint32_t key0, key1;
@@ -72,6 +77,10 @@ struct GemmArgs {
   int64_t out_ld, out_split;
   int out_m, out_n, out_bf16, accumulate;
 };
+
+// what a bf16 call keeps is f16 with 2^15 before it: 11 bits for entries down to 2^-29 of their block's largest, 2^-40 of that
+// below (the bf16 rounding of dl that follows is 2^-8)
+constexpr float KEEP_SCALE = 32768.0f;
 
 __device__ __forceinline__ float load_any(const void* p, int f32, int64_t i) {
   return f32 ? ((const float*)p)[i] : (float)((const bf16*)p)[i];
@@ -310,7 +319,7 @@ __device__ __forceinline__ void epilogue(const GemmArgs& g, const Tile& tile, f3
 #pragma unroll
     for (int r = 0; r < 4; ++r) bias[i][r] = s_bias[wm + i * 16 + 4 * q + r];
 
-  if (EPI == EPI_SCORE) {
+  if (EPI == EPI_SCORE || EPI == EPI_KEEP) {
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       const int64_t n = n0 + wn + j * 16 + c;
@@ -331,15 +340,34 @@ __device__ __forceinline__ void epilogue(const GemmArgs& g, const Tile& tile, f3
           for (int r = 0; r < 4; ++r)
             if (y == i * 16 + r) g.target[n] = acc[i][j][r];
       }
+      top = fmaxf(top, __shfl_xor(top, 16));              // one base for the wave's whole block of entries
+      top = fmaxf(top, __shfl_xor(top, 32));
       const float base = top == -__builtin_inff() ? 0.0f : top;
       float sum = 0.0f;
 #pragma unroll
       for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) sum += exp_of(acc[i][j][r] - base);
+        for (int r = 0; r < 4; ++r) {
+          const float e = exp_of(acc[i][j][r] - base);
+          sum += e;
+          if (EPI == EPI_KEEP) acc[i][j][r] = e;
+        }
+      sum += __shfl_xor(sum, 16);
+      sum += __shfl_xor(sum, 32);
+      if (EPI == EPI_KEEP && n < g.n) {
+        const int64_t v = g.v0 + m0 + wm;
+        if (q == 0) g.keep_base[v / (MT * 16) * g.n_pad + n] = base;
 #pragma unroll
-      for (int o = 16; o <= 32; o <<= 1) {
-        merge_lse(top, sum, __shfl_xor(top, o), __shfl_xor(sum, o));
+        for (int i = 0; i < MT; ++i) {
+          if (sizeof(T) == 2) {
+            f16x4 h;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) h[r] = (_Float16)(acc[i][j][r] * KEEP_SCALE);
+            *(f16x4*)((_Float16*)g.keep + n * g.keep_ld + v + i * 16 + 4 * q) = h;
+          } else {
+            *(f32x4*)((float*)g.keep + n * g.keep_ld + v + i * 16 + 4 * q) = acc[i][j];
+          }
+        }
       }
       if (q == 0) {
         s_red[((wave / WN) * BN + wn + j * 16 + c) * 2] = top;
@@ -834,7 +862,7 @@ __global__ void __launch_bounds__(GJX_BLOCK)
 // (max, sum exp) of the tiles of a row -> lse, and log p(y) = l_y - lse.  `width` rows by 256 / width parts per block.
 __global__ void __launch_bounds__(GJX_BLOCK)
     k_lincat_combine(const float2* __restrict__ part, int tiles, int64_t n_pad, int64_t n, int width,
-                     const float* __restrict__ target, float* __restrict__ lp, float* __restrict__ lse) {
+                     const float* __restrict__ target, float* __restrict__ lp, float* __restrict__ lse, float* __restrict__ lp_kept) {
   __shared__ float2 sm[GJX_BLOCK];
   const int col = threadIdx.x % width, grp = threadIdx.x / width, groups = GJX_BLOCK / width;
   const int64_t i = (int64_t)blockIdx.x * width + col;
@@ -854,7 +882,9 @@ __global__ void __launch_bounds__(GJX_BLOCK)
   if (grp == 0 && i < n) {
     const float l = top + logf(sum);
     if (lse) lse[i] = l;
-    lp[i] = target[i] - l;
+    const float p = target[i] - l;
+    lp[i] = p;
+    if (lp_kept) lp_kept[i] = p;
   }
 }
 
@@ -885,20 +915,109 @@ __global__ void __launch_bounds__(GJX_BLOCK)
   if (lane == 0) out[i] = arg;
 }
 
+// dl of a piece of the vocabulary from what the forward kept: dl = g (onehot - exp(base - lse) e), and its sums over strips
+// of rows for db.  A thread takes eight entries of a strip's rows.  Bound by memory: one read, one write.
+
+template <typename T>
+__global__ void __launch_bounds__(GJX_BLOCK)
+    k_lincat_dl(const void* __restrict__ keep, int64_t keep_ld, const float* __restrict__ base, int block, int64_t n_pad,
+                const float* __restrict__ lp, const float* __restrict__ lse, const float* __restrict__ up,
+                const int32_t* __restrict__ y, int64_t n, int64_t vocab, int64_t v0, int cols, int strip, T* __restrict__ dl,
+                int64_t dl_ld, float* __restrict__ resid, float* __restrict__ db_part, int64_t db_ld) {
+  const int col = (blockIdx.y * GJX_BLOCK + threadIdx.x) * 8;
+  if (col >= cols) return;
+  const int64_t i0 = (int64_t)blockIdx.x * strip;
+  const int rows = (int)max(min((int64_t)strip, n - i0), (int64_t)0);
+  const float* b = base + (v0 + col) / block * n_pad + i0;
+  T* out = dl + i0 * dl_ld + col;
+  float db[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll 4
+  for (int i = 0; i < rows; ++i) {
+    const int64_t row = i0 + i;
+    float x[8];
+    if constexpr (sizeof(T) == 2) {
+      const f16x8 h = *(const f16x8*)((const _Float16*)keep + row * keep_ld + v0 + col);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = (float)h[j];
+    } else {
+      const float* p = (const float*)keep + row * keep_ld + v0 + col;
+      const f32x4 lo = *(const f32x4*)p, hi = *(const f32x4*)(p + 4);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        x[j] = lo[j];
+        x[4 + j] = hi[j];
+      }
+    }
+    const float g = up[row], f = -g * exp_of(b[i] - lse[row]) * (sizeof(T) == 2 ? 1.0f / KEEP_SCALE : 1.0f);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] *= f;
+    const int64_t at = min(max((int64_t)y[row], (int64_t)0), vocab - 1) - v0 - col;
+    const bool here = at >= 0 && at < 8;
+    const float own = g - g * exp_of(lp[row]);            // the value's own entry, from its log-density
+    if (here)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = j == (int)at ? own : x[j];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) db[j] += x[j];
+    if constexpr (sizeof(T) == 2) {
+      bf16x8 h;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) h[j] = (bf16)x[j];
+      *(bf16x8*)(out + i * dl_ld) = h;
+      if (here) resid[row] = own - (float)(bf16)own;      // (see EPI_DL)
+    } else {
+      *(f32x4*)(out + i * dl_ld) = f32x4{x[0], x[1], x[2], x[3]};
+      *(f32x4*)(out + i * dl_ld + 4) = f32x4{x[4], x[5], x[6], x[7]};
+    }
+  }
+  for (int i = rows; i < strip; ++i) {         // the rows behind the last that the products' tiles reach
+#pragma unroll
+    for (int j = 0; j < 8; ++j) out[i * dl_ld + j] = (T)0.0f;
+  }
+  if (db_part) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) db_part[(int64_t)blockIdx.x * db_ld + col + j] = db[j];
+  }
+}
+
 // out[i][k] = sum over parts of part[s][i][k] in f32, stored in the output's type; rows of `width`, parts of `ld` columns.
 // With resid: + resid[i] w[y_i][k] (bf16 weights)
+struct Fold {
+  const float* part;
+  int parts;
+  int64_t part_stride, rows, ld, width;
+  void* out;
+  int out_bf16;
+  const float* resid;
+  const int32_t* y;
+  const bf16* w;
+  int64_t w_ld, vocab;
+};
+
+// one or two such sums (those of dx and of db) in one launch
 __global__ void __launch_bounds__(GJX_BLOCK)
-    k_lincat_fold(const float* __restrict__ part, int parts, int64_t part_stride, int64_t rows, int64_t ld, int64_t width,
-                  void* __restrict__ out, int out_bf16, const float* __restrict__ resid, const int32_t* __restrict__ y,
-                  const bf16* __restrict__ w, int64_t w_ld, int64_t vocab) {
-  const int64_t total = rows * width;
-  for (int64_t i = (int64_t)blockIdx.x * GJX_BLOCK + threadIdx.x; i < total; i += (int64_t)gridDim.x * GJX_BLOCK) {
-    const int64_t r = i / width, k = i - r * width;
+    k_lincat_fold(Fold one, Fold two) {
+  const int64_t total = one.rows * one.width, all = total + two.rows * two.width;
+  auto entry = [](const Fold& f, int64_t i) {
+    const int64_t r = i / f.width, k = i - r * f.width;
     float s = 0.0f;
-    for (int p = 0; p < parts; ++p) s += part[p * part_stride + r * ld + k];
-    if (resid) s += resid[r] * (float)w[min(max((int64_t)y[r], (int64_t)0), vocab - 1) * w_ld + k];
-    if (out_bf16) ((bf16*)out)[i] = (bf16)s;
-    else ((float*)out)[i] = s;
+    const float* at = f.part + r * f.ld + k;
+    int p = 0;
+    for (; p + 8 <= f.parts; p += 8, at += 8 * f.part_stride) {         // eight loads in flight, added in order
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = at[j * f.part_stride];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s += x[j];
+    }
+    for (; p < f.parts; ++p, at += f.part_stride) s += *at;
+    if (f.resid) s += f.resid[r] * (float)f.w[min(max((int64_t)f.y[r], (int64_t)0), f.vocab - 1) * f.w_ld + k];
+    if (f.out_bf16) ((bf16*)f.out)[i] = (bf16)s;
+    else ((float*)f.out)[i] = s;
+  };
+  for (int64_t u = (int64_t)blockIdx.x * GJX_BLOCK + threadIdx.x; u < all; u += (int64_t)gridDim.x * GJX_BLOCK) {
+    if (u < total) entry(one, u);
+    else entry(two, u - total);
   }
 }
 
@@ -909,6 +1028,10 @@ constexpr int64_t DL_BYTES = (int64_t)512 << 20;      // dl of one piece of the 
 constexpr int64_t PACK_BYTES = (int64_t)512 << 20;    // packed weights of one piece
 constexpr int64_t MAX_LD = 1 << 22;                   // 256 rows stay within 32-bit byte offsets
 constexpr int ROWS_MAX = 32;                          // rows up to which k_lincat_rows is used
+// What the forward of a gradient keeps (the exponentials of all logits) spares the gradient its first product and costs a
+// write and a read of them; up to this size, and from the width on where the product is the dearer one.
+constexpr int64_t KEEP_BYTES = (int64_t)2 << 30;
+constexpr int KEEP_WIDTH_F32 = 256, KEEP_WIDTH_BF16 = 1024;
 
 int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 
@@ -940,6 +1063,7 @@ struct Plan {
   int64_t piece;                // vocabulary entries per piece (multiple of 256)
   int64_t tiles;                // partial results per row
   int splits;                   // parts of dx's reduction
+  int strip;                    // rows per workgroup of k_lincat_dl
   int64_t o_x, o_w, o_part, o_target, o_dl, o_db, o_dx, o_resid, bytes;
 };
 
@@ -977,7 +1101,10 @@ Plan plan_of(const Call& c, bool grad, bool want_dx) {
   p.o_w = k.take(p.pack_w ? p.piece * p.kp * 2 : 0);
   if (grad) {
     p.o_dl = k.take(p.n_pad * p.piece * e);
-    p.o_db = k.take(p.n_tiles * p.piece * 4);
+    // strips of 64 rows, shorter ones where those would leave CUs without work
+    p.strip = 64;
+    while (p.strip > 16 && up(c.n, 64) / p.strip * (up(p.piece, GJX_BLOCK * 8) / (GJX_BLOCK * 8)) < 1024) p.strip /= 2;
+    p.o_db = k.take(std::max(p.n_tiles, up(c.n, 64) / p.strip) * p.piece * 4);
     p.o_resid = k.take(c.n * 4);
     const int64_t tiles = up(c.width, bm) / bm * p.n_tiles;
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>((c.f32() ? 768 : 512) / tiles, p.piece / BK / 8));
@@ -988,6 +1115,25 @@ Plan plan_of(const Call& c, bool grad, bool want_dx) {
   }
   p.bytes = k.at;
   return p;
+}
+
+// the buffer between a forward and its gradient
+struct Kept {
+  int64_t ld, o_base, o_lp, bytes;      // bytes = 0: nothing is kept
+  int block;                            // entries that share a base: those of a wave
+};
+
+Kept kept_of(const Call& c, const Plan& forward) {
+  Kept k = {};
+  if (forward.rows || c.width < (c.f32() ? KEEP_WIDTH_F32 : KEEP_WIDTH_BF16)) return k;
+  k.ld = up(c.vocab, BM);
+  k.block = c.f32() ? BM32 / 2 : forward.bn == 256 ? BM / 2 : BM / 4;
+  Carver at;
+  at.take(c.n * k.ld * (c.f32() ? 4 : 2));
+  k.o_base = at.take(k.ld / k.block * forward.n_pad * 4);
+  k.o_lp = at.take(c.n * 4);
+  k.bytes = at.at <= KEEP_BYTES ? at.at : 0;
+  return k;
 }
 
 // a kernel's dynamic LDS limit, raised once per device
@@ -1060,6 +1206,13 @@ int32_t check_work(const Call& c, const Plan& p, const void* work, int64_t bytes
   return GJX_OK;
 }
 
+int32_t check_kept(const Call& c, const Kept& k, const void* kept, int64_t bytes) {
+  GJX_REQUIRE(k.bytes > 0 && ((uintptr_t)kept & 255) == 0 && bytes >= k.bytes, GJX_EINVAL,
+              "%s: d_kept has %lld bytes, needs %lld aligned to 256 (0: nothing is kept at these sizes)", c.who, (long long)bytes,
+              (long long)k.bytes);
+  return GJX_OK;
+}
+
 GemmArgs common_args(const Call& c, const Plan& p) {
   GemmArgs a = {};
   a.splits = 1;
@@ -1100,6 +1253,7 @@ int depth_tiles(const Call& c, int64_t depth) { return (int)(c.f32() ? up(depth,
 // the forward product, reduced to log-densities (EPI_SCORE) or draws (EPI_DRAW)
 struct Forward {
   float *lp, *lse;
+  char* kept;
   uint32_t key0, key1;
   uint64_t offset;
   int32_t* out;
@@ -1116,10 +1270,10 @@ int32_t launch_rows(const Call& c, const Plan& p, const GemmArgs& a, hipStream_t
 }
 
 template <int EPI>
-int32_t forward(const Call& c, const Forward& f, void* d_work, int64_t work_bytes, hipStream_t s) {
-  const Plan p = plan_of(c, false, false);
+int32_t forward(const Call& c, const Plan& p, const Forward& f, void* d_work, int64_t work_bytes, hipStream_t s) {
   int32_t rc = check_work(c, p, d_work, work_bytes);
   if (rc != GJX_OK) return rc;
+  const Kept kept = f.kept ? kept_of(c, p) : Kept{};
   char* ws = (char*)d_work;
   GemmArgs a = common_args(c, p);
   a.key0 = f.key0;
@@ -1127,8 +1281,11 @@ int32_t forward(const Call& c, const Forward& f, void* d_work, int64_t work_byte
   a.offset = f.offset;
   a.part = (float2*)(ws + p.o_part);
   a.target = (float*)(ws + p.o_target);
-  if (p.rows) {
-    rc = c.f32() ? launch_rows<float, EPI>(c, p, a, s) : launch_rows<bf16, EPI>(c, p, a, s);
+  a.keep = f.kept;
+  a.keep_base = (float*)(f.kept + kept.o_base);
+  a.keep_ld = kept.ld;
+  if (EPI != EPI_KEEP && p.rows) {
+    if constexpr (EPI != EPI_KEEP) rc = c.f32() ? launch_rows<float, EPI>(c, p, a, s) : launch_rows<bf16, EPI>(c, p, a, s);
     if (rc != GJX_OK) return rc;
   } else {
     Inputs in = {};
@@ -1148,10 +1305,11 @@ int32_t forward(const Call& c, const Forward& f, void* d_work, int64_t work_byte
       if ((rc = launch<false, false, EPI>(c, p.bn > 64, a, s)) != GJX_OK) return rc;
     }
   }
-  if (EPI == EPI_SCORE) {
+  if (EPI != EPI_DRAW) {
     int cols = 1;                                            // 16 rows x 16 parts of the tiles per workgroup
     while (cols < 16 && cols < c.n) cols *= 2;
-    k_lincat_combine<<<(unsigned)(up(c.n, cols) / cols), GJX_BLOCK, 0, s>>>(a.part, (int)p.tiles, p.n_pad, c.n, cols, a.target, f.lp, f.lse);
+    k_lincat_combine<<<(unsigned)(up(c.n, cols) / cols), GJX_BLOCK, 0, s>>>(a.part, (int)p.tiles, p.n_pad, c.n, cols, a.target, f.lp, f.lse,
+                                                                               f.kept ? (float*)(f.kept + kept.o_lp) : nullptr);
   } else {
     k_lincat_pick<<<(unsigned)(up(c.n, GJX_BLOCK / 64) / (GJX_BLOCK / 64)), GJX_BLOCK, 0, s>>>(a.part, (int)p.tiles, p.n_pad, c.n, f.out);
   }
@@ -1162,28 +1320,36 @@ int32_t forward(const Call& c, const Forward& f, void* d_work, int64_t work_byte
 }  // namespace
 
 GJX_API int32_t gjx_linear_categorical_workspace(int32_t dtype, const void* d_x, int64_t x_ld, const void* d_w, int64_t w_ld,
-                                                 int64_t n, int64_t vocab, int64_t width, int32_t grad, int64_t* bytes) {
+                                                 int64_t n, int64_t vocab, int64_t width, int32_t kind, int64_t* bytes) {
   static const int32_t some_y = 0;
   const Call c = {"gjx_linear_categorical_workspace", dtype, &some_y, d_x, x_ld, d_w, w_ld, nullptr, n, vocab, width};
-  GJX_REQUIRE(bytes != nullptr && grad >= 0 && grad <= 2, GJX_EINVAL, "%s: bytes is null or grad not in [0, 2]", c.who);
+  GJX_REQUIRE(bytes != nullptr && kind >= 0 && kind <= 3, GJX_EINVAL, "%s: bytes is null or kind not in [0, 3]", c.who);
   const int32_t rc = check_args(c);
   if (rc != GJX_OK) return rc;
-  *bytes = n == 0 ? 0 : plan_of(c, grad != 0, grad == 1).bytes;
+  if (n == 0) *bytes = 0;
+  else if (kind == 3) *bytes = kept_of(c, plan_of(c, false, false)).bytes;
+  else *bytes = plan_of(c, kind != 0, kind == 1).bytes;
   return GJX_OK;
 }
 
 GJX_API int32_t gjx_linear_categorical_logpdf(int32_t dtype, const int32_t* d_y, const void* d_x, int64_t x_ld,
                                               const void* d_w, int64_t w_ld, const void* d_bias, int64_t n, int64_t vocab,
-                                              int64_t width, float* d_lp, float* d_lse, void* d_work, int64_t work_bytes,
-                                              void* stream) {
+                                              int64_t width, float* d_lp, float* d_lse, void* d_kept, int64_t kept_bytes,
+                                              void* d_work, int64_t work_bytes, void* stream) {
   const Call c = {"gjx_linear_categorical_logpdf", dtype, d_y, d_x, x_ld, d_w, w_ld, d_bias, n, vocab, width};
-  const int32_t rc = check_args(c);
+  int32_t rc = check_args(c);
   if (rc != GJX_OK || n == 0) return rc;
   GJX_REQUIRE(d_lp, GJX_EINVAL, "%s: null output", c.who);
   Forward f = {};
   f.lp = d_lp;
   f.lse = d_lse;
-  return forward<EPI_SCORE>(c, f, d_work, work_bytes, (hipStream_t)stream);
+  const Plan p = plan_of(c, false, false);
+  if (d_kept) {
+    if ((rc = check_kept(c, kept_of(c, p), d_kept, kept_bytes)) != GJX_OK) return rc;
+    f.kept = (char*)d_kept;
+    return forward<EPI_KEEP>(c, p, f, d_work, work_bytes, (hipStream_t)stream);
+  }
+  return forward<EPI_SCORE>(c, p, f, d_work, work_bytes, (hipStream_t)stream);
 }
 
 GJX_API int32_t gjx_random_linear_categorical_i32(const uint32_t key[2], uint64_t offset, int32_t dtype, const void* d_x,
@@ -1200,13 +1366,13 @@ GJX_API int32_t gjx_random_linear_categorical_i32(const uint32_t key[2], uint64_
   f.key1 = key[1];
   f.offset = offset;
   f.out = d_out;
-  return forward<EPI_DRAW>(c, f, d_work, work_bytes, (hipStream_t)stream);
+  return forward<EPI_DRAW>(c, plan_of(c, false, false), f, d_work, work_bytes, (hipStream_t)stream);
 }
 
 GJX_API int32_t gjx_linear_categorical_grad(int32_t dtype, const int32_t* d_y, const void* d_x, int64_t x_ld, const void* d_w,
                                             int64_t w_ld, const void* d_bias, int64_t n, int64_t vocab, int64_t width,
-                                            const float* d_lse, const float* d_upstream, void* d_dx, void* d_dw, void* d_db,
-                                            void* d_work, int64_t work_bytes, void* stream) {
+                                            const float* d_lse, const float* d_upstream, const void* d_kept, int64_t kept_bytes,
+                                            void* d_dx, void* d_dw, void* d_db, void* d_work, int64_t work_bytes, void* stream) {
   const Call c = {"gjx_linear_categorical_grad", dtype, d_y, d_x, x_ld, d_w, w_ld, d_bias, n, vocab, width};
   int32_t rc = check_args(c);
   if (rc != GJX_OK) return rc;
@@ -1215,6 +1381,11 @@ GJX_API int32_t gjx_linear_categorical_grad(int32_t dtype, const int32_t* d_y, c
   const bool f32 = c.f32();
   const Plan p = plan_of(c, true, d_dx != nullptr);
   if ((rc = check_work(c, p, d_work, work_bytes)) != GJX_OK) return rc;
+  Kept kept = {};
+  if (d_kept) {
+    kept = kept_of(c, plan_of(c, false, false));
+    if ((rc = check_kept(c, kept, d_kept, kept_bytes)) != GJX_OK) return rc;
+  }
   if (!d_dx && !d_dw && !d_db) return GJX_OK;
   hipStream_t s = (hipStream_t)stream;
   char* ws = (char*)d_work;
@@ -1223,33 +1394,54 @@ GJX_API int32_t gjx_linear_categorical_grad(int32_t dtype, const int32_t* d_y, c
   const bool wide = p.bn > 64;
   const int mk = (int)(up(width, p.bm) / p.bm);
   const int64_t part_ld = up(p.kp, 4);
-  float *dx_part = (float*)(ws + p.o_dx), *resid = f32 ? nullptr : (float*)(ws + p.o_resid);
+  float *dx_part = (float*)(ws + p.o_dx), *db_part = (float*)(ws + p.o_db), *resid = f32 ? nullptr : (float*)(ws + p.o_resid);
+  const bool whole = p.piece >= vocab;                       // one piece
+  const bool dx_direct = whole && f32 && p.splits == 1;      // nothing to add up
+  const int db_parts = (int)(d_kept ? up(n, 64) / p.strip : p.n_tiles);
+  Fold dx_fold = {}, db_fold = {};
+  auto fold = [&](const Fold& one, const Fold& two) -> int32_t {
+    k_lincat_fold<<<gjx_grid_for(one.rows * one.width + two.rows * two.width), GJX_BLOCK, 0, s>>>(one, two);
+    GJX_LAUNCH_CHECK();
+    return GJX_OK;
+  };
   for (int64_t v0 = 0; v0 < vocab; v0 += p.piece) {
     const int64_t rows = std::min(p.piece, vocab - v0), rows_pad = up(rows, BM);
     if ((rc = take_w(c, p, ws, v0, rows, in, s)) != GJX_OK) return rc;
     const Operand dl = {(const bf16*)(ws + p.o_dl), p.piece, (int)p.n_pad, (int)p.piece};
     const OperandF fdl = {(const float*)(ws + p.o_dl), p.piece, (int)p.n_pad, (int)rows_pad, 1};
-    GemmArgs a = common_args(c, p);                          // logits of the piece -> dl
-    a.a = in.w;
-    a.fa = in.fw;
-    a.b = in.x;
-    a.fb = in.fx;
-    a.ktiles = depth_tiles(c, p.kp);
-    a.mt = (int)(rows_pad / p.bm);
-    a.nt = (int)p.n_tiles;
-    a.v0 = v0;
-    a.lse = d_lse;
-    a.g = d_upstream;
-    a.dl = ws + p.o_dl;
-    a.resid = resid;
-    a.dl_ld = p.piece;
-    a.db_part = d_db ? (float*)(ws + p.o_db) : nullptr;
-    if ((rc = launch<false, false, EPI_DL>(c, wide, a, s)) != GJX_OK) return rc;
-    if (d_db) {
-      k_lincat_fold<<<gjx_grid_for(rows), GJX_BLOCK, 0, s>>>((const float*)(ws + p.o_db), (int)p.n_tiles, p.piece, 1, rows, rows,
-                                                           f32 ? (void*)((float*)d_db + v0) : (void*)((bf16*)d_db + v0), !f32,
-                                                           nullptr, nullptr, nullptr, 0, 0);
+    if (d_kept) {
+      const char* k = (const char*)d_kept;
+      const dim3 grid((unsigned)(up(n, 64) / p.strip), (unsigned)(up(rows_pad, GJX_BLOCK * 8) / (GJX_BLOCK * 8)));
+      if (f32)
+        k_lincat_dl<float><<<grid, GJX_BLOCK, 0, s>>>(k, kept.ld, (const float*)(k + kept.o_base), kept.block, p.n_pad,
+                                                      (const float*)(k + kept.o_lp), d_lse, d_upstream, d_y, n, vocab, v0, (int)rows_pad, p.strip,
+                                                      (float*)(ws + p.o_dl), p.piece, resid, d_db ? db_part : nullptr, p.piece);
+      else
+        k_lincat_dl<bf16><<<grid, GJX_BLOCK, 0, s>>>(k, kept.ld, (const float*)(k + kept.o_base), kept.block, p.n_pad,
+                                                     (const float*)(k + kept.o_lp), d_lse, d_upstream, d_y, n, vocab, v0, (int)rows_pad, p.strip,
+                                                     (bf16*)(ws + p.o_dl), p.piece, resid, d_db ? db_part : nullptr, p.piece);
       GJX_LAUNCH_CHECK();
+    } else {
+      GemmArgs a = common_args(c, p);                        // logits of the piece -> dl
+      a.a = in.w;
+      a.fa = in.fw;
+      a.b = in.x;
+      a.fb = in.fx;
+      a.ktiles = depth_tiles(c, p.kp);
+      a.mt = (int)(rows_pad / p.bm);
+      a.nt = (int)p.n_tiles;
+      a.v0 = v0;
+      a.lse = d_lse;
+      a.g = d_upstream;
+      a.dl = ws + p.o_dl;
+      a.resid = resid;
+      a.dl_ld = p.piece;
+      a.db_part = d_db ? db_part : nullptr;
+      if ((rc = launch<false, false, EPI_DL>(c, wide, a, s)) != GJX_OK) return rc;
+    }
+    if (d_db) {
+      db_fold = {db_part, db_parts, p.piece, 1, rows, rows, (char*)d_db + v0 * (f32 ? 4 : 2), !f32, nullptr, nullptr, nullptr, 0, 0};
+      if (!whole && (rc = fold(db_fold, Fold{})) != GJX_OK) return rc;
     }
     if (d_dx) {                                              // dx^T = W^T dl^T: m = feature, n = row, over the piece
       GemmArgs b = common_args(c, p);
@@ -1261,8 +1453,8 @@ GJX_API int32_t gjx_linear_categorical_grad(int32_t dtype, const int32_t* d_y, c
       b.mt = mk;
       b.nt = (int)p.n_tiles;
       b.splits = p.splits;
-      b.out = dx_part;
-      b.out_ld = part_ld;
+      b.out = dx_direct ? d_dx : (void*)dx_part;
+      b.out_ld = dx_direct ? width : part_ld;
       b.out_split = n * part_ld;
       b.out_m = (int)p.kp;
       b.out_n = (int)n;
@@ -1288,10 +1480,9 @@ GJX_API int32_t gjx_linear_categorical_grad(int32_t dtype, const int32_t* d_y, c
       if ((rc = launch<true, true, EPI_STORE>(c, true, b, s)) != GJX_OK) return rc;
     }
   }
-  if (d_dx) {
-    k_lincat_fold<<<gjx_grid_for(n * width), GJX_BLOCK, 0, s>>>(dx_part, p.splits, n * part_ld, n, part_ld, width, d_dx, !f32, resid,
-                                                                d_y, (const bf16*)d_w, w_ld, vocab);
-    GJX_LAUNCH_CHECK();
-  }
+  if (d_dx && !dx_direct)
+    dx_fold = {dx_part, p.splits, n * part_ld, n, part_ld, width, d_dx, !f32, resid, d_y, (const bf16*)d_w, w_ld, vocab};
+  if (!whole) db_fold = {};                                  // (done piece by piece)
+  if (dx_fold.out || db_fold.out) return fold(dx_fold, db_fold);
   return GJX_OK;
 }

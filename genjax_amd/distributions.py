@@ -120,16 +120,16 @@ categorical = _Categorical(None, lambda x, logits: B.categorical_logpdf(x, as_co
 class _LinearCategoricalFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, x, weight, bias):
-        lp, lse = B.linear_categorical_logpdf(y, x, weight, bias)
-        ctx.save_for_backward(y, x, weight, bias, lse)
+        lp, lse, kept = B.linear_categorical_logpdf(y, x, weight, bias, keep=True)
+        ctx.save_for_backward(y, x, weight, bias, lse, kept)
         return lp
 
     @staticmethod
     def backward(ctx, g):
         if torch.is_grad_enabled():
             raise B.GjxError("linear_categorical: its gradient cannot be differentiated again (create_graph=True)")
-        y, x, weight, bias, lse = ctx.saved_tensors
-        return (None, *B.linear_categorical_grad(y, x, weight, bias, lse, g, want=ctx.needs_input_grad[1:4]))
+        y, x, weight, bias, lse, kept = ctx.saved_tensors
+        return (None, *B.linear_categorical_grad(y, x, weight, bias, lse, g, want=ctx.needs_input_grad[1:4], kept=kept))
 
 
 class _LinearCategorical(Distribution):

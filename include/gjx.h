@@ -143,21 +143,24 @@ int32_t gjx_categorical_logpdf_f32(const int32_t* d_x, const float* d_logits, in
  * feature row, without keeping the n x vocab logits.  x: n rows of `width` (row stride x_ld elements), W: vocab rows
  * (stride w_ld), bias: vocab or NULL, all of type `dtype` (GJX_F32 or GJX_BF16); sums and outputs lp, lse in f32.
  * y outside [0, vocab) takes the nearest entry.  A bias of -inf takes its entry out of the distribution; a row with no
- * entry left is NaN.  The caller owns the workspace (256-byte aligned, gjx_linear_categorical_workspace bytes; grad:
+ * entry left is NaN.  The caller owns the workspace (256-byte aligned, gjx_linear_categorical_workspace bytes; kind:
  * 0 for the log-density, 1 for the gradient, 2 for the gradient without d_dx); its contents need not be kept between calls.
+ * kind 3 gives the bytes of d_kept (nullable, 256-byte aligned): what the log-density may leave for the gradient, which then
+ * does not form the logits again; 0 where they gain nothing by it (up to 32 rows, small widths) or pass 2 GiB.
+ * The inputs are finite (bias: or -inf).
  *   logpdf: lp_i = l_{i, y_i} - lse_i, lse_i = log sum_v exp(l_iv) (d_lse nullable)
  *   grad:   outputs (nullable) dx, dW, db of sum_i upstream_i lp_i, contiguous, of type dtype (what jax.grad of
  *           assess produces inside hmc, mcmc.py:59-88, 508, 523); d_lse is the log-density call's */
 int32_t gjx_linear_categorical_workspace(int32_t dtype, const void* d_x, int64_t x_ld, const void* d_w, int64_t w_ld,
-                                         int64_t n, int64_t vocab, int64_t width, int32_t grad, int64_t* bytes);
+                                         int64_t n, int64_t vocab, int64_t width, int32_t kind, int64_t* bytes);
 int32_t gjx_linear_categorical_logpdf(int32_t dtype, const int32_t* d_y, const void* d_x, int64_t x_ld,
                                       const void* d_w, int64_t w_ld, const void* d_bias, int64_t n, int64_t vocab,
-                                      int64_t width, float* d_lp, float* d_lse, void* d_work, int64_t work_bytes,
-                                      void* stream);
+                                      int64_t width, float* d_lp, float* d_lse, void* d_kept, int64_t kept_bytes,
+                                      void* d_work, int64_t work_bytes, void* stream);
 int32_t gjx_linear_categorical_grad(int32_t dtype, const int32_t* d_y, const void* d_x, int64_t x_ld, const void* d_w,
                                     int64_t w_ld, const void* d_bias, int64_t n, int64_t vocab, int64_t width,
-                                    const float* d_lse, const float* d_upstream, void* d_dx, void* d_dw, void* d_db,
-                                    void* d_work, int64_t work_bytes, void* stream);
+                                    const float* d_lse, const float* d_upstream, const void* d_kept, int64_t kept_bytes,
+                                    void* d_dx, void* d_dw, void* d_db, void* d_work, int64_t work_bytes, void* stream);
 /* its draw: argmax_v (l_iv + Gumbel), the Gumbel of entry v of row i on counter (offset + i) vocab + v of the key (the
  * layout of gjx_random_categorical_i32 with per-row logits; distributions.py:92-95), ties to the lowest entry;
  * workspace as for the log-density */

@@ -310,3 +310,82 @@ def test_same_bits_on_every_call(G):
     first = _grads(G, x, w, b, y, up)
     for _ in range(3):
         assert all(torch.equal(a, c) for a, c in zip(first, _grads(G, x, w, b, y, up)))
+
+
+# ---- what the forward keeps for the gradient ---------------------------------
+# Above 32 rows and from a width of 256 (f32) or 1024 (bf16) on, the gradient is formed from the forward's exponentials.  In
+# f32 they are kept as they are: exp(l - base) and exp(base - lse) share the error that exp(l - lse) had.  In bf16 they are
+# kept in 11 bits (2^-11, and 2^-40 of the block's largest absolutely), before dl is rounded as everywhere: dl is off by
+# |g| (2^-11 p + 2^-40) more.
+def _check_kept(G, n, vocab, width, dtype, bias=True):
+    from genjax_amd import backend as B
+
+    x, w, b, y, up = _inputs(n, vocab, width, dtype, bias=bias)
+    t = _truth(x, w, b, y, up)
+    args = [a for a in (x, w, b) if a is not None]
+    lp, lse, kept = B.linear_categorical_logpdf(y, *args, keep=True)
+    assert kept is not None
+    plain, lse2 = B.linear_categorical_logpdf(y, *args)
+    assert torch.equal(lp, plain) and torch.equal(lse, lse2)
+    _close("lp", lp, t["lp"])
+    if dtype == torch.bfloat16:
+        X, W, u = x.double().abs(), w.double().abs(), up.double().abs().unsqueeze(1)
+        L = x.double() @ w.double().t() + (0.0 if b is None else b.double())
+        extra = u * (torch.softmax(L, 1) * 2.0 ** -11 + 2.0 ** -40)
+        for name, more in (("dx", extra @ W), ("dw", extra.t() @ X), ("db", extra.sum(0))):
+            t[name] = (t[name][0], t[name][1] + more)
+    got = B.linear_categorical_grad(y, x, w, b, lse, up, kept=kept)
+    again = B.linear_categorical_grad(y, x, w, b, lse, up, kept=kept)          # what is kept is only read
+    for name, g, g2 in zip(("dx", "dw", "db"), got, again):
+        if g is not None:
+            _close(name, g, t[name])
+            assert torch.equal(g, g2)
+    for want in ((True, False, False), (False, True, False), (False, False, b is not None)):
+        part = B.linear_categorical_grad(y, x, w, b, lse, up, want=want, kept=kept)
+        for wanted, p, g in zip(want, part, got):
+            assert torch.equal(p, g) if wanted else p is None
+
+
+@pytest.mark.parametrize("n,vocab,width", [(33, 2, 256), (33, 300, 257), (64, 257, 300), (130, 4099, 512), (200, 50001, 256), (1000, 140001, 256)])
+def test_gradient_from_what_the_forward_kept_f32(G, n, vocab, width):
+    _check_kept(G, n, vocab, width, torch.float32, bias=vocab != 300)
+
+
+@pytest.mark.parametrize("n,vocab,width", [(33, 2, 1024), (33, 300, 1030), (100, 511, 1088), (257, 70000, 1024), (4000, 70001, 1024)])
+def test_gradient_from_what_the_forward_kept_bf16(G, n, vocab, width):
+    _check_kept(G, n, vocab, width, torch.bfloat16, bias=vocab != 300)
+
+
+def test_kept_rows_without_an_entry_and_masked_entries(G):
+    """Entries with a bias of -inf keep a gradient of 0, values there a log-density of -inf, rows without any entry are NaN;
+    a graph that is replayed and an eager backward in between agree."""
+    n, vocab, width = 70, 600, 256
+    x, w, b, y, up = _inputs(n, vocab, width, torch.float32)
+    b[100:500] = -float("inf")
+    y = torch.where((y >= 100) & (y < 500), 5, y).to(torch.int32)
+    t = _truth(x, w, b, y, up)
+    for name, got in zip(("lp", "dx", "dw", "db"), _grads(G, x, w, b, y, up)):
+        _close(name, got, t[name])
+        if name in ("dw", "db"):
+            assert not got[100:500].any()
+    y2 = y.clone()
+    y2[3] = 200
+    lp, dx, dw, db = _grads(G, x, w, b, y2, up)
+    assert lp[3] == -float("inf") and torch.isfinite(dx).all() and torch.isfinite(dw).all() and torch.isfinite(db).all()
+    lp, *_ = _grads(G, x, w, torch.full_like(b, -float("inf")), y, up)
+    assert torch.isnan(lp).all()
+
+
+def test_two_backwards_and_a_large_shift(G):
+    """retain_graph: the second backward gives the same; logits near 300 (a bias common to all) change nothing."""
+    x, w, b, y, up = _inputs(90, 700, 320, torch.float32)
+    leaves = [a.clone().requires_grad_(True) for a in (x, w, b + 300.0)]
+    lp = G.linear_categorical.logpdf(y, *leaves)
+    one = torch.autograd.grad(lp, leaves, up, retain_graph=True)
+    two = torch.autograd.grad(lp, leaves, up)
+    assert all(torch.equal(p, q) for p, q in zip(one, two))
+    t = _truth(x, w, b + 300.0, y, up)
+    # a logit near 300 is rounded to 2^-24 of it after the bias is added: E grows by 2^-24 * 300 < 2^-15, in p as in dl
+    P = torch.softmax(x.double() @ w.double().t() + b.double(), 1) * up.double().abs().unsqueeze(1) * 2.0 ** -14
+    for name, got, more in zip(("dx", "dw", "db"), one, (P @ w.double().abs(), P.t() @ x.double().abs(), P.sum(0))):
+        _close(name, got, (t[name][0], t[name][1] + more))
