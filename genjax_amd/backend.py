@@ -471,49 +471,66 @@ def _note_leaves(who, out):
                                "stream and still lives: drop that graph (its outputs) first, or capture with fresh leaves")
 
 
-def _unit_stride(t):
-    """`t` itself when its last axis is contiguous and its rows neither overlap nor lie too far apart, else a copy."""
-    width, (step, unit) = t.shape[1], t.stride()
-    return t if (unit == 1 or width == 1) and width <= step <= 1 << 22 else t.contiguous()
+class _LinearPlan:
+    """Checked sizes and strides of a linear-categorical call, with the workspaces it needs."""
+
+    __slots__ = ("dtype", "n", "vocab", "width", "x_ld", "w_ld", "copy_x", "copy_w", "low", "_bytes")
+
+    def bytes(self, kind):
+        size = self._bytes.get(kind)
+        if size is None:
+            out = C.c_int64()
+            N.check(N.lib().gjx_linear_categorical_workspace(self.dtype, 16 + self.low[0], self.x_ld, 16 + self.low[1], self.w_ld, self.n,
+                                                             self.vocab, self.width, kind, C.byref(out)),
+                    "gjx_linear_categorical_workspace")
+            size = self._bytes[kind] = max(out.value, 256) if kind < 3 else out.value
+        return size
 
 
 @functools.lru_cache(maxsize=1024)
-def _linear_workspace_bytes(dtype, x_low, x_ld, w_low, w_ld, n, vocab, width, kind):
-    """Workspace of a call: depends on the sizes, the row strides and the pointers' alignment (their low bits)."""
-    size = C.c_int64()
-    N.check(N.lib().gjx_linear_categorical_workspace(dtype, 16 + x_low, x_ld, 16 + w_low, w_ld, n, vocab, width, kind, C.byref(size)),
-            "gjx_linear_categorical_workspace")
-    return max(size.value, 256) if kind < 3 else size.value
+def _linear_plan(x_type, w_type, b_type, x_shape, w_shape, b_shape, x_stride, w_stride, x_low, w_low):
+    """x_low, w_low: the addresses modulo 16 (the layout of a workspace depends on the operands' alignment)."""
+    who = "linear_categorical"
+    if len(x_shape) != 2 or len(w_shape) != 2 or x_shape[1] != w_shape[1] or w_shape[0] < 1 or w_shape[1] < 1:
+        raise GjxError(f"{who}: x {tuple(x_shape)} and weight {tuple(w_shape)} must be (n, width) and (vocab, width)")
+    p = _LinearPlan()
+    p.n, (p.vocab, p.width) = x_shape[0], w_shape
+    if b_shape is not None and b_shape != (p.vocab,):
+        raise GjxError(f"{who}: bias {tuple(b_shape)} must be ({p.vocab},)")
+    p.dtype = ELEMENT_TYPES.get(x_type)
+    if p.dtype is None or w_type != x_type or b_type not in (None, x_type):
+        raise GjxError(f"{who}: x, weight and bias must all be float32 or all bfloat16 (got {x_type}, {w_type}"
+                       f"{'' if b_type is None else f', {b_type}'})")
+    # taken as they are: rows with a contiguous last axis that neither overlap nor lie too far apart
+    fits = lambda step, unit: (unit == 1 or p.width == 1) and p.width <= step <= 1 << 22        # noqa: E731
+    p.copy_x, p.copy_w = not fits(*x_stride), not fits(*w_stride)
+    p.x_ld, p.w_ld = p.width if p.copy_x else x_stride[0], p.width if p.copy_w else w_stride[0]
+    p.low = (0 if p.copy_x else x_low, 0 if p.copy_w else w_low)
+    p._bytes = {}
+    return p
 
 
 class _Linear:
     """The checked inputs of a linear-categorical call as the library takes them."""
 
-    __slots__ = ("x", "weight", "bias", "n", "vocab", "width", "head")
+    __slots__ = ("x", "weight", "bias", "n", "vocab", "width", "head", "plan")
 
     def __init__(self, x, weight, bias):
-        who = "linear_categorical"
         for name, t in (("x", x), ("weight", weight), ("bias", bias)):
             if t is not None and not isinstance(t, torch.Tensor):
-                raise GjxError(f"{who}: `{name}` must be a tensor")
-        if x.dim() != 2 or weight.dim() != 2 or x.shape[1] != weight.shape[1] or weight.shape[0] < 1 or weight.shape[1] < 1:
-            raise GjxError(f"{who}: x {tuple(x.shape)} and weight {tuple(weight.shape)} must be (n, width) and (vocab, width)")
-        self.n, (self.vocab, self.width) = x.shape[0], weight.shape
-        if bias is not None and bias.shape != (self.vocab,):
-            raise GjxError(f"{who}: bias {tuple(bias.shape)} must be ({self.vocab},)")
-        dtype = ELEMENT_TYPES.get(x.dtype)
-        if dtype is None or weight.dtype != x.dtype or (bias is not None and bias.dtype != x.dtype):
-            raise GjxError(f"{who}: x, weight and bias must all be float32 or all bfloat16 (got {x.dtype}, {weight.dtype}"
-                           f"{'' if bias is None else f', {bias.dtype}'})")
-        _on_current_device(who, ("x", x), ("weight", weight), ("bias", bias))
-        self.x, self.weight, self.bias = _unit_stride(x), _unit_stride(weight), None if bias is None else bias.contiguous()
-        self.head = (dtype, self.x.data_ptr(), max(self.x.stride(0), self.width), self.weight.data_ptr(),
-                     max(self.weight.stride(0), self.width))
+                raise GjxError(f"linear_categorical: `{name}` must be a tensor")
+        has = bias is not None
+        p = self.plan = _linear_plan(x.dtype, weight.dtype, bias.dtype if has else None, x.shape, weight.shape, bias.shape if has else None,
+                                     x.stride(), weight.stride(), x.data_ptr() & 15, weight.data_ptr() & 15)
+        _on_current_device("linear_categorical", ("x", x), ("weight", weight), ("bias", bias))
+        self.x, self.weight = x.contiguous() if p.copy_x else x, weight.contiguous() if p.copy_w else weight
+        self.bias = bias.contiguous() if has else None
+        self.n, self.vocab, self.width = p.n, p.vocab, p.width
+        self.head = (p.dtype, self.x.data_ptr(), p.x_ld, self.weight.data_ptr(), p.w_ld)
 
     def workspace(self, kind):
         """kind: 0 log-density or draw, 1 gradient, 2 gradient without x's, 3 what the first leaves for the second (or None)."""
-        dtype, xp, x_ld, wp, w_ld = self.head
-        size = _linear_workspace_bytes(dtype, xp & 15, x_ld, wp & 15, w_ld, self.n, self.vocab, self.width, kind)
+        size = self.plan.bytes(kind)
         return torch.empty(size, dtype=torch.uint8, device=self.x.device) if size else None
 
 

@@ -58,7 +58,7 @@ def test_linear_categorical_abi_refusals():
     assert L.gjx_linear_categorical_workspace(0, p, 256, p, 256, 100, 5, 256, 3, C.byref(size)) == 0 and size.value > 100 * 256 * 4
     assert code(kept=p, kept_bytes=size.value - 1, **sizes) == -1 and b"d_kept" in L.gjx_last_error()
     assert code(kept=C.c_void_p((1 << 20) + 16), kept_bytes=size.value, **sizes) == -1
-    for n, vocab, width, dtype in ((32, 1000, 512, 0), (100, 1000, 255, 0), (100, 1000, 1023, 1), (1 << 20, 1 << 20, 512, 0)):
+    for n, vocab, width, dtype in ((32, 1000, 512, 0), (100, 1000, 127, 0), (100, 1000, 511, 1), (1 << 20, 1 << 20, 512, 0)):
         assert L.gjx_linear_categorical_workspace(dtype, p, width, p, width, n, vocab, width, 3, C.byref(size)) == 0 and size.value == 0
 
     def grad(lse=p, up=p, kept=None, kept_bytes=0, work_bytes=1 << 30):
