@@ -234,8 +234,11 @@ __device__ __forceinline__ void epilogue(const GemmArgs& g, const Tile& tile, f3
   const int q = lane >> 4, c = lane & 15;
   if (EPI == EPI_STORE) {
     if (sizeof(T) == 2 && TB && g.resid_in) {
-      // dW of the rows' own values: += resid_i x_i, in ascending i (every wave looks for its own columns, 512 rows at a time)
-      for (int64_t i8 = 0; i8 < g.n; i8 += 512) {
+      // dW of the rows' own values: += resid_i x_i, in ascending i, over the rows of this part of the reduction.  Every wave
+      // looks for its own columns, 512 rows at a time; a lane takes the rows of its column, so that up to sixteen are added at
+      // once (one after the other, 500 rows of 300 values took 86 us)
+      const int64_t end = min((int64_t)g.ktiles * (split + 1) / g.splits * BK, g.n);
+      for (int64_t i8 = (int64_t)g.ktiles * split / g.splits * BK; i8 < end; i8 += 512) {
         int v8[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u) v8[u] = g.y[min(i8 + 64 * u + lane, g.n - 1)];
@@ -246,26 +249,34 @@ __device__ __forceinline__ void epilogue(const GemmArgs& g, const Tile& tile, f3
 #pragma unroll
           for (int e = 1; e < 8; ++e) yv = u == e ? v8[e] : yv;
           const int64_t v = min(max((int64_t)yv, (int64_t)0), g.vocab - 1) - g.v0 - n0 - wn;
-          uint64_t hits = __ballot(i0 + lane < g.n && v >= 0 && v < NT * 16);
-          if (!hits) continue;
+          const bool mine = i0 + lane < end && v >= 0 && v < NT * 16;
+          if (!__ballot(mine)) continue;
+          const int vl = mine ? (int)v : -1;
           const float res = g.resid_in[min(i0 + lane, g.n - 1)];
-          while (hits) {
-            const int l = __builtin_ctzll(hits);
-            hits &= hits - 1;
-            const int vl = __builtin_amdgcn_readlane((int)v, l);
-            const float rl = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(res), l));
-            if ((vl & 15) != c) continue;
-            const bf16* xr = g.a.p + (i0 + l) * g.a.ld;
+          uint64_t hits = 0;                               // the rows of this lane's column
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-              const bf16x4 xv = *(const bf16x4*)(xr + min(m0 + wm + i * 16 + 4 * q, g.a.cols - 4));
+          for (int e = 0; e < 16; ++e) {
+            const uint64_t rows = __ballot(vl >= 0 && (vl & 15) == e);
+            hits = c == e ? rows : hits;
+          }
+          while (__ballot(hits != 0)) {
+            const int l = hits ? __builtin_ctzll(hits) : 0;
+            const int vr = __shfl(vl, l);
+            const float rr = __shfl(res, l);
+            const float rl = hits ? rr : 0.0f;
+            hits &= hits - 1;
+            const bf16* xr = g.a.p + min(i0 + l, g.n - 1) * g.a.ld;
+            bf16x4 xv[MT];
+#pragma unroll
+            for (int i = 0; i < MT; ++i) xv[i] = *(const bf16x4*)(xr + min(m0 + wm + i * 16 + 4 * q, g.a.cols - 4));
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
 #pragma unroll
               for (int j = 0; j < NT; ++j) {
-                const float w = (vl >> 4) == j ? rl : 0.0f;
+                const float w = (vr >> 4) == j ? rl : 0.0f;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) acc[i][j][r] += w * (float)xv[r];
+                for (int r = 0; r < 4; ++r) acc[i][j][r] += w * (float)xv[i][r];
               }
-            }
           }
         }
       }
@@ -994,10 +1005,10 @@ struct Fold {
   int64_t w_ld, vocab;
 };
 
-// one or two such sums (those of dx and of db) in one launch
+// up to three such sums (those of dx, db and dW) in one launch
 __global__ void __launch_bounds__(GJX_BLOCK)
-    k_lincat_fold(Fold one, Fold two) {
-  const int64_t total = one.rows * one.width, all = total + two.rows * two.width;
+    k_lincat_fold(Fold one, Fold two, Fold three) {
+  const int64_t first = one.rows * one.width, second = first + two.rows * two.width, all = second + three.rows * three.width;
   auto entry = [](const Fold& f, int64_t i) {
     const int64_t r = i / f.width, k = i - r * f.width;
     float s = 0.0f;
@@ -1016,8 +1027,9 @@ __global__ void __launch_bounds__(GJX_BLOCK)
     else ((float*)f.out)[i] = s;
   };
   for (int64_t u = (int64_t)blockIdx.x * GJX_BLOCK + threadIdx.x; u < all; u += (int64_t)gridDim.x * GJX_BLOCK) {
-    if (u < total) entry(one, u);
-    else entry(two, u - total);
+    if (u < first) entry(one, u);
+    else if (u < second) entry(two, u - first);
+    else entry(three, u - second);
   }
 }
 
@@ -1064,9 +1076,9 @@ struct Plan {
   bool pack_x, pack_w;
   int64_t piece;                // vocabulary entries per piece (multiple of 256)
   int64_t tiles;                // partial results per row
-  int splits;                   // parts of dx's reduction
+  int splits, splits_w;         // parts of the reductions of dx (over the piece) and dW (over the rows)
   int strip;                    // rows per workgroup of k_lincat_dl
-  int64_t o_x, o_w, o_part, o_target, o_dl, o_db, o_dx, o_resid, bytes;
+  int64_t o_x, o_w, o_part, o_target, o_dl, o_db, o_dx, o_dw, o_resid, bytes;
 };
 
 struct Carver {
@@ -1109,7 +1121,11 @@ Plan plan_of(const Call& c, bool grad, bool want_dx) {
     p.o_db = k.take(std::max(p.n_tiles, up(c.n, 64) / p.strip) * p.piece * 4);
     p.o_resid = k.take(c.n * 4);
     const int64_t tiles = up(c.width, bm) / bm * p.n_tiles;
-    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>((c.f32() ? 768 : 512) / tiles, p.piece / BK / 8));
+    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>((c.f32() ? 768 : 512) / tiles, p.piece / (c.f32() ? 128 : 512)));
+    // few tiles of dW: their rows are shared out (1000 x 2000 x 128: 63 us in eight workgroups)
+    const int64_t tiles_w = up(c.width, bm) / bm * (up(c.vocab, c.f32() ? 128 : 256) / (c.f32() ? 128 : 256));
+    p.splits_w = p.piece < c.vocab ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>(256 / tiles_w, c.n / 128));
+    p.o_dw = k.take(p.splits_w > 1 ? p.splits_w * c.vocab * up(c.width, 4) * 4 : 0);
     p.o_dx = k.take(want_dx ? (int64_t)p.splits * c.n * up(p.kp, 4) * 4 : 0);
   } else {
     p.o_part = k.take(p.tiles * p.n_pad * 8);
@@ -1400,9 +1416,10 @@ GJX_API int32_t gjx_linear_categorical_grad(int32_t dtype, const int32_t* d_y, c
   const bool whole = p.piece >= vocab;                       // one piece
   const bool dx_direct = whole && f32 && p.splits == 1;      // nothing to add up
   const int db_parts = (int)(d_kept ? up(n, 64) / p.strip : p.n_tiles);
-  Fold dx_fold = {}, db_fold = {};
-  auto fold = [&](const Fold& one, const Fold& two) -> int32_t {
-    k_lincat_fold<<<gjx_grid_for(one.rows * one.width + two.rows * two.width), GJX_BLOCK, 0, s>>>(one, two);
+  Fold dx_fold = {}, db_fold = {}, dw_fold = {};
+  auto fold = [&](const Fold& one, const Fold& two, const Fold& three) -> int32_t {
+    const int64_t entries = one.rows * one.width + two.rows * two.width + three.rows * three.width;
+    k_lincat_fold<<<gjx_grid_for(entries), GJX_BLOCK, 0, s>>>(one, two, three);
     GJX_LAUNCH_CHECK();
     return GJX_OK;
   };
@@ -1443,7 +1460,7 @@ GJX_API int32_t gjx_linear_categorical_grad(int32_t dtype, const int32_t* d_y, c
     }
     if (d_db) {
       db_fold = {db_part, db_parts, p.piece, 1, rows, rows, (char*)d_db + v0 * (f32 ? 4 : 2), !f32, nullptr, nullptr, nullptr, 0, 0};
-      if (!whole && (rc = fold(db_fold, Fold{})) != GJX_OK) return rc;
+      if (!whole && (rc = fold(db_fold, Fold{}, Fold{})) != GJX_OK) return rc;
     }
     if (d_dx) {                                              // dx^T = W^T dl^T: m = feature, n = row, over the piece
       GemmArgs b = common_args(c, p);
@@ -1474,9 +1491,19 @@ GJX_API int32_t gjx_linear_categorical_grad(int32_t dtype, const int32_t* d_y, c
       b.nt = (int)(f32 ? up(rows, 128) / 128 : rows_pad / 256);
       b.out = f32 ? (void*)((float*)d_dw + v0 * width) : (void*)((bf16*)d_dw + v0 * width);
       b.out_ld = width;
+      b.out_bf16 = !f32;
+      if (p.splits_w > 1) {                                  // (one piece)
+        float* part = (float*)(ws + p.o_dw);
+        const int64_t ld = up(width, 4);
+        b.splits = p.splits_w;
+        b.out = part;
+        b.out_ld = ld;
+        b.out_split = vocab * ld;
+        b.out_bf16 = 0;
+        dw_fold = {part, p.splits_w, vocab * ld, vocab, ld, width, d_dw, !f32, nullptr, nullptr, nullptr, 0, 0};
+      }
       b.out_m = (int)width;
       b.out_n = (int)rows;
-      b.out_bf16 = !f32;
       b.resid_in = resid;
       b.v0 = v0;
       if ((rc = launch<true, true, EPI_STORE>(c, true, b, s)) != GJX_OK) return rc;
@@ -1485,6 +1512,6 @@ GJX_API int32_t gjx_linear_categorical_grad(int32_t dtype, const int32_t* d_y, c
   if (d_dx && !dx_direct)
     dx_fold = {dx_part, p.splits, n * part_ld, n, part_ld, width, d_dx, !f32, resid, d_y, (const bf16*)d_w, w_ld, vocab};
   if (!whole) db_fold = {};                                  // (done piece by piece)
-  if (dx_fold.out || db_fold.out) return fold(dx_fold, db_fold);
+  if (dx_fold.out || db_fold.out || dw_fold.out) return fold(dx_fold, db_fold, dw_fold);
   return GJX_OK;
 }

@@ -385,3 +385,15 @@ def test_two_backwards_and_a_large_shift(G):
     P = torch.softmax(x.double() @ w.double().t() + b.double(), 1) * up.double().abs().unsqueeze(1) * 2.0 ** -14
     for name, got, more in zip(("dx", "dw", "db"), one, (P @ w.double().abs(), P.t() @ x.double().abs(), P.sum(0))):
         _close(name, got, (t[name][0], t[name][1] + more))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("n,vocab,width", [(1500, 7, 96), (700, 300, 500), (4000, 1, 33), (1000, 2000, 64)])
+def test_many_rows_of_few_values(G, n, vocab, width, dtype):
+    """The rows of dW's sums shared out over workgroups, many of them with the same value."""
+    x, w, b, y, up = _inputs(n, vocab, width, TYPES[dtype])
+    t = _truth(x, w, b, y, up)
+    one = _grads(G, x, w, b, y, up)
+    for name, got, again in zip(("lp", "dx", "dw", "db"), one, _grads(G, x, w, b, y, up)):
+        _close(name, got, t[name])
+        assert torch.equal(got, again)
