@@ -1023,11 +1023,12 @@ __global__ void __launch_bounds__(TEAM, 2)
 // ---------------------------------------------------------------------------
 // gradients of q, k and the gates, all chunks at once
 // ---------------------------------------------------------------------------
-// Eight waves: wave w forms the rows of tokens [16 (w % 4), + 16) and the dk half w / 4.  Per 32 columns of dv, S0, dS1, e,
-// delta and dO become fragment planes in LDS once, for all waves (each wave splitting its own operands: 380 us for 1024
+// Sixteen waves: wave w forms the rows of tokens [16 (w % 4), + 16) and the dk quarter w / 4.  Per 32 columns of dv, S0, dS1,
+// e, delta and dO become fragment planes in LDS once, for all waves (each wave splitting its own operands: 380 us for 1024
 // chunks of 64 x 128 x 128), while the next columns are on their way to registers; the row sums <dS1, S0> and e.delta
-// fall out of the same registers.
-constexpr int BACK = 512;
+// fall out of the same registers.  E and F go to LDS as fragments of themselves and of their transposes, split once.
+// (Eight waves of twice the work, 194 registers: 129 us instead of 113 for them; the phases of one workgroup hardly overlapped.)
+constexpr int BACK = 1024;
 
 // eight values from LDS to a row, in vectors of 16 bytes where it is whole and aligned
 template <typename T>
@@ -1050,19 +1051,19 @@ __device__ __forceinline__ void store8(T* to, const float* x, int n, int vec) {
 }
 
 template <typename T, int DKP, int NPI>
-__global__ void __launch_bounds__(BACK, 2)
+__global__ void __launch_bounds__(BACK)
     k_delta_back(Shape sh, const T* __restrict__ d_o, const float* __restrict__ g, const int32_t* __restrict__ lengths,
                  T* __restrict__ dq, T* __restrict__ dk, float* __restrict__ dg, float* __restrict__ dbeta, Work w, int vec_o, int vec_out) {
   typedef KeyBlock<DKP, NPI> KB;
-  constexpr int MT = DKP / 16, MH = MT / 2;               // tiles of dk; of one wave
+  constexpr int MT = DKP / 16, MH = MT / 4;               // tiles of dk; of one wave
   constexpr int F_S0 = 0, F_S1 = MT * 3 * FRAG, F_E = 2 * F_S1, F_D = F_E + 12 * FRAG, F_O = F_D + 12 * FRAG, F_ALL = F_O + 4 * NPI * FRAG;
+  constexpr int E_ROW = 0, F_ROW = 24 * FRAG, E_COL = 48 * FRAG, F_COL = 72 * FRAG, EF_ALL = 96 * FRAG;     // [tile][slab][plane]
   constexpr int LO = DKP + 4;                             // row of dq or dk in LDS: the four quads of a wave miss each other's banks
-  constexpr int MATRICES = 2 * C * LD * 4, RESULTS = 2 * C * LO * 4;
-  __shared__ __attribute__((aligned(16))) char buffer[std::max(F_ALL * 2, std::max(MATRICES, RESULTS))];
-  __shared__ float s_gh[C], s_gl[C], s_row[2][C], s_db[C], s_put[8];
-  __shared__ double s_sum[8];
+  constexpr int RESULTS = 2 * C * LO * 4;
+  __shared__ __attribute__((aligned(16))) char buffer[std::max(std::max(F_ALL, EF_ALL) * 2, RESULTS)];
+  __shared__ float s_gh[C], s_gl[C], s_row[4][C], s_db[C], s_put[16];
+  __shared__ double s_sum[16];
   bf16* frag = (bf16*)buffer;
-  float *se = (float*)buffer, *sf = se + C * LD;          // E and F, once the fragments are used up
   float *sq = (float*)buffer, *sk = sq + C * LO;          // dq and dk, once E and F are
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quad = lane >> 4, c = lane & 15;
   const int wt = wave & 3, wh = wave >> 2;
@@ -1102,81 +1103,68 @@ __global__ void __launch_bounds__(BACK, 2)
     s_gl[lane] = (float)(gam - (double)(float)gam);
   }
 
-  // this thread's pieces of a slab: eight columns of one row of S0 and dS1, and of e and delta (first half) or dO
-  const int row = tid >> 2, sub = tid & 3;                // 128 rows
+  // this thread's pieces of a slab: four columns of one row of S0 and dS1, and of e and delta (first half) or dO
+  const int row = tid >> 3, sub = tid & 7;                // 128 rows
   const bool has_state = row < DKP;
-  const bool first = tid < 256;
+  const bool first = tid < 512;
   const int trow = row & 63;
-  const float *p_s0 = w.s0 + (at * DKP + min(row, DKP - 1)) * sh.dvp + 8 * sub, *p_s1 = w.ds1 + (at * DKP + min(row, DKP - 1)) * sh.dvp + 8 * sub;
-  const float *p_e = w.e + (at * C + trow) * sh.dvp + 8 * sub, *p_d = w.delta + (at * C + trow) * sh.dvp + 8 * sub;
+  const float *p_s0 = w.s0 + (at * DKP + min(row, DKP - 1)) * sh.dvp + 4 * sub, *p_s1 = w.ds1 + (at * DKP + min(row, DKP - 1)) * sh.dvp + 4 * sub;
+  const float *p_e = w.e + (at * C + trow) * sh.dvp + 4 * sub, *p_d = w.delta + (at * C + trow) * sh.dvp + 4 * sub;
   const T* p_o = d_o + ((b * sh.time + t0 + min(trow, left - 1)) * sh.heads + h) * sh.dv;
-  float x0[8], x1[8], x2[8], x3[8];
-  auto load8 = [](const float* p, float (&x)[8]) {
-    const f32x4 a = *(const f32x4*)p, z = *(const f32x4*)(p + 4);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      x[j] = a[j];
-      x[4 + j] = z[j];
-    }
-  };
+  f32x4 x0, x1, x2, x3;
   auto load = [&](int s) {
-    load8(p_s0 + 32 * s, x0);
-    load8(p_s1 + 32 * s, x1);
+    x0 = *(const f32x4*)(p_s0 + 32 * s);
+    x1 = *(const f32x4*)(p_s1 + 32 * s);
     if (first) {
-      load8(p_e + 32 * s, x2);
-      load8(p_d + 32 * s, x3);
+      x2 = *(const f32x4*)(p_e + 32 * s);
+      x3 = *(const f32x4*)(p_d + 32 * s);
     } else {
-      const int c0 = 32 * s + 8 * sub;
-      if (vec_o && c0 + 8 <= sh.dv) {
-        typedef T vec8 __attribute__((ext_vector_type(8)));
-        const vec8 v = *(const vec8*)(p_o + c0);
+      const int c0 = 32 * s + 4 * sub;
+      if (vec_o && c0 + 4 <= sh.dv) {
+        typedef T vec4 __attribute__((ext_vector_type(4)));
+        const vec4 v = *(const vec4*)(p_o + c0);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x2[j] = (float)v[j];
+        for (int j = 0; j < 4; ++j) x2[j] = (float)v[j];
       } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x2[j] = c0 + j < sh.dv ? (float)p_o[c0 + j] : 0.0f;
+        for (int j = 0; j < 4; ++j) x2[j] = c0 + j < sh.dv ? (float)p_o[c0 + j] : 0.0f;
       }
     }
   };
-  auto put8 = [&](int base, int planes, int r, const float (&x)[8]) {
-    bf16* f = frag + base + (r >> 4) * planes * FRAG + ((r & 15) + 16 * sub) * 8;
-    if (planes == 3) {
-      bf16x8 o3[3];
-      split<3>(x, o3);
+  auto put4 = [&](int base, int planes, int r, f32x4 v) {
+    bf16* f = frag + base + (r >> 4) * planes * FRAG + ((r & 15) + 16 * (sub >> 1)) * 8 + (sub & 1) * 4;
+    float x[4] = {v[0], v[1], v[2], v[3]};
+    bf16 h[4];
 #pragma unroll
-      for (int p = 0; p < 3; ++p) *(bf16x8*)(f + p * FRAG) = o3[p];
-    } else {
-      bf16x8 o1[1];
-      split<1>(x, o1);
-      *(bf16x8*)f = o1[0];
-    }
+    for (int p = 0; p < 3; ++p)
+      if (p < planes) {
+        if (planes == 3) split_planes<3, 4>(x, p, h);
+        else split_planes<1, 4>(x, p, h);
+        *(bf16x4*)(f + p * FRAG) = bf16x4{h[0], h[1], h[2], h[3]};
+      }
   };
 
-  f32x4 m1[MH], m2[MH], m3[MH], pe[2], pf[2];
+  f32x4 m1[MH], m2[MH], m3[MH], pe = {0, 0, 0, 0}, pf = {0, 0, 0, 0};
 #pragma unroll
   for (int t = 0; t < MH; ++t) m1[t] = m2[t] = m3[t] = f32x4{0, 0, 0, 0};
-#pragma unroll
-  for (int j = 0; j < 2; ++j) pe[j] = pf[j] = f32x4{0, 0, 0, 0};
   float dot = 0.0f, db = 0.0f;
   const int slabs = sh.dvp / 32;
   load(0);
   for (int s = 0; s < slabs; ++s) {
     if (has_state) {
-      put8(F_S0, 3, row, x0);
-      put8(F_S1, 3, row, x1);
+      put4(F_S0, 3, row, x0);
+      put4(F_S1, 3, row, x1);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) dot += x0[j] * x1[j];
+      for (int j = 0; j < 4; ++j) dot += x0[j] * x1[j];
     }
     if (first) {
-      put8(F_E, 3, trow, x2);
-      put8(F_D, 3, trow, x3);
+      put4(F_E, 3, trow, x2);
+      put4(F_D, 3, trow, x3);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) db += x2[j] * x3[j];
+      for (int j = 0; j < 4; ++j) db += x2[j] * x3[j];
     } else {
-      if (trow >= left)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x2[j] = 0.0f;
-      put8(F_O, NPI, trow, x2);
+      if (trow >= left) x2 = f32x4{0, 0, 0, 0};
+      put4(F_O, NPI, trow, x2);
     }
     __syncthreads();
     if (s + 1 < slabs) load(s + 1);
@@ -1193,14 +1181,12 @@ __global__ void __launch_bounds__(BACK, 2)
       m2[t] = mma_planes<3, 3, 3>(fe, f0, m2[t]);
       m3[t] = mma_planes<3, 3, 3>(fd, f1, m3[t]);
     }
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-      if (2 * wh + j <= wt) {
-        bf16x8 fj[3];
-        get_frag<3>(frag + F_D + (2 * wh + j) * 3 * FRAG, lane, fj);
-        pe[j] = mma_planes<NPI, 3, 3>(fo, fj, pe[j]);
-        pf[j] = mma_planes<3, 3, 3>(fe, fj, pf[j]);
-      }
+    if (wh <= wt) {
+      bf16x8 fj[3];
+      get_frag<3>(frag + F_D + wh * 3 * FRAG, lane, fj);
+      pe = mma_planes<NPI, 3, 3>(fo, fj, pe);
+      pf = mma_planes<3, 3, 3>(fe, fj, pf);
+    }
     __syncthreads();
   }
   {
@@ -1210,84 +1196,102 @@ __global__ void __launch_bounds__(BACK, 2)
     if (lane == 0) s_sum[wave] = d;
     db += __shfl_xor(db, 1);
     db += __shfl_xor(db, 2);
+    db += __shfl_xor(db, 4);
     if (first && sub == 0) s_db[trow] = db;
   }
-#pragma unroll
-  for (int j = 0; j < 2; ++j)
+  {
+    f32x4 ev, fv;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int i = 16 * wt + 4 * quad + r, jj = 16 * (2 * wh + j) + c;
+      const int i = 16 * wt + 4 * quad + r, jj = 16 * wh + c;
       const float d = jj <= i ? expf((s_gh[i] - s_gh[jj]) + (s_gl[i] - s_gl[jj])) * rb[jj] : 0.0f;
-      se[i * LD + jj] = jj <= i ? sh.scale * d * pe[j][r] : 0.0f;
-      sf[i * LD + jj] = jj < i ? -rb[i] * d * pf[j][r] : 0.0f;
+      ev[r] = jj <= i ? sh.scale * d * pe[r] : 0.0f;
+      fv[r] = jj < i ? -rb[i] * d * pf[r] : 0.0f;
     }
+    // their transposes (rows of the operand: jj; reduction: i) as they lie in the registers; themselves entry by entry
+    put_half<3>(frag + E_COL + (wh * 2 + (wt >> 1)) * 3 * FRAG, wt & 1, lane, ev);
+    put_half<3>(frag + F_COL + (wh * 2 + (wt >> 1)) * 3 * FRAG, wt & 1, lane, fv);
+    bf16* at_row = frag + (wt * 2 + (wh >> 1)) * 3 * FRAG + (4 * quad + 16 * (c >> 2)) * 8 + 4 * (wh & 1) + (c & 3);
+    float xe[4] = {ev[0], ev[1], ev[2], ev[3]}, xf[4] = {fv[0], fv[1], fv[2], fv[3]};
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+      bf16 he[4], hf[4];
+      split_planes<3, 4>(xe, p, he);
+      split_planes<3, 4>(xf, p, hf);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        at_row[E_ROW + p * FRAG + r * 8] = he[r];
+        at_row[F_ROW + p * FRAG + r * 8] = hf[r];
+      }
+    }
+  }
   const f32x4 be = *(const f32x4*)(rb + 16 * wt + 4 * quad), eg = *(const f32x4*)(rb + C + 16 * wt + 4 * quad);
   const f32x4 rest = *(const f32x4*)(rb + 2 * C + 16 * wt + 4 * quad);
   __syncthreads();
 
-  const int tok = 16 * wt + c;                            // this lane's row of the operands E, F (column: their transposes)
-  // E and F as rows, then as columns: half the fragments live at a time
-  auto rows_of = [&](const float* m, bool trans, bf16x8 (&out)[2][3]) {
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      float x[8];
+  for (int t = 0; t < MH; ++t) {
+    m1[t] *= eg * sh.scale;
+    m2[t] *= -(be * eg);
+    m3[t] *= be * rest;
+  }
+  f32x4 last[MH];
+  float qv[MH][4], kv[MH][4];                             // q and k where dq and dk are: entries of the fragments at hand
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = trans ? m[perm(s, quad, j) * LD + tok] : m[tok * LD + perm(s, quad, j)];
-      split<3>(x, out[s]);
-    }
-  };
-  {
-    bf16x8 fe[2][3], ff[2][3];
-    rows_of(se, false, fe);
-    rows_of(sf, false, ff);
+  for (int t = 0; t < MH; ++t) last[t] = m3[t];
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    bf16x8 kt[MH][NPI], qt[MH][NPI];
 #pragma unroll
     for (int t = 0; t < MH; ++t) {
-      m1[t] *= eg * sh.scale;
-      m2[t] *= -(be * eg);
+      load_frag<NPI>(kb + KB::KT, (wh * MH + t) * 2 + s, MT * 2 * FRAG, lane, kt[t]);
+      load_frag<NPI>(kb + KB::QT, (wh * MH + t) * 2 + s, MT * 2 * FRAG, lane, qt[t]);
+    }
+    if (s <= wt >> 1) {                                   // (E and F are lower triangular)
+      bf16x8 fe[3], ff[3];
+      get_frag<3>(frag + E_ROW + (wt * 2 + s) * 3 * FRAG, lane, fe);
+      get_frag<3>(frag + F_ROW + (wt * 2 + s) * 3 * FRAG, lane, ff);
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        bf16x8 kt[NPI];
-        load_frag<NPI>(kb + KB::KT, (wh * MH + t) * 2 + s, MT * 2 * FRAG, lane, kt);
-        m1[t] = mma_planes<3, NPI, 3>(fe[s], kt, m1[t]);
-        m2[t] = mma_planes<3, NPI, 3>(ff[s], kt, m2[t]);
+      for (int t = 0; t < MH; ++t) {
+        m1[t] = mma_planes<3, NPI, 3>(fe, kt[t], m1[t]);
+        m2[t] = mma_planes<3, NPI, 3>(ff, kt[t], m2[t]);
       }
     }
-    __builtin_amdgcn_sched_barrier(0);
+    if (s >= wt >> 1) {
+      bf16x8 fe[3], ff[3];
+      get_frag<3>(frag + E_COL + (wt * 2 + s) * 3 * FRAG, lane, fe);
+      get_frag<3>(frag + F_COL + (wt * 2 + s) * 3 * FRAG, lane, ff);
+#pragma unroll
+      for (int t = 0; t < MH; ++t) {
+        m3[t] = mma_planes<3, NPI, 3>(fe, qt[t], m3[t]);
+        m3[t] = mma_planes<3, NPI, 3>(ff, kt[t], m3[t]);
+      }
+    }
+    if (s == wt >> 1)
+#pragma unroll
+      for (int t = 0; t < MH; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          qv[t][r] = kv[t][r] = 0.0f;
+#pragma unroll
+          for (int p = NPI - 1; p >= 0; --p) {
+            qv[t][r] += (float)(wt & 1 ? qt[t][p][4 + r] : qt[t][p][r]);
+            kv[t][r] += (float)(wt & 1 ? kt[t][p][4 + r] : kt[t][p][r]);
+          }
+        }
   }
-  bf16x8 fe[2][3], ff[2][3];
-  rows_of(se, true, fe);
-  rows_of(sf, true, ff);
-  __syncthreads();
+  __syncthreads();                                        // the fragments of E and F are used up
   f32x4 sum = {0, 0, 0, 0}, put = {0, 0, 0, 0};
 #pragma unroll
   for (int t = 0; t < MH; ++t) {
-    const int tile = wh * MH + t, col = 16 * tile + c;
-    f32x4 aw = m3[t] * be * rest;
-    const f32x4 last = aw, aq = m1[t], ar = m2[t];
-    float qv[4] = {0, 0, 0, 0}, kv[4] = {0, 0, 0, 0};     // q and k where dq and dk are: entries of the fragments at hand
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      bf16x8 kt[NPI], qt[NPI];
-      load_frag<NPI>(kb + KB::KT, tile * 2 + s, MT * 2 * FRAG, lane, kt);
-      load_frag<NPI>(kb + KB::QT, tile * 2 + s, MT * 2 * FRAG, lane, qt);
-      aw = mma_planes<3, NPI, 3>(fe[s], qt, aw);
-      aw = mma_planes<3, NPI, 3>(ff[s], kt, aw);
-      if (s == wt >> 1)
-#pragma unroll
-        for (int p = NPI - 1; p >= 0; --p)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            qv[r] += (float)(wt & 1 ? qt[p][4 + r] : qt[p][r]);
-            kv[r] += (float)(wt & 1 ? kt[p][4 + r] : kt[p][r]);
-          }
-    }
+    const int col = 16 * (wh * MH + t) + c;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int i = 16 * wt + 4 * quad + r;               // (tokens behind the end and columns behind dk: q, k, E, F are 0)
-      sum[r] += qv[r] * aq[r] + kv[r] * (ar[r] - aw[r]);
-      put[r] += kv[r] * last[r];
-      sq[i * LO + col] = i < left ? aq[r] : 0.0f;
-      sk[i * LO + col] = i < left ? ar[r] + aw[r] : 0.0f;
+      sum[r] += qv[t][r] * m1[t][r] + kv[t][r] * (m2[t][r] - m3[t][r]);
+      put[r] += kv[t][r] * last[t][r];
+      sq[i * LO + col] = i < left ? m1[t][r] : 0.0f;
+      sk[i * LO + col] = i < left ? m2[t][r] + m3[t][r] : 0.0f;
     }
   }
   float all = put[0] + put[1] + put[2] + put[3];
@@ -1302,8 +1306,8 @@ __global__ void __launch_bounds__(BACK, 2)
     if (c == 0) s_row[wh][16 * wt + 4 * quad + r] = s;
   }
   __syncthreads();
-  // out of LDS in rows: pieces of eight columns (stored from the accumulators, two bytes a lane: 138 us instead of 70 for
-  // the 1024 chunks)
+  // out of LDS in rows: pieces of eight columns (stored from the accumulators, two bytes a lane, the kernel took 139 us instead
+  // of 129 for the 1024 chunks)
   for (int u = tid; u < 2 * left_o * (DKP / 8); u += BACK) {
     const bool is_k = u >= left_o * (DKP / 8);
     const int v = is_k ? u - left_o * (DKP / 8) : u, i = v / (DKP / 8), c0 = v % (DKP / 8) * 8;
@@ -1315,7 +1319,7 @@ __global__ void __launch_bounds__(BACK, 2)
     else store8((is_k ? dk : dq) + p, x, n, vec_out);
   }
   if (wave == 0) {
-    double s = (double)s_row[0][lane] + (double)s_row[1][lane];
+    double s = (double)s_row[0][lane] + (double)s_row[1][lane] + (double)s_row[2][lane] + (double)s_row[3][lane];
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
       const double down = __shfl_down(s, o);
@@ -1323,7 +1327,7 @@ __global__ void __launch_bounds__(BACK, 2)
     }
     double end = 0.0, written = 0.0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 16; ++i) {
       end += s_sum[i];
       written += (double)s_put[i];
     }
