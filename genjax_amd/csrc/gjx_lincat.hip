@@ -1324,8 +1324,8 @@ int32_t forward(const Call& c, const Plan& p, const Forward& f, void* d_work, in
     }
   }
   if (EPI != EPI_DRAW) {
-    int cols = 1;                                            // 16 rows x 16 parts of the tiles per workgroup
-    while (cols < 16 && cols < c.n) cols *= 2;
+    int cols = 16;                                           // rows per workgroup; fewer where that fills more CUs
+    while (cols > 1 && up(c.n, cols) / cols < 256) cols /= 2;
     k_lincat_combine<<<(unsigned)(up(c.n, cols) / cols), GJX_BLOCK, 0, s>>>(a.part, (int)p.tiles, p.n_pad, c.n, cols, a.target, f.lp, f.lse,
                                                                                f.kept ? (float*)(f.kept + kept.o_lp) : nullptr);
   } else {

@@ -134,8 +134,10 @@ class _LinearCategoricalFn(torch.autograd.Function):
 
 class _LinearCategorical(Distribution):
     """linear_categorical(x, weight, bias=None): a draw from softmax(x W^T + b) per row.  x: (n, width) rows or one
-    (width,) row shared by every particle; weight: (vocab, width); bias: (vocab,).  All float32 or all bfloat16;
-    sums and log-densities are float32.  Differentiable in x, weight and bias."""
+    (width,) row shared by every particle; weight: (vocab, width); bias: (vocab,).  All float32 or all bfloat16 and
+    finite, the bias or -inf (its entry is never drawn and has the log-density -inf); sums and log-densities are
+    float32.  Differentiable in x, weight and bias; above 32 rows and small widths the forward of a gradient keeps up
+    to 2 GiB for it (the exponentials of all logits), and what would take more is formed again."""
 
     def _param_event_ndims(self, a):
         return a.dim() if isinstance(a, torch.Tensor) else 0
@@ -166,7 +168,9 @@ class _LinearCategorical(Distribution):
         if y.dim() == 1 and y.numel() not in (1, n):
             raise B.GjxError(f"linear_categorical: {y.numel()} values against {n} rows of x")
         scalar = y.dim() == 0 and x.dim() == 1
-        rows, ys = self._rows(x, n), y.to(torch.int32)
+        if y.dtype != torch.int32 and weight.dim() == 2:        # outside the vocabulary: the nearest entry, in 64 bits too
+            y = y.long().clamp(0, max(weight.shape[0] - 1, 0)).to(torch.int32)
+        rows, ys = self._rows(x, n), y
         if ys.shape != (n,):
             ys = ys.reshape(-1).expand(n)
         if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):

@@ -397,3 +397,11 @@ def test_many_rows_of_few_values(G, n, vocab, width, dtype):
     for name, got, again in zip(("lp", "dx", "dw", "db"), one, _grads(G, x, w, b, y, up)):
         _close(name, got, t[name])
         assert torch.equal(got, again)
+
+
+@pytest.mark.parametrize("dtype", [torch.int64, torch.float32, torch.uint8])
+def test_values_of_other_types(G, dtype):
+    x, w, b, y, _ = _inputs(6, 9, 16, torch.float32)
+    far = torch.tensor([-5, 0, 8, 9, 2 ** 32 + 3, -2 ** 40] if dtype == torch.int64 else [0, 1, 2, 8, 9, 200], device="cuda").to(dtype)
+    near = far.long().clamp(0, 8).to(torch.int32)
+    assert torch.equal(G.linear_categorical.logpdf(far, x, w, b), G.linear_categorical.logpdf(near, x, w, b))
