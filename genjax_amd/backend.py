@@ -93,8 +93,11 @@ def _rows(t: torch.Tensor | None):
 def _raw_stream() -> int:
     """The current device's current stream as the raw hipStream_t (torch.cuda.current_stream() builds a Stream
     object and resolves the device through several Python layers: ~9 us, eight times per SMC stage)."""
-    return _RAW_STREAM(torch.cuda.current_device())
+    return _RAW_STREAM(_CURRENT_DEVICE())
 
+
+# (a tensor on a GPU exists where this is called, so torch's lazy initialisation is behind us)
+_CURRENT_DEVICE = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 _RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
@@ -448,7 +451,7 @@ def _on_current_device(who, *tensors):
         if not isinstance(t, torch.Tensor) or not t.is_cuda:
             raise GjxError(f"{who}: `{name}` must be a device tensor")
         if cur is None:
-            cur = torch.cuda.current_device()
+            cur = _CURRENT_DEVICE()
         if t.get_device() != cur:
             raise GjxError(f"{who}: `{name}` lives on {t.device} but the current device is cuda:{cur}: launches "
                            "go to the current device's stream (use torch.cuda.set_device / torch.cuda.device)")
@@ -618,10 +621,11 @@ def mvnormal_logpdf(x, mu, cov):
 class _DeltaPlan:
     """A checked set of shapes and strides as the library takes it, with its workspace sizes."""
 
-    __slots__ = ("shape", "ref", "batch", "time", "heads", "dk", "dv", "_bytes")
+    __slots__ = ("shape", "ref", "batch", "time", "heads", "dk", "dv", "spans", "_bytes")
 
-    def __init__(self, shape):
+    def __init__(self, shape, spans):
         self.shape, self.ref = shape, C.byref(shape)
+        self.spans = spans                                      # bytes from the first entry of q, k, v, the gates to the last's end
         self.batch, self.time, self.heads, self.dk, self.dv = shape.batch, shape.time, shape.heads, shape.dk, shape.dv
         self._bytes = {}
 
@@ -652,9 +656,11 @@ def _delta_plan(who, dtypes, q_shape, k_shape, v_shape, g_shape, b_shape, q_stri
     if dtypes[3] != torch.float32 or dtypes[4] != torch.float32:
         raise GjxError(f"{who}: log_decay and beta must be float32 (got {dtypes[3]}, {dtypes[4]})")
     three = C.c_int64 * 3
+    span = lambda t, shape, stride: t.itemsize * (1 + sum((n - 1) * s for n, s in zip(shape, stride))) if min(shape) > 0 else 0      # noqa: E731
+    spans = tuple(map(span, dtypes, (q_shape, k_shape, v_shape, g_shape, b_shape), (q_stride, k_stride, v_stride, g_stride, b_stride)))
     return _DeltaPlan(N.DeltaShape(ELEMENT_TYPES[dtypes[0]], kheads, heads, dk, dv, float(dk ** -0.5 if scale is None else scale),
                                    batch, time, three(*q_stride[:3]), three(*k_stride[:3]), three(*v_stride[:3]),
-                                   three(*g_stride), three(*b_stride)))
+                                   three(*g_stride), three(*b_stride)), spans)
 
 
 def _delta_inputs(who, q, k, v, log_decay, beta, scale):
@@ -673,22 +679,24 @@ def _delta_inputs(who, q, k, v, log_decay, beta, scale):
     return plan, t
 
 
-def _delta_state(who, name, state, p):
-    """A (batch, heads, dk, dv) float32 state, contiguous."""
+def _delta_state(who, name, state, p, here=True):
+    """A (batch, heads, dk, dv) float32 state, contiguous (here: on the current device)."""
     if state is None:
         return None
     if not isinstance(state, torch.Tensor) or state.shape != (p.batch, p.heads, p.dk, p.dv) or state.dtype != torch.float32:
         raise GjxError(f"{who}: `{name}` must be float32 of shape {(p.batch, p.heads, p.dk, p.dv)}")
-    _on_current_device(who, (name, state))
+    if here:
+        _on_current_device(who, (name, state))
     return state.contiguous()
 
 
-def _delta_indices(who, name, t, p):
+def _delta_indices(who, name, t, p, here=True):
     if t is None:
         return None
     if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.shape != (p.batch,):
         raise GjxError(f"{who}: `{name}` must be int32 of shape ({p.batch},)")
-    _on_current_device(who, (name, t))
+    if here:
+        _on_current_device(who, (name, t))
     return t.contiguous()
 
 
@@ -725,14 +733,6 @@ def delta_filter_grad(q, k, v, log_decay, beta, d_o, d_state, kept, scale=None, 
     return outs + [state0]
 
 
-def _overlap(a, b):
-    """Whether the address ranges of two tensors meet (strided ones count from their first entry to their last)."""
-    if a.numel() == 0 or b.numel() == 0:
-        return False
-    end = lambda t: t.data_ptr() + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()     # noqa: E731
-    return a.data_ptr() < end(b) and b.data_ptr() < end(a)
-
-
 @functools.lru_cache(maxsize=1024)
 def _delta_step_plan(dtypes, q_shape, k_shape, v_shape, g_shape, b_shape, q_stride, k_stride, v_stride, g_stride, b_stride, scale):
     who = "delta_filter_step"
@@ -759,8 +759,9 @@ def delta_filter_step(state, q, k, v, log_decay, beta, scale=None, ancestors=Non
                          None if scale is None else float(scale))
     if state is None:
         raise GjxError(f"{who}: `state` must be float32 of shape {(p.batch, p.heads, p.dk, p.dv)}")
-    state, ancestors = _delta_state(who, "state", state, p), _delta_indices(who, "ancestors", ancestors, p)
-    _on_current_device(who, ("q", q), ("k", k), ("v", v), ("log_decay", log_decay), ("beta", beta))
+    state, ancestors = _delta_state(who, "state", state, p, here=False), _delta_indices(who, "ancestors", ancestors, p, here=False)
+    _on_current_device(who, ("q", q), ("k", k), ("v", v), ("log_decay", log_decay), ("beta", beta), ("state", state),
+                       ("ancestors", ancestors), ("out", out))
     if out is None:
         if state.data_ptr() & 15:                               # a view into the middle of a buffer
             state = state.clone()
@@ -768,11 +769,14 @@ def delta_filter_step(state, q, k, v, log_decay, beta, scale=None, ancestors=Non
     else:
         if not isinstance(out, torch.Tensor) or out.shape != state.shape or out.dtype != torch.float32 or not out.is_contiguous():
             raise GjxError(f"{who}: `out` must be contiguous float32 of shape {tuple(state.shape)}")
-        _on_current_device(who, ("out", out))
-        if _overlap(out, state) and (ancestors is not None or out.data_ptr() != state.data_ptr()):
+        lo = out.data_ptr()
+        size = out.numel() * 4
+        if lo < state.data_ptr() + size and state.data_ptr() < lo + size and (ancestors is not None or lo != state.data_ptr()):
             raise GjxError(f"{who}: `out` may be the state itself without ancestors and must not overlap it otherwise")
-        for name, t in (("q", q), ("k", k), ("v", v), ("log_decay", log_decay), ("beta", beta), ("ancestors", ancestors)):
-            if t is not None and _overlap(out, t):
+        spans = p.spans if ancestors is None else (*p.spans, 4 * p.batch)
+        for name, t, span in zip(("q", "k", "v", "log_decay", "beta", "ancestors"), (q, k, v, log_decay, beta, ancestors), spans):
+            at = t.data_ptr()
+            if lo < at + span and at < lo + size:
                 raise GjxError(f"{who}: `out` must not overlap `{name}`")
     from_, to = state.data_ptr(), out.data_ptr()
     if (from_ | to) & 15:

@@ -291,3 +291,102 @@ def test_step_takes_states_inside_a_buffer_and_refuses_outputs_over_inputs(G):
     q, k, v, g, beta = m.inputs(tok)
     with pytest.raises(G.GjxError, match="must not overlap `v`"):
         delta_filter_step(m.state(2), q, k, v, g, beta, out=v.view(2, 1, 1, 1))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_two_graphs_of_a_fit_that_keeps(G, dtype):
+    """Captured log-density and gradient over what the forward keeps: two graphs, replayed in turn with eager calls between."""
+    from genjax_amd import backend as B
+
+    t = {"bf16": torch.bfloat16, "f32": torch.float32}[dtype]
+    sets = []
+    for i, (n, vocab, width) in enumerate(((100, 700, 512), (65, 3000, 576))):
+        gen = torch.Generator("cuda").manual_seed(i)
+        x = torch.randn(n, width, device="cuda", generator=gen).to(t)
+        w = (torch.randn(vocab, width, device="cuda", generator=gen) / width ** 0.5).to(t)
+        y = torch.randint(0, vocab, (n,), device="cuda", generator=gen, dtype=torch.int32)
+        up = torch.ones(n, device="cuda")
+
+        def call(x=x, w=w, y=y, up=up):
+            lp, lse, kept = B.linear_categorical_logpdf(y, x, w, keep=True)
+            assert kept is not None
+            return [lp, lse] + B.linear_categorical_grad(y, x, w, None, lse, up, want=(True, True, False), kept=kept)[:2]
+
+        call()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = call()
+        sets.append((graph, outs, call, x))
+    for turn in range(4):
+        for graph, outs, call, x in sets:
+            x.copy_(torch.randn(x.shape, device="cuda", generator=torch.Generator("cuda").manual_seed(turn)))
+            graph.replay()
+            want = call()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+def test_two_threads_on_streams_of_their_own(G):
+    """Training steps of two host threads, each on its own stream, give the bits of the same steps one after the other."""
+    import threading
+
+    from genjax_amd.families.state_space import delta_filter
+
+    models = [_Model(seed=4, dk=64, dv=64), _Model(seed=5, vocab=90, kheads=2, heads=2, dk=30, dv=33)]
+    data = [_sequences(m, 2, 150, seed=i) for i, m in enumerate(models)]
+
+    def step(m, y):
+        leaves = [t.clone().requires_grad_(True) for t in (*m.inputs(y[:, :-1]), m.w, m.b)]
+        o, last = delta_filter(*leaves[:5])
+        lp = G.linear_categorical.logpdf(y[:, 1:].reshape(-1), o.flatten(2).flatten(0, 1), *leaves[5:])
+        return [lp.detach(), last.detach(), *torch.autograd.grad(lp, leaves, torch.ones_like(lp))]
+
+    want = [step(m, y) for m, y in zip(models, data)]
+    torch.cuda.synchronize()
+    got, failed = [None, None], []
+
+    def work(i):
+        try:
+            stream = torch.cuda.Stream()
+            stream.wait_stream(torch.cuda.default_stream())
+            with torch.cuda.stream(stream):
+                for _ in range(5):
+                    got[i] = step(models[i], data[i])
+            stream.synchronize()
+        except BaseException as e:                               # noqa: BLE001  reported below, on the test's thread
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+    for a, b in zip(got, want):
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_longest_rows_and_widest_states(G):
+    """The documented ends of the ranges: width 65536, one value in the vocabulary; dv = 1024 with dk = 128, 1024 heads."""
+    from genjax_amd.families.state_space import delta_filter, delta_filter_step
+
+    gen = torch.Generator("cuda").manual_seed(0)
+    x, w = (torch.randn(n, 65536, device="cuda", generator=gen) / 256.0 for n in (40, 3))
+    y = torch.randint(0, 3, (40,), device="cuda", generator=gen, dtype=torch.int32)
+    want = torch.log_softmax(x.double() @ w.double().t(), 1).gather(1, y.long()[:, None]).squeeze(1)
+    mag = (x.double().abs() @ w.double().abs().t()).max().item()
+    tol = 2 * 2 * 65536 * 2.0 ** -23 * mag + 2.0 ** -16 + 2.0 ** -20          # a chain of 65536 products in f32, twice
+    assert ((G.linear_categorical.logpdf(y, x, w) - want).abs() <= tol).all()
+    assert torch.equal(G.linear_categorical.logpdf(y, x, w[:1]), torch.zeros(40, device="cuda"))
+    for heads, dk, dv in ((1, 128, 1024), (1024, 8, 4)):
+        q, k = (torch.nn.functional.normalize(torch.randn(1, 3, heads, dk, device="cuda", generator=gen), dim=-1) for _ in range(2))
+        v, g = torch.randn(1, 3, heads, dv, device="cuda", generator=gen), -torch.rand(1, 3, heads, device="cuda", generator=gen)
+        beta = torch.rand(1, 3, heads, device="cuda", generator=gen)
+        o, last = delta_filter(q, k, v, g, beta)
+        state = torch.zeros(1, heads, dk, dv, device="cuda")
+        for t in range(3):
+            one, state = delta_filter_step(state, *(a[:, t] for a in (q, k, v, g, beta)))
+            # each side within 2^-15 of the largest entry (its own tests)
+            assert ((one - o[:, t]).abs().max() <= 2.0 ** -14 * o.abs().max()).item()
+        assert ((state - last).abs().max() <= 2.0 ** -14 * last.abs().max()).item()

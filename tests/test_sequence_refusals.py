@@ -152,12 +152,15 @@ def test_delta_filter_step_refusals():
             S.delta_filter_step(grad, *args, ancestors=ancestors)
 
 
-def test_overlap_of_strided_tensors():
+def test_spans_of_strided_tensors():
+    """What `out` of a step is held against: the bytes from an input's first entry to the end of its last."""
     B = _B()
-    base = torch.zeros(64)
-    assert B._overlap(base[:8], base[7:9]) and not B._overlap(base[:8], base[8:9])
-    assert B._overlap(base[0:20:10], base[10:12]) and not B._overlap(base[0:20:10], base[11:12])
-    assert not B._overlap(base[:0], base) and B._overlap(base[3].expand(5), base[:4])
+    q = torch.zeros(2, 1, 8)
+    v = torch.zeros(2, 2, 9)[:, :, :4]
+    gate = torch.zeros(1, 2).expand(2, 2)
+    p = B._delta_step_plan((torch.float32,) * 5, q.shape, q.shape, v.shape, gate.shape, gate.shape, q.stride(), q.stride(), v.stride(),
+                           gate.stride(), gate.stride(), None)
+    assert p.spans == (64, 64, 4 * (9 * 3 + 4), 8, 8)
 
 
 def _shape(dtype=0, kheads=1, heads=2, dk=8, dv=4, batch=2, time=3, v_token=8):
