@@ -674,7 +674,7 @@ struct SlabLoader {
       where(i, index, group);
       bf16x8 o[3];
       split8(x[i], o);
-      char* f = lds + (index >> 4) * 3072 + (16 * group + ((index + 2 * group) & 15)) * 16;
+      char* f = lds + (index >> 4) * 3072 + (16 * group + ((index & 15) ^ (2 * (group & 1) | (group >> 1) * 12))) * 16;
 #pragma unroll
       for (int p = 0; p < 3; ++p) *(bf16x8*)(f + p * 1024) = o[p];
     }
@@ -682,7 +682,7 @@ struct SlabLoader {
   static __device__ __forceinline__ void frag(const char* lds, int i0, int lane, bf16x8 (&out)[3]) {
     const int q = lane >> 4;
 #pragma unroll
-    for (int p = 0; p < 3; ++p) out[p] = *(const bf16x8*)(lds + (i0 >> 4) * 3072 + p * 1024 + (16 * q + ((lane + 2 * q) & 15)) * 16);
+    for (int p = 0; p < 3; ++p) out[p] = *(const bf16x8*)(lds + (i0 >> 4) * 3072 + p * 1024 + (16 * q + ((lane & 15) ^ (2 * (q & 1) | (q >> 1) * 12))) * 16);
   }
 };
 
