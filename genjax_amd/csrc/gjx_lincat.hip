@@ -690,12 +690,12 @@ struct SlabLoader {
 // LDS traffic are small beside them and no packed copy of the operands is needed (packing to bf16 planes first: pack and
 // product 328 us for 200 x 50001 x 768).  One 32-deep slab in LDS, the next one in registers; three workgroups a CU
 // cover each other's splitting and barriers and leave less idle at the end than one of twice the size.  Bound by the matrix
-// unit (busy 55 % of the time) and by the splitting beside it: 200 x 50001 x 768 in 128 us (the rows padded to 256: 0.92 PFLOP/s
-// of partial products), 1000 x 20011 x 512 in 125 to 148 us per product (0.83 to 0.98).
+// unit (busy 57 % of the time), the splitting beside it and how evenly the tiles fill the CUs: 200 x 50001 x 768 in 100 us (0.92
+// PFLOP/s of partial products), 1000 x 20011 x 512 in 121 to 139 us per product (0.88 to 1.02).
 template <int BN, bool TA, bool TB, int EPI>
-__global__ void __launch_bounds__(GEMM32_THREADS, 3)
+__global__ void __launch_bounds__(GEMM32_THREADS, BN > 128 ? 2 : 3)
     k_lincat_gemm32(GemmArgs g) {
-  constexpr int BM = BM32, WN = 2, WM = 2, MT = BM / WM / 16, NT = BN / WN / 16;
+  constexpr int BM = BM32, WN = BN > 128 ? 1 : 2, WM = 4 / WN, MT = BM / WM / 16, NT = BN / WN / 16;
   constexpr int A_BYTES = BM / 16 * 3072;
   extern __shared__ char smem_raw[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -722,20 +722,22 @@ __global__ void __launch_bounds__(GEMM32_THREADS, 3)
       la.load(g.fa, (kt + 1) * 32);
       lb.load(g.fb, (kt + 1) * 32);
     }
+    __builtin_amdgcn_s_setprio(1);             // products first: splitting fills the gaps they leave (3 % faster)
 #pragma unroll
     for (int j = 0; j < NT; j += 2) {          // two column tiles at a time: with all four, registers spill
       bf16x8 fb[2][3];
       SlabLoader<BN, TB>::frag(sb, wn + j * 16, lane, fb[0]);
-      SlabLoader<BN, TB>::frag(sb, wn + j * 16 + 16, lane, fb[1]);
+      if (j + 1 < NT) SlabLoader<BN, TB>::frag(sb, wn + j * 16 + 16, lane, fb[1]);
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         bf16x8 fa[3];
         SlabLoader<BM, TA>::frag(sa, wm + i * 16, lane, fa);
         acc[i][j] = mma3(fa, fb[0], acc[i][j]);
-        acc[i][j + 1] = mma3(fa, fb[1], acc[i][j + 1]);
+        if (j + 1 < NT) acc[i][j + 1] = mma3(fa, fb[1], acc[i][j + 1]);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
+    __builtin_amdgcn_s_setprio(0);
     __syncthreads();
   }
   epilogue<float, BM, BN, WM, WN, MT, NT, TB, EPI>(g, tile, acc, smem_raw);
@@ -1046,6 +1048,16 @@ __global__ void __launch_bounds__(GJX_BLOCK)
 constexpr int64_t DL_BYTES = (int64_t)512 << 20;      // dl of one piece of the vocabulary (any size is right)
 constexpr int64_t PACK_BYTES = (int64_t)512 << 20;    // packed weights of one piece
 constexpr int64_t MAX_LD = 1 << 22;                   // 256 rows stay within 32-bit byte offsets
+// f32 density or draw of 129 to 208 rows: one tile can hold them all (208: what the accumulators of two workgroups a CU leave
+// room for), so that the weights are read and split once instead of once for each of two tiles of 128.  Two such workgroups on a
+// CU take the time of 3.55 of the smaller ones, one alone that of 2.8, so it depends on how the tiles fill the CUs: 200 rows of
+// width 256, one tile / two tiles, at 250 tiles of the vocabulary 39 / 31 us, 321: 43 / 38, 391: 44 / 51, 508: 47 / 52,
+// 625: 72 / 60, 1000: 85 / 90; 200 x 50001 x 768: 105 / 132.
+constexpr int ALL_ROWS = 208;
+bool one_row_tile(int64_t n, int64_t vocab_tiles) {
+  const int64_t each = (vocab_tiles + 255) / 256, halves = (2 * vocab_tiles + 255) / 256;        // workgroups per CU
+  return n > 128 && n <= ALL_ROWS && 71 * (each / 2) + 56 * (each % 2) < 20 * halves;
+}
 constexpr int ROWS_MAX = 32;                          // rows up to which k_lincat_rows is used
 // What the forward of a gradient keeps (the exponentials of all logits) spares the gradient its first product and costs a
 // write and a read of them; up to this size, and from the width on where the product is the dearer one.  Forward and gradient,
@@ -1097,7 +1109,8 @@ struct Carver {
   }
 };
 
-Plan plan_of(const Call& c, bool grad, bool want_dx) {
+// keeps: a forward whose tiles a gradient's have to match
+Plan plan_of(const Call& c, bool grad, bool want_dx, bool keeps) {
   Plan p = {};
   const int64_t bm = c.f32() ? BM32 : BM, vt = up(c.vocab, bm) / bm;
   p.rows = !grad && c.n <= ROWS_MAX;
@@ -1108,6 +1121,7 @@ Plan plan_of(const Call& c, bool grad, bool want_dx) {
   // wide tiles where there are enough of them to fill the 256 CUs; f32 tiles are half as wide (three planes in LDS)
   const int wide = c.f32() ? 128 : 256;
   p.bn = (c.n > 64 && up(c.n, wide) / wide * vt >= 256) ? wide : 64;
+  if (!grad && !keeps && c.f32() && one_row_tile(c.n, vt)) p.bn = ALL_ROWS;
   p.n_pad = p.rows ? up(c.n, 16) : up(c.n, p.bn);
   p.n_tiles = p.n_pad / p.bn;
   p.tiles = p.rows ? up(c.vocab, 64) / 64 : vt;
@@ -1202,6 +1216,8 @@ int32_t launch(const Call& c, bool wide, const GemmArgs& a, hipStream_t s) {
   if constexpr (TB) {           // dW: n is the vocabulary, always wide
     return c.f32() ? launch32<128, TA, TB, EPI>(a, (unsigned)blocks, s) : launch16<256, TA, TB, EPI>(a, (unsigned)blocks, s);
   } else {
+    if constexpr (EPI == EPI_SCORE || EPI == EPI_DRAW)
+      if (c.f32() && a.n_pad == ALL_ROWS) return launch32<ALL_ROWS, TA, TB, EPI>(a, (unsigned)blocks, s);
     if (c.f32()) return wide ? launch32<128, TA, TB, EPI>(a, (unsigned)blocks, s) : launch32<64, TA, TB, EPI>(a, (unsigned)blocks, s);
     return wide ? launch16<256, TA, TB, EPI>(a, (unsigned)blocks, s) : launch16<64, TA, TB, EPI>(a, (unsigned)blocks, s);
   }
@@ -1352,8 +1368,9 @@ GJX_API int32_t gjx_linear_categorical_workspace(int32_t dtype, const void* d_x,
   const int32_t rc = check_args(c);
   if (rc != GJX_OK) return rc;
   if (n == 0) *bytes = 0;
-  else if (kind == 3) *bytes = kept_of(c, plan_of(c, false, false)).bytes;
-  else *bytes = plan_of(c, kind != 0, kind == 1).bytes;
+  else if (kind == 3) *bytes = kept_of(c, plan_of(c, false, false, true)).bytes;
+  else if (kind == 0) *bytes = std::max(plan_of(c, false, false, false).bytes, plan_of(c, false, false, true).bytes);
+  else *bytes = plan_of(c, true, kind == 1, false).bytes;
   return GJX_OK;
 }
 
@@ -1368,7 +1385,7 @@ GJX_API int32_t gjx_linear_categorical_logpdf(int32_t dtype, const int32_t* d_y,
   Forward f = {};
   f.lp = d_lp;
   f.lse = d_lse;
-  const Plan p = plan_of(c, false, false);
+  const Plan p = plan_of(c, false, false, d_kept != nullptr);
   if (d_kept) {
     if ((rc = check_kept(c, kept_of(c, p), d_kept, kept_bytes)) != GJX_OK) return rc;
     f.kept = (char*)d_kept;
@@ -1391,7 +1408,7 @@ GJX_API int32_t gjx_random_linear_categorical_i32(const uint32_t key[2], uint64_
   f.key1 = key[1];
   f.offset = offset;
   f.out = d_out;
-  return forward<EPI_DRAW>(c, plan_of(c, false, false), f, d_work, work_bytes, (hipStream_t)stream);
+  return forward<EPI_DRAW>(c, plan_of(c, false, false, false), f, d_work, work_bytes, (hipStream_t)stream);
 }
 
 GJX_API int32_t gjx_linear_categorical_grad(int32_t dtype, const int32_t* d_y, const void* d_x, int64_t x_ld, const void* d_w,
@@ -1404,11 +1421,11 @@ GJX_API int32_t gjx_linear_categorical_grad(int32_t dtype, const int32_t* d_y, c
   GJX_REQUIRE(n >= 1, GJX_EINVAL, "%s: no rows (the gradients are zero; the caller fills them)", c.who);
   GJX_REQUIRE(d_lse && d_upstream, GJX_EINVAL, "%s: null input", c.who);
   const bool f32 = c.f32();
-  const Plan p = plan_of(c, true, d_dx != nullptr);
+  const Plan p = plan_of(c, true, d_dx != nullptr, false);
   if ((rc = check_work(c, p, d_work, work_bytes)) != GJX_OK) return rc;
   Kept kept = {};
   if (d_kept) {
-    kept = kept_of(c, plan_of(c, false, false));
+    kept = kept_of(c, plan_of(c, false, false, true));
     if ((rc = check_kept(c, kept, d_kept, kept_bytes)) != GJX_OK) return rc;
   }
   if (!d_dx && !d_dw && !d_db) return GJX_OK;
