@@ -429,8 +429,8 @@ __global__ void __launch_bounds__(256)
 // its rows of K^T) is used by no other wave, so it is loaded straight into registers, each fragment for the next chunk as
 // soon as it has been used for this one.
 // Bound by the chain: 1.7 us a chunk at 2.3 GHz (bf16, dk = 128; 8192 tokens in 218 us), of which the products are 0.3 us
-// and the rest is the way of S, r and V' through LDS.  With kept states 2.8 us, the gradient's scan 3.2 us a chunk (2048
-// tokens, all CUs taken: 89 and 104 us).  Tried and no faster: two chunks of operands in flight (239 against 230 us),
+// and the rest is the way of S, r and V' through LDS.  With kept states 2.8 us, the gradient's scan 3.0 us a chunk (2048
+// tokens, all CUs taken: 88 and 96 us).  Tried and no faster: two chunks of operands in flight (239 against 230 us),
 // K S split along its reduction so that S stays in registers (241 against 225).
 constexpr int TEAM = 512;
 // vmcnt(0) alone: with nothing in flight at the loop's entry, the waits inside it count the loop's own loads only
@@ -544,14 +544,15 @@ struct Columns {
   }
 };
 
-// f32 rows [row, row + 4) x this lane's column of a (rows, dvp) block
-__device__ __forceinline__ void store_rows(float* block, int row, int col, int pitch, f32x4 x) {
+// What is kept for the gradient lies in blocks of 16 columns, rows of 64 bytes one behind the other: a workgroup of the scans
+// then fills whole lines (as rows of dvp columns, which neighbours fill piece by piece, the gradient scan took 104 us instead of 96 for 32 chunks on all CUs).
+__device__ __forceinline__ void store_rows(float* block, int row, int c, f32x4 x) {
 #pragma unroll
-  for (int r = 0; r < 4; ++r) store_at(block, (uint32_t)((row + r) * pitch + col) * 4, x[r]);
+  for (int r = 0; r < 4; ++r) store_at(block, (uint32_t)((row + r) * 16 + c) * 4, x[r]);
 }
 
-// a slab of S from its three planes (their sum is exact) to rows of an f32 block
-__device__ __forceinline__ void store_slab(const bf16* frag, float* block, int s, const Place& p, int col, int pitch) {
+// a slab of S from its three planes (their sum is exact) to its rows of a block
+__device__ __forceinline__ void store_slab(const bf16* frag, float* block, int s, const Place& p) {
   bf16x8 f[3];
   get_frag<3>(frag, p.lane, f);
   f32x4 lo, hi;
@@ -560,8 +561,8 @@ __device__ __forceinline__ void store_slab(const bf16* frag, float* block, int s
     lo[j] = (float)f[0][j] + ((float)f[1][j] + (float)f[2][j]);
     hi[j] = (float)f[0][4 + j] + ((float)f[1][4 + j] + (float)f[2][4 + j]);
   }
-  store_rows(block, 32 * s + 4 * p.quad, col, pitch, lo);
-  store_rows(block, 32 * s + 16 + 4 * p.quad, col, pitch, hi);
+  store_rows(block, 32 * s + 4 * p.quad, p.c, lo);
+  store_rows(block, 32 * s + 16 + 4 * p.quad, p.c, hi);
 }
 
 template <typename T>
@@ -625,7 +626,7 @@ __global__ void __launch_bounds__(TEAM, 2)
 #pragma unroll
       for (int n = 0; n < NC; ++n) {
         if (KEEP && p.col0 + 16 * n < sh.dvp)
-          store_rows(w.delta + (p.bh * sh.chunks + ch) * C * sh.dvp, tok, p.col0 + 16 * n, sh.dvp,
+          store_rows(w.delta + ((p.bh * sh.chunks + ch) * sh.dvp + (p.tile * NC + n) * 16) * C, tok, p.c,
                      x_d[(((int)(ch & 1) * 4 + wave) * NC + n) * 64 + lane]);
         Orders<NPO> acc;
 #pragma unroll
@@ -661,7 +662,7 @@ __global__ void __launch_bounds__(TEAM, 2)
         now[n] = acc.sum() * f_eg * sh.scale;
         // what the gradient needs is stored from here: loads of the state waves would wait behind their own stores
         if (KEEP && wave < KS && p.col0 + 16 * n < sh.dvp)
-          store_slab(x_s + (wave * NC + n) * 3 * FRAG, w.s0 + (p.bh * sh.chunks + ch) * DKP * sh.dvp, wave, p, p.col0 + 16 * n, sh.dvp);
+          store_slab(x_s + (wave * NC + n) * 3 * FRAG, w.s0 + ((p.bh * sh.chunks + ch) * sh.dvp + (p.tile * NC + n) * 16) * DKP, wave, p);
       }
       load_q(next);
       lds_barrier();
@@ -892,7 +893,7 @@ __global__ void __launch_bounds__(TEAM, 2)
 #pragma unroll
         for (int n = 0; n < NC; ++n)
           if (p.col0 + 16 * n < sh.dvp)
-            store_slab(x_s + (wave * NC + n) * 3 * FRAG, w.ds1 + at * DKP * sh.dvp, wave, p, p.col0 + 16 * n, sh.dvp);
+            store_slab(x_s + (wave * NC + n) * 3 * FRAG, w.ds1 + (at * sh.dvp + (p.tile * NC + n) * 16) * DKP, wave, p);
       if (ch > 0) put_o(now);
       lds_barrier();
       if (ch > 0) products(now);
@@ -900,7 +901,7 @@ __global__ void __launch_bounds__(TEAM, 2)
 #pragma unroll
       for (int n = 0; n < NC; ++n) {
         const f32x4 e = x_l[(wave * NC + n) * 64 + lane];
-        if (p.col0 + 16 * n < sh.dvp) store_rows(w.e + at * C * sh.dvp, tok, p.col0 + 16 * n, sh.dvp, e);
+        if (p.col0 + 16 * n < sh.dvp) store_rows(w.e + (at * sh.dvp + (p.tile * NC + n) * 16) * C, tok, p.c, e);
         f32x4 out = e * f_beta;
         if (left < C)
 #pragma unroll
@@ -1114,16 +1115,17 @@ __global__ void __launch_bounds__(BACK)
   const bool has_state = row < DKP;
   const bool first = tid < 512;
   const int trow = row & 63;
-  const float *p_s0 = w.s0 + (at * DKP + min(row, DKP - 1)) * sh.dvp + 4 * sub, *p_s1 = w.ds1 + (at * DKP + min(row, DKP - 1)) * sh.dvp + 4 * sub;
-  const float *p_e = w.e + (at * C + trow) * sh.dvp + 4 * sub, *p_d = w.delta + (at * C + trow) * sh.dvp + 4 * sub;
+  const int64_t in_s = (int64_t)(sub >> 2) * 16 * DKP + min(row, DKP - 1) * 16 + 4 * (sub & 3), in_c = (sub >> 2) * 16 * C + trow * 16 + 4 * (sub & 3);
+  const float *p_s0 = w.s0 + at * sh.dvp * DKP + in_s, *p_s1 = w.ds1 + at * sh.dvp * DKP + in_s;
+  const float *p_e = w.e + at * sh.dvp * C + in_c, *p_d = w.delta + at * sh.dvp * C + in_c;
   const T* p_o = d_o + ((b * sh.time + t0 + min(trow, left - 1)) * sh.heads + h) * sh.dv;
   f32x4 x0, x1, x2, x3;
   auto load = [&](int s) {
-    x0 = *(const f32x4*)(p_s0 + 32 * s);
-    x1 = *(const f32x4*)(p_s1 + 32 * s);
+    x0 = *(const f32x4*)(p_s0 + 32 * DKP * s);
+    x1 = *(const f32x4*)(p_s1 + 32 * DKP * s);
     if (first) {
-      x2 = *(const f32x4*)(p_e + 32 * s);
-      x3 = *(const f32x4*)(p_d + 32 * s);
+      x2 = *(const f32x4*)(p_e + 32 * C * s);
+      x3 = *(const f32x4*)(p_d + 32 * C * s);
     } else {
       const int c0 = 32 * s + 4 * sub;
       if (vec_o && c0 + 4 <= sh.dv) {
