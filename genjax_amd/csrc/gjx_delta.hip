@@ -545,7 +545,8 @@ struct Columns {
 };
 
 // What is kept for the gradient lies in blocks of 16 columns, rows of 64 bytes one behind the other: a workgroup of the scans
-// then fills whole lines (as rows of dvp columns, which neighbours fill piece by piece, the gradient scan took 104 us instead of 96 for 32 chunks on all CUs).
+// then fills whole lines (as rows of dvp columns, which neighbours fill piece by piece, the gradient scan took 104 us instead of
+// 96 for 32 chunks on all CUs).
 __device__ __forceinline__ void store_rows(float* block, int row, int c, f32x4 x) {
 #pragma unroll
   for (int r = 0; r < 4; ++r) store_at(block, (uint32_t)((row + r) * 16 + c) * 4, x[r]);
