@@ -8,7 +8,8 @@
 // The products are 16x16x32 bf16 MFMA tiles with f32 accumulators.  f32 operands are split exactly into three bf16 planes
 // (8 bits each) and the six largest partial products are summed.
 //
-// Three kernels: k_lincat_rows for few rows (the weights go once from memory to the matrix unit), k_lincat_gemm for bf16
+// Where a product has few tiles and a long reduction, the reduction is cut into parts (cuts_of).  Three product kernels:
+// k_lincat_rows for few rows (the weights go once from memory to the matrix unit), k_lincat_gemm for bf16
 // (tiles straight into LDS), k_lincat_gemm32 for f32 (tiles split into planes on their way to LDS).
 #include "gjx_common.h"
 
@@ -1000,6 +1001,133 @@ __global__ void __launch_bounds__(GJX_BLOCK)
   }
 }
 
+// Few tiles and a long reduction: the product is cut along the width, and its parts [s][row][entry] (f32) are added up here.
+struct Parts {
+  const float* p;
+  int parts;
+  int64_t stride, ld;
+  const void* bias;
+  int bias_f32;
+  __device__ __forceinline__ float logit(int64_t row, int64_t v) const {
+    const float* at = p + row * ld + v;
+    float l = 0.0f;
+    for (int s = 0; s < parts; s += 8) {                    // eight loads in flight, added in order
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = at[min(s + j, parts - 1) * stride];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) l += s + j < parts ? x[j] : 0.0f;
+    }
+    return bias ? l + load_any(bias, bias_f32, v) : l;
+  }
+};
+
+// a row's log-density (and what is kept, as EPI_KEEP leaves it, with lse for every base) or draw; TPR threads a row
+template <int TPR, int EPI>
+__global__ void __launch_bounds__(TPR > GJX_BLOCK ? TPR : GJX_BLOCK)
+    k_lincat_finish(Parts parts, float* __restrict__ sums, int64_t n, int64_t vocab, const int32_t* __restrict__ y, float* __restrict__ lp,
+                    float* __restrict__ lse, void* __restrict__ keep, int keep_f32, int64_t keep_ld, float* __restrict__ base, int block,
+                    int64_t n_pad, float* __restrict__ lp_kept, uint32_t key0, uint32_t key1, uint64_t offset, int32_t* __restrict__ out) {
+  constexpr int ROWS = TPR < GJX_BLOCK ? GJX_BLOCK / TPR : 1;
+  __shared__ float s_a[TPR / 64], s_b[TPR / 64], s_c[TPR / 64];
+  const int t = threadIdx.x % TPR, wave = threadIdx.x >> 6;
+  const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR;
+  const bool live = row < n;
+  float top = -__builtin_inff(), sum = 0.0f, own = 0.0f;
+  int arg = 0x7fffffff;
+  if (live) {
+    const int64_t value = EPI == EPI_DRAW ? -1 : min(max((int64_t)y[row], (int64_t)0), vocab - 1);
+    for (int64_t v = t; v < vocab; v += TPR) {
+      const float l = parts.logit(row, v);
+      if (EPI == EPI_DRAW) {
+        const float u = gjx_uniform_at(key0, key1, (offset + (uint64_t)row) * (uint64_t)vocab + (uint64_t)v, 1.17549435e-38f, 1.0f);
+        merge_best(top, arg, l == -__builtin_inff() ? l : l + (-logf(-logf(u))), (int)v);
+      } else {
+        if (v == value) own = l;
+        merge_lse(top, sum, l, 1.0f);
+        if (EPI == EPI_KEEP) sums[row * parts.ld + v] = l;         // (the first part: this thread alone reads and writes the entry)
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    if (EPI == EPI_DRAW) {
+      merge_best(top, arg, __shfl_xor(top, o), __shfl_xor(arg, o));
+    } else {
+      merge_lse(top, sum, __shfl_xor(top, o), __shfl_xor(sum, o));
+      own += __shfl_xor(own, o);
+    }
+  }
+  if (TPR > 64) {
+    if ((threadIdx.x & 63) == 0) {
+      s_a[wave] = top;
+      s_b[wave] = EPI == EPI_DRAW ? __int_as_float(arg) : sum;
+      s_c[wave] = own;
+    }
+    __syncthreads();
+    top = s_a[0];
+    sum = s_b[0];
+    arg = __float_as_int(s_b[0]);
+    own = s_c[0];
+#pragma unroll
+    for (int w = 1; w < TPR / 64; ++w) {
+      if (EPI == EPI_DRAW) {
+        merge_best(top, arg, s_a[w], __float_as_int(s_b[w]));
+      } else {
+        merge_lse(top, sum, s_a[w], s_b[w]);
+        own += s_c[w];
+      }
+    }
+  }
+  if (!live) return;
+  if (EPI == EPI_DRAW) {
+    if (t == 0) out[row] = arg;
+    return;
+  }
+  const float all = top + logf(sum);
+  if (t == 0) {
+    lp[row] = own - all;
+    if (lse) lse[row] = all;
+    if (EPI == EPI_KEEP) lp_kept[row] = own - all;
+  }
+  if (EPI == EPI_KEEP) {
+    for (int64_t k = t; k < keep_ld / block; k += TPR) base[k * n_pad + row] = all;
+    for (int64_t v = t; v < keep_ld; v += TPR) {
+      const float e = v < vocab ? exp_of(sums[row * parts.ld + v] - all) : 0.0f;
+      if (keep_f32) ((float*)keep)[row * keep_ld + v] = e;
+      else ((_Float16*)keep)[row * keep_ld + v] = (_Float16)(e * KEEP_SCALE);
+    }
+  }
+}
+
+// dl of the whole vocabulary from the parts of the logits: 64 entries by four rows at a time of a strip (see k_lincat_dl)
+template <typename T>
+__global__ void __launch_bounds__(GJX_BLOCK)
+    k_lincat_dl_parts(Parts parts, const float* __restrict__ lse, const float* __restrict__ up, const int32_t* __restrict__ y, int64_t n,
+                      int64_t vocab, int strip, T* __restrict__ dl, int64_t dl_ld, float* __restrict__ resid, float* __restrict__ db_part,
+                      int64_t db_ld) {
+  __shared__ float s_db[4][64];
+  const int c = threadIdx.x & 63, q = threadIdx.x >> 6, col = blockIdx.y * 64 + c;
+  const int64_t i0 = (int64_t)blockIdx.x * strip;
+  float db = 0.0f;
+  for (int i = q; i < strip; i += 4) {
+    const int64_t row = i0 + i;
+    float x = 0.0f;
+    if (row < n && col < vocab) {
+      x = -up[row] * exp_of(parts.logit(row, col) - lse[row]);
+      if (min(max((int64_t)y[row], (int64_t)0), vocab - 1) == col) {
+        x += up[row];
+        if (resid) resid[row] = x - (float)(T)x;             // (see EPI_DL)
+      }
+      db += x;
+    }
+    dl[row * dl_ld + col] = (T)x;
+  }
+  s_db[q][c] = db;
+  __syncthreads();
+  if (db_part && q == 0) db_part[(int64_t)blockIdx.x * db_ld + col] = (s_db[0][c] + s_db[1][c]) + (s_db[2][c] + s_db[3][c]);
+}
+
 // out[i][k] = sum over parts of part[s][i][k] in f32, stored in the output's type; rows of `width`, parts of `ld` columns.
 // With resid: + resid[i] w[y_i][k] (bf16 weights)
 struct Fold {
@@ -1058,6 +1186,8 @@ bool one_row_tile(int64_t n, int64_t vocab_tiles) {
   const int64_t each = (vocab_tiles + 255) / 256, halves = (2 * vocab_tiles + 255) / 256;        // workgroups per CU
   return n > 128 && n <= ALL_ROWS && 71 * (each / 2) + 56 * (each % 2) < 20 * halves;
 }
+// when a reduction is cut (cuts_of), in tiles of depth and of the product
+constexpr int CUT_DEPTH_F32 = 12, CUT_DEPTH_BF16 = 24, CUT_ROWS_DEPTH = 24, CUT_TILES = 64, CUT_DEEP = 32;
 constexpr int ROWS_MAX = 32;                          // rows up to which k_lincat_rows is used
 // What the forward of a gradient keeps (the exponentials of all logits) spares the gradient its first product and costs a
 // write and a read of them; up to this size, and from the width on where the product is the dearer one.  Forward and gradient,
@@ -1097,7 +1227,9 @@ struct Plan {
   int64_t tiles;                // partial results per row
   int splits, splits_w;         // parts of the reductions of dx (over the piece) and dW (over the rows)
   int strip;                    // rows per workgroup of k_lincat_dl
-  int64_t o_x, o_w, o_part, o_target, o_dl, o_db, o_dx, o_dw, o_resid, bytes;
+  int cuts;                     // parts of the logits' reduction (1: done in the product's epilogue)
+  int64_t cut_ld;
+  int64_t o_x, o_w, o_part, o_target, o_dl, o_db, o_dx, o_dw, o_resid, o_cut, bytes;
 };
 
 struct Carver {
@@ -1108,6 +1240,17 @@ struct Carver {
     return p;
   }
 };
+
+// Few tiles and a long reduction: it is cut into parts of four tiles of depth or more, which a second launch adds up.
+// Density, whole / cut: f32 200 x 500 x 1024 42 / 13 us, 500 x 300 x 500 27 / 14, 64 x 8000 x 512 (63 tiles) 25.6 / 24.7, 64 x 12000
+// x 1024 (94 tiles, 32 deep) 42 / 34, 64 x 16000 x 1024 42 / 40; of the kernel for few rows 2 x 326 x 1024 21 / 11, 1 x 6000 x 4096
+// 82 / 38; bf16 (half as deep, twice as fast a tile) 30 x 8000 x 2048 42 / 23, 1 x 3000 x 1600 31 / 13, 64 x 12000 x 2048 31 / 34
+// with its gradient at 80 / 73.
+int cuts_of(const Call& c, int64_t tiles, bool rows) {           // tiles: of the product, at least one
+  const int64_t depth = up(c.width, c.f32() ? 32 : 64) / (c.f32() ? 32 : 64);
+  if (depth < (rows ? CUT_ROWS_DEPTH : c.f32() ? CUT_DEPTH_F32 : CUT_DEPTH_BF16)) return 1;
+  return tiles > (c.f32() && depth >= CUT_DEEP ? 2 * CUT_TILES : CUT_TILES) ? 1 : (int)std::min<int64_t>(512 / tiles, depth / 4);
+}
 
 // keeps: a forward whose tiles a gradient's have to match
 Plan plan_of(const Call& c, bool grad, bool want_dx, bool keeps) {
@@ -1124,6 +1267,15 @@ Plan plan_of(const Call& c, bool grad, bool want_dx, bool keeps) {
   if (!grad && !keeps && c.f32() && one_row_tile(c.n, vt)) p.bn = ALL_ROWS;
   p.n_pad = p.rows ? up(c.n, 16) : up(c.n, p.bn);
   p.n_tiles = p.n_pad / p.bn;
+  p.cuts = cuts_of(c, p.rows ? vt : vt * p.n_tiles, p.rows);
+  if (p.cuts > 1 && p.rows) {                               // then tiles after all
+    p.rows = false;
+    p.pack_x = !c.f32() && !direct(c.x, c.x_ld, c.width);
+    p.pack_w = !c.f32() && !direct(c.w, c.w_ld, c.width);
+    p.n_pad = up(c.n, 64);
+    p.n_tiles = 1;
+  }
+  p.cut_ld = up(c.vocab, 4);
   p.tiles = p.rows ? up(c.vocab, 64) / 64 : vt;
   const int64_t e = c.f32() ? 4 : 2;
   int64_t piece = up(c.vocab, BM);
@@ -1131,9 +1283,11 @@ Plan plan_of(const Call& c, bool grad, bool want_dx, bool keeps) {
   if (grad) piece = std::min(piece, std::max<int64_t>(BM, DL_BYTES / (p.n_pad * e) / BM * BM));
   const int64_t pieces = up(c.vocab, piece) / piece;
   p.piece = up(up(c.vocab, pieces) / pieces, BM);           // equal pieces
+  if (p.piece < c.vocab) p.cuts = 1;
   Carver k;
   p.o_x = k.take(p.pack_x ? c.n * p.kp * 2 : 0);
   p.o_w = k.take(p.pack_w ? p.piece * p.kp * 2 : 0);
+  p.o_cut = k.take(p.cuts > 1 ? p.cuts * c.n * p.cut_ld * 4 : 0);
   if (grad) {
     p.o_dl = k.take(p.n_pad * p.piece * e);
     // strips of 64 rows, shorter ones where those would leave CUs without work
@@ -1164,7 +1318,7 @@ struct Kept {
 
 Kept kept_of(const Call& c, const Plan& forward) {
   Kept k = {};
-  if (forward.rows || c.width < (c.f32() ? KEEP_WIDTH_F32 : KEEP_WIDTH_BF16)) return k;
+  if (forward.rows || c.n <= ROWS_MAX || c.width < (c.f32() ? KEEP_WIDTH_F32 : KEEP_WIDTH_BF16)) return k;
   k.ld = up(c.vocab, BM);
   k.block = c.f32() ? BM32 / 2 : forward.bn == 256 ? BM / 2 : BM / 4;
   Carver at;
@@ -1215,6 +1369,8 @@ int32_t launch(const Call& c, bool wide, const GemmArgs& a, hipStream_t s) {
   GJX_REQUIRE(blocks < ((int64_t)1 << 31), GJX_ELIMIT, "%s: %lld tiles", c.who, (long long)blocks);
   if constexpr (TB) {           // dW: n is the vocabulary, always wide
     return c.f32() ? launch32<128, TA, TB, EPI>(a, (unsigned)blocks, s) : launch16<256, TA, TB, EPI>(a, (unsigned)blocks, s);
+  } else if constexpr (EPI == EPI_STORE && !TA) {            // the cut product of few tiles
+    return c.f32() ? launch32<64, TA, TB, EPI>(a, (unsigned)blocks, s) : launch16<64, TA, TB, EPI>(a, (unsigned)blocks, s);
   } else {
     if constexpr (EPI == EPI_SCORE || EPI == EPI_DRAW)
       if (c.f32() && a.n_pad == ALL_ROWS) return launch32<ALL_ROWS, TA, TB, EPI>(a, (unsigned)blocks, s);
@@ -1291,6 +1447,27 @@ int32_t take_w(const Call& c, const Plan& p, char* ws, int64_t v0, int64_t rows,
 
 int depth_tiles(const Call& c, int64_t depth) { return (int)(c.f32() ? up(depth, 32) / 32 : up(depth, BK) / BK); }
 
+// the logits without their bias in parts, for the whole vocabulary
+int32_t cut_product(const Call& c, const Plan& p, const Inputs& in, char* ws, Parts& parts, hipStream_t s) {
+  float* out = (float*)(ws + p.o_cut);
+  GemmArgs a = common_args(c, p);
+  a.a = in.w;
+  a.fa = in.fw;
+  a.b = in.x;
+  a.fb = in.fx;
+  a.ktiles = depth_tiles(c, p.kp);
+  a.mt = (int)(up(c.vocab, p.bm) / p.bm);
+  a.nt = (int)p.n_tiles;
+  a.splits = p.cuts;
+  a.out = out;
+  a.out_ld = p.cut_ld;
+  a.out_split = c.n * p.cut_ld;
+  a.out_m = (int)c.vocab;
+  a.out_n = (int)c.n;
+  parts = {out, p.cuts, c.n * p.cut_ld, p.cut_ld, c.bias, c.f32()};
+  return launch<false, false, EPI_STORE>(c, false, a, s);
+}
+
 // the forward product, reduced to log-densities (EPI_SCORE) or draws (EPI_DRAW)
 struct Forward {
   float *lp, *lse;
@@ -1325,6 +1502,22 @@ int32_t forward(const Call& c, const Plan& p, const Forward& f, void* d_work, in
   a.keep = f.kept;
   a.keep_base = (float*)(f.kept + kept.o_base);
   a.keep_ld = kept.ld;
+  if (p.cuts > 1) {
+    Inputs in = {};
+    Parts parts = {};
+    if ((rc = take_x(c, p, ws, in, s)) != GJX_OK || (rc = take_w(c, p, ws, 0, c.vocab, in, s)) != GJX_OK) return rc;
+    if ((rc = cut_product(c, p, in, ws, parts, s)) != GJX_OK) return rc;
+    float *base = (float*)(f.kept + kept.o_base), *lp_kept = (float*)(f.kept + kept.o_lp);
+    auto finish = [&](auto* kernel, int64_t blocks, int threads) {
+      kernel<<<(unsigned)blocks, threads, 0, s>>>(parts, (float*)(ws + p.o_cut), c.n, c.vocab, c.y, f.lp, f.lse, f.kept, c.f32(), kept.ld,
+                                                  base, kept.block, p.n_pad, lp_kept, f.key0, f.key1, f.offset, f.out);
+    };
+    if (c.vocab <= 256) finish(k_lincat_finish<64, EPI>, up(c.n, 4) / 4, GJX_BLOCK);
+    else if (c.vocab <= 1024) finish(k_lincat_finish<256, EPI>, c.n, 256);
+    else finish(k_lincat_finish<1024, EPI>, c.n, 1024);
+    GJX_LAUNCH_CHECK();
+    return GJX_OK;
+  }
   if (EPI != EPI_KEEP && p.rows) {
     if constexpr (EPI != EPI_KEEP) rc = c.f32() ? launch_rows<float, EPI>(c, p, a, s) : launch_rows<bf16, EPI>(c, p, a, s);
     if (rc != GJX_OK) return rc;
@@ -1439,7 +1632,7 @@ GJX_API int32_t gjx_linear_categorical_grad(int32_t dtype, const int32_t* d_y, c
   float *dx_part = (float*)(ws + p.o_dx), *db_part = (float*)(ws + p.o_db), *resid = f32 ? nullptr : (float*)(ws + p.o_resid);
   const bool whole = p.piece >= vocab;                       // one piece
   const bool dx_direct = whole && f32 && p.splits == 1;      // nothing to add up
-  const int db_parts = (int)(d_kept ? up(n, 64) / p.strip : p.n_tiles);
+  const int db_parts = (int)(d_kept || p.cuts > 1 ? up(n, 64) / p.strip : p.n_tiles);
   Fold dx_fold = {}, db_fold = {}, dw_fold = {};
   auto fold = [&](const Fold& one, const Fold& two, const Fold& three) -> int32_t {
     const int64_t entries = one.rows * one.width + two.rows * two.width + three.rows * three.width;
@@ -1463,6 +1656,17 @@ GJX_API int32_t gjx_linear_categorical_grad(int32_t dtype, const int32_t* d_y, c
         k_lincat_dl<bf16><<<grid, GJX_BLOCK, 0, s>>>(k, kept.ld, (const float*)(k + kept.o_base), kept.block, p.n_pad,
                                                      (const float*)(k + kept.o_lp), d_lse, d_upstream, d_y, n, vocab, v0, (int)rows_pad, p.strip,
                                                      (bf16*)(ws + p.o_dl), p.piece, resid, d_db ? db_part : nullptr, p.piece);
+      GJX_LAUNCH_CHECK();
+    } else if (p.cuts > 1) {                                 // (one piece)
+      Parts parts = {};
+      if ((rc = cut_product(c, p, in, ws, parts, s)) != GJX_OK) return rc;
+      const dim3 grid((unsigned)(up(n, 64) / p.strip), (unsigned)(rows_pad / 64));
+      if (f32)
+        k_lincat_dl_parts<float><<<grid, GJX_BLOCK, 0, s>>>(parts, d_lse, d_upstream, d_y, n, vocab, p.strip,
+                                                            (float*)(ws + p.o_dl), p.piece, resid, d_db ? db_part : nullptr, p.piece);
+      else
+        k_lincat_dl_parts<bf16><<<grid, GJX_BLOCK, 0, s>>>(parts, d_lse, d_upstream, d_y, n, vocab, p.strip,
+                                                           (bf16*)(ws + p.o_dl), p.piece, resid, d_db ? db_part : nullptr, p.piece);
       GJX_LAUNCH_CHECK();
     } else {
       GemmArgs a = common_args(c, p);                        // logits of the piece -> dl

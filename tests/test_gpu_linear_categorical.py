@@ -425,3 +425,34 @@ def test_rows_of_one_wide_tile(G, n):
     # the same draws as categorical's over the rounded logits, but where two entries lie within the logits' error
     ref = B.sample_categorical(key, (x.double() @ w.double().t() + b.double()).float())
     assert (ours == ref).float().mean() >= 0.98
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("n,vocab,width", [(2, 326, 3867), (1, 1, 4096), (32, 3000, 4100), (500, 31, 3000), (64, 1500, 1024), (40, 5000, 800),
+                                           (129, 700, 2048), (2000, 3, 1000)])
+def test_few_tiles_and_long_rows(G, n, vocab, width, dtype):
+    """The products whose reduction is cut along the width: log-density, gradients (kept or formed again), draws."""
+    from genjax_amd import backend as B
+
+    x, w, b, y, up = _inputs(n, vocab, width, TYPES[dtype])
+    if vocab > 2:
+        b[1] = -float("inf")
+        y[y == 1] = 0
+    t = _truth(x, w, b, y, up)
+    one = _grads(G, x, w, b, y, up)
+    for name, got, again in zip(("lp", "dx", "dw", "db"), one, _grads(G, x, w, b, y, up)):
+        _close(name, got, t[name])
+        assert torch.equal(got, again)
+    _close("lp without a gradient", G.linear_categorical.logpdf(y, x, w, b), t["lp"])
+    lp, lse = B.linear_categorical_logpdf(y, x, w, b)
+    for name, got in zip(("dx", "dw", "db"), B.linear_categorical_grad(y, x, w, b, lse, up)):      # nothing kept
+        _close(name + " formed again", got, t[name])
+    key = G.key(11)
+    got = B.sample_linear_categorical(key, x, w, b)
+    u = B.random_uniform(key, n * vocab, 1.17549435e-38, 1.0).double().reshape(n, vocab)
+    z = x.double() @ w.double().t() + b.double() - (-u.log()).log()
+    best = z.max(dim=1)[0]
+    # the logits are off by E = 2 width 2^-23 sum |x w| at most, the noise by some units of 2^-24 of at most ~20
+    E = 2 * width * 2.0 ** -23 * (x.double().abs() @ w.double().abs().t()).max(1)[0]
+    assert (best - z.gather(1, got.long().unsqueeze(1)).squeeze(1) <= 2 * E + 1e-4).all()
+    assert vocab < 2 or (got != 1).all() or vocab <= 2
