@@ -1071,6 +1071,7 @@ __global__ void __launch_bounds__(BACK)
   __shared__ __attribute__((aligned(16))) char buffer[std::max(std::max(F_ALL, EF_ALL) * 2, RESULTS)];
   __shared__ float s_gh[C], s_gl[C], s_row[4][C], s_db[C], s_put[16];
   __shared__ double s_sum[16];
+  __shared__ int s_state[16];                             // whether S0 has an entry other than 0
   bf16* frag = (bf16*)buffer;
   float *sq = (float*)buffer, *sk = sq + C * LO;          // dq and dk, once E and F are
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quad = lane >> 4, c = lane & 15;
@@ -1157,6 +1158,7 @@ __global__ void __launch_bounds__(BACK)
 #pragma unroll
   for (int t = 0; t < MH; ++t) m1[t] = m2[t] = m3[t] = f32x4{0, 0, 0, 0};
   float dot = 0.0f, db = 0.0f;
+  bool any = false;
   const int slabs = sh.dvp / 32;
   load(0);
   for (int s = 0; s < slabs; ++s) {
@@ -1164,7 +1166,10 @@ __global__ void __launch_bounds__(BACK)
       put4(F_S0, 3, row, x0);
       put4(F_S1, 3, row, x1);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) dot += x0[j] * x1[j];
+      for (int j = 0; j < 4; ++j) {
+        dot += x0[j] * x1[j];
+        any |= x0[j] != 0.0f;
+      }
     }
     if (first) {
       put4(F_E, 3, trow, x2);
@@ -1202,7 +1207,11 @@ __global__ void __launch_bounds__(BACK)
     double d = has_state ? (double)dot : 0.0;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) d += __shfl_xor(d, o);
-    if (lane == 0) s_sum[wave] = d;
+    const uint64_t some = __ballot(any);
+    if (lane == 0) {
+      s_sum[wave] = d;
+      s_state[wave] = some != 0;
+    }
     db += __shfl_xor(db, 1);
     db += __shfl_xor(db, 2);
     db += __shfl_xor(db, 4);
@@ -1335,12 +1344,15 @@ __global__ void __launch_bounds__(BACK)
       if (lane + o < 64) s += down;
     }
     double end = 0.0, written = 0.0;
+    int state = 0;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
+      state |= s_state[i];
       end += s_sum[i];
       written += (double)s_put[i];
     }
     s += (double)rb[3 * C] * end + written;
+    if (lane == 0 && !state) s = 0.0;                     // <dS0, S0> of an empty state: exactly 0, not the sums' rounding
     if (lane < left_o) {
       dg[g_at + (int64_t)lane * sh.heads] = lane < left ? (float)s : 0.0f;
       dbeta[g_at + (int64_t)lane * sh.heads] = lane < left ? s_db[lane] : 0.0f;

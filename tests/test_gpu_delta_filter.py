@@ -316,3 +316,16 @@ def test_state_beyond_32_bit_offsets(S):
     to, ts, _ = _truth(a)
     _close("o", o[-2:], to[:, 0].detach(), 2.0 ** -19)
     _close("state", new[-2:], ts.detach(), 2.0 ** -19)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("time", [1, 2, 65])
+def test_first_decay_of_an_empty_state_has_no_gradient(S, time, dtype):
+    """Without an initial state (or with one of zeros) nothing decays at the first token: its gradient is 0, not rounding."""
+    a, d_o, d_state = _inputs(3, time, 2, 4, 40, 24, TYPES[dtype], state=False)
+    for state in (None, torch.zeros(3, 4, 40, 24, device="cuda")):
+        leaves = [a[n].clone().requires_grad_(True) for n in NAMES[:5]]
+        o, last = S.delta_filter(*leaves, initial_state=state)
+        grads = torch.autograd.grad([o, last], leaves, [d_o, d_state])
+        assert not grads[3][:, 0].any() and (time == 1 or grads[3][:, 1].any())
+        assert all(g.any() for i, g in enumerate(grads) if i != 3)
