@@ -15,11 +15,14 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 typedef __bf16 bf16;
 typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef f32x4 f32x4_any __attribute__((aligned(4)));       // 16 bytes at any entry of a row: one load all the same
+typedef bf16x8 bf16x8_any __attribute__((aligned(2)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
@@ -46,7 +49,7 @@ struct Operand {
 struct OperandF {
   const float* p;
   int64_t ld;
-  int rows, cols, vec;   // vec: rows are aligned to 16 bytes
+  int rows, cols;
 };
 
 struct GemmArgs {
@@ -601,8 +604,8 @@ __global__ void __launch_bounds__(GEMM_THREADS)
 }
 
 // One 32-deep slab of an f32 operand, R output indices wide: pieces of eight reduction entries of one output index, loaded
-// into registers, split and written to LDS as fragments (16 indices x 3 planes x 64 slots of 16 bytes).  Whole slabs of
-// aligned rows are read at a uniform base plus a kept 32-bit offset; others entry by entry, clamped and masked.
+// into registers, split and written to LDS as fragments (16 indices x 3 planes x 64 slots of 16 bytes).  Whole slabs are
+// read at a uniform base plus a kept 32-bit offset; the last one entry by entry, clamped and masked.
 // Slot (index, group) lies at 16 group + (index + 2 group) % 16: neither the four lanes that write a row's groups nor the
 // sixteen that read a group meet in a bank (without the rotation 60 % of the LDS cycles were conflicts).
 template <int R, bool T>
@@ -635,14 +638,14 @@ struct SlabLoader {
     }
   }
   __device__ __forceinline__ void load(const OperandF& o, int k0) {
-    if (T ? k0 + 32 <= o.rows : o.vec && k0 + 32 <= o.cols) {
+    if (k0 + 32 <= (T ? o.rows : o.cols)) {
 #pragma unroll
       for (int i = 0; i < PIECES; ++i) {
         if (T) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) x[i][j] = *(const float*)(base + (int64_t)j * o.ld * 4 + off[i]);
         } else {
-          const f32x4 lo = *(const f32x4*)(base + off[i]), hi = *(const f32x4*)(base + 16 + off[i]);
+          const f32x4 lo = *(const f32x4_any*)(base + off[i]), hi = *(const f32x4_any*)(base + 16 + off[i]);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             x[i][j] = lo[j];
@@ -749,7 +752,7 @@ __global__ void __launch_bounds__(GEMM32_THREADS, BN > 128 ? 2 : 3)
 // 32000 x 1024 bf16 weights in 17 us, 3.9 TB/s.
 template <typename T, int NT, int EPI>
 __global__ void __launch_bounds__(GJX_BLOCK)
-    k_lincat_rows(GemmArgs g, const T* __restrict__ x, int64_t x_ld, const T* __restrict__ w, int64_t w_ld, int width, int vec) {
+    k_lincat_rows(GemmArgs g, const T* __restrict__ x, int64_t x_ld, const T* __restrict__ w, int64_t w_ld, int width) {
   constexpr int P = sizeof(T) == 4 ? 3 : 1, U = (sizeof(T) == 4 ? 8 : 16) / NT;      // planes; slabs in flight
   __shared__ float s_red[4][16 * NT][2];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, c = lane & 15;
@@ -758,12 +761,13 @@ __global__ void __launch_bounds__(GJX_BLOCK)
   const T* xp[NT];
 #pragma unroll
   for (int j = 0; j < NT; ++j) xp[j] = x + min((int64_t)(j * 16 + c), g.n - 1) * x_ld;
-  auto load = [&](const T* p, int k, float (&f)[8], bf16x8& h) {       // eight entries from k (a multiple of 8) on, zeros behind the end
-    if (vec && k + 8 <= width) {
+  // eight entries from k (a multiple of 8) on; not whole: zeros behind the end
+  auto load = [&](auto whole, const T* p, int k, float (&f)[8], bf16x8& h) {
+    if (whole || k + 8 <= width) {
       if (P == 1) {
-        h = *(const bf16x8*)(p + k);
+        h = *(const bf16x8_any*)(p + k);
       } else {
-        const f32x4 lo = *(const f32x4*)(p + k), hi = *(const f32x4*)(p + k + 4);
+        const f32x4 lo = *(const f32x4_any*)(p + k), hi = *(const f32x4_any*)(p + k + 4);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           f[e] = lo[e];
@@ -785,20 +789,22 @@ __global__ void __launch_bounds__(GJX_BLOCK)
   f32x4 acc[NT];
 #pragma unroll
   for (int j = 0; j < NT; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  for (int k0 = 0; k0 < width; k0 += 32 * U) {
-    float fw[U][8];
-    bf16x8 hw[U];
+  // `count` slabs from k0 on, their loads of the weights all in flight; whole: inside the width
+  auto slabs = [&](int k0, auto count, auto whole) {
+    constexpr int N = decltype(count)::value;
+    float fw[N][8];
+    bf16x8 hw[N];
 #pragma unroll
-    for (int u = 0; u < U; ++u) load(wp, k0 + 32 * u + 8 * q, fw[u], hw[u]);
+    for (int u = 0; u < N; ++u) load(whole, wp, k0 + 32 * u + 8 * q, fw[u], hw[u]);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
+    for (int u = 0; u < N; ++u) {
       bf16x8 a[3];
       if (P == 3) split8(fw[u], a);
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
         float fx[8];
         bf16x8 hx, b[3];
-        load(xp[j], k0 + 32 * u + 8 * q, fx, hx);
+        load(whole, xp[j], k0 + 32 * u + 8 * q, fx, hx);
         if (P == 1) {
           acc[j] = mma(hw[u], hx, acc[j]);
         } else {
@@ -807,7 +813,13 @@ __global__ void __launch_bounds__(GJX_BLOCK)
         }
       }
     }
-  }
+  };
+  int k0 = 0;
+  for (; k0 + 32 * U <= width; k0 += 32 * U) slabs(k0, std::integral_constant<int, U>(), std::true_type());
+  if constexpr (U >= 8)
+    for (; k0 + 8 * U <= width; k0 += 8 * U) slabs(k0, std::integral_constant<int, U / 4>(), std::true_type());
+  for (; k0 + 32 <= width; k0 += 32) slabs(k0, std::integral_constant<int, 1>(), std::true_type());
+  if (k0 < width) slabs(k0, std::integral_constant<int, 1>(), std::false_type());
   float bias[4];
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
@@ -1215,8 +1227,6 @@ struct Call {
 
 // rows a tile loader can take as they are: aligned to 16 bytes, whole 64-deep tiles
 bool direct(const void* p, int64_t ld, int64_t width) { return ((uintptr_t)p & 15) == 0 && ld % 8 == 0 && width % 64 == 0; }
-// ... a vector load can take: aligned to 16 bytes
-bool vector_rows(const Call& c, const void* p, int64_t ld) { return ((uintptr_t)p & 15) == 0 && ld % (c.f32() ? 4 : 8) == 0; }
 
 struct Plan {
   bool rows;                    // k_lincat_rows
@@ -1429,7 +1439,7 @@ struct Inputs {
 };
 
 int32_t take_x(const Call& c, const Plan& p, char* ws, Inputs& in, hipStream_t s) {
-  in.fx = {(const float*)c.x, c.x_ld, (int)c.n, (int)c.width, vector_rows(c, c.x, c.x_ld)};
+  in.fx = {(const float*)c.x, c.x_ld, (int)c.n, (int)c.width};
   in.x = {(const bf16*)c.x, c.x_ld, (int)c.n, (int)p.kp};
   if (!p.pack_x) return GJX_OK;
   in.x = {(const bf16*)(ws + p.o_x), p.kp, (int)c.n, (int)p.kp};
@@ -1438,7 +1448,7 @@ int32_t take_x(const Call& c, const Plan& p, char* ws, Inputs& in, hipStream_t s
 
 int32_t take_w(const Call& c, const Plan& p, char* ws, int64_t v0, int64_t rows, Inputs& in, hipStream_t s) {
   const char* w = c.w_row(v0);
-  in.fw = {(const float*)w, c.w_ld, (int)rows, (int)c.width, vector_rows(c, w, c.w_ld)};
+  in.fw = {(const float*)w, c.w_ld, (int)rows, (int)c.width};
   in.w = {(const bf16*)w, c.w_ld, (int)rows, (int)p.kp};
   if (!p.pack_w) return GJX_OK;
   in.w = {(const bf16*)(ws + p.o_w), p.kp, (int)rows, (int)p.kp};
@@ -1479,10 +1489,9 @@ struct Forward {
 
 template <typename T, int EPI>
 int32_t launch_rows(const Call& c, const Plan& p, const GemmArgs& a, hipStream_t s) {
-  const int vec = vector_rows(c, c.x, c.x_ld) && vector_rows(c, c.w, c.w_ld);
   const unsigned blocks = (unsigned)p.tiles;
-  if (p.n_pad == 16) k_lincat_rows<T, 1, EPI><<<blocks, GJX_BLOCK, 0, s>>>(a, (const T*)c.x, c.x_ld, (const T*)c.w, c.w_ld, (int)c.width, vec);
-  else k_lincat_rows<T, 2, EPI><<<blocks, GJX_BLOCK, 0, s>>>(a, (const T*)c.x, c.x_ld, (const T*)c.w, c.w_ld, (int)c.width, vec);
+  if (p.n_pad == 16) k_lincat_rows<T, 1, EPI><<<blocks, GJX_BLOCK, 0, s>>>(a, (const T*)c.x, c.x_ld, (const T*)c.w, c.w_ld, (int)c.width);
+  else k_lincat_rows<T, 2, EPI><<<blocks, GJX_BLOCK, 0, s>>>(a, (const T*)c.x, c.x_ld, (const T*)c.w, c.w_ld, (int)c.width);
   GJX_LAUNCH_CHECK();
   return GJX_OK;
 }
@@ -1644,7 +1653,7 @@ GJX_API int32_t gjx_linear_categorical_grad(int32_t dtype, const int32_t* d_y, c
     const int64_t rows = std::min(p.piece, vocab - v0), rows_pad = up(rows, BM);
     if ((rc = take_w(c, p, ws, v0, rows, in, s)) != GJX_OK) return rc;
     const Operand dl = {(const bf16*)(ws + p.o_dl), p.piece, (int)p.n_pad, (int)p.piece};
-    const OperandF fdl = {(const float*)(ws + p.o_dl), p.piece, (int)p.n_pad, (int)rows_pad, 1};
+    const OperandF fdl = {(const float*)(ws + p.o_dl), p.piece, (int)p.n_pad, (int)rows_pad};
     if (d_kept) {
       const char* k = (const char*)d_kept;
       const dim3 grid((unsigned)(up(n, 64) / p.strip), (unsigned)(up(rows_pad, GJX_BLOCK * 8) / (GJX_BLOCK * 8)));
