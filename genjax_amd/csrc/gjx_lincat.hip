@@ -33,6 +33,7 @@ namespace {
 
 constexpr int BM = 256, BK = 64, GEMM_THREADS = 512;         // bf16 tiles: BM entries of m, 64 deep, eight waves
 constexpr int BM32 = 128, GEMM32_THREADS = 256;              // f32 tiles: 32 deep, four waves
+constexpr int SPLIT_BYTES = 3 * 64 * 16;                      // a slab of 16 of its rows: three planes of 64 lanes x 16 bytes
 
 enum { EPI_SCORE = 0, EPI_DL = 1, EPI_STORE = 2, EPI_DRAW = 3, EPI_KEEP = 4 };   // KEEP: SCORE that leaves what dl is formed from
 
@@ -678,7 +679,7 @@ struct SlabLoader {
       where(i, index, group);
       bf16x8 o[3];
       split8(x[i], o);
-      char* f = lds + (index >> 4) * 3072 + (16 * group + ((index & 15) ^ (2 * (group & 1) | (group >> 1) * 12))) * 16;
+      char* f = lds + (index >> 4) * SPLIT_BYTES + (16 * group + ((index & 15) ^ (2 * (group & 1) | (group >> 1) * 12))) * 16;
 #pragma unroll
       for (int p = 0; p < 3; ++p) *(bf16x8*)(f + p * 1024) = o[p];
     }
@@ -686,7 +687,7 @@ struct SlabLoader {
   static __device__ __forceinline__ void frag(const char* lds, int i0, int lane, bf16x8 (&out)[3]) {
     const int q = lane >> 4;
 #pragma unroll
-    for (int p = 0; p < 3; ++p) out[p] = *(const bf16x8*)(lds + (i0 >> 4) * 3072 + p * 1024 + (16 * q + ((lane & 15) ^ (2 * (q & 1) | (q >> 1) * 12))) * 16);
+    for (int p = 0; p < 3; ++p) out[p] = *(const bf16x8*)(lds + (i0 >> 4) * SPLIT_BYTES + p * 1024 + (16 * q + ((lane & 15) ^ (2 * (q & 1) | (q >> 1) * 12))) * 16);
   }
 };
 
@@ -700,7 +701,7 @@ template <int BN, bool TA, bool TB, int EPI>
 __global__ void __launch_bounds__(GEMM32_THREADS, BN > 128 ? 2 : 3)
     k_lincat_gemm32(GemmArgs g) {
   constexpr int BM = BM32, WN = BN > 128 ? 1 : 2, WM = 4 / WN, MT = BM / WM / 16, NT = BN / WN / 16;
-  constexpr int A_BYTES = BM / 16 * 3072;
+  constexpr int A_BYTES = BM / 16 * SPLIT_BYTES;
   extern __shared__ char smem_raw[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Tile tile = tile_of<BM, BN>(g);
@@ -1364,7 +1365,7 @@ int32_t launch16(const GemmArgs& a, unsigned blocks, hipStream_t s) {
 template <int BN, bool TA, bool TB, int EPI>
 int32_t launch32(const GemmArgs& a, unsigned blocks, hipStream_t s) {
   static std::atomic<uint64_t> done{0};
-  constexpr int lds = (BM32 + BN) / 16 * 3072;
+  constexpr int lds = (BM32 + BN) / 16 * SPLIT_BYTES;
   const int32_t rc = allow_lds(k_lincat_gemm32<BN, TA, TB, EPI>, lds, done);
   if (rc != GJX_OK) return rc;
   k_lincat_gemm32<BN, TA, TB, EPI><<<blocks, GEMM32_THREADS, lds, s>>>(a);
