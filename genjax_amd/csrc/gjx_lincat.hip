@@ -66,7 +66,7 @@ struct GemmArgs {
   float2* part;        // [tile m][n_pad]: (max, sum exp) of a row over one tile; drawing: (largest l + Gumbel, its entry)
   float* target;       // logit of y
   void* keep;          // EPI_KEEP: [n][keep_ld] exp(l - base), f32 or f16 x 2^15, base the row's largest l of a wave's block of entries
-  float* keep_base;    // [v / block][n_pad]
+  float* keep_base;    // [v / block][n]
   int64_t keep_ld;
   int64_t n_pad;
   int part_tile0;
@@ -373,7 +373,7 @@ __device__ __forceinline__ void epilogue(const GemmArgs& g, const Tile& tile, f3
       sum += __shfl_xor(sum, 32);
       if (EPI == EPI_KEEP && n < g.n) {
         const int64_t v = g.v0 + m0 + wm;
-        if (q == 0) g.keep_base[v / (MT * 16) * g.n_pad + n] = base;
+        if (q == 0) g.keep_base[v / (MT * 16) * g.n + n] = base;
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
           if (sizeof(T) == 2) {
@@ -832,7 +832,7 @@ __global__ void __launch_bounds__(GJX_BLOCK)
     const int64_t n = j * 16 + c;
     float top = -__builtin_inff(), sum = 0.0f;
     int arg = 0x7fffffff;
-    if (EPI == EPI_SCORE) {
+    if (EPI != EPI_DRAW) {
       const int64_t y = n < g.n ? min(max((int64_t)g.y[n], (int64_t)0), g.vocab - 1) - v0 - 4 * q : -1;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -840,9 +840,27 @@ __global__ void __launch_bounds__(GJX_BLOCK)
         top = fmaxf(top, acc[j][r]);
         if (y == r) g.target[n] = acc[j][r];
       }
+      top = fmaxf(top, __shfl_xor(top, 16));              // the wave's sixteen entries
+      top = fmaxf(top, __shfl_xor(top, 32));
       const float base = top == -__builtin_inff() ? 0.0f : top;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) sum += exp_of(acc[j][r] - base);
+      for (int r = 0; r < 4; ++r) {
+        acc[j][r] = exp_of(acc[j][r] - base);
+        sum += acc[j][r];
+      }
+      sum += __shfl_xor(sum, 16);
+      sum += __shfl_xor(sum, 32);
+      if (EPI == EPI_KEEP && n < g.n) {
+        if (q == 0) g.keep_base[(int64_t)(v0 / 16) * g.n + n] = base;
+        if (sizeof(T) == 2) {
+          f16x4 h;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) h[r] = (_Float16)(acc[j][r] * KEEP_SCALE);
+          *(f16x4*)((_Float16*)g.keep + n * g.keep_ld + v0 + 4 * q) = h;
+        } else {
+          *(f32x4*)((float*)g.keep + n * g.keep_ld + v0 + 4 * q) = acc[j];
+        }
+      }
     } else if (n < g.n) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -855,14 +873,12 @@ __global__ void __launch_bounds__(GJX_BLOCK)
         }
       }
     }
+    if (EPI == EPI_DRAW)
 #pragma unroll
-    for (int o = 16; o <= 32; o <<= 1) {
-      if (EPI == EPI_SCORE) merge_lse(top, sum, __shfl_xor(top, o), __shfl_xor(sum, o));
-      else merge_best(top, arg, __shfl_xor(top, o), __shfl_xor(arg, o));
-    }
+      for (int o = 16; o <= 32; o <<= 1) merge_best(top, arg, __shfl_xor(top, o), __shfl_xor(arg, o));
     if (q == 0) {
       s_red[wave][j * 16 + c][0] = top;
-      s_red[wave][j * 16 + c][1] = EPI == EPI_SCORE ? sum : __int_as_float(arg);
+      s_red[wave][j * 16 + c][1] = EPI == EPI_DRAW ? __int_as_float(arg) : sum;
     }
   }
   __syncthreads();
@@ -871,10 +887,10 @@ __global__ void __launch_bounds__(GJX_BLOCK)
     int arg = __float_as_int(sum);
 #pragma unroll
     for (int i = 1; i < 4; ++i) {
-      if (EPI == EPI_SCORE) merge_lse(top, sum, s_red[i][threadIdx.x][0], s_red[i][threadIdx.x][1]);
+      if (EPI != EPI_DRAW) merge_lse(top, sum, s_red[i][threadIdx.x][0], s_red[i][threadIdx.x][1]);
       else merge_best(top, arg, s_red[i][threadIdx.x][0], __float_as_int(s_red[i][threadIdx.x][1]));
     }
-    g.part[(int64_t)blockIdx.x * g.n_pad + threadIdx.x] = make_float2(top, EPI == EPI_SCORE ? sum : __int_as_float(arg));
+    g.part[(int64_t)blockIdx.x * g.n_pad + threadIdx.x] = make_float2(top, EPI == EPI_DRAW ? __int_as_float(arg) : sum);
   }
 }
 
@@ -954,7 +970,7 @@ __global__ void __launch_bounds__(GJX_BLOCK)
 
 template <typename T>
 __global__ void __launch_bounds__(GJX_BLOCK)
-    k_lincat_dl(const void* __restrict__ keep, int64_t keep_ld, const float* __restrict__ base, int block, int64_t n_pad,
+    k_lincat_dl(const void* __restrict__ keep, int64_t keep_ld, const float* __restrict__ base, int block,
                 const float* __restrict__ lp, const float* __restrict__ lse, const float* __restrict__ up,
                 const int32_t* __restrict__ y, int64_t n, int64_t vocab, int64_t v0, int cols, int strip, T* __restrict__ dl,
                 int64_t dl_ld, float* __restrict__ resid, float* __restrict__ db_part, int64_t db_ld) {
@@ -962,7 +978,7 @@ __global__ void __launch_bounds__(GJX_BLOCK)
   if (col >= cols) return;
   const int64_t i0 = (int64_t)blockIdx.x * strip;
   const int rows = (int)max(min((int64_t)strip, n - i0), (int64_t)0);
-  const float* b = base + (v0 + col) / block * n_pad + i0;
+  const float* b = base + (v0 + col) / block * n + i0;
   T* out = dl + i0 * dl_ld + col;
   float db[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll 4
@@ -1040,7 +1056,7 @@ template <int TPR, int EPI>
 __global__ void __launch_bounds__(TPR > GJX_BLOCK ? TPR : GJX_BLOCK)
     k_lincat_finish(Parts parts, float* __restrict__ sums, int64_t n, int64_t vocab, const int32_t* __restrict__ y, float* __restrict__ lp,
                     float* __restrict__ lse, void* __restrict__ keep, int keep_f32, int64_t keep_ld, float* __restrict__ base, int block,
-                    int64_t n_pad, float* __restrict__ lp_kept, uint32_t key0, uint32_t key1, uint64_t offset, int32_t* __restrict__ out) {
+                    float* __restrict__ lp_kept, uint32_t key0, uint32_t key1, uint64_t offset, int32_t* __restrict__ out) {
   constexpr int ROWS = TPR < GJX_BLOCK ? GJX_BLOCK / TPR : 1;
   __shared__ float s_a[TPR / 64], s_b[TPR / 64], s_c[TPR / 64];
   const int t = threadIdx.x % TPR, wave = threadIdx.x >> 6;
@@ -1104,7 +1120,7 @@ __global__ void __launch_bounds__(TPR > GJX_BLOCK ? TPR : GJX_BLOCK)
     if (EPI == EPI_KEEP) lp_kept[row] = own - all;
   }
   if (EPI == EPI_KEEP) {
-    for (int64_t k = t; k < keep_ld / block; k += TPR) base[k * n_pad + row] = all;
+    for (int64_t k = t; k < keep_ld / block; k += TPR) base[k * n + row] = all;
     for (int64_t v = t; v < keep_ld; v += TPR) {
       const float e = v < vocab ? exp_of(sums[row * parts.ld + v] - all) : 0.0f;
       if (keep_f32) ((float*)keep)[row * keep_ld + v] = e;
@@ -1203,7 +1219,8 @@ bool one_row_tile(int64_t n, int64_t vocab_tiles) {
 constexpr int CUT_DEPTH_F32 = 12, CUT_DEPTH_BF16 = 24, CUT_ROWS_DEPTH = 24, CUT_TILES = 64, CUT_DEEP = 32;
 constexpr int ROWS_MAX = 32;                          // rows up to which k_lincat_rows is used
 // What the forward of a gradient keeps (the exponentials of all logits) spares the gradient its first product and costs a
-// write and a read of them; up to this size, and from the width on where the product is the dearer one.  Forward and gradient,
+// write and a read of them; up to this size, and from the width on where the product is the dearer one (up to 32 rows: always,
+// the product there takes as long as the weights; 1 x 35780 x 1386 f32: 300 us with it formed again, 240 kept).  Forward and gradient,
 // kept against formed again: bf16 4096 x 32000 x 128: 475 / 460 us, x 256: 524 / 549, x 512: 610 / 666, x 1024: 915 / 1040;
 // 300 x 8000 x 256: 62 / 57, x 512: 65 / 66; f32 1000 x 20011 x 64: 180 / 180, x 128: 191 / 200, x 512: 396 / 468.
 constexpr int64_t KEEP_BYTES = (int64_t)2 << 30;
@@ -1329,12 +1346,12 @@ struct Kept {
 
 Kept kept_of(const Call& c, const Plan& forward) {
   Kept k = {};
-  if (forward.rows || c.n <= ROWS_MAX || c.width < (c.f32() ? KEEP_WIDTH_F32 : KEEP_WIDTH_BF16)) return k;
+  if (c.n > ROWS_MAX && c.width < (c.f32() ? KEEP_WIDTH_F32 : KEEP_WIDTH_BF16)) return k;
   k.ld = up(c.vocab, BM);
-  k.block = c.f32() ? BM32 / 2 : forward.bn == 256 ? BM / 2 : BM / 4;
+  k.block = forward.rows ? 16 : c.f32() ? BM32 / 2 : forward.bn == 256 ? BM / 2 : BM / 4;
   Carver at;
   at.take(c.n * k.ld * (c.f32() ? 4 : 2));
-  k.o_base = at.take(k.ld / k.block * forward.n_pad * 4);
+  k.o_base = at.take(k.ld / k.block * c.n * 4);
   k.o_lp = at.take(c.n * 4);
   k.bytes = at.at <= KEEP_BYTES ? at.at : 0;
   return k;
@@ -1520,7 +1537,7 @@ int32_t forward(const Call& c, const Plan& p, const Forward& f, void* d_work, in
     float *base = (float*)(f.kept + kept.o_base), *lp_kept = (float*)(f.kept + kept.o_lp);
     auto finish = [&](auto* kernel, int64_t blocks, int threads) {
       kernel<<<(unsigned)blocks, threads, 0, s>>>(parts, (float*)(ws + p.o_cut), c.n, c.vocab, c.y, f.lp, f.lse, f.kept, c.f32(), kept.ld,
-                                                  base, kept.block, p.n_pad, lp_kept, f.key0, f.key1, f.offset, f.out);
+                                                  base, kept.block, lp_kept, f.key0, f.key1, f.offset, f.out);
     };
     if (c.vocab <= 256) finish(k_lincat_finish<64, EPI>, up(c.n, 4) / 4, GJX_BLOCK);
     else if (c.vocab <= 1024) finish(k_lincat_finish<256, EPI>, c.n, 256);
@@ -1528,8 +1545,8 @@ int32_t forward(const Call& c, const Plan& p, const Forward& f, void* d_work, in
     GJX_LAUNCH_CHECK();
     return GJX_OK;
   }
-  if (EPI != EPI_KEEP && p.rows) {
-    if constexpr (EPI != EPI_KEEP) rc = c.f32() ? launch_rows<float, EPI>(c, p, a, s) : launch_rows<bf16, EPI>(c, p, a, s);
+  if (p.rows) {
+    rc = c.f32() ? launch_rows<float, EPI>(c, p, a, s) : launch_rows<bf16, EPI>(c, p, a, s);
     if (rc != GJX_OK) return rc;
   } else {
     Inputs in = {};
@@ -1659,11 +1676,11 @@ GJX_API int32_t gjx_linear_categorical_grad(int32_t dtype, const int32_t* d_y, c
       const char* k = (const char*)d_kept;
       const dim3 grid((unsigned)(up(n, 64) / p.strip), (unsigned)(up(rows_pad, GJX_BLOCK * 8) / (GJX_BLOCK * 8)));
       if (f32)
-        k_lincat_dl<float><<<grid, GJX_BLOCK, 0, s>>>(k, kept.ld, (const float*)(k + kept.o_base), kept.block, p.n_pad,
+        k_lincat_dl<float><<<grid, GJX_BLOCK, 0, s>>>(k, kept.ld, (const float*)(k + kept.o_base), kept.block,
                                                       (const float*)(k + kept.o_lp), d_lse, d_upstream, d_y, n, vocab, v0, (int)rows_pad, p.strip,
                                                       (float*)(ws + p.o_dl), p.piece, resid, d_db ? db_part : nullptr, p.piece);
       else
-        k_lincat_dl<bf16><<<grid, GJX_BLOCK, 0, s>>>(k, kept.ld, (const float*)(k + kept.o_base), kept.block, p.n_pad,
+        k_lincat_dl<bf16><<<grid, GJX_BLOCK, 0, s>>>(k, kept.ld, (const float*)(k + kept.o_base), kept.block,
                                                      (const float*)(k + kept.o_lp), d_lse, d_upstream, d_y, n, vocab, v0, (int)rows_pad, p.strip,
                                                      (bf16*)(ws + p.o_dl), p.piece, resid, d_db ? db_part : nullptr, p.piece);
       GJX_LAUNCH_CHECK();

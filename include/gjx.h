@@ -146,7 +146,7 @@ int32_t gjx_categorical_logpdf_f32(const int32_t* d_x, const float* d_logits, in
  * entry left is NaN.  The caller owns the workspace (256-byte aligned, gjx_linear_categorical_workspace bytes; kind:
  * 0 for the log-density, 1 for the gradient, 2 for the gradient without d_dx); its contents need not be kept between calls.
  * kind 3 gives the bytes of d_kept (nullable, 256-byte aligned): what the log-density may leave for the gradient, which then
- * does not form the logits again; 0 where they gain nothing by it (up to 32 rows, small widths) or pass 2 GiB.
+ * does not form the logits again; 0 where they gain nothing by it (more than 32 rows of small widths) or pass 2 GiB.
  * The inputs are finite (bias: or -inf).
  *   logpdf: lp_i = l_{i, y_i} - lse_i, lse_i = log sum_v exp(l_iv) (d_lse nullable)
  *   grad:   outputs (nullable) dx, dW, db of sum_i upstream_i lp_i, contiguous, of type dtype (what jax.grad of

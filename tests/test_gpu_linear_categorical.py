@@ -7,7 +7,7 @@ Tolerances (per element, from the arithmetic):
  * lse: the exponentials' relative errors (2 E and 2^-22 of expf) and at most 256 additions in a chain, 2^-16 in all;
    the subtraction and the logarithm round once more, 2^-22 of |l| + |lse|;
  * dl = g (onehot - p): p is off by (2 E + 2^-15) p, and dl is rounded to bf16 (2^-8) or split exactly (f32, 2^-22); where
-   the forward keeps its exponentials in 11 bits for it (bf16, above 32 rows, from a width of 512 on) by |g| (2^-11 p + 2^-40) more;
+   the forward keeps its exponentials in 11 bits for it (bf16, up to 32 rows or from a width of 512 on) by |g| (2^-11 p + 2^-40) more;
  * dx, dW, db: the products' sums over m terms in f32 add 2 m 2^-23 sum |terms|; the result is rounded once to its type."""
 import numpy as np
 import pytest
@@ -51,7 +51,7 @@ def _truth(x, w, b, y, up):
     D.scatter_add_(1, Y, u)
     half = HALF[x.dtype]
     dD = D.abs() * (half if x.dtype == torch.bfloat16 else 2.0 ** -22) + u.abs() * P * (2 * E + 2.0 ** -15)
-    if x.dtype == torch.bfloat16 and n > 32 and width >= 512:      # formed from what the forward kept
+    if x.dtype == torch.bfloat16 and (n <= 32 or width >= 512):      # formed from what the forward kept
         dD += u.abs() * (P * 2.0 ** -11 + 2.0 ** -40)
     out = {"lp": (lp, lp_tol)}
     dx, dw, db = D @ W, D.t() @ X, D.sum(0)
@@ -316,7 +316,7 @@ def test_same_bits_on_every_call(G):
 
 
 # ---- what the forward keeps for the gradient ---------------------------------
-# Above 32 rows and from a width of 128 (f32) or 512 (bf16) on, the gradient is formed from the forward's exponentials.  In
+# Up to 32 rows, and from a width of 128 (f32) or 512 (bf16) on, the gradient is formed from the forward's exponentials.  In
 # f32 they are kept as they are: exp(l - base) and exp(base - lse) share the error that exp(l - lse) had.  In bf16 they are
 # kept in 11 bits (2^-11, and 2^-40 of the block's largest absolutely), before dl is rounded as everywhere.
 def _check_kept(G, n, vocab, width, dtype, bias=True):
@@ -343,12 +343,12 @@ def _check_kept(G, n, vocab, width, dtype, bias=True):
             assert torch.equal(p, g) if wanted else p is None
 
 
-@pytest.mark.parametrize("n,vocab,width", [(33, 2, 128), (33, 300, 257), (64, 257, 300), (130, 4099, 512), (200, 50001, 256), (1000, 140001, 256)])
+@pytest.mark.parametrize("n,vocab,width", [(1, 1, 1), (1, 70, 33), (16, 1000, 100), (17, 9000, 65), (32, 129, 1100), (33, 2, 128), (33, 300, 257), (64, 257, 300), (130, 4099, 512), (200, 50001, 256), (1000, 140001, 256)])
 def test_gradient_from_what_the_forward_kept_f32(G, n, vocab, width):
     _check_kept(G, n, vocab, width, torch.float32, bias=vocab != 300)
 
 
-@pytest.mark.parametrize("n,vocab,width", [(33, 2, 512), (33, 300, 1030), (100, 511, 576), (257, 70000, 1024), (4000, 70001, 1024)])
+@pytest.mark.parametrize("n,vocab,width", [(1, 1, 1), (1, 70, 33), (16, 1000, 100), (17, 9000, 65), (32, 129, 2100), (33, 2, 512), (33, 300, 1030), (100, 511, 576), (257, 70000, 1024), (4000, 70001, 1024)])
 def test_gradient_from_what_the_forward_kept_bf16(G, n, vocab, width):
     _check_kept(G, n, vocab, width, torch.bfloat16, bias=vocab != 300)
 

@@ -53,19 +53,19 @@ def test_linear_categorical_abi_refusals():
     assert code(n=(1 << 24) + 1) == -4 and code(vocab=(1 << 24) + 1) == -4
     assert code(width=65537, x_ld=65537, w_ld=65537) == -4
     assert code(n=0, y=None, x=None, w=None, lp=None, lse=None, work=None, work_bytes=0) == 0       # nothing to do
-    assert code(kept=p, kept_bytes=1 << 30) == -1 and b"nothing is kept" in L.gjx_last_error()      # few rows keep nothing
+    assert code(n=100, kept=p, kept_bytes=1 << 30) == -1 and b"nothing is kept" in L.gjx_last_error()      # small widths keep nothing
     sizes = dict(n=100, vocab=5, width=256, x_ld=256, w_ld=256)
     assert L.gjx_linear_categorical_workspace(0, p, 256, p, 256, 100, 5, 256, 3, C.byref(size)) == 0 and size.value > 100 * 256 * 4
     assert code(kept=p, kept_bytes=size.value - 1, **sizes) == -1 and b"d_kept" in L.gjx_last_error()
     assert code(kept=C.c_void_p((1 << 20) + 16), kept_bytes=size.value, **sizes) == -1
-    for n, vocab, width, dtype in ((32, 1000, 512, 0), (100, 1000, 127, 0), (100, 1000, 511, 1), (1 << 20, 1 << 20, 512, 0)):
+    for n, vocab, width, dtype in ((33, 1000, 127, 0), (100, 1000, 127, 0), (100, 1000, 511, 1), (1 << 20, 1 << 20, 512, 0)):
         assert L.gjx_linear_categorical_workspace(dtype, p, width, p, width, n, vocab, width, 3, C.byref(size)) == 0 and size.value == 0
 
     def grad(lse=p, up=p, kept=None, kept_bytes=0, work_bytes=1 << 30):
         return L.gjx_linear_categorical_grad(0, p, p, 8, p, 8, None, 3, 5, 8, lse, up, kept, kept_bytes, p, p, p, p, work_bytes, None)
 
     assert grad(lse=None) == -1 and grad(up=None) == -1 and grad(work_bytes=16) == -1
-    assert grad(kept=p, kept_bytes=1 << 30) == -1
+    assert grad(kept=p, kept_bytes=1) == -1
     key = (C.c_uint32 * 2)(0, 1)
     assert L.gjx_random_linear_categorical_i32(key, 0, 0, p, 8, p, 8, None, 3, 5, 8, None, p, 1 << 30, None) == -1
 
