@@ -66,6 +66,7 @@ struct GemmArgs {
   float2* part;        // [tile m][n_pad]: (max, sum exp) of a row over one tile; drawing: (largest l + Gumbel, its entry)
   float* target;       // logit of y
   void* keep;          // EPI_KEEP: [n][keep_ld] exp(l - base), f32 or f16 x 2^15, base the row's largest l of a wave's block of entries
+                       // (-inf where none is left: the entries are 0, and so is their factor exp(base - lse), however small lse is)
   float* keep_base;    // [v / block][n]
   int64_t keep_ld;
   int64_t n_pad;
@@ -373,7 +374,7 @@ __device__ __forceinline__ void epilogue(const GemmArgs& g, const Tile& tile, f3
       sum += __shfl_xor(sum, 32);
       if (EPI == EPI_KEEP && n < g.n) {
         const int64_t v = g.v0 + m0 + wm;
-        if (q == 0) g.keep_base[v / (MT * 16) * g.n + n] = base;
+        if (q == 0) g.keep_base[v / (MT * 16) * g.n + n] = top;
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
           if (sizeof(T) == 2) {
@@ -851,7 +852,7 @@ __global__ void __launch_bounds__(GJX_BLOCK)
       sum += __shfl_xor(sum, 16);
       sum += __shfl_xor(sum, 32);
       if (EPI == EPI_KEEP && n < g.n) {
-        if (q == 0) g.keep_base[(int64_t)(v0 / 16) * g.n + n] = base;
+        if (q == 0) g.keep_base[(int64_t)(v0 / 16) * g.n + n] = top;
         if (sizeof(T) == 2) {
           f16x4 h;
 #pragma unroll

@@ -456,3 +456,34 @@ def test_few_tiles_and_long_rows(G, n, vocab, width, dtype):
     E = 2 * width * 2.0 ** -23 * (x.double().abs() @ w.double().abs().t()).max(1)[0]
     assert (best - z.gather(1, got.long().unsqueeze(1)).squeeze(1) <= 2 * E + 1e-4).all()
     assert vocab < 2 or (got != 1).all() or vocab <= 2
+
+
+def _far_below(G, n, vocab, width, dtype, shift, masked=None):
+    """Gradients where every logit lies `shift` below 0, entries `masked` taken out: a common shift changes no probability."""
+    x, w, b, y, up = _inputs(n, vocab, width, dtype)
+    b = (b.float() + shift).to(dtype)
+    if masked is not None:
+        b[masked] = -float("inf")
+        y = torch.full_like(y, vocab - 1)
+    t = _truth(x, w, b, y, up)
+    # a logit of this size is rounded to 2^-24 of it after the bias is added: dl moves by twice that of p
+    P = torch.softmax(x.double() @ w.double().t() + b.double(), 1) * up.double().abs().unsqueeze(1) * 2.0 ** -23 * (abs(shift) + 16)
+    more = (0.0, P @ w.double().abs(), P.t() @ x.double().abs(), P.sum(0))
+    for name, got, m in zip(("lp", "dx", "dw", "db"), _grads(G, x, w, b, y, up), more):
+        assert torch.isfinite(got).all(), name
+        _close(name, got, (t[name][0], t[name][1] + m))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("n", [1, 17, 32, 70])
+@pytest.mark.parametrize("vocab", [1, 7, 16, 33, 65, 257, 1040])
+def test_gradient_of_logits_far_below_zero(G, n, vocab, dtype):
+    """Entries behind the vocabulary stand in the products' tiles beside logits near -300."""
+    _far_below(G, n, vocab, 64 if n <= 32 else 576, TYPES[dtype], -300.0)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("n,width", [(1, 64), (32, 64), (70, 576), (300, 576), (300, 64)])
+def test_gradient_beside_masked_blocks_far_below_zero(G, n, width, dtype):
+    """Whole blocks of entries without one that is left, logits near -120 elsewhere."""
+    _far_below(G, n, 1300, width, TYPES[dtype], -120.0, slice(100, 1000))
