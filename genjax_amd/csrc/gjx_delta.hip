@@ -14,8 +14,12 @@
 //   E = scale D (dO V'^T), F = -beta_i D_ij (e_i.V'_j)  (i > j),
 //   dQ = scale e^gamma dO S0^T + E K,  dK as what is read = -beta e^gamma e S0^T + F K,
 //   dK as what is written = E^T Q + F^T K + e^(gamma_C - gamma) V' dS1^T,
-//   dgamma_i = q_i.dq_i + k_i.dk_i(read) - k_i.dk_i(written), + <dS1, S1> at the chunk's end,
-//   dg = reverse cumsum of dgamma within the chunk                               (k_delta_back, all chunks at once).
+//   dg_t = sum of what the decay of token t stands in, each term with it as a factor (k_delta_back, all chunks at once):
+//     q_i.(scale e^gamma dO S0^T)_i - k_i.(beta e^gamma e S0^T)_i  (i >= t)    what later tokens read of S0,
+//     X_ij = E_ij q_i.k_j + F_ij k_i.k_j  (i >= t > j)                         what they read of earlier tokens,
+//     k_j.(e^(gamma_C - gamma) V' dS1^T)_j  (j < t) and e^gamma_C <dS1, S0>    what S1 holds of earlier tokens and of S0.
+//   (As a reverse cumsum of dgamma_i = q_i.dq_i + k_i.dk_i(read) - k_i.dk_i(written), terms without that factor stand in
+//   the sums and cancel in exact arithmetic only: at log-decays below -10 what they leave behind was all of dg.)
 //
 // Arithmetic: 16x16x32 bf16 MFMA with f32 accumulators.  Whatever is not an input in bf16 is split into three bf16 planes
 // (8 bits each) and multiplied in the partial products above 2^-23, so that states, gains and gradients keep f32
@@ -162,9 +166,6 @@ __device__ __forceinline__ constexpr int lower(int i, int s) { return i < 2 ? i 
 __device__ __forceinline__ constexpr int upper(int i, int s) { return i < 2 ? 2 * i + s : 4 + (i - 2); }
 
 __device__ __forceinline__ int perm(int s, int q, int j) { return 32 * s + (j < 4 ? 4 * q + j : 12 + 4 * q + j); }
-
-template <typename T>
-__device__ __forceinline__ float to_f32(T v) { return (float)v; }
 
 __device__ __forceinline__ int64_t length_of(const int32_t* lengths, int64_t b, int64_t time) {
   return lengths ? std::min<int64_t>(std::max<int64_t>(lengths[b], 0), time) : time;
@@ -1066,12 +1067,14 @@ __global__ void __launch_bounds__(BACK)
   constexpr int MT = DKP / 16, MH = MT / 4;               // tiles of dk; of one wave
   constexpr int F_S0 = 0, F_S1 = MT * 3 * FRAG, F_E = 2 * F_S1, F_D = F_E + 12 * FRAG, F_O = F_D + 12 * FRAG, F_ALL = F_O + 4 * NPI * FRAG;
   constexpr int E_ROW = 0, F_ROW = 24 * FRAG, E_COL = 48 * FRAG, F_COL = 72 * FRAG, EF_ALL = 96 * FRAG;     // [tile][slab][plane]
+  constexpr int KS = DKP / 32, SLABS = NPI == 1 ? KS : 1, TURNS = NPI == 1 ? 2 : 1;       // f32: registers for one slab at a time
   constexpr int LO = DKP + 4;                             // row of dq or dk in LDS: the four quads of a wave miss each other's banks
   constexpr int RESULTS = 2 * C * LO * 4;
   __shared__ __attribute__((aligned(16))) char buffer[std::max(std::max(F_ALL, EF_ALL) * 2, RESULTS)];
-  __shared__ float s_gh[C], s_gl[C], s_row[4][C], s_db[C], s_put[16];
+  __shared__ float s_gh[C], s_gl[C], s_db[C];
+  __shared__ float s_x[C * LD], s_pair[16][C];            // X; its sums over i >= t > j, a wave's rows i
+  __shared__ float s_read[4][C], s_put[4][C];             // a token's terms that read S0 and that write S1, by dk quarter
   __shared__ double s_sum[16];
-  __shared__ int s_state[16];                             // whether S0 has an entry other than 0
   bf16* frag = (bf16*)buffer;
   float *sq = (float*)buffer, *sk = sq + C * LO;          // dq and dk, once E and F are
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quad = lane >> 4, c = lane & 15;
@@ -1158,7 +1161,6 @@ __global__ void __launch_bounds__(BACK)
 #pragma unroll
   for (int t = 0; t < MH; ++t) m1[t] = m2[t] = m3[t] = f32x4{0, 0, 0, 0};
   float dot = 0.0f, db = 0.0f;
-  bool any = false;
   const int slabs = sh.dvp / 32;
   load(0);
   for (int s = 0; s < slabs; ++s) {
@@ -1166,10 +1168,7 @@ __global__ void __launch_bounds__(BACK)
       put4(F_S0, 3, row, x0);
       put4(F_S1, 3, row, x1);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        dot += x0[j] * x1[j];
-        any |= x0[j] != 0.0f;
-      }
+      for (int j = 0; j < 4; ++j) dot += x0[j] * x1[j];
     }
     if (first) {
       put4(F_E, 3, trow, x2);
@@ -1207,11 +1206,7 @@ __global__ void __launch_bounds__(BACK)
     double d = has_state ? (double)dot : 0.0;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) d += __shfl_xor(d, o);
-    const uint64_t some = __ballot(any);
-    if (lane == 0) {
-      s_sum[wave] = d;
-      s_state[wave] = some != 0;
-    }
+    if (lane == 0) s_sum[wave] = d;
     db += __shfl_xor(db, 1);
     db += __shfl_xor(db, 2);
     db += __shfl_xor(db, 4);
@@ -1225,6 +1220,22 @@ __global__ void __launch_bounds__(BACK)
       const float d = jj <= i ? expf((s_gh[i] - s_gh[jj]) + (s_gl[i] - s_gl[jj])) * rb[jj] : 0.0f;
       ev[r] = jj <= i ? sh.scale * d * pe[r] : 0.0f;
       fv[r] = jj < i ? -rb[i] * d * pf[r] : 0.0f;
+    }
+    f32x4 qk = {0, 0, 0, 0}, kk = {0, 0, 0, 0};
+    if (wh <= wt)
+#pragma unroll SLABS
+      for (int s = 0; s < KS; ++s) {
+        bf16x8 fq[NPI], fi[NPI], fj[NPI];
+        load_frag<NPI>(kb + KB::QA, wt * KS + s, 4 * KS * FRAG, lane, fq);
+        load_frag<NPI>(kb + KB::KA, wt * KS + s, 4 * KS * FRAG, lane, fi);
+        load_frag<NPI>(kb + KB::KA, wh * KS + s, 4 * KS * FRAG, lane, fj);
+        qk = mma_planes<NPI, NPI, NPI>(fq, fj, qk);
+        kk = mma_planes<NPI, NPI, NPI>(fi, fj, kk);
+      }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int i = 16 * wt + 4 * quad + r, jj = 16 * wh + c;
+      s_x[i * LD + jj] = jj < i ? ev[r] * qk[r] + fv[r] * kk[r] : 0.0f;      // (E_ii does not hang on the decay)
     }
     // their transposes (rows of the operand: jj; reduction: i) as they lie in the registers; themselves entry by entry
     put_half<3>(frag + E_COL + (wh * 2 + (wt >> 1)) * 3 * FRAG, wt & 1, lane, ev);
@@ -1253,18 +1264,30 @@ __global__ void __launch_bounds__(BACK)
     m2[t] *= -(be * eg);
     m3[t] *= be * rest;
   }
-  f32x4 last[MH];
-  float qv[MH][4], kv[MH][4];                             // q and k where dq and dk are: entries of the fragments at hand
-#pragma unroll
-  for (int t = 0; t < MH; ++t) last[t] = m3[t];
-#pragma unroll
-  for (int s = 0; s < 2; ++s) {
+  f32x4 sum = {0, 0, 0, 0}, put = {0, 0, 0, 0};
+#pragma unroll TURNS
+  for (int u = 0; u < 2; ++u) {                           // the slab of this wave's tokens, then the other
+    const int s = u ^ (wt >> 1);
     bf16x8 kt[MH][NPI], qt[MH][NPI];
 #pragma unroll
     for (int t = 0; t < MH; ++t) {
       load_frag<NPI>(kb + KB::KT, (wh * MH + t) * 2 + s, MT * 2 * FRAG, lane, kt[t]);
       load_frag<NPI>(kb + KB::QT, (wh * MH + t) * 2 + s, MT * 2 * FRAG, lane, qt[t]);
     }
+    if (u == 0)                                           // q and k where dq and dk are: entries of the fragments at hand
+#pragma unroll
+      for (int t = 0; t < MH; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {                     // (tokens behind the end and columns behind dk: q and k are 0)
+          float qv = 0.0f, kv = 0.0f;
+#pragma unroll
+          for (int p = NPI - 1; p >= 0; --p) {
+            qv += (float)(wt & 1 ? qt[t][p][4 + r] : qt[t][p][r]);
+            kv += (float)(wt & 1 ? kt[t][p][4 + r] : kt[t][p][r]);
+          }
+          sum[r] += qv * m1[t][r] + kv * m2[t][r];
+          put[r] += kv * m3[t][r];
+        }
     if (s <= wt >> 1) {                                   // (E and F are lower triangular)
       bf16x8 fe[3], ff[3];
       get_frag<3>(frag + E_ROW + (wt * 2 + s) * 3 * FRAG, lane, fe);
@@ -1285,43 +1308,44 @@ __global__ void __launch_bounds__(BACK)
         m3[t] = mma_planes<3, NPI, 3>(ff, kt[t], m3[t]);
       }
     }
-    if (s == wt >> 1)
-#pragma unroll
-      for (int t = 0; t < MH; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          qv[t][r] = kv[t][r] = 0.0f;
-#pragma unroll
-          for (int p = NPI - 1; p >= 0; --p) {
-            qv[t][r] += (float)(wt & 1 ? qt[t][p][4 + r] : qt[t][p][r]);
-            kv[t][r] += (float)(wt & 1 ? kt[t][p][4 + r] : kt[t][p][r]);
-          }
-        }
   }
+  float pair = 0.0f;                                      // lane t: rows i >= t of every sixteenth, columns j < t
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int i = 16 * u + wave;
+    float x = s_x[i * LD + lane];
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const float before = __shfl_up(x, o);
+      if (lane >= o) x += before;
+    }
+    x = __shfl_up(x, 1);
+    pair += lane > 0 && i >= lane ? x : 0.0f;
+  }
+  s_pair[wave][lane] = pair;
   __syncthreads();                                        // the fragments of E and F are used up
-  f32x4 sum = {0, 0, 0, 0}, put = {0, 0, 0, 0};
 #pragma unroll
   for (int t = 0; t < MH; ++t) {
     const int col = 16 * (wh * MH + t) + c;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int i = 16 * wt + 4 * quad + r;               // (tokens behind the end and columns behind dk: q, k, E, F are 0)
-      sum[r] += qv[t][r] * m1[t][r] + kv[t][r] * (m2[t][r] - m3[t][r]);
-      put[r] += kv[t][r] * last[t][r];
+      const int i = 16 * wt + 4 * quad + r;
       sq[i * LO + col] = i < left ? m1[t][r] : 0.0f;
       sk[i * LO + col] = i < left ? m2[t][r] + m3[t][r] : 0.0f;
     }
   }
-  float all = put[0] + put[1] + put[2] + put[3];
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) all += __shfl_xor(all, o);
-  if (lane == 0) s_put[wave] = all;
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
-    float s = sum[r];
+    float a = sum[r], b = put[r];
 #pragma unroll
-    for (int o = 1; o < 16; o <<= 1) s += __shfl_xor(s, o);
-    if (c == 0) s_row[wh][16 * wt + 4 * quad + r] = s;
+    for (int o = 1; o < 16; o <<= 1) {
+      a += __shfl_xor(a, o);
+      b += __shfl_xor(b, o);
+    }
+    if (c == 0) {
+      s_read[wh][16 * wt + 4 * quad + r] = a;
+      s_put[wh][16 * wt + 4 * quad + r] = b;
+    }
   }
   __syncthreads();
   // out of LDS in rows: pieces of eight columns (stored from the accumulators, two bytes a lane, the kernel took 139 us instead
@@ -1337,22 +1361,22 @@ __global__ void __launch_bounds__(BACK)
     else store8((is_k ? dk : dq) + p, x, n, vec_out);
   }
   if (wave == 0) {
-    double s = (double)s_row[0][lane] + (double)s_row[1][lane] + (double)s_row[2][lane] + (double)s_row[3][lane];
+    double reads = 0.0, puts = 0.0, s = 0.0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      reads += (double)s_read[i][lane];
+      puts += (double)s_put[i][lane];
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s += (double)s_pair[i][lane] + (double)rb[3 * C] * s_sum[i];
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-      const double down = __shfl_down(s, o);
-      if (lane + o < 64) s += down;
+      const double later = __shfl_down(reads, o), earlier = __shfl_up(puts, o);
+      if (lane + o < 64) reads += later;
+      if (lane >= o) puts += earlier;
     }
-    double end = 0.0, written = 0.0;
-    int state = 0;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      state |= s_state[i];
-      end += s_sum[i];
-      written += (double)s_put[i];
-    }
-    s += (double)rb[3 * C] * end + written;
-    if (lane == 0 && !state) s = 0.0;                     // <dS0, S0> of an empty state: exactly 0, not the sums' rounding
+    puts = __shfl_up(puts, 1);
+    s += reads + (lane > 0 ? puts : 0.0);
     if (lane < left_o) {
       dg[g_at + (int64_t)lane * sh.heads] = lane < left ? (float)s : 0.0f;
       dbeta[g_at + (int64_t)lane * sh.heads] = lane < left ? s_db[lane] : 0.0f;

@@ -329,3 +329,36 @@ def test_first_decay_of_an_empty_state_has_no_gradient(S, time, dtype):
         grads = torch.autograd.grad([o, last], leaves, [d_o, d_state])
         assert not grads[3][:, 0].any() and (time == 1 or grads[3][:, 1].any())
         assert all(g.any() for i, g in enumerate(grads) if i != 3)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("low,high", [(-25.0, -8.0), (-40.0, -39.0), (-9.0, -0.01)])
+@pytest.mark.parametrize("time,kheads,heads,dk,dv,state", [(1, 1, 2, 64, 64, True), (65, 1, 2, 32, 48, True), (130, 2, 2, 128, 40, True),
+                                                           (70, 1, 1, 50, 33, False)])
+def test_gradient_of_strong_decays(S, time, kheads, heads, dk, dv, state, low, high, dtype):
+    """dg_t = a_t <G_t, S_{t-1}>, G_t the gradient of the decayed state: each entry is held against its own size,
+    a_t |G_t| |S_{t-1}| (Cauchy and Schwarz bound every term of its sums by that), however small the decay is."""
+    a, d_o, d_state = _inputs(2, time, kheads, heads, dk, dv, TYPES[dtype], state=state)
+    u = torch.rand(2, time, heads, device="cuda", generator=torch.Generator("cuda").manual_seed(time))
+    a["log_decay"] = low + (high - low) * u
+    leaf = {n: t.detach().double() for n, t in a.items() if t is not None}
+    q, k = (leaf[n].repeat_interleave(heads // kheads, 2) for n in "qk")
+    mem = leaf.get("state", torch.zeros(2, heads, dk, dv, dtype=torch.float64, device="cuda"))
+    before, faded, outs = [], [], []
+    for t in range(time):
+        before.append(mem)
+        new = (mem * leaf["log_decay"][:, t].exp()[..., None, None]).requires_grad_(True)
+        faded.append(new)
+        w = leaf["beta"][:, t, :, None] * (leaf["v"][:, t] - (new * k[:, t, :, :, None]).sum(2))
+        mem = new + k[:, t, :, :, None] * w[:, :, None, :]
+        outs.append(dk ** -0.5 * (mem * q[:, t, :, :, None]).sum(2))
+    G = torch.autograd.grad([torch.stack(outs, 1), mem], faded, [d_o.double(), d_state.double()])
+    decay = leaf["log_decay"].exp()
+    before = [b.detach() for b in before]
+    want = decay * torch.stack([(g * b).sum((2, 3)) for g, b in zip(G, before)], 1)
+    size = decay * torch.stack([g.norm(dim=(2, 3)) * b.norm(dim=(2, 3)) for g, b in zip(G, before)], 1)
+    leaves = [a[n].clone().requires_grad_(True) for n in NAMES[:5]]
+    o, last = S.delta_filter(*leaves, initial_state=a["state"])
+    got = torch.autograd.grad([o, last], leaves, [d_o, d_state])[3]
+    worst = ((got.double() - want).abs() / (2.0 ** -14 * size + 2.0 ** -126)).max().item()
+    assert worst <= 1.0, f"{worst:.3g} times its bound"
