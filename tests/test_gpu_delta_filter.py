@@ -362,3 +362,39 @@ def test_gradient_of_strong_decays(S, time, kheads, heads, dk, dv, state, low, h
     got = torch.autograd.grad([o, last], leaves, [d_o, d_state])[3]
     worst = ((got.double() - want).abs() / (2.0 ** -14 * size + 2.0 ** -126)).max().item()
     assert worst <= 1.0, f"{worst:.3g} times its bound"
+
+
+# 320 or 384 tiles of 16 columns: more than the 256 up to which a workgroup of the scans takes one of them
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("batch,time,kheads,heads,dk,dv", [(5, 130, 8, 8, 50, 112), (5, 200, 8, 8, 128, 112), (2, 330, 3, 12, 64, 250),
+                                                           (3, 70, 2, 64, 20, 17)])
+def test_wide_scans_over_several_chunks(S, batch, time, kheads, heads, dk, dv, dtype):
+    assert batch * heads * (-(-dv // 32) * 2) > 256
+    a, d_o, d_state = _inputs(batch, time, kheads, heads, dk, dv, TYPES[dtype])
+    _check(S, a, d_o, d_state)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_wide_scans_of_ragged_sequences(S, dtype):
+    a, d_o, d_state = _inputs(6, 150, 2, 8, 100, 100, TYPES[dtype], state=False)
+    lengths = torch.tensor([0, 1, 64, 65, 127, 150], dtype=torch.int32, device="cuda")
+    _check(S, a, d_o, d_state, lengths=lengths)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("slow", [False, True])
+def test_many_chunks(S, dtype, slow):
+    """70 chunks.  What is forgotten within a chunk keeps the bounds of few chunks; with decays of 0.001 a token the
+    roundings of all 70 add up, 18 times those of the four chunks that the bounds count (2^-11 and 2^-9)."""
+    a, d_o, d_state = _inputs(1, 4485, 1, 2, 64, 32, TYPES[dtype])
+    if slow:
+        a["log_decay"] = a["log_decay"] * 0.004
+    o, last, leaf = _truth(a)
+    mine = {n: t.detach().clone().requires_grad_(True) for n, t in a.items()}
+    got = S.delta_filter(*(mine[n] for n in NAMES[:5]), initial_state=mine["state"])
+    more = 32.0 if slow else 1.0
+    _close("o", got[0].detach(), o.detach(), 2.0 ** -15 * more)
+    _close("state", got[1].detach(), last.detach(), 2.0 ** -16 * more)
+    want = torch.autograd.grad([o, last], [leaf[n] for n in NAMES], [d_o.double(), d_state.double()])
+    for n, x, y in zip(NAMES, torch.autograd.grad(got, [mine[n] for n in NAMES], [d_o, d_state]), want):
+        _close("d" + n, x, y, 2.0 ** -14 * more)

@@ -487,3 +487,45 @@ def test_gradient_of_logits_far_below_zero(G, n, vocab, dtype):
 def test_gradient_beside_masked_blocks_far_below_zero(G, n, width, dtype):
     """Whole blocks of entries without one that is left, logits near -120 elsewhere."""
     _far_below(G, n, 1300, width, TYPES[dtype], -120.0, slice(100, 1000))
+
+
+@pytest.mark.parametrize("n,vocab,width,dtype", [(4000, 70001, 64, "bf16"), (2000, 70001, 65, "f32"), (1000, 560001, 130, "f32")])
+def test_gradient_formed_again_in_pieces_of_the_vocabulary(G, n, vocab, width, dtype):
+    """Nothing is kept (too narrow, or above 2 GiB) and dl passes 512 MiB: each piece adds to dx, fills its own rows of dW and
+    db, and holds the values of its own entries."""
+    from genjax_amd import backend as B
+
+    t = TYPES[dtype]
+    x, w, b, y, up = _inputs(n, vocab, width, t)
+    assert B.linear_categorical_logpdf(y, x, w, b, keep=True)[2] is None
+    half = -(-(-(-vocab // 2)) // 256) * 256                # where the second of two equal pieces begins
+    for i, v in enumerate((0, half - 1, half, half + 1, vocab - 1)):
+        y[7 * i:7 * i + 7] = v
+    want = _truth(x, w, b, y, up)
+    for name, got in zip(("lp", "dx", "dw", "db"), _grads(G, x, w, b, y, up)):
+        _close(name, got, want[name])
+
+
+@pytest.mark.parametrize("n", [40, 70])
+def test_packed_weights_in_pieces(G, n):
+    """bf16 weights whose rows are packed for the tile loader, 547 MiB of them: two pieces."""
+    from genjax_amd import backend as B
+
+    vocab, width = 140001, 2000
+    x, w, b, y, up = _inputs(n, vocab, width, torch.bfloat16)
+    half = -(-(-(-vocab // 2)) // 256) * 256
+    y[:3] = torch.tensor([half - 1, half, vocab - 1], dtype=torch.int32, device="cuda")
+    want = _truth(x, w, b, y, up)
+    for name, got in zip(("lp", "dx", "dw", "db"), _grads(G, x, w, b, y, up)):
+        _close(name, got, want[name])
+    lp, lse = B.linear_categorical_logpdf(y, x, w, b)
+    _close("lp that keeps nothing", lp, want["lp"])
+    for name, got in zip(("dx", "dw", "db"), B.linear_categorical_grad(y, x, w, b, lse, up)):
+        _close(name + " formed again", got, want[name])
+    key = G.key(5)
+    got = B.sample_linear_categorical(key, x, w, b)
+    u = B.random_uniform(key, n * vocab, 1.17549435e-38, 1.0).double().reshape(n, vocab)
+    z = x.double() @ w.double().t() + b.double() - (-u.log()).log()
+    E = 2 * width * 2.0 ** -23 * (x.double().abs() @ w.double().abs().t()).max(1)[0]
+    assert (z.max(dim=1)[0] - z.gather(1, got.long().unsqueeze(1)).squeeze(1) <= 2 * E + 1e-4).all()
+    assert (got >= half).any() and (got < half).any()
