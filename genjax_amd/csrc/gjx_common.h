@@ -161,6 +161,14 @@ static inline int gjx_grid_for(int64_t n) {
   return (int)(b > GJX_MAX_GRID ? GJX_MAX_GRID : b);
 }
 
+// A workgroup per piece of work, in rows of 2^21: a launch takes fewer than 2^32 threads along x (1024 a workgroup at
+// most).  The last row is not full: kernels return where gjx_block() is behind their last piece.
+static inline dim3 gjx_grid_rows(int64_t blocks) {
+  const int64_t row = (int64_t)1 << 21;
+  return blocks <= row ? dim3((unsigned)blocks) : dim3((unsigned)row, (unsigned)((blocks + row - 1) / row));
+}
+__device__ __forceinline__ uint32_t gjx_block() { return blockIdx.y * gridDim.x + blockIdx.x; }
+
 // Grid of the VALU-bound per-particle kernels (extend / mh / hmc).  Measured on MI355X at
 // N = 2^24 (k_loc_mh, 10 moves): 1280 blocks 4.99 ms, 2048 4.64, 4096 4.43, 8192 4.32,
 // 16384 4.26, 65536 4.27 -- many short blocks let the dispatcher even out the tail.  Re-measured with

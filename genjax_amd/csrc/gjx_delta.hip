@@ -285,7 +285,8 @@ __global__ void __launch_bounds__(256)
   float* sn = (float*)sk;                       // N
   float* st = sn + C * LD;                      // That
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, quad = lane >> 4, c = lane & 15;
-  const int64_t chunk = blockIdx.x % sh.chunks, bh = blockIdx.x / sh.chunks, b = bh / sh.heads;
+  const int64_t chunk = gjx_block() % sh.chunks, bh = gjx_block() / sh.chunks, b = bh / sh.heads;
+  if (b >= sh.batch) return;
   const int h = (int)(bh % sh.heads), kh = h / sh.group;
   const int64_t len = length_of(lengths, b, sh.time), t0 = chunk * C;
   if (t0 >= len) return;
@@ -480,7 +481,7 @@ __device__ __forceinline__ bool place_of(const Shape& sh, const int32_t* lengths
   p.reads = w >= 4;
   p.quad = p.lane >> 4;
   p.c = p.lane & 15;
-  if (!scan_place(blockIdx.x, (sh.dvp / 16 + NC - 1) / NC, sh.batch * sh.heads, p.bh, p.tile)) return false;
+  if (!scan_place(gjx_block(), (sh.dvp / 16 + NC - 1) / NC, sh.batch * sh.heads, p.bh, p.tile)) return false;
   p.b = p.bh / sh.heads;
   p.h = (int)(p.bh % sh.heads);
   p.kh = p.h / sh.group;
@@ -1079,7 +1080,8 @@ __global__ void __launch_bounds__(BACK)
   float *sq = (float*)buffer, *sk = sq + C * LO;          // dq and dk, once E and F are
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quad = lane >> 4, c = lane & 15;
   const int wt = wave & 3, wh = wave >> 2;
-  const int64_t chunk = blockIdx.x % sh.chunks, bh = blockIdx.x / sh.chunks, b = bh / sh.heads;
+  const int64_t chunk = gjx_block() % sh.chunks, bh = gjx_block() / sh.chunks, b = bh / sh.heads;
+  if (b >= sh.batch) return;
   const int h = (int)(bh % sh.heads), kh = h / sh.group;
   const int64_t len = length_of(lengths, b, sh.time), t0 = chunk * C, at = bh * sh.chunks + chunk;
   const bool shared = sh.group > 1;
@@ -1417,10 +1419,10 @@ __global__ void __launch_bounds__(256)
   __shared__ float s_q[128], s_k[128];
   __shared__ f32x4 s_pk[RG][CG], s_pq[RG][CG];
   const int tid = threadIdx.x, cg = tid % CG, rg = tid / CG;
-  const int64_t bh = blockIdx.x / col_tiles;
-  const int64_t b = bh / sh.heads;
+  const int64_t bh = gjx_block() / col_tiles, b = bh / sh.heads;
+  if (b >= sh.batch) return;
   const int h = (int)(bh % sh.heads), kh = h / sh.group;
-  const int col = (int)(blockIdx.x % col_tiles) * CG * 4 + cg * 4;
+  const int col = (int)(gjx_block() % col_tiles) * CG * 4 + cg * 4;
   if (tid < 128) {
     s_q[tid] = tid < sh.dk ? (float)q[b * sh.qs[0] + kh * sh.qs[2] + tid] : 0.0f;
     s_k[tid] = tid < sh.dk ? (float)k[b * sh.ks[0] + kh * sh.ks[2] + tid] : 0.0f;
@@ -1594,7 +1596,7 @@ bool aligned_rows(const T* p, const int64_t (&s)[3]) {
 // until the 256 CUs are taken; wider ones then read each fragment once for twice the columns
 constexpr int wide_tiles(int dkp, int npi) { return dkp == 128 && npi == 3 ? 1 : 2; }      // f32 at dk > 64: registers for one
 bool scan_wide(const Shape& sh) { return sh.batch * sh.heads * (sh.dvp / 16) > 256; }
-unsigned scan_grid(const Shape& sh, int nc) { return (unsigned)(up(sh.batch * sh.heads, 8) * (up(sh.dvp / 16, nc) / nc)); }
+dim3 scan_grid(const Shape& sh, int nc) { return gjx_grid_rows(up(sh.batch * sh.heads, 8) * (up(sh.dvp / 16, nc) / nc)); }
 
 template <typename T, int DKP, bool KEEP>
 int32_t run_filter(const Shape& sh, const T* q, const T* k, const T* v, const float* g, const float* beta, const float* state0,
@@ -1603,7 +1605,7 @@ int32_t run_filter(const Shape& sh, const T* q, const T* k, const T* v, const fl
   if (sh.chunks > 0) {
     constexpr int lds = std::max(2 * NPI * C * (DKP + 8) * 2, 2 * C * LD * 4) + C * LD * 4 + 3 * C * 4;
     GJX_CHECK_HIP(hipFuncSetAttribute((const void*)k_delta_prepare<T, DKP, NPI, KEEP>, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-    k_delta_prepare<T, DKP, NPI, KEEP><<<(unsigned)(sh.batch * sh.heads * sh.chunks), 256, lds, s>>>(
+    k_delta_prepare<T, DKP, NPI, KEEP><<<gjx_grid_rows(sh.batch * sh.heads * sh.chunks), 256, lds, s>>>(
         sh, q, k, g, beta, lengths, w, aligned_rows(q, sh.qs) && aligned_rows(k, sh.ks) && sh.dk % 8 == 0);
     GJX_LAUNCH_CHECK();
   }
@@ -1629,7 +1631,7 @@ int32_t run_grad(const Shape& sh, const float* g, const int32_t* lengths, const 
   if (sh.chunks == 0) return GJX_OK;
   const int vec_o = ((uintptr_t)d_o & 15) == 0 && sh.dv % 8 == 0;
   const int vec_out = (((uintptr_t)dq | (uintptr_t)dk) & 15) == 0 && sh.dk % 8 == 0;
-  k_delta_back<T, DKP, NPI><<<(unsigned)(sh.batch * sh.heads * sh.chunks), BACK, 0, s>>>(sh, d_o, g, lengths, dq, dk, dg, dbeta, w, vec_o, vec_out);
+  k_delta_back<T, DKP, NPI><<<gjx_grid_rows(sh.batch * sh.heads * sh.chunks), BACK, 0, s>>>(sh, d_o, g, lengths, dq, dk, dg, dbeta, w, vec_o, vec_out);
   GJX_LAUNCH_CHECK();
   if (sh.group > 1) {
     k_delta_shared_heads<T><<<gjx_grid_for(sh.batch * sh.time * sh.kheads * sh.dk), GJX_BLOCK, 0, s>>>(sh, w.dq, w.dk, dq, dk);
@@ -1643,8 +1645,8 @@ int32_t run_step(const Shape& sh, const float* state, const int32_t* anc, const 
                  const float* beta, T* o, float* out, hipStream_t s) {
   const int64_t bh = sh.batch * sh.heads;
 #define GJX_STEP(CG, R)                                                                                                       \
-  k_delta_step<T, CG, R><<<(unsigned)(bh * (up(sh.dv, CG * 4) / (CG * 4))), 256, 0, s>>>(sh, state, anc, q, k, v, g, beta, o, out, \
-                                                                                         (int)(up(sh.dv, CG * 4) / (CG * 4)))
+  k_delta_step<T, CG, R><<<gjx_grid_rows(bh * (up(sh.dv, CG * 4) / (CG * 4))), 256, 0, s>>>(sh, state, anc, q, k, v, g, beta, o, out, \
+                                                                                            (int)(up(sh.dv, CG * 4) / (CG * 4)))
   if (sh.dv <= 64) {
     if (sh.dk <= 64) GJX_STEP(16, 4);
     else GJX_STEP(16, 8);

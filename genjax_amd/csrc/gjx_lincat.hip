@@ -217,11 +217,12 @@ struct Tile {
 
 // neighbouring tiles to one XCD (workgroups go round the eight of them), eight m-tiles by all n-tiles at a time
 template <int BM, int BN>
-__device__ __forceinline__ Tile tile_of(const GemmArgs& g) {
-  int id = blockIdx.x;
-  const int total = g.mt * g.nt * g.splits, per = total / 8, extra = total % 8, xcd = id % 8;
+__device__ __forceinline__ bool tile_of(const GemmArgs& g, Tile& t) {
+  const int total = g.mt * g.nt * g.splits, per = total / 8, extra = total % 8;
+  int id = (int)gjx_block();                                  // (rows of a multiple of eight workgroups)
+  if (id >= total) return false;
+  const int xcd = id % 8;
   id = xcd * per + min(xcd, extra) + id / 8;
-  Tile t;
   t.split = id / (g.mt * g.nt);
   id -= t.split * g.mt * g.nt;
   const int group = id / (8 * g.nt), in = id - group * 8 * g.nt, height = min(8, g.mt - group * 8);
@@ -229,7 +230,7 @@ __device__ __forceinline__ Tile tile_of(const GemmArgs& g) {
   t.tn = in / height;
   t.m0 = t.tm * BM;
   t.n0 = t.tn * BN;
-  return t;
+  return true;
 }
 
 // what becomes of a tile's accumulators (rows m0 + wm + 16 i + 4 q + r, columns n0 + wn + 16 j + lane % 16); T: the operands' type
@@ -535,7 +536,8 @@ __global__ void __launch_bounds__(GEMM_THREADS)
   extern __shared__ char smem_raw[];
   LDS_AS char* smem = (LDS_AS char*)smem_raw;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const Tile tile = tile_of<BM, BN>(g);
+  Tile tile;
+  if (!tile_of<BM, BN>(g, tile)) return;
   const int kt0 = (int)((int64_t)g.ktiles * tile.split / g.splits), kt1 = (int)((int64_t)g.ktiles * (tile.split + 1) / g.splits);
 
   f32x4 acc[MT][NT];
@@ -705,7 +707,8 @@ __global__ void __launch_bounds__(GEMM32_THREADS, BN > 128 ? 2 : 3)
   constexpr int A_BYTES = BM / 16 * SPLIT_BYTES;
   extern __shared__ char smem_raw[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const Tile tile = tile_of<BM, BN>(g);
+  Tile tile;
+  if (!tile_of<BM, BN>(g, tile)) return;
   const int kt0 = (int)((int64_t)g.ktiles * tile.split / g.splits), kt1 = (int)((int64_t)g.ktiles * (tile.split + 1) / g.splits);
   f32x4 acc[MT][NT];
 #pragma unroll
@@ -1370,23 +1373,23 @@ int32_t allow_lds(K* kernel, int bytes, std::atomic<uint64_t>& done) {
 }
 
 template <int BN, bool TA, bool TB, int EPI>
-int32_t launch16(const GemmArgs& a, unsigned blocks, hipStream_t s) {
+int32_t launch16(const GemmArgs& a, int64_t blocks, hipStream_t s) {
   static std::atomic<uint64_t> done{0};
   constexpr int lds = 2 * (BM + BN) * BK * 2;
   const int32_t rc = allow_lds(k_lincat_gemm<BN, TA, TB, EPI>, lds, done);
   if (rc != GJX_OK) return rc;
-  k_lincat_gemm<BN, TA, TB, EPI><<<blocks, GEMM_THREADS, lds, s>>>(a);
+  k_lincat_gemm<BN, TA, TB, EPI><<<gjx_grid_rows(blocks), GEMM_THREADS, lds, s>>>(a);
   GJX_LAUNCH_CHECK();
   return GJX_OK;
 }
 
 template <int BN, bool TA, bool TB, int EPI>
-int32_t launch32(const GemmArgs& a, unsigned blocks, hipStream_t s) {
+int32_t launch32(const GemmArgs& a, int64_t blocks, hipStream_t s) {
   static std::atomic<uint64_t> done{0};
   constexpr int lds = (BM32 + BN) / 16 * SPLIT_BYTES;
   const int32_t rc = allow_lds(k_lincat_gemm32<BN, TA, TB, EPI>, lds, done);
   if (rc != GJX_OK) return rc;
-  k_lincat_gemm32<BN, TA, TB, EPI><<<blocks, GEMM32_THREADS, lds, s>>>(a);
+  k_lincat_gemm32<BN, TA, TB, EPI><<<gjx_grid_rows(blocks), GEMM32_THREADS, lds, s>>>(a);
   GJX_LAUNCH_CHECK();
   return GJX_OK;
 }
@@ -1395,16 +1398,16 @@ int32_t launch32(const GemmArgs& a, unsigned blocks, hipStream_t s) {
 template <bool TA, bool TB, int EPI>
 int32_t launch(const Call& c, bool wide, const GemmArgs& a, hipStream_t s) {
   const int64_t blocks = (int64_t)a.mt * a.nt * a.splits;
-  GJX_REQUIRE(blocks < ((int64_t)1 << 31), GJX_ELIMIT, "%s: %lld tiles", c.who, (long long)blocks);
+  GJX_REQUIRE(blocks < ((int64_t)1 << 31) - (1 << 21), GJX_ELIMIT, "%s: %lld tiles", c.who, (long long)blocks);
   if constexpr (TB) {           // dW: n is the vocabulary, always wide
-    return c.f32() ? launch32<128, TA, TB, EPI>(a, (unsigned)blocks, s) : launch16<256, TA, TB, EPI>(a, (unsigned)blocks, s);
+    return c.f32() ? launch32<128, TA, TB, EPI>(a, blocks, s) : launch16<256, TA, TB, EPI>(a, blocks, s);
   } else if constexpr (EPI == EPI_STORE && !TA) {            // the cut product of few tiles
-    return c.f32() ? launch32<64, TA, TB, EPI>(a, (unsigned)blocks, s) : launch16<64, TA, TB, EPI>(a, (unsigned)blocks, s);
+    return c.f32() ? launch32<64, TA, TB, EPI>(a, blocks, s) : launch16<64, TA, TB, EPI>(a, blocks, s);
   } else {
     if constexpr (EPI == EPI_SCORE || EPI == EPI_DRAW)
-      if (c.f32() && a.n_pad == ALL_ROWS) return launch32<ALL_ROWS, TA, TB, EPI>(a, (unsigned)blocks, s);
-    if (c.f32()) return wide ? launch32<128, TA, TB, EPI>(a, (unsigned)blocks, s) : launch32<64, TA, TB, EPI>(a, (unsigned)blocks, s);
-    return wide ? launch16<256, TA, TB, EPI>(a, (unsigned)blocks, s) : launch16<64, TA, TB, EPI>(a, (unsigned)blocks, s);
+      if (c.f32() && a.n_pad == ALL_ROWS) return launch32<ALL_ROWS, TA, TB, EPI>(a, blocks, s);
+    if (c.f32()) return wide ? launch32<128, TA, TB, EPI>(a, blocks, s) : launch32<64, TA, TB, EPI>(a, blocks, s);
+    return wide ? launch16<256, TA, TB, EPI>(a, blocks, s) : launch16<64, TA, TB, EPI>(a, blocks, s);
   }
 }
 

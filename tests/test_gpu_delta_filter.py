@@ -398,3 +398,19 @@ def test_many_chunks(S, dtype, slow):
     want = torch.autograd.grad([o, last], [leaf[n] for n in NAMES], [d_o.double(), d_state.double()])
     for n, x, y in zip(NAMES, torch.autograd.grad(got, [mine[n] for n in NAMES], [d_o, d_state]), want):
         _close("d" + n, x, y, 2.0 ** -14 * more)
+
+
+def test_more_workgroups_than_a_row_of_the_grid(S):
+    """2^24 (particle, head) pairs: a launch along one axis would pass 2^32 threads."""
+    n, heads = 1 << 20, 16
+    gen = torch.Generator("cuda").manual_seed(1)
+    q, k, v, g, beta = (torch.rand(*s, device="cuda", generator=gen) for s in [(n, heads, 1)] * 3 + [(n, heads)] * 2)
+    state = torch.rand(n, heads, 1, 1, device="cuda", generator=gen)
+    o, new = S.delta_filter_step(state, q, k, v, -g, beta)
+    faded = state[..., 0, 0].double() * (-g.double()).exp()
+    want = faded + k[..., 0] * beta * (v[..., 0] - faded * k[..., 0])
+    assert ((new[..., 0, 0] - want).abs() <= 2.0 ** -20).all()                  # a handful of roundings of values below 2
+    assert ((o[..., 0] - want * q[..., 0]).abs() <= 2.0 ** -19).all()
+    none = [t[:, None, :8][:, :0] for t in (q, k, v, -g, beta)]                 # no token: 2^23 workgroups of 512 threads
+    o, new = S.delta_filter(*none, initial_state=state[:, :8])
+    assert o.shape == (n, 0, 8, 1) and torch.equal(new, state[:, :8])

@@ -529,3 +529,15 @@ def test_packed_weights_in_pieces(G, n):
     E = 2 * width * 2.0 ** -23 * (x.double().abs() @ w.double().abs().t()).max(1)[0]
     assert (z.max(dim=1)[0] - z.gather(1, got.long().unsqueeze(1)).squeeze(1) <= 2 * E + 1e-4).all()
     assert (got >= half).any() and (got < half).any()
+
+
+@pytest.mark.parametrize("dtype,vocab", [("bf16", 1 << 19), ("f32", 1 << 18)])
+def test_more_tiles_than_a_row_of_the_grid(G, dtype, vocab):
+    """2^20 rows: the product's tiles along one axis would pass 2^32 threads."""
+    n, width = 1 << 20, 32
+    x, w, b, y, _ = _inputs(n, vocab, width, TYPES[dtype])
+    lp = G.linear_categorical.logpdf(y, x, w, b)
+    for i in (0, 1000, n // 2 - 1, n // 2, n - 3):
+        part = slice(i, i + 3)
+        _close("lp", lp[part], _truth(x[part], w, b, y[part], torch.ones(3, device="cuda"))["lp"])
+    assert torch.isfinite(lp).all() and (lp < 0).all()
