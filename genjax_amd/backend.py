@@ -464,14 +464,23 @@ def _address(t):
 def _note_leaves(who, out):
     """Refuse, while a graph is being captured, a differentiable call whose leaves an eager autograd graph still holds: a
     leaf's node keeps the stream it was made on, and a captured backward that reaches such a node waits across the capture
-    border, which ends the process.  (Leaves seen by this call are noted on their nodes, which live as long as the graph.)"""
+    border, which ends the process.  Leaves are noted on their nodes, which live as long as the graph; an eager call notes
+    those of the 32 nodes nearest to it (the entry points put up to two of their own between a leaf and the call, a gather or
+    a reshape and a broadcast), a captured one looks through its whole graph."""
     stream = _raw_stream()
-    for node, _ in out.grad_fn.next_functions:
-        if node is not None and hasattr(node, "variable"):
-            first = node.metadata.setdefault("gjx_stream", stream)
-            if first != stream and torch.cuda.is_current_stream_capturing():
-                raise GjxError(f"{who}: a leaf of this captured call belongs to an autograd graph that was built on another "
-                               "stream and still lives: drop that graph (its outputs) first, or capture with fresh leaves")
+    capturing = torch.cuda.is_current_stream_capturing()
+    nodes, seen = collections.deque([out.grad_fn]), set()
+    while nodes and (capturing or len(seen) < 32):
+        for down, _ in nodes.popleft().next_functions:
+            if down is None or down in seen:
+                continue
+            seen.add(down)
+            if hasattr(down, "variable"):
+                if down.metadata.setdefault("gjx_stream", stream) != stream and capturing:
+                    raise GjxError(f"{who}: a leaf of this captured call belongs to an autograd graph that was built on another "
+                                   "stream and still lives: drop that graph (its outputs) first, or capture with fresh leaves")
+            else:
+                nodes.append(down)
 
 
 class _LinearPlan:

@@ -390,3 +390,25 @@ def test_longest_rows_and_widest_states(G):
             # each side within 2^-15 of the largest entry (its own tests)
             assert ((one - o[:, t]).abs().max() <= 2.0 ** -14 * o.abs().max()).item()
         assert ((state - last).abs().max() <= 2.0 ** -14 * last.abs().max()).item()
+
+
+@pytest.mark.parametrize("which", ["row", "step"])
+def test_captured_calls_refuse_leaves_behind_the_entry_points_own_operations(G, which):
+    """As above, where the entry point itself broadcasts the leaf (a shared feature row) or adds an axis to it (one token)."""
+    from genjax_amd.families.state_space import delta_filter_step
+
+    m = _Model(kheads=1, heads=1, dk=8, dv=8)
+    tok = torch.tensor([1, 2, 3], dtype=torch.int32, device="cuda")
+    q, k, v, g, beta = m.inputs(tok)
+    leaf = (torch.ones(m.w.shape[1], device="cuda") if which == "row" else v.detach().clone()).requires_grad_(True)
+    call = (lambda: G.linear_categorical.logpdf(tok, leaf, m.w)) if which == "row" else \
+        (lambda: delta_filter_step(m.state(3), q, k, leaf, g, beta)[0])
+    alive = call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(G.GjxError, match="still lives"):
+        with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+            torch.zeros(4, device="cuda").add_(1.0)
+            call()
+    torch.cuda.synchronize()
+    assert torch.isfinite(torch.autograd.grad(alive.sum(), leaf)[0]).all()

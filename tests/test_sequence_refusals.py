@@ -226,3 +226,48 @@ def test_linear_categorical_far_rows():
     assert L.gjx_linear_categorical_workspace(0, p, (1 << 22) + 1, p, 8, 3, 5, 8, 0, C.byref(size)) == -4
     assert L.gjx_linear_categorical_workspace(0, p, 8, p, (1 << 22) + 1, 3, 5, 8, 0, C.byref(size)) == -4
     assert L.gjx_linear_categorical_workspace(0, p, 8, p, 8, 3, 5, 8, 4, C.byref(size)) == -1
+
+
+def _on_host(monkeypatch, stream, capturing):
+    """The entry points' autograd side on host tensors: kernels that return zeros, a stream that the test names."""
+    from genjax_amd import distributions as D
+
+    B = _B()
+    monkeypatch.setattr(B, "_raw_stream", lambda: stream[0])
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+    monkeypatch.setattr(B, "delta_filter", lambda q, k, v, g, beta, state, *rest, **kw: (
+        torch.zeros(v.shape), torch.zeros(v.shape[0], v.shape[2], k.shape[3], v.shape[3]), torch.zeros(1)))
+    monkeypatch.setattr(B, "linear_categorical_logpdf", lambda y, x, *rest, **kw: (torch.zeros(x.shape[0]), torch.zeros(x.shape[0]), None))
+    monkeypatch.setattr(D, "as_col", lambda t: t)
+    return B
+
+
+@pytest.mark.parametrize("which", ["state", "state by ancestors", "v", "row", "rows", "weight", "behind operations"])
+def test_captured_calls_find_the_leaves_behind_the_entry_points_own_operations(monkeypatch, which):
+    """The one-token form adds the time axis and gathers the states, a shared feature row is broadcast: the leaf stands
+    behind them all the same."""
+    from genjax_amd import linear_categorical
+    from genjax_amd.families import state_space as S
+
+    stream, capturing = [1], [False]
+    B = _on_host(monkeypatch, stream, capturing)
+    args = [t[:, 0] for t in _delta_args()]
+    ancestors = torch.zeros(2, dtype=torch.int32)
+    y, w = torch.zeros(3, dtype=torch.int32), torch.zeros(5, 8)
+    leaf = {"state": torch.zeros(2, 2, 8, 4), "state by ancestors": torch.zeros(2, 2, 8, 4), "v": args[2].clone(), "row": torch.zeros(8),
+            "rows": torch.zeros(3, 8), "weight": w.clone(), "behind operations": torch.zeros(3, 8)}[which].requires_grad_(True)
+    calls = {"state": lambda: S.delta_filter_step(leaf, *args)[0],
+             "state by ancestors": lambda: S.delta_filter_step(leaf, *args, ancestors=ancestors)[0],
+             "v": lambda: S.delta_filter_step(torch.zeros(2, 2, 8, 4), args[0], args[1], leaf, *args[3:])[0],
+             "row": lambda: linear_categorical.logpdf(y, leaf, w), "rows": lambda: linear_categorical.logpdf(y, leaf, w),
+             "weight": lambda: linear_categorical.logpdf(y, torch.zeros(3, 8), leaf),
+             "behind operations": lambda: linear_categorical.logpdf(y, (leaf * 2.0).tanh() + 1.0 if capturing[0] else leaf, w)}
+    monkeypatch.setattr(type(y), "is_cuda", property(lambda t: True))
+    alive = calls[which]()
+    stream[0] = 2
+    assert calls[which]() is not None                       # another stream, but no capture: nothing to refuse
+    capturing[0] = True
+    with pytest.raises(B.GjxError, match="still lives"):
+        calls[which]()
+    del alive
+    assert calls[which]().grad_fn is not None               # its graph is gone
