@@ -771,7 +771,8 @@ def delta_filter_step(state, q, k, v, log_decay, beta, scale=None, ancestors=Non
     state, ancestors = _delta_state(who, "state", state, p, here=False), _delta_indices(who, "ancestors", ancestors, p, here=False)
     _on_current_device(who, ("q", q), ("k", k), ("v", v), ("log_decay", log_decay), ("beta", beta), ("state", state),
                        ("ancestors", ancestors), ("out", out))
-    if out is None:
+    written = out is not None
+    if not written:
         if state.data_ptr() & 15:                               # a view into the middle of a buffer
             state = state.clone()
         out = torch.empty_like(state)
@@ -790,6 +791,8 @@ def delta_filter_step(state, q, k, v, log_decay, beta, scale=None, ancestors=Non
     from_, to = state.data_ptr(), out.data_ptr()
     if (from_ | to) & 15:
         raise GjxError(f"{who}: `state` and `out` must be aligned to 16 bytes")
+    if written and not out.is_inference():
+        torch.autograd.graph.increment_version(out)             # as an in-place operation: a graph that saved it must not use it
     o = torch.empty((p.batch, p.heads, p.dv), dtype=v.dtype, device=v.device)
     N.check(N.lib().gjx_delta_filter_step(p.ref, from_, _address(ancestors), q.data_ptr(), k.data_ptr(), v.data_ptr(),
                                           log_decay.data_ptr(), beta.data_ptr(), o.data_ptr(), to, _raw_stream()),

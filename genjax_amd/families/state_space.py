@@ -296,7 +296,7 @@ def delta_filter_step(state, q, k, v, log_decay, beta, scale=None, ancestors=Non
     the gather costs no pass of its own.  Indices are clamped to [0, n).  out: buffer for the new state -- the state
     itself (in place) when there are no ancestors.  Where a gradient is wanted the call is delta_filter over one
     token."""
-    if _wants_gradient(state, q, k, v, log_decay, beta):
+    if _wants_gradient(state, q, k, v, log_decay, beta, out):
         if out is not None:
             raise GjxError("delta_filter_step: `out` cannot be given where a gradient is wanted")
         for name, t in (("state", state), ("q", q), ("k", k), ("v", v), ("log_decay", log_decay), ("beta", beta)):

@@ -414,3 +414,24 @@ def test_more_workgroups_than_a_row_of_the_grid(S):
     none = [t[:, None, :8][:, :0] for t in (q, k, v, -g, beta)]                 # no token: 2^23 workgroups of 512 threads
     o, new = S.delta_filter(*none, initial_state=state[:, :8])
     assert o.shape == (n, 0, 8, 1) and torch.equal(new, state[:, :8])
+
+
+def test_step_into_a_buffer_that_a_graph_saved(S):
+    """The new state written over a tensor that an autograd graph needs: its backward says so, as for torch's own operations."""
+    a, _, _ = _inputs(2, 1, 1, 1, 8, 8, torch.float32)
+    args = [a[n][:, 0] for n in NAMES[:5]]
+    w = torch.ones_like(a["state"], requires_grad=True)
+    for state, out in ((a["state"].clone(), None), (a["state"].clone(), torch.zeros_like(a["state"]))):
+        target = state if out is None else out
+        y = (w * target).sum()
+        S.delta_filter_step(state, *args, out=target)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    y = (w * a["state"]).sum()
+    S.delta_filter_step(a["state"], *args)                  # a state that is only read
+    y.backward()
+    assert torch.equal(w.grad, a["state"])
+    with torch.inference_mode():                            # tensors without a version
+        plain = a["state"].clone()
+        S.delta_filter_step(plain, *args, out=plain)
+    assert torch.equal(plain, S.delta_filter_step(a["state"], *args)[1])

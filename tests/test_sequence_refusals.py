@@ -271,3 +271,12 @@ def test_captured_calls_find_the_leaves_behind_the_entry_points_own_operations(m
         calls[which]()
     del alive
     assert calls[which]().grad_fn is not None               # its graph is gone
+
+
+def test_step_refuses_an_output_buffer_that_requires_a_gradient():
+    from genjax_amd.families import state_space as S
+
+    B = _B()
+    args = [t[:, 0] for t in _delta_args()]
+    with pytest.raises(B.GjxError, match="`out` cannot be given"):
+        S.delta_filter_step(torch.zeros(2, 2, 8, 4), *args, out=torch.zeros(2, 2, 8, 4, requires_grad=True))
