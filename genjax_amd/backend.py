@@ -791,7 +791,7 @@ def delta_filter_step(state, q, k, v, log_decay, beta, scale=None, ancestors=Non
     from_, to = state.data_ptr(), out.data_ptr()
     if (from_ | to) & 15:
         raise GjxError(f"{who}: `state` and `out` must be aligned to 16 bytes")
-    if written and not out.is_inference():
+    if written:
         torch.autograd.graph.increment_version(out)             # as an in-place operation: a graph that saved it must not use it
     o = torch.empty((p.batch, p.heads, p.dv), dtype=v.dtype, device=v.device)
     N.check(N.lib().gjx_delta_filter_step(p.ref, from_, _address(ancestors), q.data_ptr(), k.data_ptr(), v.data_ptr(),

@@ -134,7 +134,7 @@ class _LinearCategoricalFn(torch.autograd.Function):
 
 class _LinearCategorical(Distribution):
     """linear_categorical(x, weight, bias=None): a draw from softmax(x W^T + b) per row.  x: (n, width) rows or one
-    (width,) row shared by every particle; weight: (vocab, width); bias: (vocab,).  All float32 or all bfloat16 and
+    (width,) row shared by every particle (sample_shape=(m,): m draws from it); weight: (vocab, width); bias: (vocab,).  All float32 or all bfloat16 and
     finite, the bias or -inf (its entry is never drawn and has the log-density -inf); sums and log-densities are
     float32.  Differentiable in x, weight and bias; the forward of a gradient keeps up to 2 GiB for it (the exponentials
     of all logits), and what would take more, or many rows of a small width, is formed again."""
@@ -148,14 +148,17 @@ class _LinearCategorical(Distribution):
             raise B.GjxError(f"linear_categorical: x {tuple(x.shape)} must be (width,) or (n, width)")
         return x if x.dim() == 2 and x.shape[0] == n else x.reshape(-1, x.shape[-1]).expand(n, x.shape[-1])
 
-    def sample(self, x, weight, bias=None, **kwargs):
+    def sample(self, x, weight, bias=None, sample_shape=None, **kwargs):
         from .core import _next_key, batch_size
 
         x, weight, bias = as_col(x), as_col(weight), None if bias is None else as_col(bias)
-        n = x.shape[0] if x.dim() == 2 else (batch_size() or 1)
+        if sample_shape and (x.dim() != 1 or len(sample_shape) != 1):
+            raise B.GjxError(f"linear_categorical: sample_shape {tuple(sample_shape)} must be one number of draws from one (width,) row "
+                             f"(x: {tuple(x.shape)})")
+        n = x.shape[0] if x.dim() == 2 else (sample_shape[0] if sample_shape else (batch_size() or 1))
         out = B.sample_linear_categorical(_next_key(), self._rows(x.detach(), n), weight.detach(),
                                           None if bias is None else bias.detach())
-        return out if (x.dim() == 2 or batch_size()) else out[0]
+        return out if (x.dim() == 2 or sample_shape or batch_size()) else out[0]
 
     def logpdf(self, y, x, weight, bias=None, **kwargs):
         x, weight, bias = as_col(x), as_col(weight), None if bias is None else as_col(bias)

@@ -541,3 +541,18 @@ def test_more_tiles_than_a_row_of_the_grid(G, dtype, vocab):
         part = slice(i, i + 3)
         _close("lp", lp[part], _truth(x[part], w, b, y[part], torch.ones(3, device="cuda"))["lp"])
     assert torch.isfinite(lp).all() and (lp < 0).all()
+
+
+def test_draws_of_a_shape(G):
+    """sample_shape as categorical takes it: that many draws from one row; anything else is refused, not ignored."""
+    from genjax_amd import backend as B
+
+    x, w, b, _, _ = _inputs(3, 6, 8, torch.float32)
+    draw = lambda *a, **k: G.seed(lambda: G.linear_categorical.sample(*a, **k))(G.key(1))      # noqa: E731
+    assert draw(x[0], w, b, sample_shape=(50,)).shape == (50,) and draw(x[0], w, b).shape == () and draw(x, w, b).shape == (3,)
+    logits = x[0] @ w.t() + b
+    ref = G.seed(lambda: G.categorical.sample(logits, sample_shape=(50,)))(G.key(1))
+    assert ref.shape == (50,) and len(set(draw(x[0], w, b, sample_shape=(50,)).tolist())) > 1
+    for bad in (dict(x=x, sample_shape=(50,)), dict(x=x[0], sample_shape=(5, 10))):
+        with pytest.raises(B.GjxError, match="sample_shape"):
+            draw(bad["x"], w, b, sample_shape=bad["sample_shape"])
