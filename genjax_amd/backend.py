@@ -14,6 +14,7 @@ from typing import Sequence
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as N
 from ._native import GjxError, LgssmParams, LocWorld, OutlierModel
@@ -459,6 +460,14 @@ def _on_current_device(who, *tensors):
 
 def _address(t):
     return 0 if t is None else t.data_ptr()
+
+
+def no_tangents(who, *values):
+    """Refuse dual tensors: what the library computes has no forward-mode derivative, and their tangents would be dropped."""
+    if forward_ad._current_level >= 0:                         # inside a dual_level()
+        for t in values:
+            if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+                raise GjxError(f"{who}: forward-mode derivatives (dual tensors) are not supported; use reverse mode")
 
 
 def _note_leaves(who, out):

@@ -161,6 +161,7 @@ class _LinearCategorical(Distribution):
         return out if (x.dim() == 2 or sample_shape or batch_size()) else out[0]
 
     def logpdf(self, y, x, weight, bias=None, **kwargs):
+        B.no_tangents(self.name, x, weight, bias)
         x, weight, bias = as_col(x), as_col(weight), None if bias is None else as_col(bias)
         y = y if isinstance(y, torch.Tensor) and y.is_cuda else torch.as_tensor(y, device=x.device)
         if y.dim() > 1:
@@ -198,6 +199,7 @@ class _MvNormal(Distribution):
         return out if (mu.dim() == 2 or cov.dim() == 3 or batch_size()) else out[0]
 
     def logpdf(self, x, mu, cov, **kwargs):
+        B.no_tangents(self.name, x, mu, cov)
         x, mu, cov = as_col(x), as_col(mu), as_col(cov)
         single = x.dim() == 1 and mu.dim() == 1 and cov.dim() == 2
         out = B.mvnormal_logpdf(x.reshape(-1, x.shape[-1]), mu, cov)

@@ -281,6 +281,7 @@ def delta_filter(q, k, v, log_decay, beta, initial_state=None, scale=None, lengt
 
     Returns (o (batch, time, heads, dv) of v's type, S_time (batch, heads, dk, dv) float32); differentiable in q, k, v,
     log_decay, beta and initial_state.  Chunks of 64 tokens run as matrix products; delta_filter_step takes one token."""
+    B.no_tangents("delta_filter", q, k, v, log_decay, beta, initial_state)
     if _wants_gradient(q, k, v, log_decay, beta, initial_state):
         out = _DeltaFilterFn.apply(q, k, v, log_decay, beta, initial_state, scale, lengths)
         B._note_leaves("delta_filter", out[0])
@@ -296,6 +297,7 @@ def delta_filter_step(state, q, k, v, log_decay, beta, scale=None, ancestors=Non
     the gather costs no pass of its own.  Indices are clamped to [0, n).  out: buffer for the new state -- the state
     itself (in place) when there are no ancestors.  Where a gradient is wanted the call is delta_filter over one
     token."""
+    B.no_tangents("delta_filter_step", state, q, k, v, log_decay, beta)
     if _wants_gradient(state, q, k, v, log_decay, beta, out):
         if out is not None:
             raise GjxError("delta_filter_step: `out` cannot be given where a gradient is wanted")

@@ -280,3 +280,30 @@ def test_step_refuses_an_output_buffer_that_requires_a_gradient():
     args = [t[:, 0] for t in _delta_args()]
     with pytest.raises(B.GjxError, match="`out` cannot be given"):
         S.delta_filter_step(torch.zeros(2, 2, 8, 4), *args, out=torch.zeros(2, 2, 8, 4, requires_grad=True))
+
+
+def test_dual_tensors_are_refused():
+    """Forward mode: the plain route would return a result without its tangent."""
+    from torch.autograd import forward_ad
+
+    import genjax_amd as G
+    from genjax_amd.families import state_space as S
+
+    B = _B()
+    args, state = _delta_args(), torch.zeros(2, 2, 8, 4)
+    x, w, b, y = torch.zeros(3, 8), torch.zeros(5, 8), torch.zeros(5), torch.zeros(3, dtype=torch.int32)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))        # noqa: E731
+        calls = [lambda i=i: S.delta_filter(*(dual(t) if i == j else t for j, t in enumerate(args))) for i in range(5)]
+        calls += [lambda: S.delta_filter(*args, initial_state=dual(state)),
+                  lambda: S.delta_filter_step(dual(state), *(t[:, 0] for t in args)),
+                  lambda: S.delta_filter_step(state, *(dual(t[:, 0]) for t in args)),
+                  lambda: G.linear_categorical.logpdf(y, dual(x), w, b), lambda: G.linear_categorical.logpdf(y, x, dual(w), b),
+                  lambda: G.linear_categorical.logpdf(y, x, w, dual(b)),
+                  lambda: G.normal.logpdf(dual(b), 0.0, 1.0), lambda: G.normal.logpdf(b, dual(b), 1.0),
+                  lambda: G.categorical.logpdf(y, dual(x)), lambda: G.multivariate_normal.logpdf(x, dual(x[0]), torch.eye(8))]
+        for call in calls:
+            with pytest.raises(B.GjxError, match="forward-mode"):
+                call()
+        with pytest.raises(B.GjxError, match="device tensor"):              # no tangent: as outside
+            S.delta_filter(*args)
