@@ -119,8 +119,8 @@ categorical = _Categorical(None, lambda x, logits: B.categorical_logpdf(x, as_co
 # row of them per particle.  The gradient (x, weight, bias) is the library's, as for the densities above.
 class _LinearCategoricalFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, y, x, weight, bias):
-        lp, lse, kept = B.linear_categorical_logpdf(y, x, weight, bias, keep=True)
+    def forward(ctx, y, x, weight, bias, keep):
+        lp, lse, kept = (*B.linear_categorical_logpdf(y, x, weight, bias, keep=keep), None)[:3]
         ctx.save_for_backward(y, x, weight, bias, lse, kept)
         return lp
 
@@ -129,7 +129,7 @@ class _LinearCategoricalFn(torch.autograd.Function):
         if torch.is_grad_enabled():
             raise B.GjxError("linear_categorical: its gradient cannot be differentiated again (create_graph=True)")
         y, x, weight, bias, lse, kept = ctx.saved_tensors
-        return (None, *B.linear_categorical_grad(y, x, weight, bias, lse, g, want=ctx.needs_input_grad[1:4], kept=kept))
+        return (None, *B.linear_categorical_grad(y, x, weight, bias, lse, g, want=ctx.needs_input_grad[1:4], kept=kept), None)
 
 
 class _LinearCategorical(Distribution):
@@ -137,7 +137,8 @@ class _LinearCategorical(Distribution):
     (width,) row shared by every particle (sample_shape=(m,): m draws from it); weight: (vocab, width); bias: (vocab,).  All float32 or all bfloat16 and
     finite, the bias or -inf (its entry is never drawn and has the log-density -inf); sums and log-densities are
     float32.  Differentiable in x, weight and bias; the forward of a gradient keeps up to 2 GiB for it (the exponentials
-    of all logits), and what would take more, or many rows of a small width, is formed again."""
+    of all logits) until the backward, and what would take more, or many rows of a small width, is formed again.  With
+    keep=False nothing is kept: for losses over many calls, whose kept exponentials would add up."""
 
     def _param_event_ndims(self, a):
         return a.dim() if isinstance(a, torch.Tensor) else 0
@@ -160,7 +161,7 @@ class _LinearCategorical(Distribution):
                                           None if bias is None else bias.detach())
         return out if (x.dim() == 2 or sample_shape or batch_size()) else out[0]
 
-    def logpdf(self, y, x, weight, bias=None, **kwargs):
+    def logpdf(self, y, x, weight, bias=None, keep=True, **kwargs):
         B.no_tangents(self.name, x, weight, bias)
         x, weight, bias = as_col(x), as_col(weight), None if bias is None else as_col(bias)
         y = y if isinstance(y, torch.Tensor) and y.is_cuda else torch.as_tensor(y, device=x.device)
@@ -178,7 +179,7 @@ class _LinearCategorical(Distribution):
         if ys.shape != (n,):
             ys = ys.reshape(-1).expand(n)
         if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
-            out = _LinearCategoricalFn.apply(ys, rows, weight, bias)
+            out = _LinearCategoricalFn.apply(ys, rows, weight, bias, bool(keep))
             B._note_leaves("linear_categorical", out)
         else:
             out = B.linear_categorical_logpdf(ys, rows, weight, bias, want_lse=False)[0]

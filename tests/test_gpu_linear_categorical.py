@@ -556,3 +556,24 @@ def test_draws_of_a_shape(G):
     for bad in (dict(x=x, sample_shape=(50,)), dict(x=x[0], sample_shape=(5, 10))):
         with pytest.raises(B.GjxError, match="sample_shape"):
             draw(bad["x"], w, b, sample_shape=bad["sample_shape"])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("n,vocab,width", [(20, 3000, 64), (100, 9000, 640)])
+def test_a_gradient_without_kept_exponentials(G, n, vocab, width, dtype):
+    """keep=False: the same bounds, and between forward and backward no more than the outputs and the inputs are held."""
+    x, w, b, y, up = _inputs(n, vocab, width, TYPES[dtype])
+    want = _truth(x, w, b, y, up)
+    held = []
+    for keep in (True, False):
+        leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        lp = G.linear_categorical.logpdf(y, *leaves, keep=keep)
+        held.append(torch.cuda.memory_allocated() - before)
+        _close("lp", lp.detach(), want["lp"])
+        for name, got in zip(("dx", "dw", "db"), torch.autograd.grad(lp, leaves, up)):
+            _close(name, got, want[name])
+    assert held[0] >= n * vocab * (2 if dtype == "bf16" else 4) and held[1] <= 4096
+    tr, _ = G.seed(lambda: G.linear_categorical.generate(y, x, w, b, keep=False))(G.key(0))      # through the interface, too
+    assert torch.equal(tr.get_score(), -G.linear_categorical.logpdf(y, x, w, b))
