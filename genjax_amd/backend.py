@@ -462,6 +462,14 @@ def _address(t):
     return 0 if t is None else t.data_ptr()
 
 
+def _upstream(who, name, t, shape, dtype, device):
+    """What a gradient entry reads besides its forward's inputs: of the outputs' shape and type, on the inputs' device."""
+    if not isinstance(t, torch.Tensor) or t.shape != shape or t.dtype != dtype or t.device != device:
+        what = f"{t.dtype} {tuple(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
+        raise GjxError(f"{who}: `{name}` must be {dtype} of shape {tuple(shape)} on {device}, got {what}")
+    return t.contiguous()
+
+
 def no_tangents(who, *values):
     """Refuse dual tensors: what the library computes has no forward-mode derivative, and their tangents would be dropped."""
     if forward_ad._current_level >= 0:                         # inside a dual_level()
@@ -590,7 +598,8 @@ def linear_categorical_grad(y, x, weight, bias, lse, upstream, want=(True, True,
     if a.n == 0:
         return [None if o is None else o.zero_() for o in outs]
     if any(o is not None for o in outs):
-        upstream = _f32(upstream).contiguous()
+        lse = _upstream("linear_categorical", "lse", lse, (a.n,), torch.float32, a.x.device)
+        upstream = _upstream("linear_categorical", "upstream", _f32(upstream), (a.n,), torch.float32, a.x.device)
         dtype, xp, x_ld, wp, w_ld = a.head
         work = a.workspace(1 if outs[0] is not None else 2)
         N.check(N.lib().gjx_linear_categorical_grad(dtype, y.data_ptr(), xp, x_ld, wp, w_ld, _address(a.bias), a.n, a.vocab, a.width,
@@ -740,7 +749,8 @@ def delta_filter_grad(q, k, v, log_decay, beta, d_o, d_state, kept, scale=None, 
     lengths = _delta_indices(who, "lengths", lengths, p)
     d_state = _delta_state(who, "d_state", d_state, p)
     dev = v.device
-    d_o = torch.zeros((p.batch, p.time, p.heads, p.dv), dtype=v.dtype, device=dev) if d_o is None else d_o.contiguous()
+    o_shape = (p.batch, p.time, p.heads, p.dv)
+    d_o = torch.zeros(o_shape, dtype=v.dtype, device=dev) if d_o is None else _upstream(who, "d_o", d_o, o_shape, v.dtype, dev)
     outs = [torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v, g, be)]
     state0 = torch.empty((p.batch, p.heads, p.dk, p.dv), dtype=torch.float32, device=dev) if want_state0 else None
     work = p.workspace(2, dev)

@@ -307,3 +307,22 @@ def test_dual_tensors_are_refused():
                 call()
         with pytest.raises(B.GjxError, match="device tensor"):              # no tangent: as outside
             S.delta_filter(*args)
+
+
+def test_gradient_entries_check_their_upstream(monkeypatch):
+    """An upstream gradient of another shape or type would be read behind its end."""
+    B = _B()
+    monkeypatch.setattr(B, "_on_current_device", lambda *a: None)
+    x, w, y = torch.zeros(3, 8), torch.zeros(5, 8), torch.zeros(3, dtype=torch.int32)
+    good = torch.zeros(3)
+    for lse, up, name in ((good, torch.zeros(()), "upstream"), (good, torch.zeros(2), "upstream"), (good, torch.zeros(3, 1), "upstream"),
+                          (torch.zeros(2), good, "lse"), (good.double(), good, "lse"), (None, good, "lse")):
+        with pytest.raises(B.GjxError, match=f"`{name}` must be"):
+            B.linear_categorical_grad(y, x, w, None, lse, up)
+    args = _delta_args()
+    o = torch.zeros(args[2].shape)
+    for bad in (o[:1], o[:, :1], o.double(), o.bfloat16(), o.to("meta"), 1.0):
+        with pytest.raises(B.GjxError, match="`d_o` must be"):
+            B.delta_filter_grad(*args, bad, None, torch.zeros(1, dtype=torch.uint8))
+    with pytest.raises(B.GjxError, match="`d_state` must be"):
+        B.delta_filter_grad(*args, o, torch.zeros(1, 2, 8, 4), torch.zeros(1, dtype=torch.uint8))
