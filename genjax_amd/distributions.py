@@ -167,7 +167,7 @@ class _LinearCategorical(Distribution):
         y = y if isinstance(y, torch.Tensor) and y.is_cuda else torch.as_tensor(y, device=x.device)
         if y.dim() > 1:
             raise B.GjxError(f"linear_categorical: y {tuple(y.shape)} must be one value or one per row")
-        n = x.shape[0] if x.dim() == 2 else max(1, y.numel())
+        n = x.shape[0] if x.dim() == 2 else y.numel()
         if y.dim() == 1 and x.dim() == 2 and n == 1:
             n = y.numel()
         if y.dim() == 1 and y.numel() not in (1, n):

@@ -577,3 +577,14 @@ def test_a_gradient_without_kept_exponentials(G, n, vocab, width, dtype):
     assert held[0] >= n * vocab * (2 if dtype == "bf16" else 4) and held[1] <= 4096
     tr, _ = G.seed(lambda: G.linear_categorical.generate(y, x, w, b, keep=False))(G.key(0))      # through the interface, too
     assert torch.equal(tr.get_score(), -G.linear_categorical.logpdf(y, x, w, b))
+
+
+def test_no_value_of_a_shared_row(G):
+    x, w, b, y, _ = _inputs(1, 6, 8, torch.float32)
+    for row in (x[0], x):
+        leaves = [t.clone().requires_grad_(True) for t in (row, w, b)]
+        assert G.linear_categorical.logpdf(y[:0], row, w, b).shape == (0,)
+        lp = G.linear_categorical.logpdf(y[:0], *leaves)
+        assert lp.shape == (0,)
+        for g, t in zip(torch.autograd.grad(lp.sum(), leaves), leaves):
+            assert torch.equal(g, torch.zeros_like(t))
