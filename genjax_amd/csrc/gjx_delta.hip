@@ -1035,9 +1035,10 @@ __global__ void __launch_bounds__(TEAM, 2)
 // Sixteen waves: wave w forms the rows of tokens [16 (w % 4), + 16) and the dk quarter w / 4.  Per 32 columns of dv, S0, dS1,
 // e, delta and dO become fragment planes in LDS once, for all waves (each wave splitting its own operands: 380 us for 1024
 // chunks of 64 x 128 x 128), while the next columns are on their way to registers; the row sums <dS1, S0> and e.delta
-// fall out of the same registers.  1024 chunks in 112 us, 290 MB at 2.6 TB/s: memory, splitting and products of the one
-// workgroup that a CU holds take turns.  E and F go to LDS as fragments of themselves and of their transposes, split once.
-// (Eight waves of twice the work, 194 registers: 129 us instead of 113 for them; the phases of one workgroup hardly overlapped.)
+// fall out of the same registers.  1024 chunks in 119 to 128 us, 320 MB at 2.6 TB/s: memory, splitting and products of the one
+// workgroup that a CU holds take turns (8 us of them are the products q.k and k.k that the decays' gradient takes).  E and F go
+// to LDS as fragments of themselves and of their transposes, split once.  (Eight waves of twice the work, 194 registers, before
+// those products: 129 us against 113; the phases of one workgroup hardly overlapped.)
 constexpr int BACK = 1024;
 
 // eight values from LDS to a row, in vectors of 16 bytes where it is whole and aligned

@@ -485,7 +485,7 @@ __device__ __forceinline__ void epilogue(const GemmArgs& g, const Tile& tile, f3
 #pragma unroll
       for (int r = 0; r < 4; ++r) dbs[i][r] += acc[i][j][r];
       if (sizeof(T) == 2) {
-        // rounded to bf16 (the products that follow take bf16 operands): each entry is off by at most 2^-9 of it,
+        // rounded to bf16 (the products that follow take bf16 operands): each entry is off by at most 2^-8 of it,
         // independently of its neighbours.  The value's own entry is usually far larger than the others, so that ONE
         // rounding would show in whole rows of the gradients: what it loses is kept apart and added in f32.
         bf16x4 h;
@@ -522,8 +522,8 @@ __device__ __forceinline__ void epilogue(const GemmArgs& g, const Tile& tile, f3
 }
 
 // C[m][n] = sum_k A(m, k) B(n, k) in bf16; BM x BN per workgroup of eight waves.  Bound by the matrix unit at the clock that
-// it sustains: 4096 x 128000 x 4096 (log-densities) in 3.15 ms = 1.36 PFLOP/s, where a library product of these sizes reaches
-// 1.2 to 1.4; dx and dW of 4096 x 128000 x 2048 at 1.21 and 1.05.  Two LDS buffers of one 64-deep tile each
+// it sustains: 4096 x 128000 x 4096 (log-densities) in 3.06 to 3.3 ms once the clock has settled = 1.3 to 1.4 PFLOP/s, where a
+// library product of these sizes reaches 1.2 to 1.4; dx and dW of 4096 x 128000 x 2048 at 1.27 and 1.12.  Two LDS buffers of one 64-deep tile each
 // and two register sets of fragments: while the products of one 32-deep slab run, the next slab is read (across the tile's
 // end: the one barrier of a tile stands between its two slabs, when its last slab is in registers), and the tile after the
 // next one is on its way into the buffer just emptied.
@@ -697,9 +697,10 @@ struct SlabLoader {
 // the same product of f32 operands: six matrix instructions per fragment pair, so the splitting (once per tile) and the
 // LDS traffic are small beside them and no packed copy of the operands is needed (packing to bf16 planes first: pack and
 // product 328 us for 200 x 50001 x 768).  One 32-deep slab in LDS, the next one in registers; three workgroups a CU
-// cover each other's splitting and barriers and leave less idle at the end than one of twice the size.  Bound by the matrix
-// unit (busy 57 % of the time), the splitting beside it and how evenly the tiles fill the CUs: 200 x 50001 x 768 in 100 us (0.92
-// PFLOP/s of partial products), 1000 x 20011 x 512 in 121 to 139 us per product (0.88 to 1.02).
+// cover each other's splitting and barriers and leave less idle at the end than one of twice the size.  No one unit is the
+// bound: the matrix unit is busy 57 % of the time, the rest goes to splitting, LDS and barriers where the workgroups of a CU
+// do not cover each other, and to CUs that the last tiles leave idle: 200 x 50001 x 768 in 109 to 119 us (0.83 PFLOP/s of
+// partial products), 1000 x 20011 x 512 in 112 to 150 us per product (0.82 to 1.1).
 template <int BN, bool TA, bool TB, int EPI>
 __global__ void __launch_bounds__(GEMM32_THREADS, BN > 128 ? 2 : 3)
     k_lincat_gemm32(GemmArgs g) {
@@ -1213,7 +1214,9 @@ constexpr int64_t MAX_LD = 1 << 22;                   // 256 rows stay within 32
 // room for), so that the weights are read and split once instead of once for each of two tiles of 128.  Two such workgroups on a
 // CU take the time of 3.55 of the smaller ones, one alone that of 2.8, so it depends on how the tiles fill the CUs: 200 rows of
 // width 256, one tile / two tiles, at 250 tiles of the vocabulary 39 / 31 us, 321: 43 / 38, 391: 44 / 51, 508: 47 / 52,
-// 625: 72 / 60, 1000: 85 / 90; 200 x 50001 x 768: 105 / 132.
+// 625: 72 / 60, 1000: 85 / 90; 200 x 50001 x 768: 105 / 132.  The row count moves neither side (130, 150, 180, 200 and 208 rows
+// within 4 %): width 256 at 391 tiles 44 / 52, 508: 48 / 56, 560: 75 / 62, 1000: 95 / 100; width 768 at 321: 104 / 100, 391:
+// 109 / 133, 508: 125 / 144, 625: 191 / 169, 1000: 240 / 263.
 constexpr int ALL_ROWS = 208;
 bool one_row_tile(int64_t n, int64_t vocab_tiles) {
   const int64_t each = (vocab_tiles + 255) / 256, halves = (2 * vocab_tiles + 255) / 256;        // workgroups per CU
@@ -1223,9 +1226,11 @@ bool one_row_tile(int64_t n, int64_t vocab_tiles) {
 constexpr int CUT_DEPTH_F32 = 12, CUT_DEPTH_BF16 = 24, CUT_ROWS_DEPTH = 24, CUT_TILES = 64, CUT_DEEP = 32;
 constexpr int ROWS_MAX = 32;                          // rows up to which k_lincat_rows is used
 // What the forward of a gradient keeps (the exponentials of all logits) spares the gradient its first product and costs a
-// write and a read of them; up to this size, and from the width on where the product is the dearer one (up to 32 rows: always,
-// the product there takes as long as the weights; 1 x 35780 x 1386 f32: 300 us with it formed again, 240 kept).  Forward and gradient,
-// kept against formed again: bf16 4096 x 32000 x 128: 475 / 460 us, x 256: 524 / 549, x 512: 610 / 666, x 1024: 915 / 1040;
+// write and a read of them; up to this size, and from the width on where the product is the dearer one; up to 32 rows
+// always, since the product there takes as long as the weights.  Forward and gradient, kept against formed again, on the GPU alone:
+// f32 1 x 35780 x 1386: 237 / 298 us, 8 x 128000 x 256: 133 / 160, 32 x 20011 x 512: 78 / 90, 32 x 128000 x 32: 98 / 100, 32 x 300 x 32:
+// 33 / 32; bf16 1 x 32000 x 1024: 73 / 90, 8 x 128000 x 256: 96 / 107, 32 x 128000 x 512: 168 / 181, x 64: 83 / 84, 32 x 32000 x 64:
+// 51 / 49, 16 x 1000 x 64: 40 / 39.  More rows: bf16 4096 x 32000 x 128: 475 / 460 us, x 256: 524 / 549, x 512: 610 / 666, x 1024: 915 / 1040;
 // 300 x 8000 x 256: 62 / 57, x 512: 65 / 66; f32 1000 x 20011 x 64: 180 / 180, x 128: 191 / 200, x 512: 396 / 468.
 constexpr int64_t KEEP_BYTES = (int64_t)2 << 30;
 constexpr int KEEP_WIDTH_F32 = 128, KEEP_WIDTH_BF16 = 512;
