@@ -258,6 +258,7 @@ _SIGNATURES = {
     "gjx_delta_filter_workspace": ([C.POINTER(DeltaShape), _i32, C.POINTER(_i64)], _i32),
     "gjx_delta_filter": ([C.POINTER(DeltaShape)] + [_vp] * 9 + [_i32, _vp, _i64, _vp], _i32),
     "gjx_delta_filter_grad": ([C.POINTER(DeltaShape)] + [_vp] * 15 + [_i64, _vp, _i64, _vp], _i32),
+    "gjx_gather_states_grad_f32": ([_vp] * 3 + [_i64] * 2 + [_vp] * 3, _i32),
     "gjx_delta_filter_step": ([C.POINTER(DeltaShape)] + [_vp] * 10, _i32),
     "gjx_lgssm_smc_run": ([_vp, C.POINTER(LgssmParams), _u32p, _i32, _f32p, _i64, _i32] + [_vp] * 11
                           + [C.POINTER(C.c_int32), _vp], _i32),

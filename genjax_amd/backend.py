@@ -761,6 +761,20 @@ def delta_filter_grad(q, k, v, log_decay, beta, d_o, d_state, kept, scale=None, 
     return outs + [state0]
 
 
+def gather_states_grad(grad, ancestors):
+    """Gradient of state[ancestors] over the first axis (n rows from n): row j sums the rows of grad whose ancestor is j, in order."""
+    n = ancestors.shape[0]
+    _on_current_device("gather_states_grad", ("grad", grad), ("ancestors", ancestors))
+    grad = _upstream("gather_states_grad", "grad", grad, (n, *grad.shape[1:]), torch.float32, ancestors.device)
+    out = torch.empty_like(grad)
+    if out.numel() > 0:
+        values, order = torch.sort(ancestors.clamp(0, n - 1), stable=True)
+        starts = torch.empty(n + 1, dtype=torch.int64, device=grad.device)
+        N.check(N.lib().gjx_gather_states_grad_f32(grad.data_ptr(), values.data_ptr(), order.data_ptr(), n, grad.numel() // n,
+                                                   starts.data_ptr(), out.data_ptr(), _raw_stream()), "gjx_gather_states_grad_f32")
+    return out
+
+
 @functools.lru_cache(maxsize=1024)
 def _delta_step_plan(dtypes, q_shape, k_shape, v_shape, g_shape, b_shape, q_stride, k_stride, v_stride, g_stride, b_stride, scale):
     who = "delta_filter_step"

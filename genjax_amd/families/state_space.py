@@ -267,6 +267,19 @@ class _DeltaFilterFn(torch.autograd.Function):
         return (*grads, None, None)
 
 
+class _GatherStatesFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, state, ancestors):
+        ctx.save_for_backward(ancestors)
+        return state.index_select(0, ancestors.clamp(0, state.shape[0] - 1))
+
+    @staticmethod
+    def backward(ctx, grad):
+        if torch.is_grad_enabled():
+            raise GjxError("delta_filter_step: its gradient cannot be differentiated again (create_graph=True)")
+        return B.gather_states_grad(grad, *ctx.saved_tensors), None
+
+
 def delta_filter(q, k, v, log_decay, beta, initial_state=None, scale=None, lengths=None):
     """The gated delta filter over whole sequences: per batch element and head, with a_t = exp(log_decay_t),
 
@@ -309,7 +322,7 @@ def delta_filter_step(state, q, k, v, log_decay, beta, scale=None, ancestors=Non
             if not isinstance(ancestors, torch.Tensor) or ancestors.dtype != torch.int32 or ancestors.shape != (n,):
                 raise GjxError(f"delta_filter_step: `ancestors` must be int32 of shape ({n},)")
             if n > 0:
-                state = state.index_select(0, ancestors.long().clamp(0, n - 1))
+                state = _GatherStatesFn.apply(state, ancestors)
         o, new = delta_filter(*(t.unsqueeze(1) for t in (q, k, v, log_decay, beta)), initial_state=state, scale=scale)
         return o.squeeze(1), new
     return B.delta_filter_step(state, q, k, v, log_decay, beta, scale, ancestors, out)

@@ -772,6 +772,13 @@ int32_t gjx_delta_filter_step(const gjx_delta_shape* shape, const float* d_state
                               const void* d_q, const void* d_k, const void* d_v, const float* d_g, const float* d_beta,
                               void* d_o, float* d_state_out, void* stream);
 
+/* Gradient of a gather of n states by ancestors (out_i = state_{ancestor_i}; smc.py:170-174): d_out[j] = sum of the rows
+ * d_grad[i] of the i with ancestor j, added in a fixed order; a row without one is 0.  `row`: entries of a state; d_sorted: the
+ * ancestors in ascending order, all in [0, n); d_order: where each came from, ascending among equals (a stable sort);
+ * d_starts: n + 1 entries of scratch. */
+int32_t gjx_gather_states_grad_f32(const float* d_grad, const int32_t* d_sorted, const int64_t* d_order, int64_t n, int64_t row,
+                                   int64_t* d_starts, float* d_out, void* stream);
+
 /* ---- Game-of-Life inversion by single-site Gibbs sweeps (examples/gol/core.py) ----
  * Boards: n_chains x n x n cells, one byte (0 / 1) per cell, row-major, square (the
  * reference's range mask, core.py:141-149, mixes the axes; all its boards are square).

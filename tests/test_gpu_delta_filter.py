@@ -435,3 +435,59 @@ def test_step_into_a_buffer_that_a_graph_saved(S):
         plain = a["state"].clone()
         S.delta_filter_step(plain, *args, out=plain)
     assert torch.equal(plain, S.delta_filter_step(a["state"], *args)[1])
+
+
+@pytest.mark.parametrize("n,shape", [(1, (1, 1, 1)), (5, (2, 3, 5)), (300, (4, 16, 16)), (2000, (1, 1, 2)), (700, (3, 7, 11)), (40, (8, 128, 128)),
+                                     (3000, (2, 8, 8))])
+def test_gradient_of_gathered_states(S, n, shape):
+    """Rows summed by ancestor: spread, sorted, half of them one ancestor's, all of them one's; the same bits every time.
+    A sum of c terms in f32, in any order, is off by at most c 2^-24 of the sum of their sizes."""
+    from genjax_amd import backend as B
+
+    gen = torch.Generator("cuda").manual_seed(n)
+    d = torch.randn(n, *shape, device="cuda", generator=gen)
+    spread = torch.randint(0, n, (n,), device="cuda", generator=gen, dtype=torch.int32)
+    half = torch.where(torch.rand(n, device="cuda", generator=gen) < 0.5, n // 3, spread).to(torch.int32)
+    for anc in (spread, spread.sort()[0], half, torch.full_like(spread, n - 1), torch.arange(n, device="cuda", dtype=torch.int32)):
+        want, size = (torch.zeros(n, *shape, device="cuda", dtype=torch.float64).index_add_(0, anc.long(), t.double()) for t in (d, d.abs()))
+        got = B.gather_states_grad(d, anc)
+        count = torch.bincount(anc.long(), minlength=n).reshape(n, 1, 1, 1)
+        assert ((got.double() - want).abs() <= count * 2.0 ** -24 * size).all()
+        for _ in range(3):
+            assert torch.equal(got, B.gather_states_grad(d, anc))
+    far = spread.clone()
+    far[0], far[-1] = -7, 10 ** 9                            # taken to the nearest particle, as the forward takes them
+    assert torch.equal(B.gather_states_grad(d, far), B.gather_states_grad(d, far.clamp(0, n - 1)))
+    odd = torch.empty(d.numel() + 1, device="cuda")[1:].view_as(d).copy_(d)      # not aligned to 16 bytes
+    assert ((B.gather_states_grad(odd, half) - B.gather_states_grad(d, half)).abs() <= 2.0 ** -12 * d.abs().max()).all()
+
+
+def test_gradients_through_repeated_ancestors_have_the_same_bits(S):
+    """Eager calls and replays of a captured one, with other ancestors each time."""
+    n = 200
+    a, d_o, d_state = _inputs(n, 1, 1, 2, 16, 24, torch.float32)
+    args = [a[x][:, 0] for x in NAMES[:5]]
+    leaf = a["state"].clone().requires_grad_(True)
+    gen = torch.Generator("cuda").manual_seed(3)
+    anc = torch.randint(0, 9, (n,), device="cuda", generator=gen, dtype=torch.int32)
+
+    def grad():
+        o, new = S.delta_filter_step(leaf, *args, ancestors=anc)
+        return torch.autograd.grad([o, new], leaf, [d_o[:, 0], d_state])[0]
+
+    first = grad()
+    assert all(torch.equal(first, grad()) for _ in range(4))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        grad()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        out = grad()
+    for turn in range(5):
+        anc.copy_(torch.randint(0, 1 + 40 * turn, (n,), device="cuda", generator=gen))
+        graph.replay()
+        want = grad()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)

@@ -326,3 +326,14 @@ def test_gradient_entries_check_their_upstream(monkeypatch):
             B.delta_filter_grad(*args, bad, None, torch.zeros(1, dtype=torch.uint8))
     with pytest.raises(B.GjxError, match="`d_state` must be"):
         B.delta_filter_grad(*args, o, torch.zeros(1, 2, 8, 4), torch.zeros(1, dtype=torch.uint8))
+
+
+def test_gather_gradient_abi_refusals():
+    from genjax_amd import _native as N
+
+    L, p = N.lib(), C.c_void_p(1 << 20)
+    run = lambda d=p, s=p, o=p, n=3, row=4, w=p, out=p: L.gjx_gather_states_grad_f32(d, s, o, n, row, w, out, None)      # noqa: E731
+    assert run(n=-1) == -1 and run(row=0) == -1
+    assert run(d=None) == -1 and run(s=None) == -1 and run(o=None) == -1 and run(w=None) == -1 and run(out=None) == -1
+    assert run(n=(1 << 24) + 1) == -4 and run(row=(1 << 30) + 1) == -4 and run(n=1 << 24, row=1 << 20) == -4
+    assert run(n=0, d=None, s=None, o=None, w=None, out=None) == 0
