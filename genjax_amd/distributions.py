@@ -145,6 +145,8 @@ class _LinearCategorical(Distribution):
 
     @staticmethod
     def _rows(x, n):
+        # (a shared row's gradient is the sum of the n rows', each in x's type: in bfloat16 as many roundings of 2^-8 of a
+        # row's gradient, which add up as their signs fall, besides the sum's own)
         if x.dim() not in (1, 2):
             raise B.GjxError(f"linear_categorical: x {tuple(x.shape)} must be (width,) or (n, width)")
         return x if x.dim() == 2 and x.shape[0] == n else x.reshape(-1, x.shape[-1]).expand(n, x.shape[-1])

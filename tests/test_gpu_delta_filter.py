@@ -491,3 +491,30 @@ def test_gradients_through_repeated_ancestors_have_the_same_bits(S):
         want = grad()
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+
+
+def test_sequences_beyond_32_bit_offsets(S):
+    """v, o and their gradients pass 2^31 entries.  With log-decays of -0.5 nothing reaches further than e^-64 over 128 tokens, so
+    the last tokens' outputs are those of the last 192 alone, the first tokens' gradients those of the first 192."""
+    time, heads, dk, dv = (1 << 20) + 70, 16, 32, 128
+    gen = torch.Generator("cuda").manual_seed(8)
+    r = lambda *s: torch.randn(s, generator=gen, device="cuda", dtype=torch.bfloat16)        # noqa: E731
+    q, k = (torch.nn.functional.normalize(r(1, time, 1, dk), dim=-1) for _ in range(2))
+    v, d_o = r(1, time, heads, dv), r(1, time, heads, dv)
+    assert v.numel() > 1 << 31
+    g = torch.full((1, 1, 1), -0.5, device="cuda").expand(1, time, heads)
+    beta = torch.full((1, 1, 1), 0.5, device="cuda").expand(1, time, heads)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    o, last = S.delta_filter(q, k, v, g, beta)
+    grads = torch.autograd.grad(o, leaves, d_o)
+    first = ((time - 192) // 64) * 64                       # where a chunk begins
+    for part, out, gradients in ((slice(first, time), slice(128, None), False), (slice(0, 192), slice(0, 64), True),
+                                 (slice(first, time), slice(128, None), True)):
+        short = [t.detach()[:, part].clone().requires_grad_(True) for t in leaves]
+        o2, s2 = S.delta_filter(*short, g[:, part], beta[:, part])
+        if not gradients:
+            _close("o", o[:, part][:, out].detach(), o2[:, out].detach().double(), 2.0 ** -14)
+            _close("state", last.detach(), s2.detach().double(), 2.0 ** -14)
+        else:
+            for name, x, y in zip("qkv", grads, torch.autograd.grad(o2, short, d_o[:, part])):
+                _close("d" + name, x[:, part][:, out], y[:, out].double(), 2.0 ** -13)

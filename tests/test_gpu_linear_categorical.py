@@ -588,3 +588,30 @@ def test_no_value_of_a_shared_row(G):
         assert lp.shape == (0,)
         for g, t in zip(torch.autograd.grad(lp.sum(), leaves), leaves):
             assert torch.equal(g, torch.zeros_like(t))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("n,vocab,width", [(100000, 50, 64), (300, 100, 2048)])
+def test_captured_gradient_of_a_shared_row(G, n, vocab, width, dtype):
+    """The row's gradient is a sum over all values; every replay against the eager result."""
+    x, w, _, y, up = _inputs(n, vocab, width, TYPES[dtype])
+    leaf = x[0].clone().requires_grad_(True)
+
+    def grad():
+        return torch.autograd.grad(G.linear_categorical.logpdf(y, leaf, w), leaf, up)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        grad()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        out = grad()
+    for turn in range(5):
+        with torch.no_grad():
+            leaf.copy_(torch.randn(width, device="cuda", generator=torch.Generator("cuda").manual_seed(turn)))
+        graph.replay()
+        want = grad()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
