@@ -483,11 +483,11 @@ def _note_leaves(who, out):
     leaf's node keeps the stream it was made on, and a captured backward that reaches such a node waits across the capture
     border, which ends the process.  Leaves are noted on their nodes, which live as long as the graph; an eager call notes
     those of the 32 nodes nearest to it (the entry points put up to two of their own between a leaf and the call, a gather or
-    a reshape and a broadcast), a captured one looks through its whole graph."""
+    a reshape and a broadcast), a captured one looks through the nearest 1024 (long chains of calls walk it each time)."""
     stream = _raw_stream()
     capturing = torch.cuda.is_current_stream_capturing()
     nodes, seen = collections.deque([out.grad_fn]), set()
-    while nodes and (capturing or len(seen) < 32):
+    while nodes and len(seen) < (1024 if capturing else 32):
         for down, _ in nodes.popleft().next_functions:
             if down is None or down in seen:
                 continue

@@ -464,7 +464,7 @@ class Distribution(GFI):
         return self._sampler(_next_key(), self._shape(args), *args, **kwargs)
 
     def logpdf(self, x, *args, **kwargs):
-        B.no_tangents(self.name, x, *args)
+        B.no_tangents(self.name, x, *args, *kwargs.values())
         return self._logpdf(as_col(x) if not isinstance(x, torch.Tensor) else x, *args, **kwargs)
 
     def simulate(self, *args, **kwargs):

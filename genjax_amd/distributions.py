@@ -134,11 +134,11 @@ class _LinearCategoricalFn(torch.autograd.Function):
 
 class _LinearCategorical(Distribution):
     """linear_categorical(x, weight, bias=None): a draw from softmax(x W^T + b) per row.  x: (n, width) rows or one
-    (width,) row shared by every particle (sample_shape=(m,): m draws from it); weight: (vocab, width); bias: (vocab,).  All float32 or all bfloat16 and
-    finite, the bias or -inf (its entry is never drawn and has the log-density -inf); sums and log-densities are
-    float32.  Differentiable in x, weight and bias; the forward of a gradient keeps up to 2 GiB for it (the exponentials
-    of all logits) until the backward, and what would take more, or many rows of a small width, is formed again.  With
-    keep=False nothing is kept: for losses over many calls, whose kept exponentials would add up."""
+    (width,) row shared by every particle (sample_shape=(m,): m draws from it); weight: (vocab, width); bias: (vocab,).
+    All float32 or all bfloat16 and finite, the bias or -inf (its entry is never drawn and has the log-density -inf);
+    sums and log-densities are float32.  Differentiable in x, weight and bias; the forward of a gradient keeps up to 2 GiB
+    for it (the exponentials of all logits) until the backward, and what would take more, or many rows of a small width, is
+    formed again.  With keep=False nothing is kept: for losses over many calls, whose kept exponentials would add up."""
 
     def _param_event_ndims(self, a):
         return a.dim() if isinstance(a, torch.Tensor) else 0
